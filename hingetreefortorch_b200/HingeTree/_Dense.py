@@ -1,0 +1,31 @@
+"""The dense layers around a forest as functions: a gated projection in front of one, the loss of a linear layer's class scores
+behind one.
+
+The reference has neither as an operator: its pipelines put torch.nn modules in front of a forest and take the loss of the scores that
+a (fused) linear layer writes (README.md:110-129).
+"""
+from .._ext import hingetree_cpp
+
+
+def gated_linear(x, gate_weight, value_weight, gate_bias=None, value_bias=None, activation="silu"):
+    """act(x @ gate_weight.T + gate_bias) * (x @ value_weight.T + value_bias), both projections, the activation and the product in
+    one kernel.
+
+    x: [..., features]; weights: [outputs, features]; biases: [outputs] or None; all torch.float32, bfloat16 or float16, one type for all.
+    activation: 'silu', 'gelu' (with the normal distribution function), 'relu' or 'sigmoid'.  Sums are fp32 whatever the type, and
+    fp32 results are as accurate as fp32 products.  Nothing but the inputs is kept for the backward, which forms the projections again."""
+    return hingetree_cpp.gated_linear(x, gate_weight, value_weight, gate_bias, value_bias, activation)
+
+
+def linear_class_loss(x, weight, bias, target, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the class scores x @ weight.T + bias, which never lie in memory, and its gradient.
+
+    x: [..., features]; weight: [classes, features]; bias: [classes] or None; one type of torch.float32, bfloat16 or float16 for all;
+    target: int64, [...].  The loss is float32 whatever the type: one number for 'mean' (over the rows that count; NaN where none
+    does) and 'sum', one per row for 'none'.
+
+    A row whose target is ignore_index has loss and gradient 0 whatever it holds.  A target that is neither a class nor ignore_index
+    makes the loss NaN, and the next call that reads the device's status word (hingetree_cpp.pipeline_status(), or the first call on new
+    ordinals) raises RuntimeError.  The backward holds the gradient of the scores in pieces of 512 MiB at the most, less with
+    hingetree_cpp.set_backward_scratch_limit(bytes)."""
+    return hingetree_cpp.linear_class_loss(x, weight, bias, target, ignore_index, reduction)

@@ -1,4 +1,5 @@
-"""Autograd functions of the hinge tree drop-in (same exported names as the reference package)."""
+"""Autograd functions of the hinge tree drop-in (same exported names as the reference package, plus the dense
+layers around a forest)."""
 from ._HingeTree import (  # noqa: F401
     contract, expand, Contract, Expand,
     HingeTree, HingeFern, SparseHingeTree, SparseHingeFern,
@@ -7,3 +8,4 @@ from ._HingeTree import (  # noqa: F401
     HingeTreeConv1d, HingeTreeConv2d, HingeTreeConv3d, HingeFernConv1d, HingeFernConv2d, HingeFernConv3d,
     HingeTrie,
 )
+from ._Dense import gated_linear, linear_class_loss  # noqa: F401

@@ -191,6 +191,16 @@ class RandomHingeForestFusedLinear(_FusedLinearMixin, RandomHingeForest):
     def forward(self, x):
         return self._linear_function.apply(x, *self._params())
 
+    def class_loss(self, x, target, ignore_index: int = -100, reduction: str = "mean"):
+        """Softmax cross entropy of forward(x) as class scores against target (int64, [B] or [B, *inner]), which takes the trees'
+        outputs and the linear layer as they are and never writes the scores (HingeTree.linear_class_loss)."""
+        if self.weights.dim() != 2:
+            raise RuntimeError("class_loss takes forests without extra_outputs: a leaf holds one number.")
+        features = self._function.apply(x, *self._tree_params())
+        if features.dim() > 2:  # trees last
+            features = features.movedim(1, -1)
+        return _F.linear_class_loss(features, self.linear_weights, self.linear_bias, target, ignore_index, reduction)
+
     def _tree_params(self):
         return self.thresholds, self.ordinals, self.weights
 
@@ -213,6 +223,7 @@ class RandomHingeFernFusedLinear(_FusedLinearMixin, RandomHingeFern):
         self._init_linear(number_of_trees, out_channels, bias)
 
     forward = RandomHingeForestFusedLinear.forward
+    class_loss = RandomHingeForestFusedLinear.class_loss
     _tree_params = RandomHingeForestFusedLinear._tree_params
     reachability = RandomHingeForestFusedLinear.reachability
     leafmap = RandomHingeForestFusedLinear.leafmap

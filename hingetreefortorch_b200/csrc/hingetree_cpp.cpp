@@ -9,6 +9,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
@@ -145,7 +146,17 @@ torch::Tensor sticky_word(const c10::Device &device, bool create) {
   bad_runtime("Error: a bounded wait inside a hinge tree kernel ran out (a parameter or gradient copy never arrived); "
               "the results of the calls since the last check are incomplete.");
 }
+
+[[noreturn]] void raise_target_range() {
+  bad_runtime("Error: a class loss since the last check was given a target that is neither a class nor the ignored one.");
+}
 }  // namespace
+
+uint32_t *long_lived_word(const torch::Tensor &like) {
+  const bool capturing = c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+  const torch::Tensor word = sticky_word(like.device(), !capturing);
+  return word.defined() ? reinterpret_cast<uint32_t *>(word.data_ptr<int32_t>()) : nullptr;
+}
 
 OrdinalGuard::OrdinalGuard(const torch::Tensor &ord, int64_t channels) : ord_(ord), channels_(channels) {
   check_ = g_ordinal_check != OrdinalCheck::Never && !seen_valid(ord, channels);
@@ -169,6 +180,7 @@ void OrdinalGuard::finish() {
   const int32_t flags = both.data_ptr<int32_t>()[0], earlier = both.data_ptr<int32_t>()[1];
   if (earlier != 0) sticky_.zero_();
   if (((uint32_t)flags | (uint32_t)earlier) & HT_FLAG_PIPELINE_TIMEOUT) raise_pipeline_timeout();
+  if ((uint32_t)earlier & HT_FLAG_TARGET_RANGE) raise_target_range();
   if (flags & (int32_t)HT_FLAG_ORDINAL_RANGE)
     bad_runtime("Error: An ordinal value is either negative or larger than or equal to the number of channels.");
   remember_valid(ord_, channels_);
@@ -181,6 +193,7 @@ int64_t pipeline_status() {
   const int32_t flags = word.item<int32_t>();
   if (flags != 0) word.zero_();
   if ((uint32_t)flags & HT_FLAG_PIPELINE_TIMEOUT) raise_pipeline_timeout();
+  if ((uint32_t)flags & HT_FLAG_TARGET_RANGE) raise_target_range();
   return flags;
 }
 
@@ -902,11 +915,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pipeline_status", &pipeline_status,
         "Reads and clears the current device's long-lived kernel status word (calls on ordinals already known to be "
         "valid do not synchronise; a kernel that gave up on a bounded wait leaves its flag there). Raises RuntimeError "
-        "when a timeout was flagged; returns the other flag bits.");
+        "when a timeout was flagged, or a class loss's target that is no class; returns the other flag bits.");
   m.def("set_ordinal_check", &set_ordinal_check,
         "When to read the ordinal range flag back from the device: 'cached' (default: once per ordinals tensor "
         "version), 'always' (every call, like the reference) or 'never'.");
   m.def("abi_version", []() { return ht_version(); });
   htx::bind_more_ops(m);
   htx::bind_autograd(m);
+  htx::bind_dense(m);
 }

@@ -31,6 +31,8 @@ bool may_keep(int64_t bytes);                  // from a forward to its backward
 bool may_keep(const torch::Tensor &scratch);
 void set_ordinal_check(const std::string &mode);
 int64_t pipeline_status();
+// The device's long-lived status word (null while a stream capture runs that would have to create it).
+uint32_t *long_lived_word(const torch::Tensor &like);
 
 // Owns the device status word of one call and turns a flagged ordinal into the reference's
 // RuntimeError.  When this ordinals tensor is already known to be valid nothing is read back and word() is the
@@ -95,6 +97,9 @@ std::vector<torch::Tensor> forest_normalised_backward(int kind, torch::Tensor z,
 
 // Registers the autograd nodes (hingetree_cpp_autograd.cpp).
 void bind_autograd(pybind11::module_ &m);
+
+// Registers the dense layers around a forest (hingetree_cpp_dense.cpp).
+void bind_dense(pybind11::module_ &m);
 
 // Registers the convolution, fused-linear, fusion, sparse, trie and contract/expand operators.
 void bind_more_ops(pybind11::module_ &m);

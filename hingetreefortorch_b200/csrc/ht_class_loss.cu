@@ -1,0 +1,460 @@
+// Softmax cross entropy of a linear layer's class scores, with its gradient, without the scores in memory:
+//
+//     s[n, v] = sum_k x[n, k] w[v, k] + bias[v]        loss[n] = log sum_v exp s[n, v] - s[n, target[n]]
+//     g[n, v] = r_n (exp(s[n, v]) / sum_v exp s[n, v] - [v = target[n]])     dx = g w     dw = g^T x     dbias = sum_n g
+//
+// r_n is the upstream gradient of row n (of a mean: divided by the rows that count); rows whose target is the ignored one
+// have loss 0 and no gradient, whatever they hold.
+//
+// Forward: one tile product whose epilogue keeps, per row and half a tile's columns, the largest score m and
+// l = sum exp(s - m) in fp32, and the target's score; a second kernel joins the pieces in a fixed order.  The row's (m, l) are
+// what the backward needs besides the inputs.
+// Backward: a piece of the classes at a time (so that g of a piece, in the operands' type, stays within a bound), the scores are
+// formed again, turned into g in the epilogue, and g enters the two products of ht_dense_products.cu.  That is 8 N V K
+// operations for a training step where 6 N V K are needed; keeping the scores would cost 4 N V bytes and their traffic.
+// g is rounded to the operands' 16 bits: 2^-9 (bf16) of a term that enters sums, below what rounding the sums themselves
+// costs; for fp16 it is scaled by 2^14 first, so that probabilities down to 4e-9 are normal numbers; for fp32 it is split
+// into planes like x and w.
+#include "ht_dense.cuh"
+
+namespace ht {
+namespace dense {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Joins two pieces of a softmax: largest score m and l = sum exp(s - m); an empty piece has m = -inf, l = 0.
+__device__ __forceinline__ void join(float &m, float &l, float m2, float l2) {
+  const float top = fmaxf(m, m2), at = top == -INFINITY ? 0.0f : top;
+  l = l * exp2_fast((m - at) * kLog2e) + l2 * exp2_fast((m2 - at) * kLog2e);
+  m = top;
+}
+
+// What a row's gradient is made of: exp((s - m)) scale - [v = target] factor.
+struct RowGrad {
+  float m, scale, factor;
+  int target;
+};
+
+template <typename T>
+struct LossEpilogue {
+  static constexpr bool kPair = false;
+  struct State {
+    float m, l;
+    int target;
+  };
+  int rows, cols;
+  const T *bias;
+  const int64_t *target;
+  float2 *partial;      // [2 n_blocks][rows]
+  float *target_score;  // [rows]
+  __device__ __forceinline__ void begin(State &s, const Where &w) const {
+    s.m = -INFINITY, s.l = 0.0f, s.target = -1;
+    if (w.inside) {
+      const int64_t t = __ldg(target + w.row);
+      if (t >= 0 && t < cols) s.target = (int)t;
+    }
+  }
+  __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
+    const int n = cols - col;
+    if (n <= 0) return;
+    if (bias != nullptr) {
+      float b[32];
+      load_columns(bias + col, b, n, true);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += b[i];
+    }
+    if (n < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i >= n) v[i] = -INFINITY;
+    }
+    const int at = s.target - col;
+    if (at >= 0 && at < 32) {
+      float score = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i == at) score = v[i];
+      target_score[w.row] = score;
+    }
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
+    top = fmaxf(top, s.m);
+    const float m = top == -INFINITY ? 0.0f : top;  // (every score so far is -inf: their exponentials are 0)
+    float sum = 0.0f, sum2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      sum += exp2_fast((v[i] - m) * kLog2e);
+      sum2 += exp2_fast((v[i + 1] - m) * kLog2e);
+    }
+    s.l = s.l * exp2_fast((s.m - m) * kLog2e) + (sum + sum2);
+    s.m = top;
+  }
+  __device__ __forceinline__ void end(State &s, const Where &w) const {
+    if (w.inside) partial[(size_t)(w.n_block * 2 + w.half) * (size_t)rows + w.row] = make_float2(s.m, s.l);
+  }
+};
+
+// g of one piece of the classes as an operand, and its sums over 32 rows for the bias's gradient.
+template <typename T>
+struct LossGradEpilogue {
+  static constexpr bool kPair = false;
+  struct State {
+    RowGrad r;
+  };
+  int rows, cols, first;  // the piece: classes first .. first + cols - 1
+  const T *bias;
+  const RowGrad *row_grad;
+  typename Kind<T>::Operand *g;  // [planes][rows][pitch]
+  int pitch;
+  size_t plane;
+  float *row_sums;  // [4 m_blocks][pitch] or null
+  __device__ __forceinline__ void begin(State &s, const Where &w) const {
+    s.r = {0.0f, 0.0f, 0.0f, -1};
+    if (w.inside) {
+      const float4 q = __ldg(reinterpret_cast<const float4 *>(row_grad + w.row));
+      s.r = {q.x, q.y, q.z, __float_as_int(q.w)};
+    }
+  }
+  __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
+    const int n = cols - col;
+    if (n <= 0) return;
+    if (bias != nullptr) {
+      float b[32];
+      load_columns(bias + first + col, b, n, true);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += b[i];
+    }
+    const int at = s.r.target - first - col;
+    const bool none = s.r.factor == 0.0f;  // a row that does not count, or is not there
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float p = exp2_fast((v[i] - s.r.m) * kLog2e) * s.r.scale;
+      v[i] = none || i >= n ? 0.0f : i == at ? p - s.r.factor : p;
+    }
+    if (w.inside) store_operand<T>(g + (size_t)w.row * (size_t)pitch + col, plane, v);
+    if (row_sums != nullptr) row_sums[(size_t)(w.m_block * 4 + w.quarter) * (size_t)pitch + col + w.lane] = sum_rows(v, w.lane);
+  }
+  __device__ __forceinline__ void end(State &, const Where &) const {}
+};
+
+// Joins the pieces of every row: 32 rows a block, 8 strands of pieces a row, joined in order.  stats[row] = (m, l); the row's
+// loss to `loss`.  A row whose target is no class: loss NaN and a flag.
+__global__ void __launch_bounds__(256) join_rows_kernel(const float2 *__restrict__ partial, int slots, const float *__restrict__ target_score,
+                                                        const int64_t *__restrict__ target, int64_t ignore, int64_t rows, int64_t classes,
+                                                        float2 *__restrict__ stats, float *__restrict__ loss, uint32_t *status_word) {
+  __shared__ float2 strand[8][33];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  float m = -INFINITY, l = 0.0f;
+  if (row < rows)
+    for (int s = y; s < slots; s += 8) {
+      const float2 q = __ldg(partial + (size_t)s * (size_t)rows + row);
+      join(m, l, q.x, q.y);
+    }
+  strand[y][lane] = make_float2(m, l);
+  __syncthreads();
+  if (y != 0 || row >= rows) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) join(m, l, strand[i][lane].x, strand[i][lane].y);
+  if (stats != nullptr) stats[row] = make_float2(m, l);
+  const int64_t t = target[row];
+  float result = 0.0f;
+  if (t != ignore) {
+    if (t >= 0 && t < classes) {
+      result = (float)((double)logf(l) + ((double)m - (double)target_score[row]));
+    } else {
+      result = NAN;
+      if (status_word != nullptr) atomicOr(status_word, HT_FLAG_TARGET_RANGE);
+    }
+  }
+  loss[row] = result;
+}
+
+// Sum or mean of the rows' losses in fp64, strand by strand in a fixed order; summary = the number of rows that count.
+__global__ void __launch_bounds__(1024) reduce_loss_kernel(const float *__restrict__ row_loss, const int64_t *__restrict__ target, int64_t ignore,
+                                                           int64_t rows, int mean, float *__restrict__ loss, float *__restrict__ summary) {
+  __shared__ double sums[32];
+  __shared__ long long counts[32];
+  double sum = 0.0;
+  long long count = 0;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    if (target[r] == ignore) continue;
+    sum += (double)row_loss[r];
+    ++count;
+  }
+  for (int s = 16; s > 0; s >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    count += __shfl_xor_sync(0xffffffffu, count, s);
+  }
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum, counts[threadIdx.x >> 5] = count;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 32; ++i) sum += sums[i], count += counts[i];
+    loss[0] = (float)(mean ? sum / (double)count : sum);
+    if (summary != nullptr) summary[0] = (float)count;
+  }
+}
+
+// The power of two at or below the largest |g|, over `unit`: what gradients of single rows are scaled by.
+__global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict__ grad, int64_t rows, float unit, float *__restrict__ alpha) {
+  __shared__ uint32_t tops[32];
+  uint32_t top = 0;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) top = max(top, __float_as_uint(fabsf(grad[r])));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 32; ++i) top = max(top, tops[i]);
+    const uint32_t e = top & 0x7f800000u;
+    // (the quotient stays a normal number; an infinity or no number is left to the rows)
+    alpha[0] = (e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e)) / unit;
+  }
+}
+
+// One upstream gradient for all rows (sum, mean) or one each, as what the rows' epilogue multiplies by; alpha: what their sums are
+// multiplied by.  The factors are at most `unit`.
+__global__ void __launch_bounds__(256) row_grad_kernel(const float2 *__restrict__ stats, const float *__restrict__ summary, const int64_t *__restrict__ target,
+                                                       int64_t ignore, int64_t rows, int64_t classes, const float *__restrict__ grad, int reduction,
+                                                       float unit, RowGrad *__restrict__ row_grad, float *__restrict__ alpha) {
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row == 0 && reduction != HT_REDUCTION_NONE) {
+    const float count = summary[0];
+    alpha[0] = reduction == HT_REDUCTION_SUM ? grad[0] / unit : count > 0.0f ? grad[0] / count / unit : 0.0f;
+  }
+  if (row >= rows) return;
+  const float2 q = stats[row];
+  const int64_t t = target[row];
+  const bool counts = t != ignore, valid = t >= 0 && t < classes;
+  float factor = 0.0f;
+  if (counts) factor = !valid ? NAN : reduction == HT_REDUCTION_NONE ? grad[row] / alpha[0] : unit;
+  float4 r;
+  r.x = q.x;
+  r.y = factor / q.y;
+  r.z = factor;
+  r.w = __int_as_float(valid && counts ? (int)t : -1);
+  reinterpret_cast<float4 *>(row_grad)[row] = r;
+}
+
+constexpr int kPlanSMs = 148;  // what tiles and workspaces are planned for
+constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // g of one piece, unless the caller sets less
+
+int screen(const ht_dense_problem *p) {
+  if (p == nullptr || p->rows < 0 || p->features < 1 || p->outputs < 1 || p->x_stride < p->features) return HT_ERR_INVALID_ARGUMENT;
+  if (p->dtype != HT_DTYPE_F32 && p->dtype != HT_DTYPE_BF16 && p->dtype != HT_DTYPE_F16) return HT_ERR_INVALID_ARGUMENT;
+  if (p->rows > 0x7fffff00 || p->features > 0x3fffff00 || p->outputs > 0x3fffff00) return HT_ERR_UNSUPPORTED;
+  return HT_OK;
+}
+
+template <typename T>
+struct ForwardPlan {
+  Operand<T> x, w;
+  int bn, slots;
+  float2 *partial;
+  float *target_score, *row_loss;
+  size_t bytes;
+  ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, void *ws) {
+    Arena arena(ws);
+    x.set(arena, xp, p.rows, p.features, p.x_stride);
+    w.set(arena, wp, p.outputs, p.features, p.features);
+    bn = tile_columns(p.rows, p.outputs, p.features, Kind<T>::kPlanes, false, kPlanSMs);
+    slots = (int)(2 * ((p.outputs + bn - 1) / bn));
+    partial = arena.take<float2>((int64_t)slots * p.rows);
+    target_score = arena.take<float>(p.rows);
+    row_loss = arena.take<float>(p.rows);
+    bytes = arena.used;
+  }
+};
+
+template <typename T>
+int forward(const ht_dense_problem &p, const void *x, const void *w, const void *bias, const int64_t *target, int64_t ignore, int reduction,
+            float *loss, float *stats, void *ws, size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
+  ForwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), ws);
+  if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
+  int sms = 0, rc;
+  float *row_loss = reduction == HT_REDUCTION_NONE ? loss : plan.row_loss;
+  if (p.rows > 0) {
+    if ((rc = sm_count(&sms)) != HT_OK) return rc;
+    if ((rc = plan.x.lay_out(stream)) != HT_OK) return rc;
+    if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
+    TileProblem t;
+    t.a[0] = plan.x.m;
+    t.b[0] = plan.w.m;
+    t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
+    t.f16 = p.dtype == HT_DTYPE_F16;
+    t.status_word = status_word;
+    LossEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), target, plan.partial, plan.target_score};
+    if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, plan.bn, sms, stream)) != HT_OK) return rc;
+    join_rows_kernel<<<(unsigned)((p.rows + 31) / 32), 256, 0, stream>>>(plan.partial, plan.slots, plan.target_score, target, ignore, p.rows,
+                                                                       p.outputs, reinterpret_cast<float2 *>(stats), row_loss, status_word);
+    HT_CHECK_LAUNCH();
+  }
+  if (reduction != HT_REDUCTION_NONE) {
+    reduce_loss_kernel<<<1, 1024, 0, stream>>>(row_loss, target, ignore, p.rows, reduction == HT_REDUCTION_MEAN, loss,
+                                               stats == nullptr ? nullptr : stats + 2 * p.rows);
+    HT_CHECK_LAUNCH();
+  }
+  return HT_OK;
+}
+
+template <typename T>
+struct BackwardPlan {
+  Operand<T> x, w;
+  int64_t piece, pitch;  // classes of a piece, elements of a row of g
+  typename Kind<T>::Operand *g;
+  RowGrad *row_grad;
+  float *alpha, *sum, *row_sums;
+  size_t bytes;
+  BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, void *ws) {
+    Arena arena(ws);
+    static const int64_t some = 0;
+    x.set(arena, xp, p.rows, p.features, p.x_stride, target != nullptr ? target : &some, ignore);
+    w.set(arena, wp, p.outputs, p.features, p.features);
+    const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
+    const int64_t per_class = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 2;
+    // pieces of whole tiles; at least one tile, and all classes where they fit
+    piece = std::max<int64_t>(limit / per_class / 256 * 256, 256);
+    if (piece >= p.outputs) piece = p.outputs;
+    pitch = round_up(piece, 64);
+    g = arena.take<typename Kind<T>::Operand>(p.rows * pitch * Kind<T>::kPlanes);
+    row_grad = arena.take<RowGrad>(p.rows);
+    alpha = arena.take<float>(1);
+    sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
+    row_sums = has_db ? arena.take<float>((p.rows + kTileM - 1) / kTileM * 4 * pitch) : nullptr;
+    bytes = arena.used;
+  }
+};
+
+template <typename T>
+int backward(const ht_dense_problem &p, const void *x, const void *w, const void *bias, const int64_t *target, int64_t ignore, int reduction,
+             const float *grad, const float *stats, void *dx_, void *dw_, void *db_, void *ws, size_t ws_bytes, uint32_t *status_word,
+             cudaStream_t stream) {
+  T *dx = static_cast<T *>(dx_), *dw = static_cast<T *>(dw_), *db = static_cast<T *>(db_);
+  BackwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), target, ignore, dx != nullptr, db != nullptr, ws);
+  if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
+  if (p.rows == 0) {
+    if (dw != nullptr) HT_CUDA_TRY(cudaMemsetAsync(dw, 0, sizeof(T) * (size_t)(p.outputs * p.features), stream));
+    if (db != nullptr) HT_CUDA_TRY(cudaMemsetAsync(db, 0, sizeof(T) * (size_t)p.outputs, stream));
+    return HT_OK;
+  }
+  int sms = 0, rc;
+  if ((rc = sm_count(&sms)) != HT_OK) return rc;
+  if ((rc = plan.x.lay_out(stream)) != HT_OK) return rc;
+  if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
+  const float unit = p.dtype == HT_DTYPE_F16 ? 16384.0f : 1.0f;
+  if (reduction == HT_REDUCTION_NONE) {
+    row_scale_kernel<<<1, 1024, 0, stream>>>(grad, p.rows, unit, plan.alpha);
+    HT_CHECK_LAUNCH();
+  }
+  row_grad_kernel<<<(unsigned)((p.rows + 255) / 256), 256, 0, stream>>>(reinterpret_cast<const float2 *>(stats), stats + 2 * p.rows, target, ignore,
+                                                                       p.rows, p.outputs, grad, reduction, unit, plan.row_grad, plan.alpha);
+  HT_CHECK_LAUNCH();
+  constexpr int kPlanes = Kind<T>::kPlanes;
+  const bool whole = p.features * (int64_t)sizeof(T) % 16 == 0;
+  for (int64_t first = 0; first < p.outputs; first += plan.piece) {
+    const int64_t count = std::min(plan.piece, p.outputs - first);
+    TileProblem t;
+    t.f16 = p.dtype == HT_DTYPE_F16;
+    t.status_word = status_word;
+    t.a[0] = plan.x.m;
+    t.b[0] = plan.w.m;
+    t.rows = p.rows, t.cols = count, t.k = p.features, t.b_n0 = first;
+    LossGradEpilogue<T> e = {};
+    e.rows = (int)p.rows, e.cols = (int)count, e.first = (int)first;
+    e.bias = static_cast<const T *>(bias);
+    e.row_grad = plan.row_grad;
+    e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = (size_t)(p.rows * plan.pitch);
+    e.row_sums = plan.row_sums;
+    if ((rc = launch_tiles<kPlanes, false, false>(t, e, tile_columns(p.rows, count, p.features, kPlanes, false, kPlanSMs), sms, stream)) != HT_OK) return rc;
+    Matrix g;
+    g.data = plan.g, g.rows = p.rows, g.cols = count, g.pitch = plan.pitch, g.planes = kPlanes, g.plane = p.rows * plan.pitch;
+    StoreEpilogue<T> store = {};
+    store.alpha = plan.alpha;
+    store.cols = (int)p.features;
+    store.whole = whole;
+    store.split = 0x7fffffff;
+    if (dx != nullptr) {
+      TileProblem q = t;
+      q.a[0] = g;
+      q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = first;
+      store.rows = store.part = (int)p.rows;
+      store.out = dx;
+      store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
+      if ((rc = product_dx<T>(q, store, sms, stream)) != HT_OK) return rc;
+    }
+    if (dw != nullptr) {
+      TileProblem q = t;
+      q.a[0] = g;
+      q.b[0] = plan.x.m;
+      q.rows = count, q.cols = p.features, q.k = p.rows, q.b_n0 = 0;
+      store.rows = store.part = (int)count;
+      store.out = dw + (size_t)first * (size_t)p.features;
+      store.sum = nullptr, store.keep = false;
+      if ((rc = product_dw<T>(q, store, sms, stream)) != HT_OK) return rc;
+    }
+    if (db != nullptr && (rc = column_sums<T>(plan.row_sums, (p.rows + kTileM - 1) / kTileM * 4, plan.pitch, count, plan.alpha, db + first, stream)) != HT_OK)
+      return rc;
+  }
+  return HT_OK;
+}
+
+template <typename F>
+auto by_type(int dtype, F &&f) {
+  return dtype == HT_DTYPE_F32 ? f(float()) : dtype == HT_DTYPE_BF16 ? f(__nv_bfloat16()) : f(__half());
+}
+
+}  // namespace
+}  // namespace dense
+}  // namespace ht
+
+using namespace ht;
+using namespace ht::dense;
+
+extern "C" size_t ht_linear_class_loss_workspace_bytes(const ht_dense_problem *p, int backward) {
+  if (screen(p) != HT_OK) return 0;
+  return by_type(p->dtype, [&](auto zero) -> size_t {
+    typedef decltype(zero) T;
+    return backward != 0 ? BackwardPlan<T>(*p, nullptr, nullptr, nullptr, 0, true, true, nullptr).bytes
+                         : ForwardPlan<T>(*p, nullptr, nullptr, nullptr).bytes;
+  });
+}
+
+extern "C" int ht_linear_class_loss_forward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
+                                            int64_t ignore_index, int reduction, float *loss, float *stats, void *workspace,
+                                            size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream) {
+  int rc = screen(p);
+  if (rc != HT_OK) return rc;
+  if (reduction != HT_REDUCTION_NONE && reduction != HT_REDUCTION_MEAN && reduction != HT_REDUCTION_SUM) return HT_ERR_INVALID_ARGUMENT;
+  if (p->rows == 0 && reduction == HT_REDUCTION_NONE) return HT_OK;
+  if (loss == nullptr || (p->rows > 0 && (x == nullptr || w == nullptr || target == nullptr))) return HT_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(stats) |
+        reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+    return HT_ERR_UNSUPPORTED;
+  return by_type(p->dtype, [&](auto zero) -> int {
+    return forward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, loss, stats, workspace, workspace_bytes, status_word,
+                                   reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int ht_linear_class_loss_backward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
+                                             int64_t ignore_index, int reduction, const float *grad, const float *stats, void *dx, void *dw,
+                                             void *dbias, void *workspace, size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream) {
+  int rc = screen(p);
+  if (rc != HT_OK) return rc;
+  if (reduction != HT_REDUCTION_NONE && reduction != HT_REDUCTION_MEAN && reduction != HT_REDUCTION_SUM) return HT_ERR_INVALID_ARGUMENT;
+  if (p->rows > 0 && (x == nullptr || w == nullptr || target == nullptr || grad == nullptr || stats == nullptr)) return HT_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(stats) |
+        reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+    return HT_ERR_UNSUPPORTED;
+  return by_type(p->dtype, [&](auto zero) -> int {
+    return backward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, grad, stats, dx, dw, dbias, workspace, workspace_bytes,
+                                    status_word, reinterpret_cast<cudaStream_t>(stream));
+  });
+}

@@ -1,0 +1,335 @@
+// What the dense layers around a forest share (ht_gated_linear.cu, ht_class_loss.cu): element types, the layout of operands for the tile
+// product, stores of a thread's 32 columns, column sums, the kernel for few rows, and the two products of a backward pass.
+#pragma once
+
+#include "ht_dense_tile.cuh"
+
+namespace ht {
+namespace dense {
+
+// Element types of a call: fp32 is held as three bf16 planes for the tensor cores.
+template <typename T>
+struct Kind;
+template <>
+struct Kind<float> {
+  static constexpr int kPlanes = 3;
+  typedef __nv_bfloat16 Operand;
+};
+template <>
+struct Kind<__nv_bfloat16> {
+  static constexpr int kPlanes = 1;
+  typedef __nv_bfloat16 Operand;
+};
+template <>
+struct Kind<__half> {
+  static constexpr int kPlanes = 1;
+  typedef __half Operand;
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, const __nv_bfloat16 *) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, const __half *) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// v = p0 + p1 + p2, each the rounding to bf16 of what the ones before leave: 24 bits.  A value that rounds to infinity without being
+// it is truncated instead; an infinity or no number stays in the first plane alone.
+__device__ __forceinline__ void split_planes(float v, float &p0, float &p1, float &p2) {
+  p0 = __bfloat162float(__float2bfloat16_rn(v));
+  if (!(fabsf(p0) < INFINITY)) {
+    p0 = fabsf(v) < INFINITY ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : v;
+    if (!(fabsf(v) < INFINITY)) {
+      p1 = p2 = 0.0f;
+      return;
+    }
+  }
+  const float r = v - p0;
+  p1 = __bfloat162float(__float2bfloat16_rn(r));
+  p2 = r - p1;
+}
+
+// 32 columns of one row (n of them inside the matrix).  `whole`: the row's address is a multiple of 16 bytes.
+template <typename T>
+__device__ __forceinline__ void store_columns(T *out, const float (&v)[32], int n, bool whole) {
+  if (whole && n >= 32) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(out + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)
+        *reinterpret_cast<uint4 *>(out + i) = make_uint4(pack_pair(v[i], v[i + 1], out), pack_pair(v[i + 2], v[i + 3], out),
+                                                         pack_pair(v[i + 4], v[i + 5], out), pack_pair(v[i + 6], v[i + 7], out));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) out[i] = from_float<T>(v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load_columns(const T *in, float (&v)[32], int n, bool whole) {
+  if (whole && n >= 32) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4 *>(in + i));
+        v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(in + i));
+        const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          T pair[2];
+          *reinterpret_cast<uint32_t *>(pair) = words[j];
+          v[i + 2 * j] = to_float(pair[0]);
+          v[i + 2 * j + 1] = to_float(pair[1]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = i < n ? to_float(in[i]) : 0.0f;
+  }
+}
+
+// The same as operands of a later product: [planes][rows][pitch], rows of a multiple of 64 elements.
+template <typename T>
+__device__ __forceinline__ void store_operand(typename Kind<T>::Operand *out, size_t plane, const float (&v)[32]) {
+  if constexpr (Kind<T>::kPlanes == 1) {
+    store_columns(out, v, 32, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      float p[3][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split_planes(v[i + j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<uint4 *>(out + (size_t)q * plane + i) =
+            make_uint4(pack_pair(p[q][0], p[q][1], out), pack_pair(p[q][2], p[q][3], out), pack_pair(p[q][4], p[q][5], out),
+                       pack_pair(p[q][6], p[q][7], out));
+    }
+  }
+}
+
+// The sum over the warp's 32 rows of column `lane`: every step halves the columns that a lane holds.
+__device__ __forceinline__ float sum_rows(const float (&v)[32], int lane) {
+  float h[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const bool up = (lane & 16) != 0;
+    h[i] = (up ? v[i + 16] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + 16], 16);
+  }
+#pragma unroll
+  for (int s = 8; s >= 1; s >>= 1) {
+    const bool up = (lane & s) != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < s) h[i] = (up ? h[i + s] : h[i]) + __shfl_xor_sync(0xffffffffu, up ? h[i] : h[i + s], s);
+  }
+  return h[0];
+}
+
+// ---- epilogue: the products themselves, scaled -----------------------------------------------------------------------
+// out = alpha (acc + products): `sum` holds what earlier pieces of k have given, in fp32; `keep`: the sum goes on (then all rows go to one matrix).
+template <typename T>
+struct StoreEpilogue {
+  static constexpr bool kPair = false;
+  struct State {
+    float alpha;
+  };
+  int rows, cols;
+  T *out, *out2;       // [part, cols] each: of the products' rows, those from `split` on go to out2
+  int split, part;
+  const float *alpha;  // on the device; null: 1
+  float *sum;          // [rows, cols] or null
+  bool begins, keep;   // the first piece of a sum, not the last one
+  bool whole;          // rows of out start on 16 bytes
+  __device__ __forceinline__ void begin(State &s, const Where &) const { s.alpha = alpha != nullptr ? __ldg(alpha) : 1.0f; }
+  __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
+    const int n = cols - col, row = w.row < split ? w.row : w.row - split;
+    if (!w.inside || n <= 0 || row >= part) return;
+    if (sum != nullptr) {
+      float *acc = sum + (size_t)w.row * (size_t)cols + col;
+      const bool quads = (cols & 3) == 0;
+      if (!begins) {
+        float before[32];
+        if (quads && n >= 32) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 q = *reinterpret_cast<const float4 *>(acc + i);
+            before[i] = q.x, before[i + 1] = q.y, before[i + 2] = q.z, before[i + 3] = q.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) before[i] = i < n ? acc[i] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] += before[i];
+      }
+      if (keep) {
+        store_columns(acc, v, n, quads);
+        return;
+      }
+    }
+    T *to = (w.row < split ? out : out2) + (size_t)row * (size_t)cols;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= s.alpha;
+    store_columns(to + col, v, n, whole);
+  }
+  __device__ __forceinline__ void end(State &, const Where &) const {}
+};
+
+// ---- operands ---------------------------------------------------------------------------------------------------------
+
+constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Memory handed out of a workspace in pieces of 256 bytes; with no base it only counts.
+struct Arena {
+  char *base;
+  size_t used = 0;
+  explicit Arena(void *at) : base(static_cast<char *>(at)) {}
+  template <typename P>
+  P *take(int64_t count) {
+    P *p = base == nullptr ? nullptr : reinterpret_cast<P *>(base + used);
+    used += align_up((size_t)std::max<int64_t>(count, 0) * sizeof(P), 256);
+    return p;
+  }
+};
+
+// A matrix as the tile product reads it: itself, or laid out anew (`copy`).  fp32 is split into planes, 16-bit rows that do not start on 16
+// bytes are padded, and rows whose target is `ignore` come as zeros where `target` is given.
+template <typename T>
+struct Operand {
+  Matrix m;
+  typename Kind<T>::Operand *copy = nullptr;
+  const T *source = nullptr;
+  int64_t stride = 0;
+  const int64_t *target = nullptr;
+  int64_t ignore = 0;
+  static bool direct(int64_t stride) { return Kind<T>::kPlanes == 1 && stride % 8 == 0; }
+  void set(Arena &arena, const T *data, int64_t rows, int64_t cols, int64_t row_stride, const int64_t *skip = nullptr, int64_t skipped = 0) {
+    source = data, stride = row_stride, target = skip, ignore = skipped;
+    m.rows = rows, m.cols = cols, m.planes = Kind<T>::kPlanes;
+    if (direct(row_stride) && skip == nullptr) {
+      m.data = data, m.pitch = row_stride;
+      return;
+    }
+    m.pitch = round_up(cols, 8);
+    m.plane = rows * m.pitch;
+    copy = arena.template take<typename Kind<T>::Operand>(m.plane * m.planes);
+    m.data = copy;
+  }
+  int lay_out(cudaStream_t stream) const;
+};
+
+// 8 columns a thread.  x is read once, the copy written once: 10 bytes a value from fp32, 4 from 16 bits.
+template <typename T>
+__global__ void __launch_bounds__(256) lay_out_kernel(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t stride, int64_t pitch,
+                                                      int64_t plane, typename Kind<T>::Operand *__restrict__ copy,
+                                                      const int64_t *__restrict__ target, int64_t ignore, bool whole) {
+  const int64_t per_row = pitch / 8, n = rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    float v[8];
+    const T *from = x + r * stride + c;
+    if (target != nullptr && __ldg(target + r) == ignore) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    } else if (whole && c + 8 <= cols) {
+      T t[8];
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(from));
+        *reinterpret_cast<uint4 *>(t + 4) = __ldg(reinterpret_cast<const uint4 *>(from + 4));
+      } else {
+        *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(from));
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_float(from[j]) : 0.0f;
+    }
+    typename Kind<T>::Operand *to = copy + r * pitch + c;
+    if constexpr (Kind<T>::kPlanes == 1) {
+      *reinterpret_cast<uint4 *>(to) = make_uint4(pack_pair(v[0], v[1], to), pack_pair(v[2], v[3], to), pack_pair(v[4], v[5], to), pack_pair(v[6], v[7], to));
+    } else {
+      float p[3][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split_planes(v[j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<uint4 *>(to + q * plane) =
+            make_uint4(pack_pair(p[q][0], p[q][1], to), pack_pair(p[q][2], p[q][3], to), pack_pair(p[q][4], p[q][5], to), pack_pair(p[q][6], p[q][7], to));
+    }
+  }
+}
+
+inline unsigned blocks_for(int64_t work, int64_t per_block, int64_t most) {
+  return (unsigned)std::min<int64_t>(std::max<int64_t>((work + per_block - 1) / per_block, 1), most);
+}
+
+template <typename T>
+int Operand<T>::lay_out(cudaStream_t stream) const {
+  if (copy == nullptr || m.rows == 0) return HT_OK;
+  const bool whole = (reinterpret_cast<uintptr_t>(source) & 15u) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
+  const int64_t work = m.rows * (m.pitch / 8);
+  lay_out_kernel<T><<<blocks_for(work, 256, 148 * 16), 256, 0, stream>>>(source, m.rows, m.cols, stride, m.pitch, m.plane, copy, target, ignore, whole);
+  HT_CHECK_LAUNCH();
+  return HT_OK;
+}
+
+// Column sums from the sums of 32 rows each that the epilogues leave: out[c] = alpha sum_r partial[r, c], r ascending in 8
+// strands that are added in order.  32 columns a block.
+template <typename T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols,
+                                                          const float *__restrict__ alpha, T *__restrict__ out) {
+  __shared__ float strand[8][33];
+  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float sum = 0.0f;
+  if (c < cols)
+    for (int64_t r = y; r < rows; r += 8) sum += __ldg(partial + r * pitch + c);
+  strand[y][lane] = sum;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += strand[i][lane];
+    out[c] = from_float<T>((alpha != nullptr ? __ldg(alpha) : 1.0f) * sum);
+  }
+}
+
+template <typename T>
+int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols, const float *alpha, T *out, cudaStream_t stream) {
+  column_sums_kernel<T><<<(unsigned)((cols + 31) / 32), 256, 0, stream>>>(partial, rows, pitch, cols, alpha, out);
+  HT_CHECK_LAUNCH();
+  return HT_OK;
+}
+
+// dx (+)= g w over a piece of outputs, dw = g^T x (ht_dense_products.cu).
+template <typename T>
+int product_dx(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream);
+template <typename T>
+int product_dw(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream);
+
+}  // namespace dense
+}  // namespace ht

@@ -1,0 +1,483 @@
+// Tile product of the dense layers around a forest (ht_gated_linear.cu, ht_class_loss.cu) on the tensor cores:
+//
+//     out[m, n] = sum_k A(m, k) B(n, k)        16-bit operands (bf16 or fp16), fp32 accumulation in tensor memory
+//
+// handed to an epilogue 32 columns at a time, so that what a layer does with its products (softmax sums, the loss's gradient,
+// activation and gate, a scaled store) happens before they leave the registers.  Either operand is stored with k
+// contiguous ([rows][k]) or with m / n contiguous ([k][rows], "MN"), which is what the three products of a layer need of
+// one stored matrix: y = x w^T, dx = dy w, dw = dy^T x, without a transposed copy.
+//
+// fp32 operands come as three bf16 planes (x = x0 + x1 + x2, each the rounding of what is left: 24 bits): the products x0 y0 in one
+// accumulator, and x0 y1, x1 y0, x1 y1, x0 y2, x2 y0 in a second; what is left out is below 2^-24 of a term.  The tensor core truncates
+// when it adds to an accumulator, always towards zero (measured: 32 instructions in a row lose about 9e-7 of the sum, which is more than an fp32
+// sum loses to rounding).  So the large products leave for registers every 8 instructions (128 values of k) and are added there in
+// fp32; the small ones are 2^-8 of those and stay to the end.
+//
+// A persistent kernel, one CTA per SM, 320 threads:
+//   warp 0      one lane issues the TMA loads (cp.async.bulk.tensor, 128-byte swizzle) into a ring of stages of 64 values of k;
+//   warp 1      allocates tensor memory, and one lane issues tcgen05.mma.kind::f16 (M 128, N up to 256, K 16) and commits
+//               each stage back to the loads and each finished accumulator to the epilogue;
+//   warps 2-9   the epilogue, under the main loop of the next tile (two accumulators): two warps per quarter of the 128 lanes, each
+//               with one half of the columns.
+// Tiles are walked in groups of 16 row blocks, rows fastest, so that what the SMs read at one time is shared in L2.
+// Every wait is bounded: when one runs out the kernel flags HT_FLAG_PIPELINE_TIMEOUT, every role stops at its own next wait, the
+// loads wait for their copies in flight, the tensor memory is freed and the kernel returns.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "ht_common.cuh"
+#include "ht_tile_common.cuh"
+#include "ht_tma.cuh"
+
+namespace ht {
+namespace dense {
+
+using namespace tile;
+
+constexpr int kTileM = 128, kTileK = 64;
+constexpr int kTileThreads = 320;
+constexpr int kEpilogueWarps = 8;
+constexpr int kChunkBlocks = 2;  // blocks of 64 values of k between two visits of the registers (three planes)
+constexpr int kMostStages = 12;
+constexpr uint32_t kStageBudget = 220 * 1024;
+constexpr size_t kTileSmem = 1024 + kStageBudget + 512;
+
+// A 16-bit matrix in device memory, row-major, `pitch` elements from row to row (a multiple of 8, base on 16 bytes); with
+// three planes, `plane` elements apart.
+struct Matrix {
+  const void *data = nullptr;
+  int64_t rows = 0, cols = 0, pitch = 0;
+  int planes = 1;
+  int64_t plane = 0;
+};
+
+struct alignas(64) TileArgs {
+  CUtensorMap a[2], b[2];
+  uint32_t *status_word;
+  uint32_t instruction;
+  int m_blocks, n_blocks, tiles;
+  int bn;                  // columns of a tile: both halves of a pair together
+  int k, k_blocks;         // of one segment
+  int segments;            // 2: the sum over k goes on in a[1], b[1]
+  int b_n0, b_k0;          // where B's rows / values of k begin
+  int stages;
+  uint32_t a_bytes, stage_bytes;
+};
+
+// What an epilogue thread is at: one row of the tile, and one half of its columns.
+struct Where {
+  int row;       // of the output
+  bool inside;   // row < rows of the output
+  int m_block, n_block, half, quarter, lane;
+};
+
+__device__ __forceinline__ uint64_t k_major_descriptor(uint32_t address) {
+  uint64_t desc = (uint64_t)((address >> 4) & 0x3fffu);
+  desc |= (uint64_t)1u << 16;              // leading byte offset: not used with k contiguous
+  desc |= (uint64_t)(1024u >> 4) << 32;    // stride byte offset: from 8 rows to the next 8
+  desc |= (uint64_t)1u << 46;              // descriptor version of this architecture
+  desc |= (uint64_t)2u << 61;              // 128-byte swizzle
+  return desc;
+}
+// m (n) contiguous: boxes of 64 of them by 64 values of k; `group`: bytes from one box to the next 64.
+__device__ __forceinline__ uint64_t mn_major_descriptor(uint32_t address, uint32_t group) {
+  uint64_t desc = (uint64_t)((address >> 4) & 0x3fffu);
+  desc |= (uint64_t)(group >> 4) << 16;    // leading byte offset: to the next 64 of m
+  desc |= (uint64_t)(1024u >> 4) << 32;    // stride byte offset: from 8 values of k to the next 8
+  desc |= (uint64_t)1u << 46;
+  desc |= (uint64_t)2u << 61;
+  return desc;
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instruction, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      :
+      : "r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instruction), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// 32 columns of this warp's lanes: issued and waited for in one statement, so that nothing reads a register before it arrives.
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *map, int col, int row, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(col), "r"(row), "r"(0), "r"(smem_addr(bar))
+      : "memory");
+}
+
+template <int PLANES, bool A_MN, bool B_MN, class Epilogue>
+__global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ Epilogue epilogue) {
+  constexpr bool kPair = Epilogue::kPair;  // the tile's columns are those of two matrices, half and half
+  static_assert(!kPair || !B_MN, "a pair's weights have k contiguous");
+  constexpr int kPlanes = PLANES;
+  constexpr bool kThree = PLANES == 3;
+  extern __shared__ __align__(1024) unsigned char tile_smem[];
+  unsigned char *base = tile_smem + ((1024u - (smem_addr(tile_smem) & 1023u)) & 1023u);
+  const uint32_t stages = smem_addr(base);
+  uint64_t *full = reinterpret_cast<uint64_t *>(base + kStageBudget);  // [stages]
+  uint64_t *empty = full + kMostStages;                                // [stages]
+  uint64_t *accumulated = empty + kMostStages;                         // [2] an accumulator is complete
+  uint64_t *drained = accumulated + 2;                                 // [2] ... and has been read out
+  uint64_t *drained_small = drained + 2;                               // [2] the second accumulator of three planes
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained_small + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int blocks = a.segments * a.k_blocks;
+  constexpr uint32_t kColumns = 512;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accumulated[b], 1);
+      mbar_init(&drained[b], kEpilogueWarps);
+      mbar_init(&drained_small[b], kEpilogueWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+
+  auto give_up = [&]() {
+    if (a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_PIPELINE_TIMEOUT);
+  };
+  // Tile -> (row block, column block): groups of 16 row blocks, the rows of a group fastest.
+  auto place = [&](int tile, int &mb, int &nb) {
+    constexpr int kGroup = 16;
+    const int per_group = kGroup * a.n_blocks, g = tile / per_group, in = tile - g * per_group;
+    const int rows = min(kGroup, a.m_blocks - g * kGroup);
+    nb = in / rows;
+    mb = g * kGroup + (in - nb * rows);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0, s = 0, phase = 1;
+      bool ok = true;
+      for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x) {
+        int mb, nb;
+        place(tile, mb, nb);
+        const int m0 = mb * kTileM, n0 = a.b_n0 + nb * (kPair ? a.bn / 2 : a.bn);
+        for (int kb = 0; kb < blocks; ++kb, ++it) {
+          if (!mbar_wait(&empty[s], phase)) {
+            give_up();
+            ok = false;
+            break;
+          }
+          const int segment = kb >= a.k_blocks ? 1 : 0;
+          const int k0 = (kb - segment * a.k_blocks) * kTileK;
+          const uint32_t at = stages + s * a.stage_bytes, bt = at + a.a_bytes;
+          mbar_expect_tx(&full[s], a.stage_bytes);
+          const CUtensorMap *am = &a.a[segment], *bm = &a.b[segment];
+          if (A_MN) {
+            for (int g = 0; g < kTileM / 64; ++g) load_3d(at + (uint32_t)g * (8192u * kPlanes), am, m0 + 64 * g, k0, &full[s]);
+          } else {
+            load_3d(at, am, k0, m0, &full[s]);
+          }
+          if (B_MN) {
+            for (int g = 0; g < a.bn / 64; ++g) load_3d(bt + (uint32_t)g * (8192u * kPlanes), bm, n0 + 64 * g, a.b_k0 + k0, &full[s]);
+          } else if (kPair) {  // plane by plane the gate's rows and the value's: what one instruction reads is contiguous
+            load_3d(bt, &a.b[0], k0, n0, &full[s]);
+            load_3d(bt + (uint32_t)(a.bn / 2) * 128u * kPlanes, &a.b[1], k0, n0, &full[s]);
+          } else {
+            load_3d(bt, bm, a.b_k0 + k0, n0, &full[s]);
+          }
+          if (++s == (uint32_t)a.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {  // the copies still in flight arrive before the CTA leaves
+        const uint32_t issued = min(it, (uint32_t)a.stages);
+        for (uint32_t j = 1; j <= issued; ++j) {
+          const uint32_t i = it - j;
+          mbar_wait(&full[i % (uint32_t)a.stages], (i / (uint32_t)a.stages) & 1u, 4096);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t s = 0, phase = 0, chunk = 0, t = 0;
+      bool ok = true;
+      const uint32_t a_plane = A_MN ? 8192u : (uint32_t)kTileM * 128u;
+      const uint32_t b_plane = B_MN ? 8192u : (uint32_t)(kPair ? a.bn / 2 : a.bn) * 128u;
+      const uint32_t step_a = A_MN ? 128u : 2u, step_b = B_MN ? 128u : 2u;  // 16 values of k, in units of 16 bytes
+      for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x, ++t) {
+        const uint32_t small = tmem + 256u + (t & 1u) * 128u;
+        uint32_t d = 0;
+        if (kThree && !mbar_wait(&drained_small[t & 1u], ((t >> 1) & 1u) ^ 1u)) {
+          give_up();
+          break;
+        }
+        for (int kb = 0; kb < blocks; ++kb) {
+          const bool first = kThree ? kb % kChunkBlocks == 0 : kb == 0;
+          if (first) {
+            if (!mbar_wait(&drained[chunk & 1u], ((chunk >> 1) & 1u) ^ 1u)) {
+              give_up();
+              ok = false;
+              break;
+            }
+            d = tmem + (chunk & 1u) * (kThree ? 128u : 256u);
+          }
+          if (!mbar_wait(&full[s], phase)) {
+            give_up();
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const int left = a.k - (kb >= a.k_blocks ? kb - a.k_blocks : kb) * kTileK;
+          const int steps = left >= kTileK ? 4 : (left + 15) / 16;
+          const uint32_t at = stages + s * a.stage_bytes, bt = at + a.a_bytes;
+          const uint64_t da = A_MN ? mn_major_descriptor(at, 8192u * kPlanes) : k_major_descriptor(at);
+          const uint64_t db = B_MN ? mn_major_descriptor(bt, 8192u * kPlanes) : k_major_descriptor(bt);
+          for (int kk = 0; kk < steps; ++kk) {
+            const uint64_t ak = da + (uint64_t)(step_a * (uint32_t)kk), bk = db + (uint64_t)(step_b * (uint32_t)kk);
+            const uint32_t into = !(first && kk == 0);
+            if (!kThree) {
+              mma_f16(d, ak, bk, a.instruction, into);
+            } else {
+              // a pair's planes lie gate by gate and value by value: two instructions of half the columns each
+              constexpr int kParts = kPair ? 2 : 1;
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) {
+                const uint32_t col = kPair ? (uint32_t)part * (uint32_t)(a.bn / 2) : 0u;
+                const uint64_t bp = bk + (uint64_t)((uint32_t)part * ((b_plane * 3u) >> 4));
+                const uint64_t ap = a_plane >> 4, pb = b_plane >> 4;
+                mma_f16(d + col, ak, bp, a.instruction, into);
+                mma_f16(small + col, ak + 2 * ap, bp, a.instruction, !(kb == 0 && kk == 0));
+                mma_f16(small + col, ak, bp + 2 * pb, a.instruction, 1u);
+                mma_f16(small + col, ak + ap, bp + pb, a.instruction, 1u);
+                mma_f16(small + col, ak + ap, bp, a.instruction, 1u);
+                mma_f16(small + col, ak, bp + pb, a.instruction, 1u);
+              }
+            }
+          }
+          mma_commit(&empty[s]);
+          if (++s == (uint32_t)a.stages) {
+            s = 0;
+            phase ^= 1u;
+          }
+          if (kb == blocks - 1 || (kThree && kb % kChunkBlocks == kChunkBlocks - 1)) {
+            mma_commit(&accumulated[chunk & 1u]);
+            ++chunk;
+          }
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp may only touch the lanes 32 (warp % 4) ...
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    uint32_t chunk = 0, t = 0;
+    const int units = kPair ? a.bn / 128 : a.bn / 64;  // of 32 columns (a pair: 32 of each), for this half
+    Where w;
+    w.half = half, w.quarter = quarter, w.lane = lane;
+    auto wait_for = [&](uint32_t c) {
+      bool there = mbar_wait(&accumulated[c & 1u], (c >> 1) & 1u);
+      if (!there) give_up();
+      there = __all_sync(0xffffffffu, there);  // a warp reads tensor memory together or not at all
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      return there;
+    };
+    auto release = [&](uint64_t *bar) {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    for (int tile = (int)blockIdx.x; tile < a.tiles; tile += (int)gridDim.x, ++t) {
+      place(tile, w.m_block, w.n_block);
+      w.row = w.m_block * kTileM + quarter * 32 + lane;
+      w.inside = w.row < epilogue.rows;
+      typename Epilogue::State state;
+      const int col0 = w.n_block * (kPair ? a.bn / 2 : a.bn);
+      if constexpr (!kThree) {
+        epilogue.begin(state, w);
+        if (!wait_for(chunk)) break;
+        const uint32_t acc = lanes + (chunk & 1u) * 256u;
+#pragma unroll 1
+        for (int u = 0; u < units; ++u) {
+          const int c = (half * units + u) * 32;
+          float v[32];
+          tmem_load_32(acc + (uint32_t)c, v);
+          if constexpr (kPair) {
+            float v2[32];
+            tmem_load_32(acc + (uint32_t)(a.bn / 2 + c), v2);
+            if (u == units - 1) release(&drained[chunk & 1u]);
+            epilogue.unit(state, w, col0 + c, v, v2);
+          } else {
+            if (u == units - 1) release(&drained[chunk & 1u]);
+            epilogue.unit(state, w, col0 + c, v);
+          }
+        }
+        ++chunk;
+      } else {
+        // 64 columns a thread at the most (bn <= 128), summed over the chunks of k
+        const int first = half * (units * 32), second = kPair ? a.bn / 2 + first : first + 32;
+        const bool two = kPair || units == 2;
+        float s0[32], s1[32], v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s0[i] = s1[i] = 0.0f;
+        bool there = true;
+        const int chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
+        for (int c = 0; c <= chunks; ++c) {
+          if (c < chunks && !(there = wait_for(chunk))) break;
+          const uint32_t acc = lanes + (c < chunks ? (chunk & 1u) * 128u : 256u + (t & 1u) * 128u);
+          tmem_load_32(acc + (uint32_t)first, v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s0[i] += v[i];
+          if (two) {
+            tmem_load_32(acc + (uint32_t)second, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s1[i] += v[i];
+          }
+          if (c < chunks) {
+            release(&drained[chunk & 1u]);
+            ++chunk;
+          } else {
+            release(&drained_small[t & 1u]);
+          }
+        }
+        if (!there) break;
+        epilogue.begin(state, w);
+        if constexpr (kPair) {
+          epilogue.unit(state, w, col0 + first, s0, s1);
+        } else {
+          epilogue.unit(state, w, col0 + first, s0);
+          if (two) epilogue.unit(state, w, col0 + second, s1);
+        }
+      }
+      epilogue.end(state, w);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+
+// Boxes of 64 columns (128 bytes) by `box_rows` rows of every plane.
+inline bool encode_matrix_16(CUtensorMap *map, const Matrix &m, int box_rows) {
+  tma::EncodeTiledFn fn = tma::encode_tiled_fn();
+  if (fn == nullptr) return false;
+  if ((reinterpret_cast<uintptr_t>(m.data) & 15u) != 0 || (m.pitch & 7) != 0 || (m.plane & 7) != 0) return false;
+  if (m.rows < 1 || m.cols < 1 || m.rows > 0x7fffffff || m.cols > 0x7fffffff || box_rows < 1 || box_rows > 256) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)m.pitch * 2u, (cuuint64_t)(m.planes > 1 ? m.plane : m.pitch) * 2u};
+  const cuuint32_t box[3] = {64u, (cuuint32_t)box_rows, (cuuint32_t)m.planes};
+  const cuuint32_t elem[3] = {1u, 1u, 1u};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(m.data), dims, strides, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct TileProblem {
+  Matrix a[2], b[2];       // a pair: b[0] and b[1] side by side; two segments: a[0] b[0] + a[1] b[1]
+  int segments = 1;
+  int64_t rows = 0, cols = 0, k = 0;  // cols: of the output (a pair: of each matrix)
+  int64_t b_n0 = 0, b_k0 = 0;
+  bool f16 = false;        // operands in fp16, else bf16
+  uint32_t *status_word = nullptr;
+};
+
+inline int sm_count(int *sms) {
+  int device = 0;
+  HT_CUDA_TRY(cudaGetDevice(&device));
+  HT_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+  return HT_OK;
+}
+
+// Columns of a tile: the width with which the SMs are done first.  A step of 16 values of k takes the tensor core bn / 2 cycles, and its
+// operands (128 + bn rows of 32 bytes) leave shared memory at 128 bytes a cycle; a tile costs about 2000 cycles besides.
+inline int tile_columns(int64_t rows, int64_t cols, int64_t k, int planes, bool pair, int sms) {
+  const int64_t m_blocks = (rows + kTileM - 1) / kTileM;
+  const int most = planes == 3 ? 128 : 256, step = pair ? 128 : 64;
+  int best = most;
+  double least = 0.0;
+  for (int bn = most; bn >= step; bn -= step) {
+    const int64_t n = pair ? bn / 2 : bn, tiles = m_blocks * ((cols + n - 1) / n);
+    const double rounds = (double)((tiles + sms - 1) / sms);
+    const double cycles = (planes == 3 ? 6.0 : 1.0) * (double)((k + 15) / 16) * std::max(bn / 2.0, 32.0 + bn / 4.0) + 2000.0;
+    if (bn == most || rounds * cycles < least * 0.999) {
+      best = bn;
+      least = rounds * cycles;
+    }
+  }
+  return best;
+}
+
+template <int PLANES, bool A_MN, bool B_MN, class Epilogue>
+int launch_tiles(const TileProblem &p, const Epilogue &epilogue, int bn, int sms, cudaStream_t stream) {
+  constexpr bool kPair = Epilogue::kPair;
+  if (p.rows < 1 || p.cols < 1 || p.k < 1) return HT_ERR_INVALID_ARGUMENT;
+  TileArgs a = {};
+  const int b_rows = kPair ? bn / 2 : bn;
+  for (int s = 0; s < p.segments || (kPair && s < 2); ++s) {
+    if (s < p.segments && !encode_matrix_16(&a.a[s], p.a[s], A_MN ? kTileK : kTileM)) return HT_ERR_UNSUPPORTED;
+    if (!encode_matrix_16(&a.b[s], p.b[s], B_MN ? kTileK : b_rows)) return HT_ERR_UNSUPPORTED;
+  }
+  const int64_t m_blocks = (p.rows + kTileM - 1) / kTileM, n_blocks = (p.cols + b_rows - 1) / b_rows;
+  if (m_blocks * n_blocks > 0x3fffffff || p.k > 0x3fffffff) return HT_ERR_UNSUPPORTED;
+  a.status_word = p.status_word;
+  const int n = PLANES == 3 ? b_rows : bn;  // of one instruction
+  a.instruction = (1u << 4) | ((p.f16 ? 0u : 1u) << 7) | ((p.f16 ? 0u : 1u) << 10) | ((A_MN ? 1u : 0u) << 15) |
+                  ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+  a.m_blocks = (int)m_blocks;
+  a.n_blocks = (int)n_blocks;
+  a.tiles = (int)(m_blocks * n_blocks);
+  a.bn = bn;
+  a.k = (int)p.k;
+  a.k_blocks = (int)((p.k + kTileK - 1) / kTileK);
+  a.segments = p.segments;
+  a.b_n0 = (int)p.b_n0;
+  a.b_k0 = (int)p.b_k0;
+  a.a_bytes = (uint32_t)kTileM * 128u * PLANES;
+  a.stage_bytes = a.a_bytes + (uint32_t)bn * 128u * PLANES;
+  a.stages = (int)std::min<uint32_t>(kStageBudget / a.stage_bytes, kMostStages);
+  auto kernel = dense_tile_kernel<PLANES, A_MN, B_MN, Epilogue>;
+  HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem));
+  kernel<<<(unsigned)std::min(a.tiles, std::max(sms, 1)), kTileThreads, kTileSmem, stream>>>(a, epilogue);
+  HT_CHECK_LAUNCH();
+  return HT_OK;
+}
+
+}  // namespace dense
+}  // namespace ht

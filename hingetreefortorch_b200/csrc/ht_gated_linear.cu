@@ -1,0 +1,363 @@
+// A gated projection in front of a forest: both projections, the activation and the product in one kernel, and its gradient.
+//
+//     a = x wg^T + bg      u = x wv^T + bv      h = act(a) u
+//     da = dh u act'(a)    du = dh act(a)       dx = da wg + du wv     dwg = da^T x     dwv = du^T x     dbg, dbv: column sums
+//
+// Forward: one tile product over the rows of both weights side by side, 64 or 128 columns of each; the epilogue has the two products
+// of an element in one thread and writes h alone.
+// Backward: nothing but x is kept.  The projections are formed again, the epilogue reads dh and writes da and du in the operands' type,
+// and those enter the products of ht_dense_products.cu: dx as one sum over both, dwg and dwv as one product.  16 N K H
+// operations for a training step where 12 N K H are needed; keeping a and u in fp32, which the gradient's accuracy asks for,
+// would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to the operands' 16 bits (2^-9 of a term
+// that enters sums, for bf16); for fp16 dh is scaled to a largest value in [1, 2) first, so that small gradients stay normal numbers; fp32
+// is split into planes.
+#include "ht_dense.cuh"
+
+namespace ht {
+namespace dense {
+namespace {
+
+// The activation g and its derivative d at a.  EXACT: fp32 results; otherwise what is rounded to 16 bits afterwards.
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid(float a) {
+  return EXACT ? 1.0f / (1.0f + expf(-a)) : __fdividef(1.0f, 1.0f + __expf(-a));
+}
+template <bool EXACT, bool SLOPE>
+__device__ __forceinline__ void activate(int act, const float (&a)[32], float (&g)[32], float (&d)[32]) {
+  if (act == HT_ACTIVATION_SILU || act == HT_ACTIVATION_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float s = sigmoid<EXACT>(a[i]);
+      g[i] = act == HT_ACTIVATION_SILU ? a[i] * s : s;
+      if (SLOPE) d[i] = act == HT_ACTIVATION_SILU ? s * (1.0f + a[i] * (1.0f - s)) : s * (1.0f - s);
+    }
+  } else if (act == HT_ACTIVATION_GELU) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float phi = 0.5f * erfcf(a[i] * -0.70710678118654752f);  // the normal distribution function
+      g[i] = a[i] * phi;
+      if (SLOPE) d[i] = phi + a[i] * 0.39894228040143268f * (EXACT ? expf(-0.5f * a[i] * a[i]) : __expf(-0.5f * a[i] * a[i]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      g[i] = a[i] < 0.0f ? 0.0f : a[i];  // (no number stays none)
+      if (SLOPE) d[i] = a[i] > 0.0f ? 1.0f : 0.0f;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void add_bias(const T *bias, int col, int n, float (&v)[32]) {
+  if (bias == nullptr) return;
+  float b[32];
+  load_columns(bias + col, b, n, true);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] += b[i];
+}
+
+template <typename T>
+struct GatedEpilogue {
+  static constexpr bool kPair = true;
+  static constexpr bool kExact = sizeof(T) == 4;
+  struct State {};
+  int rows, cols, act;
+  const T *bg, *bv;
+  T *h;        // [rows, cols]
+  bool whole;  // rows of h start on 16 bytes
+  __device__ __forceinline__ void begin(State &, const Where &) const {}
+  __device__ __forceinline__ void unit(State &, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
+    const int n = cols - col;
+    if (n <= 0) return;
+    add_bias(bg, col, n, a);
+    add_bias(bv, col, n, u);
+    float g[32];
+    activate<kExact, false>(act, a, g, g);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) g[i] *= u[i];
+    if (w.inside) store_columns(h + (size_t)w.row * (size_t)cols + col, g, n, whole);
+  }
+  __device__ __forceinline__ void end(State &, const Where &) const {}
+};
+
+// The power of two at or below the largest |dh| (its bits in *top), 1 where there is none.
+__device__ __forceinline__ float scale_of(const uint32_t *top) {
+  const uint32_t e = __ldg(top) & 0x7f800000u;
+  return e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
+}
+
+// da and du of a piece of the outputs, side by side in one operand, and their sums over 32 rows for the biases' gradients.
+template <typename T>
+struct GatedGradEpilogue {
+  static constexpr bool kPair = true;
+  static constexpr bool kExact = sizeof(T) == 4;
+  struct State {
+    float scale;
+  };
+  int rows, cols, act, first, outputs;  // the piece: outputs first .. first + cols - 1
+  const T *bg, *bv;
+  const T *dh;          // [rows, outputs]
+  bool whole;           // rows of dh start on 16 bytes
+  const uint32_t *top;  // fp16: dh is divided by this power of two; else null
+  typename Kind<T>::Operand *g;  // [planes][rows][2 pitch]: da, then du
+  int pitch;
+  size_t plane;
+  float *row_sums;  // [4 m_blocks][2 pitch] or null
+  __device__ __forceinline__ void begin(State &s, const Where &) const { s.scale = top != nullptr ? 1.0f / scale_of(top) : 1.0f; }
+  __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
+    const int n = cols - col;
+    if (n <= 0) return;
+    add_bias(bg, first + col, n, a);
+    add_bias(bv, first + col, n, u);
+    float act_a[32], slope[32], dh_[32];
+    activate<kExact, true>(act, a, act_a, slope);
+    load_columns(dh + (size_t)(w.inside ? w.row : 0) * (size_t)outputs + first + col, dh_, n, whole);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float d = dh_[i] * s.scale;
+      a[i] = w.inside && i < n ? d * u[i] * slope[i] : 0.0f;
+      u[i] = w.inside && i < n ? d * act_a[i] : 0.0f;
+    }
+    typename Kind<T>::Operand *to = g + (size_t)w.row * (size_t)(2 * pitch) + col;
+    if (w.inside) {
+      store_operand<T>(to, plane, a);
+      store_operand<T>(to + pitch, plane, u);
+    }
+    if (row_sums != nullptr) {
+      float *sums = row_sums + (size_t)(w.m_block * 4 + w.quarter) * (size_t)(2 * pitch) + col + w.lane;
+      sums[0] = sum_rows(a, w.lane);
+      sums[pitch] = sum_rows(u, w.lane);
+    }
+  }
+  __device__ __forceinline__ void end(State &, const Where &) const {}
+};
+
+// The bits of the largest |dh| (fp16) into *top, which starts as 0: bits of numbers without a sign order like the numbers.
+__global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__ v, int64_t n, uint32_t *top) {
+  uint32_t most = 0;
+  const int64_t quads = n / 8, step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = at; i < quads; i += step) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(v) + i);
+    const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = max(most, max(words[j] & 0x7fffu, (words[j] >> 16) & 0x7fffu));
+  }
+  if (at == 0)
+    for (int64_t i = quads * 8; i < n; ++i) most = max(most, (uint32_t)__half_as_ushort(v[i]) & 0x7fffu);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) atomicMax(top, __float_as_uint(__half2float(__ushort_as_half((unsigned short)most))));
+}
+__global__ void scale_kernel(const uint32_t *top, float *alpha) { *alpha = scale_of(top); }
+
+constexpr int kPlanSMs = 148;  // what tiles and workspaces are planned for
+constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // da and du of one piece, unless the caller sets less
+
+int screen(const ht_dense_problem *p) {
+  if (p == nullptr || p->rows < 0 || p->features < 1 || p->outputs < 1 || p->x_stride < p->features) return HT_ERR_INVALID_ARGUMENT;
+  if (p->dtype != HT_DTYPE_F32 && p->dtype != HT_DTYPE_BF16 && p->dtype != HT_DTYPE_F16) return HT_ERR_INVALID_ARGUMENT;
+  if (p->activation < HT_ACTIVATION_SILU || p->activation > HT_ACTIVATION_SIGMOID) return HT_ERR_INVALID_ARGUMENT;
+  if (p->rows > 0x7fffff00 || p->features > 0x3fffff00 || p->outputs > 0x3fffff00) return HT_ERR_UNSUPPORTED;
+  return HT_OK;
+}
+
+template <typename T>
+struct Plan {
+  Operand<T> x, wg, wv;
+  int64_t piece = 0, pitch = 0;
+  typename Kind<T>::Operand *g = nullptr;
+  uint32_t *top = nullptr;
+  float *alpha = nullptr, *sum = nullptr, *row_sums = nullptr;
+  size_t bytes;
+  Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, void *ws) {
+    Arena arena(ws);
+    x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
+    wg.set(arena, static_cast<const T *>(wgp), p.outputs, p.features, p.features);
+    wv.set(arena, static_cast<const T *>(wvp), p.outputs, p.features, p.features);
+    if (backward) {
+      const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
+      const int64_t per_output = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 4;
+      piece = std::max<int64_t>(limit / per_output / 256 * 256, 256);
+      if (piece >= p.outputs) piece = p.outputs;
+      pitch = round_up(piece, 64);
+      g = arena.template take<typename Kind<T>::Operand>(p.rows * 2 * pitch * Kind<T>::kPlanes);
+      top = arena.take<uint32_t>(1);
+      alpha = arena.take<float>(1);
+      sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
+      row_sums = has_bias ? arena.take<float>((p.rows + kTileM - 1) / kTileM * 4 * 2 * pitch) : nullptr;
+    }
+    bytes = arena.used;
+  }
+  int lay_out(cudaStream_t stream) const {
+    int rc = x.lay_out(stream);
+    if (rc == HT_OK) rc = wg.lay_out(stream);
+    if (rc == HT_OK) rc = wv.lay_out(stream);
+    return rc;
+  }
+};
+
+template <typename T>
+int forward(const ht_dense_problem &p, const void *x, const void *wg, const void *wv, const void *bg, const void *bv, void *h, void *ws,
+            size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
+  Plan<T> plan(p, x, wg, wv, false, false, false, ws);
+  if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
+  int sms = 0, rc;
+  if ((rc = sm_count(&sms)) != HT_OK) return rc;
+  if ((rc = plan.lay_out(stream)) != HT_OK) return rc;
+  TileProblem t;
+  t.a[0] = plan.x.m;
+  t.b[0] = plan.wg.m;
+  t.b[1] = plan.wv.m;
+  t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
+  t.f16 = p.dtype == HT_DTYPE_F16;
+  t.status_word = status_word;
+  GatedEpilogue<T> e = {(int)p.rows, (int)p.outputs, p.activation, static_cast<const T *>(bg), static_cast<const T *>(bv), static_cast<T *>(h),
+                        p.outputs * (int64_t)sizeof(T) % 16 == 0};
+  return launch_tiles<Kind<T>::kPlanes, false, false>(t, e, tile_columns(p.rows, p.outputs, p.features, Kind<T>::kPlanes, true, kPlanSMs), sms, stream);
+}
+
+struct Gradients {
+  void *dx, *dwg, *dwv, *dbg, *dbv;
+};
+
+template <typename T>
+int backward(const ht_dense_problem &p, const void *x, const void *wg, const void *wv, const void *bg, const void *bv, const void *dh,
+             const Gradients &out, void *ws, size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
+  const bool has_bias = out.dbg != nullptr || out.dbv != nullptr;
+  Plan<T> plan(p, x, wg, wv, true, out.dx != nullptr, has_bias, ws);
+  if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
+  T *dwg = static_cast<T *>(out.dwg), *dwv = static_cast<T *>(out.dwv), *dbg = static_cast<T *>(out.dbg), *dbv = static_cast<T *>(out.dbv);
+  if (p.rows == 0) {
+    for (T *q : {dwg, dwv})
+      if (q != nullptr) HT_CUDA_TRY(cudaMemsetAsync(q, 0, sizeof(T) * (size_t)(p.outputs * p.features), stream));
+    for (T *q : {dbg, dbv})
+      if (q != nullptr) HT_CUDA_TRY(cudaMemsetAsync(q, 0, sizeof(T) * (size_t)p.outputs, stream));
+    return HT_OK;
+  }
+  int sms = 0, rc;
+  if ((rc = sm_count(&sms)) != HT_OK) return rc;
+  if ((rc = plan.lay_out(stream)) != HT_OK) return rc;
+  const bool scaled = p.dtype == HT_DTYPE_F16;
+  if (scaled) {
+    const int64_t n = p.rows * p.outputs;
+    HT_CUDA_TRY(cudaMemsetAsync(plan.top, 0, sizeof(uint32_t), stream));
+    largest_kernel<<<blocks_for(n, 256 * 32, 148 * 8), 256, 0, stream>>>(static_cast<const __half *>(dh), n, plan.top);
+    HT_CHECK_LAUNCH();
+    scale_kernel<<<1, 1, 0, stream>>>(plan.top, plan.alpha);
+    HT_CHECK_LAUNCH();
+  }
+  const float *alpha = scaled ? plan.alpha : nullptr;
+  constexpr int kPlanes = Kind<T>::kPlanes;
+  const bool whole = p.features * (int64_t)sizeof(T) % 16 == 0;
+  const size_t plane = (size_t)(p.rows * 2 * plan.pitch);
+  for (int64_t first = 0; first < p.outputs; first += plan.piece) {
+    const int64_t count = std::min(plan.piece, p.outputs - first);
+    TileProblem t;
+    t.f16 = scaled;
+    t.status_word = status_word;
+    t.a[0] = plan.x.m;
+    t.b[0] = plan.wg.m;
+    t.b[1] = plan.wv.m;
+    t.rows = p.rows, t.cols = count, t.k = p.features, t.b_n0 = first;
+    GatedGradEpilogue<T> e = {};
+    e.rows = (int)p.rows, e.cols = (int)count, e.act = p.activation, e.first = (int)first, e.outputs = (int)p.outputs;
+    e.bg = static_cast<const T *>(bg), e.bv = static_cast<const T *>(bv), e.dh = static_cast<const T *>(dh);
+    e.whole = p.outputs * (int64_t)sizeof(T) % 16 == 0;
+    e.top = scaled ? plan.top : nullptr;
+    e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = plane, e.row_sums = plan.row_sums;
+    if ((rc = launch_tiles<kPlanes, false, false>(t, e, tile_columns(p.rows, count, p.features, kPlanes, true, kPlanSMs), sms, stream)) != HT_OK) return rc;
+    StoreEpilogue<T> store = {};
+    store.alpha = alpha;
+    store.cols = (int)p.features;
+    store.whole = whole;
+    store.split = 0x7fffffff;
+    Matrix g;
+    g.rows = p.rows, g.pitch = 2 * plan.pitch, g.planes = kPlanes, g.plane = (int64_t)plane;
+    if (out.dx != nullptr) {
+      TileProblem q = t;
+      g.cols = count;
+      g.data = plan.g, q.a[0] = g;
+      g.data = plan.g + plan.pitch, q.a[1] = g;
+      q.segments = 2;
+      q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = first;
+      store.rows = store.part = (int)p.rows;
+      store.out = static_cast<T *>(out.dx);
+      store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
+      if ((rc = product_dx<T>(q, store, sms, stream)) != HT_OK) return rc;
+    }
+    if (dwg != nullptr || dwv != nullptr) {
+      // rows of the product: da's columns, then du's; one of the two weights alone takes its half
+      TileProblem q = t;
+      const bool both = dwg != nullptr && dwv != nullptr;
+      g.data = dwg != nullptr ? plan.g : plan.g + plan.pitch;
+      g.cols = both ? plan.pitch + count : count;
+      q.a[0] = g;
+      q.b[0] = plan.x.m;
+      q.rows = g.cols, q.cols = p.features, q.k = p.rows, q.b_n0 = 0;
+      store.rows = (int)g.cols;
+      store.part = (int)count;
+      store.split = both ? (int)plan.pitch : 0x7fffffff;
+      store.out = (dwg != nullptr ? dwg : dwv) + (size_t)first * (size_t)p.features;
+      store.out2 = both ? dwv + (size_t)first * (size_t)p.features : nullptr;
+      store.sum = nullptr, store.keep = false;
+      if ((rc = product_dw<T>(q, store, sms, stream)) != HT_OK) return rc;
+    }
+    const int64_t blocks = (p.rows + kTileM - 1) / kTileM * 4;
+    if (dbg != nullptr && (rc = column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, alpha, dbg + first, stream)) != HT_OK) return rc;
+    if (dbv != nullptr && (rc = column_sums<T>(plan.row_sums + plan.pitch, blocks, 2 * plan.pitch, count, alpha, dbv + first, stream)) != HT_OK) return rc;
+  }
+  return HT_OK;
+}
+
+template <typename F>
+auto by_type(int dtype, F &&f) {
+  return dtype == HT_DTYPE_F32 ? f(float()) : dtype == HT_DTYPE_BF16 ? f(__nv_bfloat16()) : f(__half());
+}
+
+bool aligned(std::initializer_list<const void *> pointers) {
+  uintptr_t all = 0;
+  for (const void *p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & 15u) == 0;
+}
+
+}  // namespace
+}  // namespace dense
+}  // namespace ht
+
+using namespace ht;
+using namespace ht::dense;
+
+extern "C" size_t ht_gated_linear_workspace_bytes(const ht_dense_problem *p, int backward) {
+  if (screen(p) != HT_OK) return 0;
+  return by_type(p->dtype, [&](auto zero) -> size_t {
+    return Plan<decltype(zero)>(*p, nullptr, nullptr, nullptr, backward != 0, true, true, nullptr).bytes;
+  });
+}
+
+extern "C" int ht_gated_linear_forward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
+                                       const void *gate_bias, const void *value_bias, void *h, void *workspace, size_t workspace_bytes,
+                                       uint32_t *status_word, ht_stream_t stream) {
+  const int rc = screen(p);
+  if (rc != HT_OK) return rc;
+  if (p->rows == 0) return HT_OK;
+  if (x == nullptr || gate_weight == nullptr || value_weight == nullptr || h == nullptr) return HT_ERR_INVALID_ARGUMENT;
+  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, h, workspace})) return HT_ERR_UNSUPPORTED;
+  return by_type(p->dtype, [&](auto zero) -> int {
+    return forward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, h, workspace, workspace_bytes, status_word,
+                                   reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" int ht_gated_linear_backward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
+                                        const void *gate_bias, const void *value_bias, const void *dh, void *dx, void *dgate_weight,
+                                        void *dvalue_weight, void *dgate_bias, void *dvalue_bias, void *workspace, size_t workspace_bytes,
+                                        uint32_t *status_word, ht_stream_t stream) {
+  const int rc = screen(p);
+  if (rc != HT_OK) return rc;
+  if (p->rows > 0 && (x == nullptr || gate_weight == nullptr || value_weight == nullptr || dh == nullptr)) return HT_ERR_INVALID_ARGUMENT;
+  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, dh, dx, dgate_weight, dvalue_weight, workspace})) return HT_ERR_UNSUPPORTED;
+  const Gradients out = {dx, dgate_weight, dvalue_weight, dgate_bias, dvalue_bias};
+  return by_type(p->dtype, [&](auto zero) -> int {
+    return backward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, dh, out, workspace, workspace_bytes, status_word,
+                                    reinterpret_cast<cudaStream_t>(stream));
+  });
+}

@@ -44,6 +44,7 @@ typedef enum ht_status {
 
 /* bits OR-ed into the device status word */
 #define HT_FLAG_ORDINAL_RANGE 1u /* an ordinal was < 0 or >= C (reference: RuntimeError) */
+#define HT_FLAG_TARGET_RANGE 2u /* a class loss was given a target that is neither a class nor the ignored one */
 #define HT_FLAG_PIPELINE_TIMEOUT 0x80000000u /* a bounded wait inside a kernel ran out; outputs are incomplete */
 
 #define HT_KIND_TREE 0 /* complete binary tree: HingeTreeCommon<>  (HingeTreeCommon.h:129) */
@@ -417,6 +418,57 @@ int ht_init_medians_f64(int kind, const double *x, double *thr, const int64_t *o
  * tree t was changed.  result: T bytes in device memory. */
 int ht_thresholds_f32(int fix, float *thr, const int64_t *ord, int64_t T, int depth, unsigned char *result, ht_stream_t stream);
 int ht_thresholds_f64(int fix, double *thr, const int64_t *ord, int64_t T, int depth, unsigned char *result, ht_stream_t stream);
+
+/* ---- dense layers around a forest -------------------------------------------------------------------------
+ * A gated projection in front of a forest and the loss of a linear layer's class scores behind one, on the tensor cores.  The reference has
+ * neither (its pipelines put torch.nn modules there, README.md:110-129); they stand beside ht_linear_tf32_stats_f32 and the fused
+ * linear forests.  All matrices are row-major in the problem's type: x [rows, features] with x_stride >= features elements
+ * from row to row, weights [outputs, features], biases [outputs] or NULL, gradients like what they belong to.  Sums, softmax statistics and
+ * losses are fp32; fp32 products are as accurate as fp32 ones (three bf16 planes a value).  Pointers to matrices, biases,
+ * statistics and workspaces start on 16 bytes (HT_ERR_UNSUPPORTED otherwise).  No atomics: the same call gives the same bits.
+ * Workspaces: the matching *_workspace_bytes (0 for a bad problem). */
+#define HT_DTYPE_F32 0
+#define HT_DTYPE_BF16 1
+#define HT_DTYPE_F16 2
+#define HT_ACTIVATION_SILU 0 /* a / (1 + exp(-a)) */
+#define HT_ACTIVATION_GELU 1 /* a times the normal distribution function at a */
+#define HT_ACTIVATION_RELU 2
+#define HT_ACTIVATION_SIGMOID 3
+#define HT_REDUCTION_NONE 0
+#define HT_REDUCTION_MEAN 1 /* over the rows that count; NaN where none does */
+#define HT_REDUCTION_SUM 2
+
+typedef struct ht_dense_problem {
+  int32_t dtype;
+  int32_t activation; /* gated linear only */
+  int64_t rows, features, outputs;
+  int64_t x_stride;
+  int64_t scratch_limit; /* backward: most bytes of the gradient with respect to the products that are held at a time (0: 512 MiB);
+                          * they are then formed and used a piece of the outputs at a time, 256 of them at the least */
+} ht_dense_problem;
+
+/* h[n, o] = act(x[n] . gate_weight[o] + gate_bias[o]) * (x[n] . value_weight[o] + value_bias[o]).  The backward forms the projections
+ * again; gradients that are NULL are not computed.  rows = 0: nothing to write, or zeros for the weights. */
+size_t ht_gated_linear_workspace_bytes(const ht_dense_problem *p, int backward);
+int ht_gated_linear_forward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
+                            const void *gate_bias, const void *value_bias, void *h, void *workspace, size_t workspace_bytes,
+                            uint32_t *status_word, ht_stream_t stream);
+int ht_gated_linear_backward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
+                             const void *gate_bias, const void *value_bias, const void *dh, void *dx, void *dgate_weight,
+                             void *dvalue_weight, void *dgate_bias, void *dvalue_bias, void *workspace, size_t workspace_bytes,
+                             uint32_t *status_word, ht_stream_t stream);
+
+/* loss[n] = log sum_o exp(s[n, o]) - s[n, target[n]] with s = x w^T + bias, never in memory; a row whose target is ignore_index has loss
+ * and gradients 0 whatever it holds; a target outside [0, outputs) makes the row's loss (and gradients that it enters) NaN and
+ * sets HT_FLAG_TARGET_RANGE.  loss: [rows] floats, or one for a sum or mean.  stats (may be NULL: no backward follows):
+ * 2 rows + 2 floats that the backward is given.  grad: the upstream gradient, shaped like loss. */
+size_t ht_linear_class_loss_workspace_bytes(const ht_dense_problem *p, int backward);
+int ht_linear_class_loss_forward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
+                                 int64_t ignore_index, int reduction, float *loss, float *stats, void *workspace,
+                                 size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
+int ht_linear_class_loss_backward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
+                                  int64_t ignore_index, int reduction, const float *grad, const float *stats, void *dx, void *dw,
+                                  void *dbias, void *workspace, size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
 
 #ifdef __cplusplus
 }
