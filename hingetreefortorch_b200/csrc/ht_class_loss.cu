@@ -66,7 +66,7 @@ struct LossEpilogue {
     if (n <= 0) return;
     if (bias != nullptr) {
       float b[32];
-      load_columns(bias + col, b, n, true);
+      load_columns(bias + col, b, n);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += b[i];
     }
@@ -115,7 +115,7 @@ struct LossGradEpilogue {
   typename Kind<T>::Operand *g;  // [planes][rows][pitch]
   int pitch;
   size_t plane;
-  float *row_sums;  // [4 m_blocks][pitch] or null
+  float *row_sums;  // [row_sum_count][pitch] or null
   __device__ __forceinline__ void begin(State &s, const Where &w) const {
     s.r = {0.0f, 0.0f, 0.0f, -1};
     if (w.inside) {
@@ -128,7 +128,7 @@ struct LossGradEpilogue {
     if (n <= 0) return;
     if (bias != nullptr) {
       float b[32];
-      load_columns(bias + first + col, b, n, true);
+      load_columns(bias + first + col, b, n);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += b[i];
     }
@@ -243,7 +243,6 @@ __global__ void __launch_bounds__(256) row_grad_kernel(const float2 *__restrict_
   reinterpret_cast<float4 *>(row_grad)[row] = r;
 }
 
-constexpr int kPlanSMs = 148;  // what tiles and workspaces are planned for
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // g of one piece, unless the caller sets less
 
 int screen(const ht_dense_problem *p) {
@@ -256,7 +255,8 @@ int screen(const ht_dense_problem *p) {
 template <typename T>
 struct ForwardPlan {
   Operand<T> x, w;
-  int bn, slots;
+  TileShape shape;
+  int slots;
   float2 *partial;
   float *target_score, *row_loss;
   size_t bytes;
@@ -264,8 +264,8 @@ struct ForwardPlan {
     Arena arena(ws);
     x.set(arena, xp, p.rows, p.features, p.x_stride);
     w.set(arena, wp, p.outputs, p.features, p.features);
-    bn = tile_columns(p.rows, p.outputs, p.features, Kind<T>::kPlanes, false, kPlanSMs);
-    slots = (int)(2 * ((p.outputs + bn - 1) / bn));
+    shape = tile_shape(p.rows, p.outputs, p.features, Kind<T>::kPlanes, false);
+    slots = (int)(2 * ((p.outputs + shape.bn - 1) / shape.bn));
     partial = arena.take<float2>((int64_t)slots * p.rows);
     target_score = arena.take<float>(p.rows);
     row_loss = arena.take<float>(p.rows);
@@ -291,7 +291,7 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
     t.f16 = p.dtype == HT_DTYPE_F16;
     t.status_word = status_word;
     LossEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), target, plan.partial, plan.target_score};
-    if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, plan.bn, sms, stream)) != HT_OK) return rc;
+    if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, plan.shape, sms, stream)) != HT_OK) return rc;
     join_rows_kernel<<<(unsigned)((p.rows + 31) / 32), 256, 0, stream>>>(plan.partial, plan.slots, plan.target_score, target, ignore, p.rows,
                                                                        p.outputs, reinterpret_cast<float2 *>(stats), row_loss, status_word);
     HT_CHECK_LAUNCH();
@@ -327,7 +327,7 @@ struct BackwardPlan {
     row_grad = arena.take<RowGrad>(p.rows);
     alpha = arena.take<float>(1);
     sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
-    row_sums = has_db ? arena.take<float>((p.rows + kTileM - 1) / kTileM * 4 * pitch) : nullptr;
+    row_sums = has_db ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * pitch) : nullptr;
     bytes = arena.used;
   }
 };
@@ -357,7 +357,6 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
                                                                        p.rows, p.outputs, grad, reduction, unit, plan.row_grad, plan.alpha);
   HT_CHECK_LAUNCH();
   constexpr int kPlanes = Kind<T>::kPlanes;
-  const bool whole = p.features * (int64_t)sizeof(T) % 16 == 0;
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
     const int64_t count = std::min(plan.piece, p.outputs - first);
     TileProblem t;
@@ -372,20 +371,21 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     e.row_grad = plan.row_grad;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = (size_t)(p.rows * plan.pitch);
     e.row_sums = plan.row_sums;
-    if ((rc = launch_tiles<kPlanes, false, false>(t, e, tile_columns(p.rows, count, p.features, kPlanes, false, kPlanSMs), sms, stream)) != HT_OK) return rc;
+    const TileShape shape = tile_shape(p.rows, count, p.features, kPlanes, false);
+    if ((rc = launch_tiles<kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
     Matrix g;
     g.data = plan.g, g.rows = p.rows, g.cols = count, g.pitch = plan.pitch, g.planes = kPlanes, g.plane = p.rows * plan.pitch;
     StoreEpilogue<T> store = {};
     store.alpha = plan.alpha;
     store.cols = (int)p.features;
-    store.whole = whole;
     store.split = 0x7fffffff;
+    store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));
     if (dx != nullptr) {
       TileProblem q = t;
       q.a[0] = g;
       q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = first;
       store.rows = store.part = (int)p.rows;
-      store.out = dx;
+      store.out = dx, store.align = row_alignment(dx, p.features * (int64_t)sizeof(T));
       store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
       if ((rc = product_dx<T>(q, store, sms, stream)) != HT_OK) return rc;
     }
@@ -395,11 +395,11 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
       q.b[0] = plan.x.m;
       q.rows = count, q.cols = p.features, q.k = p.rows, q.b_n0 = 0;
       store.rows = store.part = (int)count;
-      store.out = dw + (size_t)first * (size_t)p.features;
+      store.out = dw + (size_t)first * (size_t)p.features, store.align = row_alignment(store.out, p.features * (int64_t)sizeof(T));
       store.sum = nullptr, store.keep = false;
       if ((rc = product_dw<T>(q, store, sms, stream)) != HT_OK) return rc;
     }
-    if (db != nullptr && (rc = column_sums<T>(plan.row_sums, (p.rows + kTileM - 1) / kTileM * 4, plan.pitch, count, plan.alpha, db + first, stream)) != HT_OK)
+    if (db != nullptr && (rc = column_sums<T>(plan.row_sums, row_sum_count(p.rows, shape), plan.pitch, count, plan.alpha, db + first, stream)) != HT_OK)
       return rc;
   }
   return HT_OK;

@@ -63,47 +63,17 @@ __device__ __forceinline__ void split_planes(float v, float &p0, float &p1, floa
   p2 = r - p1;
 }
 
-// 32 columns of one row (n of them inside the matrix).  `whole`: the row's address is a multiple of 16 bytes.
+// n numbers of one row, contiguous; all lanes read the same ones.
 template <typename T>
-__device__ __forceinline__ void store_columns(T *out, const float (&v)[32], int n, bool whole) {
-  if (whole && n >= 32) {
-    if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void load_columns(const T *in, float (&v)[32], int n) {
+  if (n >= 32) {
+    constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(out + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
+    for (int i = 0; i < 32; i += kPer) {
+      T t[kPer];
+      *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(in + i));
 #pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        *reinterpret_cast<uint4 *>(out + i) = make_uint4(pack_pair(v[i], v[i + 1], out), pack_pair(v[i + 2], v[i + 3], out),
-                                                         pack_pair(v[i + 4], v[i + 5], out), pack_pair(v[i + 6], v[i + 7], out));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) out[i] = from_float<T>(v[i]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void load_columns(const T *in, float (&v)[32], int n, bool whole) {
-  if (whole && n >= 32) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const float4 q = __ldg(reinterpret_cast<const float4 *>(in + i));
-        v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(in + i));
-        const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          T pair[2];
-          *reinterpret_cast<uint32_t *>(pair) = words[j];
-          v[i + 2 * j] = to_float(pair[0]);
-          v[i + 2 * j + 1] = to_float(pair[1]);
-        }
-      }
+      for (int j = 0; j < kPer; ++j) v[i + j] = to_float(t[j]);
     }
   } else {
 #pragma unroll
@@ -111,22 +81,197 @@ __device__ __forceinline__ void load_columns(const T *in, float (&v)[32], int n,
   }
 }
 
-// The same as operands of a later product: [planes][rows][pitch], rows of a multiple of 64 elements.
+__device__ __forceinline__ void store_32_bytes(void *to, const uint32_t (&q)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]), "r"(q[4]),
+               "r"(q[5]), "r"(q[6]), "r"(q[7])
+               : "memory");
+}
+__device__ __forceinline__ void load_32_bytes(const void *from, uint32_t (&q)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
+               : "l"(from)
+               : "memory");
+}
+
+// A warp's 32 rows of 32 columns between registers (a lane has a row) and a matrix: `first` points at the first row's first column of
+// the box, `rows` and `cols` of the box are inside the matrix (32 or fewer), `align` is the power of two of bytes that every row starts on
+// (32 at the most).  Rows on 32 bytes go lane by lane in whole sectors; others through the warp's shared memory, so that neighbouring lanes
+// read or write neighbouring addresses, `align` bytes each (rows of 12700 bf16, written two bytes a lane and row, took 5 times the
+// product's time).
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> {
+  typedef uint16_t type;
+};
+template <>
+struct Word<4> {
+  typedef uint32_t type;
+};
+template <>
+struct Word<8> {
+  typedef uint2 type;
+};
+template <>
+struct Word<16> {
+  typedef uint4 type;
+};
+// 16-byte piece q of row r of the box
+template <typename T>
+__device__ __forceinline__ uint32_t box_offset(uint32_t r, uint32_t q) {
+  return sizeof(T) == 4 ? 128u * r + 16u * (q ^ (r & 7u)) : 64u * r + 16u * (q ^ ((r >> 1) & 3u));
+}
+template <typename T, int BYTES, bool STORE>
+__device__ __forceinline__ void move_box(uint32_t box, T *first, size_t pitch, int rows, int cols, int lane) {
+  typedef typename Word<BYTES>::type W;
+  constexpr int kPerRow = 32 * (int)sizeof(T) / BYTES, kRows = 32 / kPerRow, kValues = BYTES / (int)sizeof(T);
+  const int piece = lane % kPerRow, c = piece * kValues;
+#pragma unroll 4
+  for (int r = lane / kPerRow; r < 32; r += kRows) {
+    if (r >= rows || c >= cols) continue;
+    const uint32_t at = box + box_offset<T>((uint32_t)r, (uint32_t)(piece * BYTES / 16)) + (uint32_t)(piece * BYTES % 16);
+    W *const shared = reinterpret_cast<W *>(__cvta_shared_to_generic(at));
+    T *const global = first + (size_t)r * pitch + c;
+    if (c + kValues <= cols) {
+      if (STORE)
+        *reinterpret_cast<W *>(global) = *shared;
+      else
+        *shared = __ldg(reinterpret_cast<const W *>(global));
+    } else {
+      T *const each = reinterpret_cast<T *>(shared);
+      for (int j = 0; j < cols - c; ++j) {
+        if (STORE)
+          global[j] = each[j];
+        else
+          each[j] = global[j];
+      }
+    }
+  }
+}
+template <typename T, bool STORE>
+__device__ __forceinline__ void move_box_by(uint32_t box, T *first, size_t pitch, int rows, int cols, int align, int lane) {
+  if (align >= 16)
+    move_box<T, 16, STORE>(box, first, pitch, rows, cols, lane);
+  else if (align == 8)
+    move_box<T, 8, STORE>(box, first, pitch, rows, cols, lane);
+  else if (align == 4 || sizeof(T) == 4)
+    move_box<T, 4, STORE>(box, first, pitch, rows, cols, lane);
+  else if constexpr (sizeof(T) == 2)
+    move_box<T, 2, STORE>(box, first, pitch, rows, cols, lane);
+}
+
+template <typename T>
+__device__ __forceinline__ void to_words(const float (&v)[32], int from, uint32_t (&q)[8]) {  // 32 bytes
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4)
+      q[i] = __float_as_uint(v[from + i]);
+    else
+      q[i] = pack_pair(v[from + 2 * i], v[from + 2 * i + 1], static_cast<const T *>(nullptr));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void from_words(const uint32_t (&q)[8], int from, float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[from + i] = __uint_as_float(q[i]);
+    } else {
+      T pair[2];
+      *reinterpret_cast<uint32_t *>(pair) = q[i];
+      v[from + 2 * i] = to_float(pair[0]);
+      v[from + 2 * i + 1] = to_float(pair[1]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_box(const Where &w, T *first, size_t pitch, int rows, int cols, int align, const float (&v)[32]) {
+  constexpr int kStep = 32 / (int)sizeof(T);
+  if (align >= 32 && cols >= 32) {
+    if (w.lane < rows) {
+      T *to = first + (size_t)w.lane * pitch;
+#pragma unroll
+      for (int i = 0; i < 32; i += kStep) {
+        uint32_t q[8];
+        to_words<T>(v, i, q);
+        store_32_bytes(to + i, q);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; i += kStep) {
+    uint32_t q[8];
+    to_words<T>(v, i, q);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(w.box + box_offset<T>((uint32_t)w.lane, (uint32_t)(i / kStep * 2 + h))),
+                   "r"(q[4 * h]), "r"(q[4 * h + 1]), "r"(q[4 * h + 2]), "r"(q[4 * h + 3])
+                   : "memory");
+  }
+  __syncwarp();
+  move_box_by<T, true>(w.box, first, pitch, rows, cols, align, w.lane);
+  __syncwarp();
+}
+// (columns and rows outside the matrix come as what the box held before)
+template <typename T>
+__device__ __forceinline__ void load_box(const Where &w, const T *first, size_t pitch, int rows, int cols, int align, float (&v)[32]) {
+  constexpr int kStep = 32 / (int)sizeof(T);
+  if (align >= 32 && cols >= 32) {
+    const T *from = first + (size_t)min(w.lane, rows - 1) * pitch;
+#pragma unroll
+    for (int i = 0; i < 32; i += kStep) {
+      uint32_t q[8];
+      load_32_bytes(from + i, q);
+      from_words<T>(q, i, v);
+    }
+    return;
+  }
+  move_box_by<T, false>(w.box, const_cast<T *>(first), pitch, rows, cols, align, w.lane);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 32; i += kStep) {
+    uint32_t q[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 t = lds_b128(w.box + box_offset<T>((uint32_t)w.lane, (uint32_t)(i / kStep * 2 + h)));
+      q[4 * h] = t.x, q[4 * h + 1] = t.y, q[4 * h + 2] = t.z, q[4 * h + 3] = t.w;
+    }
+    from_words<T>(q, i, v);
+  }
+  __syncwarp();
+}
+// The alignment of a matrix's rows for the two above.
+inline int row_alignment(const void *data, int64_t row_bytes) {
+  const uint64_t bits = (uint64_t)reinterpret_cast<uintptr_t>(data) | (uint64_t)row_bytes | 32u;
+  return (int)(bits & (~bits + 1));
+}
+
+// The same as operands of a later product: [planes][rows][pitch], rows of a multiple of 64 elements; a lane's row.
 template <typename T>
 __device__ __forceinline__ void store_operand(typename Kind<T>::Operand *out, size_t plane, const float (&v)[32]) {
-  if constexpr (Kind<T>::kPlanes == 1) {
-    store_columns(out, v, 32, true);
-  } else {
+  typedef typename Kind<T>::Operand O;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      float p[3][8];
+  for (int i = 0; i < 32; i += 16) {
+    uint32_t q[8];
+    if constexpr (Kind<T>::kPlanes == 1) {
+      to_words<O>(v, i, q);
+      store_32_bytes(out + i, q);
+    } else {
+      uint32_t q1[8], q2[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) split_planes(v[i + j], p[0][j], p[1][j], p[2][j]);
-#pragma unroll
-      for (int q = 0; q < 3; ++q)
-        *reinterpret_cast<uint4 *>(out + (size_t)q * plane + i) =
-            make_uint4(pack_pair(p[q][0], p[q][1], out), pack_pair(p[q][2], p[q][3], out), pack_pair(p[q][4], p[q][5], out),
-                       pack_pair(p[q][6], p[q][7], out));
+      for (int j = 0; j < 8; ++j) {
+        float a[3], b[3];
+        split_planes(v[i + 2 * j], a[0], a[1], a[2]);
+        split_planes(v[i + 2 * j + 1], b[0], b[1], b[2]);
+        q[j] = pack_pair(a[0], b[0], out);
+        q1[j] = pack_pair(a[1], b[1], out);
+        q2[j] = pack_pair(a[2], b[2], out);
+      }
+      store_32_bytes(out + i, q);
+      store_32_bytes(out + plane + i, q1);
+      store_32_bytes(out + 2 * plane + i, q2);
     }
   }
 }
@@ -158,43 +303,33 @@ struct StoreEpilogue {
     float alpha;
   };
   int rows, cols;
-  T *out, *out2;       // [part, cols] each: of the products' rows, those from `split` on go to out2
+  T *out, *out2;       // [part, cols] each: of the products' rows, those from `split` (a multiple of 32) on go to out2
   int split, part;
   const float *alpha;  // on the device; null: 1
   float *sum;          // [rows, cols] or null
   bool begins, keep;   // the first piece of a sum, not the last one
-  bool whole;          // rows of out start on 16 bytes
+  int align, sum_align;
   __device__ __forceinline__ void begin(State &s, const Where &) const { s.alpha = alpha != nullptr ? __ldg(alpha) : 1.0f; }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
-    const int n = cols - col, row = w.row < split ? w.row : w.row - split;
-    if (!w.inside || n <= 0 || row >= part) return;
+    const int top = w.row - w.lane, row = top < split ? top : top - split;
+    const int m = min(32, min(part - row, rows - top)), n = min(32, cols - col);
+    if (m <= 0 || n <= 0) return;
     if (sum != nullptr) {
-      float *acc = sum + (size_t)w.row * (size_t)cols + col;
-      const bool quads = (cols & 3) == 0;
+      float *acc = sum + (size_t)top * (size_t)cols + col;
       if (!begins) {
         float before[32];
-        if (quads && n >= 32) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 q = *reinterpret_cast<const float4 *>(acc + i);
-            before[i] = q.x, before[i + 1] = q.y, before[i + 2] = q.z, before[i + 3] = q.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) before[i] = i < n ? acc[i] : 0.0f;
-        }
+        load_box(w, acc, (size_t)cols, m, n, sum_align, before);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] += before[i];
       }
       if (keep) {
-        store_columns(acc, v, n, quads);
+        store_box(w, acc, (size_t)cols, m, n, sum_align, v);
         return;
       }
     }
-    T *to = (w.row < split ? out : out2) + (size_t)row * (size_t)cols;
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] *= s.alpha;
-    store_columns(to + col, v, n, whole);
+    store_box(w, (top < split ? out : out2) + (size_t)row * (size_t)cols + col, (size_t)cols, m, n, align, v);
   }
   __device__ __forceinline__ void end(State &, const Where &) const {}
 };
@@ -283,6 +418,9 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const T *__restrict__ x, i
     }
   }
 }
+
+// Sums of 32 rows that an epilogue leaves for these rows: of every tile's, inside the matrix or not.
+inline int64_t row_sum_count(int64_t rows, const TileShape &shape) { return (rows + shape.rows() - 1) / shape.rows() * shape.rows() / 32; }
 
 inline unsigned blocks_for(int64_t work, int64_t per_block, int64_t most) {
   return (unsigned)std::min<int64_t>(std::max<int64_t>((work + per_block - 1) / per_block, 1), most);

@@ -10,12 +10,12 @@ namespace dense {
 template <typename T>
 int product_dx(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream) {
   constexpr int kPlanes = Kind<T>::kPlanes;
-  return launch_tiles<kPlanes, false, true>(p, e, tile_columns(p.rows, p.cols, p.k * p.segments, kPlanes, false, sms), sms, stream);
+  return launch_tiles<kPlanes, false, true>(p, e, tile_shape(p.rows, p.cols, p.k * p.segments, kPlanes, false), sms, stream);
 }
 template <typename T>
 int product_dw(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream) {
   constexpr int kPlanes = Kind<T>::kPlanes;
-  return launch_tiles<kPlanes, true, true>(p, e, tile_columns(p.rows, p.cols, p.k, kPlanes, false, sms), sms, stream);
+  return launch_tiles<kPlanes, true, true>(p, e, tile_shape(p.rows, p.cols, p.k, kPlanes, false), sms, stream);
 }
 
 #define HT_DENSE_PRODUCTS(T)                                                                       \

@@ -13,12 +13,18 @@
 // sum loses to rounding).  So the large products leave for registers every 8 instructions (128 values of k) and are added there in
 // fp32; the small ones are 2^-8 of those and stay to the end.
 //
-// A persistent kernel, one CTA per SM, 320 threads:
-//   warp 0      one lane issues the TMA loads (cp.async.bulk.tensor, 128-byte swizzle) into a ring of stages of 64 values of k;
-//   warp 1      allocates tensor memory, and one lane issues tcgen05.mma.kind::f16 (M 128, N up to 256, K 16) and commits
-//               each stage back to the loads and each finished accumulator to the epilogue;
-//   warps 2-9   the epilogue, under the main loop of the next tile (two accumulators): two warps per quarter of the 128 lanes, each
-//               with one half of the columns.
+// A persistent kernel of 320 threads a CTA, one CTA per SM, alone (CTAS = 1, tiles of 128 rows) or in clusters of two that share a
+// tile of 256 rows (CTAS = 2): tcgen05.mma.cta_group::2 reads each CTA's 128 rows of A and half of B's rows from that CTA's shared
+// memory, which halves what a product moves of B into and out of shared memory, the resource that bounds the single form
+// (16384 x 16384 x 1024, bf16: 1110 TFLOP/s alone).
+//   warp 0      one lane issues the TMA loads (cp.async.bulk.tensor, 128-byte swizzle, no multicast) into a ring of stages of 64 values of
+//               k; in a pair both CTAs load their part and their bytes arrive at the first CTA's barrier;
+//   warp 1      allocates tensor memory, and one lane (of the first CTA) issues tcgen05.mma.kind::f16 (M 128 or 256, N up to 256,
+//               K 16) and commits each stage back to the loads and each finished accumulator to the epilogue, of both CTAs;
+//   warps 2-9   the epilogue, under the main loop of the next tile: two warps per quarter of the CTA's 128 lanes, each with one half
+//               of the columns.
+// Tensor memory: two accumulators of 256 columns, used in turn; with three planes one for the large and one for the small products,
+// and the small ones of a block are issued first, so that the large ones' accumulator is read out meanwhile.
 // Tiles are walked in groups of 16 row blocks, rows fastest, so that what the SMs read at one time is shared in L2.
 // Every wait is bounded: when one runs out the kernel flags HT_FLAG_PIPELINE_TIMEOUT, every role stops at its own next wait, the
 // loads wait for their copies in flight, the tensor memory is freed and the kernel returns.
@@ -43,8 +49,9 @@ constexpr int kTileThreads = 320;
 constexpr int kEpilogueWarps = 8;
 constexpr int kChunkBlocks = 2;  // blocks of 64 values of k between two visits of the registers (three planes)
 constexpr int kMostStages = 12;
-constexpr uint32_t kStageBudget = 220 * 1024;
-constexpr size_t kTileSmem = 1024 + kStageBudget + 512;
+constexpr uint32_t kStageBudget = 192 * 1024;
+constexpr uint32_t kBoxBytes = 4096;  // of an epilogue warp: 32 rows of 32 columns on their way to or from memory
+constexpr size_t kTileSmem = 1024 + kStageBudget + kEpilogueWarps * kBoxBytes + 512;
 
 // A 16-bit matrix in device memory, row-major, `pitch` elements from row to row (a multiple of 8, base on 16 bytes); with
 // three planes, `plane` elements apart.
@@ -65,13 +72,20 @@ struct alignas(64) TileArgs {
   int segments;            // 2: the sum over k goes on in a[1], b[1]
   int b_n0, b_k0;          // where B's rows / values of k begin
   int stages;
-  uint32_t a_bytes, stage_bytes;
+  uint32_t a_bytes, stage_bytes;  // of one CTA
+};
+
+// How a product is cut: CTAs that share a tile of 128 rows each, and its columns.
+struct TileShape {
+  int ctas, bn;
+  int rows() const { return 128 * ctas; }
 };
 
 // What an epilogue thread is at: one row of the tile, and one half of its columns.
 struct Where {
   int row;       // of the output
   bool inside;   // row < rows of the output
+  uint32_t box;  // shared memory of the warp
   int m_block, n_block, half, quarter, lane;
 };
 
@@ -93,18 +107,73 @@ __device__ __forceinline__ uint64_t mn_major_descriptor(uint32_t address, uint32
   return desc;
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instruction, uint32_t accumulate) {
+// The warps that issue loads and products run as a whole, and `one` (set in one lane, by elect.sync) predicates the instruction itself:
+// descriptors, addresses and coordinates stay in uniform registers.  In a branch that one lane takes they are moved there for
+// every instruction, and a product of 16 values of k took 240 cycles, whatever its columns, where 256 columns need 128.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-      :
-      : "r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instruction), "r"(accumulate), "r"(0u)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one;
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+template <int CTAS>
+__device__ __forceinline__ void mma_f16(uint32_t one, uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instruction, uint32_t accumulate) {
+  if constexpr (CTAS == 2) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instruction), "r"(accumulate), "r"(one)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instruction), "r"(accumulate), "r"(one)
+        : "memory");
+  }
+}
+
+// Arrives on the barrier (in a pair: on both CTAs') once every tcgen05 operation this thread issued before has completed.
+template <int CTAS>
+__device__ __forceinline__ void mma_commit(uint32_t one, uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+        "h"((uint16_t)3), "r"(one)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one)
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of the first CTA's counterpart of a barrier.
+__device__ __forceinline__ uint32_t of_first_cta(const uint64_t *bar) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_addr(bar)));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // 32 columns of this warp's lanes: issued and waited for in one statement, so that nothing reads a register before it arrives.
@@ -124,30 +193,46 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *map, int col, int row, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(col), "r"(row), "r"(0), "r"(smem_addr(bar))
-      : "memory");
+// global -> this CTA's shared memory, issued by the lane that has `one`; `bar`: the barrier that counts the bytes, in a pair the first
+// CTA's.
+template <int CTAS>
+__device__ __forceinline__ void load_3d(uint32_t one, uint32_t dst, const CUtensorMap *map, int col, int row, uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];\n\t}" ::"r"(dst),
+        "l"(map), "r"(col), "r"(row), "r"(0), "r"(bar), "r"(one)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+        "l"(map), "r"(col), "r"(row), "r"(0), "r"(bar), "r"(one)
+        : "memory");
 }
 
-template <int PLANES, bool A_MN, bool B_MN, class Epilogue>
+template <int CTAS, int PLANES, bool A_MN, bool B_MN, class Epilogue>
 __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ Epilogue epilogue) {
   constexpr bool kPair = Epilogue::kPair;  // the tile's columns are those of two matrices, half and half
   static_assert(!kPair || !B_MN, "a pair's weights have k contiguous");
-  constexpr int kPlanes = PLANES;
   constexpr bool kThree = PLANES == 3;
+  constexpr int kBuffers = kThree ? 1 : 2;  // accumulators that are used in turn
   extern __shared__ __align__(1024) unsigned char tile_smem[];
   unsigned char *base = tile_smem + ((1024u - (smem_addr(tile_smem) & 1023u)) & 1023u);
   const uint32_t stages = smem_addr(base);
-  uint64_t *full = reinterpret_cast<uint64_t *>(base + kStageBudget);  // [stages]
+  uint64_t *full = reinterpret_cast<uint64_t *>(base + kStageBudget + kEpilogueWarps * kBoxBytes);  // [stages]
   uint64_t *empty = full + kMostStages;                                // [stages]
   uint64_t *accumulated = empty + kMostStages;                         // [2] an accumulator is complete
   uint64_t *drained = accumulated + 2;                                 // [2] ... and has been read out
-  uint64_t *drained_small = drained + 2;                               // [2] the second accumulator of three planes
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained_small + 2);
+  uint64_t *drained_small = drained + 2;                               // the small products' accumulator
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained_small + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
+  const int first_tile = (int)blockIdx.x / CTAS, tile_step = (int)gridDim.x / CTAS;
   const int blocks = a.segments * a.k_blocks;
   constexpr uint32_t kColumns = 512;
 
@@ -158,19 +243,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accumulated[b], 1);
-      mbar_init(&drained[b], kEpilogueWarps);
-      mbar_init(&drained_small[b], kEpilogueWarps);
+      mbar_init(&drained[b], kEpilogueWarps * CTAS);
     }
+    mbar_init(drained_small, kEpilogueWarps * CTAS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CTAS == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  auto everybody = [&]() {  // the CTA's threads, or the pair's
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if constexpr (CTAS == 2)
+      cluster_sync();
+    else
+      __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  };
+  everybody();
   const uint32_t tmem = *tmem_slot;
 
   auto give_up = [&]() {
@@ -185,16 +280,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
     mb = g * kGroup + (in - nb * rows);
   };
 
+  // A wait of the whole warp.
+  auto arrived = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
+
   if (warp == 0) {
-    if (lane == 0) {
+    {
+      const uint32_t one = elect_one();
       uint32_t it = 0, s = 0, phase = 1;
       bool ok = true;
-      for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x) {
+      for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
         int mb, nb;
         place(tile, mb, nb);
-        const int m0 = mb * kTileM, n0 = a.b_n0 + nb * (kPair ? a.bn / 2 : a.bn);
+        const int m0 = (mb * CTAS + rank) * kTileM;
+        const int half = a.bn / 2;
+        // a pair of matrices: one each to the CTAs of a pair, both to one alone
+        const int n0 = a.b_n0 + nb * (kPair ? half : a.bn) + (CTAS == 2 && !kPair ? rank * half : 0);
         for (int kb = 0; kb < blocks; ++kb, ++it) {
-          if (!mbar_wait(&empty[s], phase)) {
+          if (!arrived(&empty[s], phase)) {
             give_up();
             ok = false;
             break;
@@ -202,20 +304,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           const int segment = kb >= a.k_blocks ? 1 : 0;
           const int k0 = (kb - segment * a.k_blocks) * kTileK;
           const uint32_t at = stages + s * a.stage_bytes, bt = at + a.a_bytes;
-          mbar_expect_tx(&full[s], a.stage_bytes);
+          const uint32_t bar = CTAS == 2 ? of_first_cta(&full[s]) : smem_addr(&full[s]);
+          if (rank == 0 && one) mbar_expect_tx(&full[s], a.stage_bytes * CTAS);
           const CUtensorMap *am = &a.a[segment], *bm = &a.b[segment];
           if (A_MN) {
-            for (int g = 0; g < kTileM / 64; ++g) load_3d(at + (uint32_t)g * (8192u * kPlanes), am, m0 + 64 * g, k0, &full[s]);
+            for (int g = 0; g < kTileM / 64; ++g) load_3d<CTAS>(one, at + (uint32_t)g * (8192u * PLANES), am, m0 + 64 * g, k0, bar);
           } else {
-            load_3d(at, am, k0, m0, &full[s]);
+            load_3d<CTAS>(one, at, am, k0, m0, bar);
           }
           if (B_MN) {
-            for (int g = 0; g < a.bn / 64; ++g) load_3d(bt + (uint32_t)g * (8192u * kPlanes), bm, n0 + 64 * g, a.b_k0 + k0, &full[s]);
-          } else if (kPair) {  // plane by plane the gate's rows and the value's: what one instruction reads is contiguous
-            load_3d(bt, &a.b[0], k0, n0, &full[s]);
-            load_3d(bt + (uint32_t)(a.bn / 2) * 128u * kPlanes, &a.b[1], k0, n0, &full[s]);
+            for (int g = 0; g < a.bn / (64 * CTAS); ++g) load_3d<CTAS>(one, bt + (uint32_t)g * (8192u * PLANES), bm, n0 + 64 * g, a.b_k0 + k0, bar);
+          } else if (kPair) {
+            load_3d<CTAS>(one, bt, &a.b[rank], k0, n0, bar);
+            if (CTAS == 1) load_3d<CTAS>(one, bt + (uint32_t)half * 128u * PLANES, &a.b[1], k0, n0, bar);
           } else {
-            load_3d(bt, bm, a.b_k0 + k0, n0, &full[s]);
+            load_3d<CTAS>(one, bt, bm, a.b_k0 + k0, n0, bar);
           }
           if (++s == (uint32_t)a.stages) {
             s = 0;
@@ -223,78 +326,89 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           }
         }
       }
-      if (!ok) {  // the copies still in flight arrive before the CTA leaves
-        const uint32_t issued = min(it, (uint32_t)a.stages);
-        for (uint32_t j = 1; j <= issued; ++j) {
-          const uint32_t i = it - j;
-          mbar_wait(&full[i % (uint32_t)a.stages], (i / (uint32_t)a.stages) & 1u, 4096);
-        }
+      // The last use of every stage ends before the CTA leaves: the commits that arrive here (in a pair, from the other CTA), or, where a
+      // wait ran out, the copies still in flight.
+      const uint32_t issued = min(it, (uint32_t)a.stages);
+      for (uint32_t j = 1; j <= issued; ++j) {
+        const uint32_t i = it - j, s = i % (uint32_t)a.stages;
+        mbar_wait(ok ? &empty[s] : &full[s], (i / (uint32_t)a.stages) & 1u, ok ? kMaxSpins : 4096);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0) {
+      const uint32_t one = elect_one();
+      const uint32_t tmem_d = __reduce_or_sync(0xffffffffu, tmem);  // the same in a uniform register
       uint32_t s = 0, phase = 0, chunk = 0, t = 0;
+      // A lane whose wait ran out waits no more, and the warp goes on: the products of what the stages hold are thrown away, and no branch
+      // depends on a wait.
       bool ok = true;
-      const uint32_t a_plane = A_MN ? 8192u : (uint32_t)kTileM * 128u;
-      const uint32_t b_plane = B_MN ? 8192u : (uint32_t)(kPair ? a.bn / 2 : a.bn) * 128u;
-      const uint32_t step_a = A_MN ? 128u : 2u, step_b = B_MN ? 128u : 2u;  // 16 values of k, in units of 16 bytes
-      for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x, ++t) {
-        const uint32_t small = tmem + 256u + (t & 1u) * 128u;
-        uint32_t d = 0;
-        if (kThree && !mbar_wait(&drained_small[t & 1u], ((t >> 1) & 1u) ^ 1u)) {
+      auto wait_here = [&](uint64_t *bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity)) {
+          ok = false;
           give_up();
-          break;
         }
+      };
+      // rows of B in a CTA; two matrices in one CTA lie one after the other, plane by plane
+      const uint32_t b_rows = (uint32_t)(CTAS == 2 || kPair ? a.bn / 2 : a.bn);
+      const uint64_t a_plane = (A_MN ? 8192u : (uint32_t)kTileM * 128u) >> 4, b_plane = (B_MN ? 8192u : b_rows * 128u) >> 4;
+      constexpr uint32_t step_a = A_MN ? 128u : 2u, step_b = B_MN ? 128u : 2u;  // 16 values of k, in units of 16 bytes
+      for (int tile = first_tile; tile < a.tiles; tile += tile_step, ++t) {
+        uint32_t d = tmem_d;
         for (int kb = 0; kb < blocks; ++kb) {
           const bool first = kThree ? kb % kChunkBlocks == 0 : kb == 0;
-          if (first) {
-            if (!mbar_wait(&drained[chunk & 1u], ((chunk >> 1) & 1u) ^ 1u)) {
-              give_up();
-              ok = false;
-              break;
-            }
-            d = tmem + (chunk & 1u) * (kThree ? 128u : 256u);
-          }
-          if (!mbar_wait(&full[s], phase)) {
-            give_up();
-            ok = false;
-            break;
-          }
+          if (kThree && kb == 0) wait_here(drained_small, (t & 1u) ^ 1u);
+          const uint32_t buffer = chunk % kBuffers;
+          auto turn = [&]() {  // the accumulator's previous sum has been read
+            if (!first) return;
+            d = tmem_d + buffer * 256u;
+            wait_here(&drained[buffer], ((chunk / kBuffers) & 1u) ^ 1u);
+          };
+          if (!kThree) turn();
+          wait_here(&full[s], phase);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const int left = a.k - (kb >= a.k_blocks ? kb - a.k_blocks : kb) * kTileK;
           const int steps = left >= kTileK ? 4 : (left + 15) / 16;
           const uint32_t at = stages + s * a.stage_bytes, bt = at + a.a_bytes;
-          const uint64_t da = A_MN ? mn_major_descriptor(at, 8192u * kPlanes) : k_major_descriptor(at);
-          const uint64_t db = B_MN ? mn_major_descriptor(bt, 8192u * kPlanes) : k_major_descriptor(bt);
-          for (int kk = 0; kk < steps; ++kk) {
-            const uint64_t ak = da + (uint64_t)(step_a * (uint32_t)kk), bk = db + (uint64_t)(step_b * (uint32_t)kk);
-            const uint32_t into = !(first && kk == 0);
-            if (!kThree) {
-              mma_f16(d, ak, bk, a.instruction, into);
-            } else {
-              // a pair's planes lie gate by gate and value by value: two instructions of half the columns each
-              constexpr int kParts = kPair ? 2 : 1;
+          const uint64_t da = A_MN ? mn_major_descriptor(at, 8192u * PLANES) : k_major_descriptor(at);
+          const uint64_t db = B_MN ? mn_major_descriptor(bt, 8192u * PLANES) : k_major_descriptor(bt);
+          constexpr int kParts = kThree && kPair && CTAS == 1 ? 2 : 1;  // two matrices in one CTA, three planes: an instruction each
+          auto large = [&](int kk) {
 #pragma unroll
-              for (int part = 0; part < kParts; ++part) {
-                const uint32_t col = kPair ? (uint32_t)part * (uint32_t)(a.bn / 2) : 0u;
-                const uint64_t bp = bk + (uint64_t)((uint32_t)part * ((b_plane * 3u) >> 4));
-                const uint64_t ap = a_plane >> 4, pb = b_plane >> 4;
-                mma_f16(d + col, ak, bp, a.instruction, into);
-                mma_f16(small + col, ak + 2 * ap, bp, a.instruction, !(kb == 0 && kk == 0));
-                mma_f16(small + col, ak, bp + 2 * pb, a.instruction, 1u);
-                mma_f16(small + col, ak + ap, bp + pb, a.instruction, 1u);
-                mma_f16(small + col, ak + ap, bp, a.instruction, 1u);
-                mma_f16(small + col, ak, bp + pb, a.instruction, 1u);
-              }
+            for (int part = 0; part < kParts; ++part)
+              mma_f16<CTAS>(one, d + (uint32_t)part * b_rows, da + (uint64_t)(step_a * (uint32_t)kk),
+                            db + (uint64_t)part * (3u * b_plane) + (uint64_t)(step_b * (uint32_t)kk), a.instruction, kk > 0 || !first);
+          };
+          auto small = [&](int kk) {
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              const uint64_t ak = da + (uint64_t)(step_a * (uint32_t)kk);
+              const uint64_t bk = db + (uint64_t)part * (3u * b_plane) + (uint64_t)(step_b * (uint32_t)kk);
+              const uint32_t to = tmem_d + 256u + (uint32_t)part * b_rows;
+              mma_f16<CTAS>(one, to, ak + 2 * a_plane, bk, a.instruction, kk > 0 || kb > 0);
+              mma_f16<CTAS>(one, to, ak, bk + 2 * b_plane, a.instruction, 1u);
+              mma_f16<CTAS>(one, to, ak + a_plane, bk + b_plane, a.instruction, 1u);
+              mma_f16<CTAS>(one, to, ak + a_plane, bk, a.instruction, 1u);
+              mma_f16<CTAS>(one, to, ak, bk + b_plane, a.instruction, 1u);
             }
+          };
+          if (kThree) {
+            for (int kk = 0; kk < steps; ++kk) small(kk);
+            turn();
+            if (first) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
-          mma_commit(&empty[s]);
+          if (steps == 4) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) large(kk);
+          } else {
+            for (int kk = 0; kk < steps; ++kk) large(kk);
+          }
+          mma_commit<CTAS>(one, smem_addr(&empty[s]));
           if (++s == (uint32_t)a.stages) {
             s = 0;
             phase ^= 1u;
           }
           if (kb == blocks - 1 || (kThree && kb % kChunkBlocks == kChunkBlocks - 1)) {
-            mma_commit(&accumulated[chunk & 1u]);
+            mma_commit<CTAS>(one, smem_addr(&accumulated[buffer]));
             ++chunk;
           }
         }
@@ -303,12 +417,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp may only touch the lanes 32 (warp % 4) ...
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    uint32_t chunk = 0, t = 0;
+    uint32_t chunk = 0;
     const int units = kPair ? a.bn / 128 : a.bn / 64;  // of 32 columns (a pair: 32 of each), for this half
     Where w;
     w.half = half, w.quarter = quarter, w.lane = lane;
+    w.box = stages + kStageBudget + (uint32_t)(warp - 2) * kBoxBytes;
     auto wait_for = [&](uint32_t c) {
-      bool there = mbar_wait(&accumulated[c & 1u], (c >> 1) & 1u);
+      bool there = mbar_wait(&accumulated[c % kBuffers], (c / kBuffers) & 1u);
       if (!there) give_up();
       there = __all_sync(0xffffffffu, there);  // a warp reads tensor memory together or not at all
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -317,10 +432,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
     auto release = [&](uint64_t *bar) {
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
+      if (lane == 0) {
+        if constexpr (CTAS == 2)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(of_first_cta(bar)) : "memory");
+        else
+          mbar_arrive(bar);
+      }
     };
-    for (int tile = (int)blockIdx.x; tile < a.tiles; tile += (int)gridDim.x, ++t) {
-      place(tile, w.m_block, w.n_block);
+    for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
+      int mb;
+      place(tile, mb, w.n_block);
+      w.m_block = mb * CTAS + rank;
       w.row = w.m_block * kTileM + quarter * 32 + lane;
       w.inside = w.row < epilogue.rows;
       typename Epilogue::State state;
@@ -346,50 +468,54 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
         }
         ++chunk;
       } else {
-        // 64 columns a thread at the most (bn <= 128), summed over the chunks of k
-        const int first = half * (units * 32), second = kPair ? a.bn / 2 + first : first + 32;
-        const bool two = kPair || units == 2;
-        float s0[32], s1[32], v[32];
+        // sums over the chunks of k in registers: up to 4 x 32 columns (a pair: 2 x 32 of each matrix, the gate's first)
+        constexpr int kMostUnits = CTAS == 2 ? 4 : 2;
+        float sum[kMostUnits][32];
+        const int parts = kPair ? 2 * units : units;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s0[i] = s1[i] = 0.0f;
+        for (int u = 0; u < kMostUnits; ++u)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[u][i] = 0.0f;
+        auto column = [&](int u) { return kPair ? (u & 1) * (a.bn / 2) + (half * units + (u >> 1)) * 32 : (half * units + u) * 32; };
         bool there = true;
         const int chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
         for (int c = 0; c <= chunks; ++c) {
           if (c < chunks && !(there = wait_for(chunk))) break;
-          const uint32_t acc = lanes + (c < chunks ? (chunk & 1u) * 128u : 256u + (t & 1u) * 128u);
-          tmem_load_32(acc + (uint32_t)first, v);
+          const uint32_t acc = lanes + (c < chunks ? 0u : 256u);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s0[i] += v[i];
-          if (two) {
-            tmem_load_32(acc + (uint32_t)second, v);
+          for (int u = 0; u < kMostUnits; ++u) {
+            if (u >= parts) break;
+            float v[32];
+            tmem_load_32(acc + (uint32_t)column(u), v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s1[i] += v[i];
+            for (int i = 0; i < 32; ++i) sum[u][i] += v[i];
           }
-          if (c < chunks) {
-            release(&drained[chunk & 1u]);
-            ++chunk;
-          } else {
-            release(&drained_small[t & 1u]);
-          }
+          if (c < chunks) ++chunk;
+          release(c < chunks ? &drained[0] : drained_small);
         }
         if (!there) break;
         epilogue.begin(state, w);
-        if constexpr (kPair) {
-          epilogue.unit(state, w, col0 + first, s0, s1);
-        } else {
-          epilogue.unit(state, w, col0 + first, s0);
-          if (two) epilogue.unit(state, w, col0 + second, s1);
+#pragma unroll
+        for (int u = 0; u < kMostUnits; ++u) {
+          if (u >= parts) break;
+          if constexpr (kPair) {
+            if ((u & 1) == 0) epilogue.unit(state, w, col0 + column(u), sum[u], sum[u + 1]);
+          } else {
+            epilogue.unit(state, w, col0 + column(u), sum[u]);
+          }
         }
       }
       epilogue.end(state, w);
     }
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  everybody();
   if (warp == 1) {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+    if constexpr (CTAS == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
   }
+  if constexpr (CTAS == 2) cluster_sync();
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -425,41 +551,66 @@ inline int sm_count(int *sms) {
   return HT_OK;
 }
 
-// Columns of a tile: the width with which the SMs are done first.  A step of 16 values of k takes the tensor core bn / 2 cycles, and its
-// operands (128 + bn rows of 32 bytes) leave shared memory at 128 bytes a cycle; a tile costs about 2000 cycles besides.
-inline int tile_columns(int64_t rows, int64_t cols, int64_t k, int planes, bool pair, int sms) {
-  const int64_t m_blocks = (rows + kTileM - 1) / kTileM;
-  const int most = planes == 3 ? 128 : 256, step = pair ? 128 : 64;
-  int best = most;
+// How to cut a product: the shape with which the SMs are done first.  Cycles of a step of 16 values of k, measured: a pair of CTAs with 256
+// columns 140, with 128 columns 100 (shared memory bounds it); one CTA with 256 columns 240, with 128 220, with 64 200 (three planes: 6 of
+// those, of 128 columns at the most alone).  A tile costs about 2000 cycles besides.
+inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, bool pair) {
+  constexpr int kPlanSMs = 148;
+  TileShape best = {1, 128};
   double least = 0.0;
-  for (int bn = most; bn >= step; bn -= step) {
-    const int64_t n = pair ? bn / 2 : bn, tiles = m_blocks * ((cols + n - 1) / n);
-    const double rounds = (double)((tiles + sms - 1) / sms);
-    const double cycles = (planes == 3 ? 6.0 : 1.0) * (double)((k + 15) / 16) * std::max(bn / 2.0, 32.0 + bn / 4.0) + 2000.0;
-    if (bn == most || rounds * cycles < least * 0.999) {
-      best = bn;
-      least = rounds * cycles;
+  for (int ctas = 2; ctas >= 1; --ctas)
+    for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 64) {
+      if (bn % (ctas == 2 || pair ? 128 : 64) != 0) continue;
+      const int64_t n = pair ? bn / 2 : bn;
+      const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n);
+      const double rounds = (double)((tiles * ctas + kPlanSMs - 1) / kPlanSMs);
+      const double step = ctas == 2 ? (bn == 256 ? 140.0 : 100.0) : 180.0 + 0.235 * bn;
+      const double cycles = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k + 15) / 16) * step + 2000.0);
+      if (least == 0.0 || cycles < least * 0.999) {
+        best = {ctas, bn};
+        least = cycles;
+      }
     }
-  }
   return best;
 }
 
+template <int CTAS, int PLANES, bool A_MN, bool B_MN, class Epilogue>
+int launch_shape(const TileArgs &a, const Epilogue &epilogue, int sms, cudaStream_t stream) {
+  auto kernel = dense_tile_kernel<CTAS, PLANES, A_MN, B_MN, Epilogue>;
+  HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem));
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(CTAS * std::min(a.tiles, std::max(sms / CTAS, 1))));
+  config.blockDim = dim3(kTileThreads);
+  config.dynamicSmemBytes = kTileSmem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = CTAS;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = CTAS > 1 ? 1 : 0;
+  HT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a, epilogue));
+  HT_CHECK_LAUNCH();
+  return HT_OK;
+}
+
 template <int PLANES, bool A_MN, bool B_MN, class Epilogue>
-int launch_tiles(const TileProblem &p, const Epilogue &epilogue, int bn, int sms, cudaStream_t stream) {
+int launch_tiles(const TileProblem &p, const Epilogue &epilogue, const TileShape &shape, int sms, cudaStream_t stream) {
   constexpr bool kPair = Epilogue::kPair;
   if (p.rows < 1 || p.cols < 1 || p.k < 1) return HT_ERR_INVALID_ARGUMENT;
   TileArgs a = {};
-  const int b_rows = kPair ? bn / 2 : bn;
+  const int bn = shape.bn, columns = kPair ? bn / 2 : bn;  // of the output
+  const int b_rows = kPair || shape.ctas == 2 ? bn / 2 : bn;   // of one load
   for (int s = 0; s < p.segments || (kPair && s < 2); ++s) {
     if (s < p.segments && !encode_matrix_16(&a.a[s], p.a[s], A_MN ? kTileK : kTileM)) return HT_ERR_UNSUPPORTED;
     if (!encode_matrix_16(&a.b[s], p.b[s], B_MN ? kTileK : b_rows)) return HT_ERR_UNSUPPORTED;
   }
-  const int64_t m_blocks = (p.rows + kTileM - 1) / kTileM, n_blocks = (p.cols + b_rows - 1) / b_rows;
+  const int64_t m_blocks = (p.rows + shape.rows() - 1) / shape.rows(), n_blocks = (p.cols + columns - 1) / columns;
   if (m_blocks * n_blocks > 0x3fffffff || p.k > 0x3fffffff) return HT_ERR_UNSUPPORTED;
   a.status_word = p.status_word;
-  const int n = PLANES == 3 ? b_rows : bn;  // of one instruction
+  const int n = PLANES == 3 && kPair && shape.ctas == 1 ? bn / 2 : bn;  // columns of one instruction
   a.instruction = (1u << 4) | ((p.f16 ? 0u : 1u) << 7) | ((p.f16 ? 0u : 1u) << 10) | ((A_MN ? 1u : 0u) << 15) |
-                  ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+                  ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(shape.rows() >> 4) << 24);
   a.m_blocks = (int)m_blocks;
   a.n_blocks = (int)n_blocks;
   a.tiles = (int)(m_blocks * n_blocks);
@@ -470,13 +621,9 @@ int launch_tiles(const TileProblem &p, const Epilogue &epilogue, int bn, int sms
   a.b_n0 = (int)p.b_n0;
   a.b_k0 = (int)p.b_k0;
   a.a_bytes = (uint32_t)kTileM * 128u * PLANES;
-  a.stage_bytes = a.a_bytes + (uint32_t)bn * 128u * PLANES;
+  a.stage_bytes = a.a_bytes + (uint32_t)(bn / shape.ctas) * 128u * PLANES;
   a.stages = (int)std::min<uint32_t>(kStageBudget / a.stage_bytes, kMostStages);
-  auto kernel = dense_tile_kernel<PLANES, A_MN, B_MN, Epilogue>;
-  HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem));
-  kernel<<<(unsigned)std::min(a.tiles, std::max(sms, 1)), kTileThreads, kTileSmem, stream>>>(a, epilogue);
-  HT_CHECK_LAUNCH();
-  return HT_OK;
+  return shape.ctas == 2 ? launch_shape<2, PLANES, A_MN, B_MN>(a, epilogue, sms, stream) : launch_shape<1, PLANES, A_MN, B_MN>(a, epilogue, sms, stream);
 }
 
 }  // namespace dense

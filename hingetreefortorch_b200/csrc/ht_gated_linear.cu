@@ -51,7 +51,7 @@ template <typename T>
 __device__ __forceinline__ void add_bias(const T *bias, int col, int n, float (&v)[32]) {
   if (bias == nullptr) return;
   float b[32];
-  load_columns(bias + col, b, n, true);
+  load_columns(bias + col, b, n);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] += b[i];
 }
@@ -63,8 +63,8 @@ struct GatedEpilogue {
   struct State {};
   int rows, cols, act;
   const T *bg, *bv;
-  T *h;        // [rows, cols]
-  bool whole;  // rows of h start on 16 bytes
+  T *h;  // [rows, cols]
+  int align;
   __device__ __forceinline__ void begin(State &, const Where &) const {}
   __device__ __forceinline__ void unit(State &, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
     const int n = cols - col;
@@ -75,7 +75,8 @@ struct GatedEpilogue {
     activate<kExact, false>(act, a, g, g);
 #pragma unroll
     for (int i = 0; i < 32; ++i) g[i] *= u[i];
-    if (w.inside) store_columns(h + (size_t)w.row * (size_t)cols + col, g, n, whole);
+    const int top = w.row - w.lane;
+    if (top < rows) store_box(w, h + (size_t)top * (size_t)cols + col, (size_t)cols, min(32, rows - top), min(32, n), align, g);
   }
   __device__ __forceinline__ void end(State &, const Where &) const {}
 };
@@ -97,12 +98,12 @@ struct GatedGradEpilogue {
   int rows, cols, act, first, outputs;  // the piece: outputs first .. first + cols - 1
   const T *bg, *bv;
   const T *dh;          // [rows, outputs]
-  bool whole;           // rows of dh start on 16 bytes
+  int align;
   const uint32_t *top;  // fp16: dh is divided by this power of two; else null
   typename Kind<T>::Operand *g;  // [planes][rows][2 pitch]: da, then du
   int pitch;
   size_t plane;
-  float *row_sums;  // [4 m_blocks][2 pitch] or null
+  float *row_sums;  // [row_sum_count][2 pitch] or null
   __device__ __forceinline__ void begin(State &s, const Where &) const { s.scale = top != nullptr ? 1.0f / scale_of(top) : 1.0f; }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
     const int n = cols - col;
@@ -111,7 +112,8 @@ struct GatedGradEpilogue {
     add_bias(bv, first + col, n, u);
     float act_a[32], slope[32], dh_[32];
     activate<kExact, true>(act, a, act_a, slope);
-    load_columns(dh + (size_t)(w.inside ? w.row : 0) * (size_t)outputs + first + col, dh_, n, whole);
+    const int top = w.row - w.lane;
+    if (top < rows) load_box(w, dh + (size_t)top * (size_t)outputs + first + col, (size_t)outputs, min(32, rows - top), min(32, n), align, dh_);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float d = dh_[i] * s.scale;
@@ -149,7 +151,6 @@ __global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__
 }
 __global__ void scale_kernel(const uint32_t *top, float *alpha) { *alpha = scale_of(top); }
 
-constexpr int kPlanSMs = 148;  // what tiles and workspaces are planned for
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // da and du of one piece, unless the caller sets less
 
 int screen(const ht_dense_problem *p) {
@@ -183,7 +184,7 @@ struct Plan {
       top = arena.take<uint32_t>(1);
       alpha = arena.take<float>(1);
       sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
-      row_sums = has_bias ? arena.take<float>((p.rows + kTileM - 1) / kTileM * 4 * 2 * pitch) : nullptr;
+      row_sums = has_bias ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * 2 * pitch) : nullptr;
     }
     bytes = arena.used;
   }
@@ -211,8 +212,8 @@ int forward(const ht_dense_problem &p, const void *x, const void *wg, const void
   t.f16 = p.dtype == HT_DTYPE_F16;
   t.status_word = status_word;
   GatedEpilogue<T> e = {(int)p.rows, (int)p.outputs, p.activation, static_cast<const T *>(bg), static_cast<const T *>(bv), static_cast<T *>(h),
-                        p.outputs * (int64_t)sizeof(T) % 16 == 0};
-  return launch_tiles<Kind<T>::kPlanes, false, false>(t, e, tile_columns(p.rows, p.outputs, p.features, Kind<T>::kPlanes, true, kPlanSMs), sms, stream);
+                        row_alignment(h, p.outputs * (int64_t)sizeof(T))};
+  return launch_tiles<Kind<T>::kPlanes, false, false>(t, e, tile_shape(p.rows, p.outputs, p.features, Kind<T>::kPlanes, true), sms, stream);
 }
 
 struct Gradients {
@@ -247,7 +248,6 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
   }
   const float *alpha = scaled ? plan.alpha : nullptr;
   constexpr int kPlanes = Kind<T>::kPlanes;
-  const bool whole = p.features * (int64_t)sizeof(T) % 16 == 0;
   const size_t plane = (size_t)(p.rows * 2 * plan.pitch);
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
     const int64_t count = std::min(plan.piece, p.outputs - first);
@@ -261,15 +261,16 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
     GatedGradEpilogue<T> e = {};
     e.rows = (int)p.rows, e.cols = (int)count, e.act = p.activation, e.first = (int)first, e.outputs = (int)p.outputs;
     e.bg = static_cast<const T *>(bg), e.bv = static_cast<const T *>(bv), e.dh = static_cast<const T *>(dh);
-    e.whole = p.outputs * (int64_t)sizeof(T) % 16 == 0;
+    e.align = row_alignment(e.dh, p.outputs * (int64_t)sizeof(T));
     e.top = scaled ? plan.top : nullptr;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = plane, e.row_sums = plan.row_sums;
-    if ((rc = launch_tiles<kPlanes, false, false>(t, e, tile_columns(p.rows, count, p.features, kPlanes, true, kPlanSMs), sms, stream)) != HT_OK) return rc;
+    const TileShape shape = tile_shape(p.rows, count, p.features, kPlanes, true);
+    if ((rc = launch_tiles<kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
     StoreEpilogue<T> store = {};
     store.alpha = alpha;
     store.cols = (int)p.features;
-    store.whole = whole;
     store.split = 0x7fffffff;
+    store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));
     Matrix g;
     g.rows = p.rows, g.pitch = 2 * plan.pitch, g.planes = kPlanes, g.plane = (int64_t)plane;
     if (out.dx != nullptr) {
@@ -280,7 +281,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
       q.segments = 2;
       q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = first;
       store.rows = store.part = (int)p.rows;
-      store.out = static_cast<T *>(out.dx);
+      store.out = static_cast<T *>(out.dx), store.align = row_alignment(store.out, p.features * (int64_t)sizeof(T));
       store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
       if ((rc = product_dx<T>(q, store, sms, stream)) != HT_OK) return rc;
     }
@@ -298,10 +299,11 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
       store.split = both ? (int)plan.pitch : 0x7fffffff;
       store.out = (dwg != nullptr ? dwg : dwv) + (size_t)first * (size_t)p.features;
       store.out2 = both ? dwv + (size_t)first * (size_t)p.features : nullptr;
+      store.align = std::min(row_alignment(dwg, p.features * (int64_t)sizeof(T)), row_alignment(dwv, p.features * (int64_t)sizeof(T)));
       store.sum = nullptr, store.keep = false;
       if ((rc = product_dw<T>(q, store, sms, stream)) != HT_OK) return rc;
     }
-    const int64_t blocks = (p.rows + kTileM - 1) / kTileM * 4;
+    const int64_t blocks = row_sum_count(p.rows, shape);
     if (dbg != nullptr && (rc = column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, alpha, dbg + first, stream)) != HT_OK) return rc;
     if (dbv != nullptr && (rc = column_sums<T>(plan.row_sums + plan.pitch, blocks, 2 * plan.pitch, count, alpha, dbv + first, stream)) != HT_OK) return rc;
   }
