@@ -15,7 +15,7 @@
 // g is rounded to the operands' 16 bits: 2^-9 (bf16) of a term that enters sums, below what rounding the sums themselves
 // costs; for fp16 it is scaled by 2^14 first, so that probabilities down to 4e-9 are normal numbers; for fp32 it is split
 // into planes like x and w.
-#include "ht_dense.cuh"
+#include "ht_dense_rows.cuh"
 
 namespace ht {
 namespace dense {
@@ -52,7 +52,8 @@ struct LossEpilogue {
   int rows, cols;
   const T *bias;
   const int64_t *target;
-  float2 *partial;      // [2 n_blocks][rows]
+  float2 *partial;      // [rows][slots], slots = 2 n_blocks
+  int slots;
   float *target_score;  // [rows]
   __device__ __forceinline__ void begin(State &s, const Where &w) const {
     s.m = -INFINITY, s.l = 0.0f, s.target = -1;
@@ -98,7 +99,7 @@ struct LossEpilogue {
     s.m = top;
   }
   __device__ __forceinline__ void end(State &s, const Where &w) const {
-    if (w.inside) partial[(size_t)(w.n_block * 2 + w.half) * (size_t)rows + w.row] = make_float2(s.m, s.l);
+    if (w.inside) partial[(size_t)w.row * (size_t)slots + (size_t)(w.n_block * 2 + w.half)] = make_float2(s.m, s.l);
   }
 };
 
@@ -145,25 +146,87 @@ struct LossGradEpilogue {
   __device__ __forceinline__ void end(State &, const Where &) const {}
 };
 
-// Joins the pieces of every row: 32 rows a block, 8 strands of pieces a row, joined in order.  stats[row] = (m, l); the row's
-// loss to `loss`.  A row whose target is no class: loss NaN and a flag.
+// The same for few rows: a lane's scores are those of two rows a tile of 8.
+template <typename T>
+struct FewLossEpilogue {
+  static constexpr bool kPair = false;
+  template <int NT>
+  struct State {
+    float m[NT][2], l[NT][2];
+  };
+  int rows, slots;
+  const T *bias;
+  const int64_t *target;
+  float2 *partial;
+  float *target_score;
+  template <typename S>
+  __device__ __forceinline__ void begin(S &s) const {
+    for (auto &m : s.m) m[0] = m[1] = -INFINITY;
+    for (auto &l : s.l) l[0] = l[1] = 0.0f;
+  }
+  template <int NT>
+  __device__ __forceinline__ void values(State<NT> &s, int n, int row, int o, int outputs, const float (&c)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (row + i >= rows) continue;
+      const int64_t t = __ldg(target + row + i);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = o + 8 * h;
+        if (at >= outputs) continue;
+        const float v = c[2 * h + i] + (bias != nullptr ? to_float(bias[at]) : 0.0f);
+        if (t == at) target_score[row + i] = v;
+        const float top = fmaxf(s.m[n][i], v), m = top == -INFINITY ? 0.0f : top;
+        s.l[n][i] = s.l[n][i] * exp2_fast((s.m[n][i] - m) * kLog2e) + exp2_fast((v - m) * kLog2e);
+        s.m[n][i] = top;
+      }
+    }
+  }
+  template <int NT>
+  __device__ __forceinline__ void end(State<NT> &s, int row0, int lane) const {
+    // the lanes with the same rows, then (each warp has its own outputs) the warps: a block's scores are one piece
+    __shared__ float2 pieces[kFewWarps][8 * NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          const float m = __shfl_xor_sync(0xffffffffu, s.m[n][i], d), l = __shfl_xor_sync(0xffffffffu, s.l[n][i], d);
+          join(s.m[n][i], s.l[n][i], m, l);
+        }
+        if (lane < 4) pieces[threadIdx.x >> 5][8 * n + 2 * lane + i] = make_float2(s.m[n][i], s.l[n][i]);
+      }
+    __syncthreads();
+    if (threadIdx.x >= 8 * NT || row0 + (int)threadIdx.x >= rows) return;
+    float2 all = pieces[0][threadIdx.x];
+    for (int i = 1; i < kFewWarps; ++i) join(all.x, all.y, pieces[i][threadIdx.x].x, pieces[i][threadIdx.x].y);
+    partial[(size_t)(row0 + (int)threadIdx.x) * (size_t)slots + blockIdx.x] = all;
+  }
+};
+
+// Joins the pieces of every row, a warp each, in a fixed order: stats[row] = (m, l), the row's loss to `loss`.  A row whose target is
+// no class: loss NaN and a flag.
 __global__ void __launch_bounds__(256) join_rows_kernel(const float2 *__restrict__ partial, int slots, const float *__restrict__ target_score,
                                                         const int64_t *__restrict__ target, int64_t ignore, int64_t rows, int64_t classes,
                                                         float2 *__restrict__ stats, float *__restrict__ loss, uint32_t *status_word) {
-  __shared__ float2 strand[8][33];
-  const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+  after_previous_kernel();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
   float m = -INFINITY, l = 0.0f;
-  if (row < rows)
-    for (int s = y; s < slots; s += 8) {
-      const float2 q = __ldg(partial + (size_t)s * (size_t)rows + row);
-      join(m, l, q.x, q.y);
-    }
-  strand[y][lane] = make_float2(m, l);
-  __syncthreads();
-  if (y != 0 || row >= rows) return;
+  const float2 *pieces = partial + (size_t)row * (size_t)slots;
+#pragma unroll 4
+  for (int s = lane; s < slots; s += 32) {
+    const float2 q = __ldg(pieces + s);
+    join(m, l, q.x, q.y);
+  }
 #pragma unroll
-  for (int i = 1; i < 8; ++i) join(m, l, strand[i][lane].x, strand[i][lane].y);
+  for (int d = 16; d > 0; d >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
+    join(m, l, m2, l2);
+  }
+  if (lane != 0) return;
   if (stats != nullptr) stats[row] = make_float2(m, l);
   const int64_t t = target[row];
   float result = 0.0f;
@@ -181,6 +244,7 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const float2 *__restrict
 // Sum or mean of the rows' losses in fp64, strand by strand in a fixed order; summary = the number of rows that count.
 __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float *__restrict__ row_loss, const int64_t *__restrict__ target, int64_t ignore,
                                                            int64_t rows, int mean, float *__restrict__ loss, float *__restrict__ summary) {
+  after_previous_kernel();
   __shared__ double sums[32];
   __shared__ long long counts[32];
   double sum = 0.0;
@@ -205,6 +269,7 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(const float *__restri
 
 // The power of two at or below the largest |g|, over `unit`: what gradients of single rows are scaled by.
 __global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict__ grad, int64_t rows, float unit, float *__restrict__ alpha) {
+  after_previous_kernel();
   __shared__ uint32_t tops[32];
   uint32_t top = 0;
   for (int64_t r = threadIdx.x; r < rows; r += 1024) top = max(top, __float_as_uint(fabsf(grad[r])));
@@ -224,6 +289,7 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict
 __global__ void __launch_bounds__(256) row_grad_kernel(const float2 *__restrict__ stats, const float *__restrict__ summary, const int64_t *__restrict__ target,
                                                        int64_t ignore, int64_t rows, int64_t classes, const float *__restrict__ grad, int reduction,
                                                        float unit, RowGrad *__restrict__ row_grad, float *__restrict__ alpha) {
+  after_previous_kernel();
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (row == 0 && reduction != HT_REDUCTION_NONE) {
     const float count = summary[0];
@@ -254,6 +320,8 @@ int screen(const ht_dense_problem *p) {
 
 template <typename T>
 struct ForwardPlan {
+  bool few;
+  FewPlan few_plan;
   Operand<T> x, w;
   TileShape shape;
   int slots;
@@ -262,10 +330,13 @@ struct ForwardPlan {
   size_t bytes;
   ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, void *ws) {
     Arena arena(ws);
-    x.set(arena, xp, p.rows, p.features, p.x_stride);
-    w.set(arena, wp, p.outputs, p.features, p.features);
+    few = few_rows<T>(p.rows, p.features, p.outputs, false, &few_plan);
+    if (!few) {
+      x.set(arena, xp, p.rows, p.features, p.x_stride);
+      w.set(arena, wp, p.outputs, p.features, p.features);
+    }
     shape = tile_shape(p.rows, p.outputs, p.features, Kind<T>::kPlanes, false);
-    slots = (int)(2 * ((p.outputs + shape.bn - 1) / shape.bn));
+    slots = few ? few_plan.blocks : (int)(2 * ((p.outputs + shape.bn - 1) / shape.bn));
     partial = arena.take<float2>((int64_t)slots * p.rows);
     target_score = arena.take<float>(p.rows);
     row_loss = arena.take<float>(p.rows);
@@ -281,25 +352,29 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
   int sms = 0, rc;
   float *row_loss = reduction == HT_REDUCTION_NONE ? loss : plan.row_loss;
   if (p.rows > 0) {
-    if ((rc = sm_count(&sms)) != HT_OK) return rc;
-    if ((rc = plan.x.lay_out(stream)) != HT_OK) return rc;
-    if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
-    TileProblem t;
-    t.a[0] = plan.x.m;
-    t.b[0] = plan.w.m;
-    t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
-    t.f16 = p.dtype == HT_DTYPE_F16;
-    t.status_word = status_word;
-    LossEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), target, plan.partial, plan.target_score};
-    if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, plan.shape, sms, stream)) != HT_OK) return rc;
-    join_rows_kernel<<<(unsigned)((p.rows + 31) / 32), 256, 0, stream>>>(plan.partial, plan.slots, plan.target_score, target, ignore, p.rows,
-                                                                       p.outputs, reinterpret_cast<float2 *>(stats), row_loss, status_word);
-    HT_CHECK_LAUNCH();
+    if (plan.few) {
+      const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(w), nullptr}, p.x_stride, (int)p.rows, (int)p.features, (int)p.outputs};
+      const FewLossEpilogue<T> e = {(int)p.rows, plan.slots, static_cast<const T *>(bias), target, plan.partial, plan.target_score};
+      if ((rc = launch_few(a, e, plan.few_plan, stream)) != HT_OK) return rc;
+    } else {
+      if ((rc = sm_count(&sms)) != HT_OK) return rc;
+      if ((rc = plan.x.lay_out(stream)) != HT_OK) return rc;
+      if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
+      TileProblem t;
+      t.a[0] = plan.x.m;
+      t.b[0] = plan.w.m;
+      t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
+      t.f16 = p.dtype == HT_DTYPE_F16;
+      t.status_word = status_word;
+      const LossEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), target, plan.partial, plan.slots, plan.target_score};
+      if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, plan.shape, sms, stream)) != HT_OK) return rc;
+    }
+    HT_TRY(launch_next(join_rows_kernel, dim3((unsigned)((p.rows + 7) / 8)), 256, 0, stream, 1, plan.partial, plan.slots, plan.target_score, target, ignore, p.rows,
+                                                                       p.outputs, reinterpret_cast<float2 *>(stats), row_loss, status_word));
   }
   if (reduction != HT_REDUCTION_NONE) {
-    reduce_loss_kernel<<<1, 1024, 0, stream>>>(row_loss, target, ignore, p.rows, reduction == HT_REDUCTION_MEAN, loss,
-                                               stats == nullptr ? nullptr : stats + 2 * p.rows);
-    HT_CHECK_LAUNCH();
+    HT_TRY(launch_next(reduce_loss_kernel, dim3(1), 1024, 0, stream, 1, row_loss, target, ignore, p.rows, reduction == HT_REDUCTION_MEAN, loss,
+                                               stats == nullptr ? nullptr : stats + 2 * p.rows));
   }
   return HT_OK;
 }
@@ -350,12 +425,10 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
   if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
   const float unit = p.dtype == HT_DTYPE_F16 ? 16384.0f : 1.0f;
   if (reduction == HT_REDUCTION_NONE) {
-    row_scale_kernel<<<1, 1024, 0, stream>>>(grad, p.rows, unit, plan.alpha);
-    HT_CHECK_LAUNCH();
+    HT_TRY(launch_next(row_scale_kernel, dim3(1), 1024, 0, stream, 1, grad, p.rows, unit, plan.alpha));
   }
-  row_grad_kernel<<<(unsigned)((p.rows + 255) / 256), 256, 0, stream>>>(reinterpret_cast<const float2 *>(stats), stats + 2 * p.rows, target, ignore,
-                                                                       p.rows, p.outputs, grad, reduction, unit, plan.row_grad, plan.alpha);
-  HT_CHECK_LAUNCH();
+  HT_TRY(launch_next(row_grad_kernel, dim3((unsigned)((p.rows + 255) / 256)), 256, 0, stream, 1, reinterpret_cast<const float2 *>(stats), stats + 2 * p.rows, target, ignore,
+                                                                       p.rows, p.outputs, grad, reduction, unit, plan.row_grad, plan.alpha));
   constexpr int kPlanes = Kind<T>::kPlanes;
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
     const int64_t count = std::min(plan.piece, p.outputs - first);

@@ -382,6 +382,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t stride, int64_t pitch,
                                                       int64_t plane, typename Kind<T>::Operand *__restrict__ copy,
                                                       const int64_t *__restrict__ target, int64_t ignore, bool whole) {
+  after_previous_kernel();
   const int64_t per_row = pitch / 8, n = rows * per_row;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / per_row, c = (i - r * per_row) * 8;
@@ -431,8 +432,7 @@ int Operand<T>::lay_out(cudaStream_t stream) const {
   if (copy == nullptr || m.rows == 0) return HT_OK;
   const bool whole = (reinterpret_cast<uintptr_t>(source) & 15u) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
   const int64_t work = m.rows * (m.pitch / 8);
-  lay_out_kernel<T><<<blocks_for(work, 256, 148 * 16), 256, 0, stream>>>(source, m.rows, m.cols, stride, m.pitch, m.plane, copy, target, ignore, whole);
-  HT_CHECK_LAUNCH();
+  HT_TRY(launch_next(lay_out_kernel<T>, dim3(blocks_for(work, 256, 148 * 16)), 256, 0, stream, 1, source, m.rows, m.cols, stride, m.pitch, m.plane, copy, target, ignore, whole));
   return HT_OK;
 }
 
@@ -441,6 +441,7 @@ int Operand<T>::lay_out(cudaStream_t stream) const {
 template <typename T>
 __global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols,
                                                           const float *__restrict__ alpha, T *__restrict__ out) {
+  after_previous_kernel();
   __shared__ float strand[8][33];
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
@@ -458,8 +459,7 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float *__restric
 
 template <typename T>
 int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols, const float *alpha, T *out, cudaStream_t stream) {
-  column_sums_kernel<T><<<(unsigned)((cols + 31) / 32), 256, 0, stream>>>(partial, rows, pitch, cols, alpha, out);
-  HT_CHECK_LAUNCH();
+  HT_TRY(launch_next(column_sums_kernel<T>, dim3((unsigned)((cols + 31) / 32)), 256, 0, stream, 1, partial, rows, pitch, cols, alpha, out));
   return HT_OK;
 }
 

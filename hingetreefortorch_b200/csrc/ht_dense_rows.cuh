@@ -1,0 +1,250 @@
+// The dense layers for few rows (answers to single samples, small batches): every weight is read once, straight into registers.
+//
+// A warp takes 16 rows of the weights (of a pair: 8 of each matrix) as one operand of mma.sync and up to 8 NT rows of x, which lie in shared
+// memory, as the other.  A sum of products does not mind in which order its terms come, so a lane's share of k is 16 contiguous bytes
+// of a row, not what the instruction's layout spreads over it: whole sectors are read, and a lane fetches what it uses itself, into a ring of 8
+// steps of its own in shared memory (cp.async), across the ends of rows.  128 KB an SM are then in flight; with the loads of 4 steps in registers
+// instead, 205 MB of fp32 weights took 73 us.
+// fp32 values are taken as two TF32 numbers (x = x0 + x1, 22 bits and a sign) and the products x0 w0 + x0 w1 + x1 w0, summed 4 steps at a time
+// in a fresh accumulator and in fp32 from there on (the tensor core truncates when it adds).
+// With few weights several warps of a block share 16 rows and take k in turn.
+// What bounds it: the weights' bytes; the launch with few of them.
+#pragma once
+
+#include "ht_dense.cuh"
+
+namespace ht {
+namespace dense {
+
+constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;
+constexpr int kFewRing = 8;  // steps of k in flight
+constexpr uint32_t kFewRingBytes = kFewWarps * kFewRing * 1024;
+constexpr int64_t kFewMostBytes = 224 * 1024 - (int64_t)kFewRingBytes;  // of x in shared memory, and of the warps' sums
+
+template <typename T>
+struct FewArgs {
+  const T *x, *w[2];
+  int64_t x_stride;
+  int rows, features, outputs;
+  int pitch;     // bytes of a row of x in shared memory: 64 more than a multiple of 128, so that 8 rows of 64 bytes meet in no bank
+  bool x_whole;  // rows of x start on 16 bytes
+  int split;     // warps that share 16 rows of the weights: a power of two
+};
+
+template <typename T>
+__device__ __forceinline__ void mma_few(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, float>::value)
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// v = high + low: high is v rounded to 11 bits (in integers: the conversion instruction runs at an eighth of their rate and bound the kernel,
+// 70 us for 205 MB of weights), low the rest, of which the tensor core drops what is below 2^-23 of v.
+__device__ __forceinline__ void split_tf32(uint32_t v, uint32_t &high, uint32_t &low) {
+  high = (v + 0x1000u) & 0xffffe000u;
+  low = __float_as_uint(__uint_as_float(v) - __uint_as_float(high));
+}
+
+// A lane's 16 bytes of a row from place `k` on, zeros behind its end, value by value.
+template <typename T>
+__device__ __forceinline__ uint4 load_values(const T *row, int k, int features) {
+  constexpr int kValues = 16 / (int)sizeof(T);
+  T t[kValues];
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) t[j] = k + j < features ? row[k + j] : from_float<T>(0.0f);
+  return *reinterpret_cast<uint4 *>(t);
+}
+// The same into shared memory, without waiting where the row starts on 16 bytes (FULL).
+template <typename T, bool FULL>
+__device__ __forceinline__ void fetch_values(uint32_t to, const T *row, int k, int features) {
+  if constexpr (FULL) {
+    const int bytes = k < features ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row + (k < features ? k : 0)), "r"(bytes) : "memory");
+  } else {
+    const uint4 q = load_values(row, k, features);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+  }
+}
+
+template <typename T, int NT, bool FULL, class Epilogue>
+__global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<T> a, const Epilogue epilogue) {
+  constexpr bool kPair = Epilogue::kPair;
+  constexpr bool kFloat = std::is_same<T, float>::value;
+  constexpr int kValues = 16 / (int)sizeof(T), kStep = 4 * kValues;  // of k: a lane's, a warp's
+  constexpr int kOutputs = kPair ? 8 : 16;
+  extern __shared__ __align__(128) unsigned char few_smem[];  // the rings, x, then (split) the warps' sums
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  const int row0 = (int)blockIdx.y * (8 * NT), held = min(8 * NT, a.rows - row0);
+  const int steps = (a.features + kStep - 1) / kStep;
+  const int groups = (a.outputs + kOutputs - 1) / kOutputs;
+  const int part = warp % a.split;
+  // this warp's groups: neighbours go to different blocks, so that every SM reads as much
+  const int first = (warp / a.split) * (int)gridDim.x + (int)blockIdx.x, stride = kFewWarps / a.split * (int)gridDim.x;
+  const int own = part < steps ? (steps - part + a.split - 1) / a.split : 0;  // steps of this warp in a group
+  const uint32_t ring = smem_addr(few_smem) + (uint32_t)(warp * kFewRing) * 1024u + (uint32_t)lane * 16u;
+
+  // What is fetched next: step `fetch_i` of this warp's in the group `fetch_group`.
+  int fetch_group = first, fetch_i = 0;
+  uint32_t fetch_slot = 0;
+  const T *fetch_a = nullptr, *fetch_b = nullptr;
+  auto rows_of = [&](int group) {
+    const int o = group * kOutputs + g;
+    fetch_a = a.w[0] + (int64_t)min(o, a.outputs - 1) * a.features;
+    fetch_b = kPair ? a.w[1] + (int64_t)min(o, a.outputs - 1) * a.features : a.w[0] + (int64_t)min(o + 8, a.outputs - 1) * a.features;
+  };
+  rows_of(fetch_group);
+  after_previous_kernel();
+  auto fetch = [&]() {
+    if (fetch_group < groups && own > 0) {
+      const int k = (part + fetch_i * a.split) * kStep + j * kValues;
+      fetch_values<T, FULL>(ring + fetch_slot * 1024u, fetch_a, k, a.features);
+      fetch_values<T, FULL>(ring + fetch_slot * 1024u + 512u, fetch_b, k, a.features);
+      if (++fetch_i == own) {
+        fetch_i = 0;
+        fetch_group += stride;
+        rows_of(fetch_group);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    fetch_slot = (fetch_slot + 1) % kFewRing;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kFewRing - 1; ++i) fetch();
+
+  unsigned char *const xs = few_smem + kFewRingBytes;
+  for (int r = warp; r < held; r += kFewWarps) {
+    const T *from = a.x + (int64_t)(row0 + r) * a.x_stride;
+    for (int i = lane; i < steps * 4; i += 32)
+      *reinterpret_cast<uint4 *>(xs + (size_t)r * (size_t)a.pitch + 16 * i) =
+          a.x_whole && (i + 1) * kValues <= a.features ? __ldg(reinterpret_cast<const uint4 *>(from) + i) : load_values(from, i * kValues, a.features);
+  }
+  __syncthreads();
+  const uint32_t x_lane = smem_addr(xs) + (uint32_t)(g * a.pitch + 16 * j);
+  float4 *sums = reinterpret_cast<float4 *>(xs + (size_t)min(8 * NT, a.rows) * (size_t)a.pitch);  // [warps][NT][32]
+  typename Epilogue::template State<NT> state;
+  epilogue.begin(state);
+  uint32_t slot = 0;
+  for (int base = 0; base < groups; base += stride) {  // (as often in every warp)
+    const int group = base + first;
+    float c[NT][4], fresh[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[n][i] = fresh[n][i] = 0.0f;
+    for (int i = 0; i < (group < groups ? own : 0); ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kFewRing - 2) : "memory");
+      const uint4 qa = lds_b128(ring + slot * 1024u), qb = lds_b128(ring + slot * 1024u + 512u);
+      slot = (slot + 1) % kFewRing;
+      const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
+      uint32_t ha[4], la[4], hb[4], lb[4];
+      if constexpr (kFloat) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          split_tf32(wa[h], ha[h], la[h]);
+          split_tf32(wb[h], hb[h], lb[h]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        if (8 * n + g < held) q = lds_b128(x_lane + (uint32_t)(8 * n * a.pitch + 64 * (part + i * a.split)));
+        const uint32_t x[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          if constexpr (kFloat) {
+            uint32_t h0, l0, h1, l1;
+            split_tf32(x[h], h0, l0);
+            split_tf32(x[h + 1], h1, l1);
+            const uint32_t high[4] = {ha[h], hb[h], ha[h + 1], hb[h + 1]}, low[4] = {la[h], lb[h], la[h + 1], lb[h + 1]};
+            mma_few<T>(fresh[n], low, h0, h1);
+            mma_few<T>(fresh[n], high, l0, l1);
+            mma_few<T>(fresh[n], high, h0, h1);
+          } else {
+            const uint32_t w[4] = {wa[h], wb[h], wa[h + 1], wb[h + 1]};
+            mma_few<T>(c[n], w, x[h], x[h + 1]);
+          }
+        }
+      }
+      if (kFloat && ((i & 3) == 3 || i == own - 1)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            c[n][h] += fresh[n][h];
+            fresh[n][h] = 0.0f;
+          }
+      }
+      fetch();
+    }
+    if (a.split > 1) {
+      __syncthreads();  // the sums of the groups before have been read
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sums[(warp * NT + n) * 32 + lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+      __syncthreads();
+      if (part != 0) continue;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        for (int i = 1; i < a.split; ++i) {
+          const float4 q = sums[((warp + i) * NT + n) * 32 + lane];
+          c[n][0] += q.x, c[n][1] += q.y, c[n][2] += q.z, c[n][3] += q.w;
+        }
+    }
+    // this lane: rows row0 + 8 n + 2 j and the next; outputs o and o + 8, or the gate and the value of o
+    const int o = group * kOutputs + g;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) epilogue.template values<NT>(state, n, row0 + 8 * n + 2 * j, o, a.outputs, c[n]);
+  }
+  epilogue.template end<NT>(state, row0, lane);
+}
+
+// How few rows are computed: n-tiles of 8 rows, row groups, blocks.
+struct FewPlan {
+  int tiles, blocks, pitch, split;
+};
+
+// Whether the rows are few enough, and how: 32 rows at the most, in groups whose x fits beside the rings.
+template <typename T>
+bool few_rows(int64_t rows, int64_t features, int64_t outputs, bool pair, FewPlan *plan) {
+  if (rows < 1 || rows > 32 || features > (1 << 20)) return false;
+  const int64_t pitch = round_up(features * (int64_t)sizeof(T), 128) + 64;
+  int tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  auto bytes = [&]() { return std::min<int64_t>(rows, 8 * tiles) * pitch + (int64_t)sizeof(float4) * 32 * kFewWarps * tiles; };
+  while (tiles > 1 && bytes() > kFewMostBytes) tiles /= 2;
+  if (bytes() > kFewMostBytes) return false;
+  const int64_t groups = (outputs + (pair ? 7 : 15)) / (pair ? 8 : 16), most = 148;
+  plan->tiles = tiles;
+  plan->pitch = (int)pitch;
+  plan->split = 1;
+  while (plan->split < kFewWarps && groups * plan->split * 2 <= most * kFewWarps) plan->split *= 2;
+  plan->blocks = (int)std::min<int64_t>((groups * plan->split + kFewWarps - 1) / kFewWarps, most);
+  return true;
+}
+
+template <typename T, class Epilogue>
+int launch_few(FewArgs<T> a, const Epilogue &e, const FewPlan &plan, cudaStream_t stream) {
+  a.pitch = plan.pitch;
+  a.x_whole = a.x_stride * (int64_t)sizeof(T) % 16 == 0 || a.rows == 1;
+  a.split = plan.split;
+  const size_t x_bytes = (size_t)std::min(a.rows, 8 * plan.tiles) * (size_t)plan.pitch;
+  const size_t bytes = kFewRingBytes + x_bytes + (plan.split > 1 ? sizeof(float4) * 32 * kFewWarps * (size_t)plan.tiles : 0);
+  const dim3 grid((unsigned)plan.blocks, (unsigned)((a.rows + 8 * plan.tiles - 1) / (8 * plan.tiles)));
+  auto run = [&](auto kernel) { return launch_next(kernel, grid, kFewThreads, bytes, stream, 1, a, e); };
+  auto by_tiles = [&](auto full) -> int {
+    constexpr bool kFull = decltype(full)::value;
+    return plan.tiles == 1   ? run(few_rows_kernel<T, 1, kFull, Epilogue>)
+           : plan.tiles == 2 ? run(few_rows_kernel<T, 2, kFull, Epilogue>)
+                             : run(few_rows_kernel<T, 4, kFull, Epilogue>);
+  };
+  return a.features * (int64_t)sizeof(T) % 16 == 0 ? by_tiles(std::true_type()) : by_tiles(std::false_type());
+}
+
+}  // namespace dense
+}  // namespace ht

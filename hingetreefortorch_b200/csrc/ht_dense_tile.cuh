@@ -34,6 +34,9 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "ht_common.cuh"
 #include "ht_tile_common.cuh"
@@ -52,6 +55,53 @@ constexpr int kMostStages = 12;
 constexpr uint32_t kStageBudget = 192 * 1024;
 constexpr uint32_t kBoxBytes = 4096;  // of an epilogue warp: 32 rows of 32 columns on their way to or from memory
 constexpr size_t kTileSmem = 1024 + kStageBudget + kEpilogueWarps * kBoxBytes + 512;
+
+#define HT_TRY(expr)                    \
+  do {                                  \
+    const int rc_ = (expr);             \
+    if (rc_ != HT_OK) return rc_;       \
+  } while (0)
+
+// The kernels of these layers follow one another closely: each lets the next one's blocks start as SMs become free, and waits for the one before
+// to have ended, with its results in memory, before it touches memory that others touch (2 to 4 us less a kernel than one after the
+// other).
+__device__ __forceinline__ void after_previous_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Launches a kernel that begins with after_previous_kernel(), in clusters of `ctas`.
+template <typename... Parameters, typename... Arguments>
+int launch_next(void (*kernel)(Parameters...), dim3 grid, int threads, size_t shared, cudaStream_t stream, int ctas, const Arguments &...arguments) {
+  if (shared > 48 * 1024) {  // asked for once a kernel and device; more than is asked for does no harm
+    int device = 0;
+    HT_CUDA_TRY(cudaGetDevice(&device));
+    static std::mutex mutex;
+    static std::map<std::pair<const void *, int>, size_t> granted;
+    std::lock_guard<std::mutex> lock(mutex);
+    size_t &most = granted[{reinterpret_cast<const void *>(kernel), device}];
+    if (shared > most) {
+      HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+      most = shared;
+    }
+  }
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = (unsigned)ctas;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3((unsigned)threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  config.attrs = attributes;
+  config.numAttrs = ctas > 1 ? 2 : 1;
+  HT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...));
+  HT_CHECK_LAUNCH();
+  return HT_OK;
+}
 
 // A 16-bit matrix in device memory, row-major, `pitch` elements from row to row (a multiple of 8, base on 16 bytes); with
 // three planes, `plane` elements apart.
@@ -267,6 +317,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
   };
   everybody();
   const uint32_t tmem = *tmem_slot;
+  after_previous_kernel();
 
   auto give_up = [&]() {
     if (a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_PIPELINE_TIMEOUT);
@@ -552,46 +603,31 @@ inline int sm_count(int *sms) {
 }
 
 // How to cut a product: the shape with which the SMs are done first.  Cycles of a step of 16 values of k, measured: a pair of CTAs with 256
-// columns 140, with 128 columns 100 (shared memory bounds it); one CTA with 256 columns 240, with 128 220, with 64 200 (three planes: 6 of
-// those, of 128 columns at the most alone).  A tile costs about 2000 cycles besides.
+// columns 160, with 128 columns 110; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120 (three planes: 6 of those, of
+// 128 columns at the most alone).  A tile costs about 2500 cycles besides.  Against that, the operands have to come from memory once,
+// 23 bytes a cycle and SM where all read, twice that where few do.
 inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, bool pair) {
   constexpr int kPlanSMs = 148;
+  constexpr double kBytesPerCycle = 23.0;
   TileShape best = {1, 128};
   double least = 0.0;
   for (int ctas = 2; ctas >= 1; --ctas)
     for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 64) {
       if (bn % (ctas == 2 || pair ? 128 : 64) != 0) continue;
       const int64_t n = pair ? bn / 2 : bn;
-      const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n);
-      const double rounds = (double)((tiles * ctas + kPlanSMs - 1) / kPlanSMs);
-      const double step = ctas == 2 ? (bn == 256 ? 140.0 : 100.0) : 180.0 + 0.235 * bn;
-      const double cycles = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k + 15) / 16) * step + 2000.0);
+      const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n) * ctas, last = tiles % kPlanSMs;
+      const double rounds = (double)((tiles + kPlanSMs - 1) / kPlanSMs);
+      const double step = ctas == 2 ? (bn == 256 ? 160.0 : 110.0) : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
+      const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k + 15) / 16) * step + 2500.0);
+      const double bytes = 2.0 * planes * (double)k * (double)(rows + cols * (pair ? 2 : 1)) / (double)tiles;
+      const double memory = bytes / kBytesPerCycle * ((double)(tiles / kPlanSMs) + (last > 0 ? std::max(0.5, (double)last / kPlanSMs) : 0.0));
+      const double cycles = std::max(products, memory);
       if (least == 0.0 || cycles < least * 0.999) {
         best = {ctas, bn};
         least = cycles;
       }
     }
   return best;
-}
-
-template <int CTAS, int PLANES, bool A_MN, bool B_MN, class Epilogue>
-int launch_shape(const TileArgs &a, const Epilogue &epilogue, int sms, cudaStream_t stream) {
-  auto kernel = dense_tile_kernel<CTAS, PLANES, A_MN, B_MN, Epilogue>;
-  HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem));
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(CTAS * std::min(a.tiles, std::max(sms / CTAS, 1))));
-  config.blockDim = dim3(kTileThreads);
-  config.dynamicSmemBytes = kTileSmem;
-  config.stream = stream;
-  cudaLaunchAttribute attribute = {};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = CTAS;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute;
-  config.numAttrs = CTAS > 1 ? 1 : 0;
-  HT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a, epilogue));
-  HT_CHECK_LAUNCH();
-  return HT_OK;
 }
 
 template <int PLANES, bool A_MN, bool B_MN, class Epilogue>
@@ -623,7 +659,9 @@ int launch_tiles(const TileProblem &p, const Epilogue &epilogue, const TileShape
   a.a_bytes = (uint32_t)kTileM * 128u * PLANES;
   a.stage_bytes = a.a_bytes + (uint32_t)(bn / shape.ctas) * 128u * PLANES;
   a.stages = (int)std::min<uint32_t>(kStageBudget / a.stage_bytes, kMostStages);
-  return shape.ctas == 2 ? launch_shape<2, PLANES, A_MN, B_MN>(a, epilogue, sms, stream) : launch_shape<1, PLANES, A_MN, B_MN>(a, epilogue, sms, stream);
+  const dim3 grid((unsigned)(shape.ctas * std::min(a.tiles, std::max(sms / shape.ctas, 1))));
+  return shape.ctas == 2 ? launch_next(dense_tile_kernel<2, PLANES, A_MN, B_MN, Epilogue>, grid, kTileThreads, kTileSmem, stream, 2, a, epilogue)
+                         : launch_next(dense_tile_kernel<1, PLANES, A_MN, B_MN, Epilogue>, grid, kTileThreads, kTileSmem, stream, 1, a, epilogue);
 }
 
 }  // namespace dense

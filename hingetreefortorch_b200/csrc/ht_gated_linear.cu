@@ -11,7 +11,7 @@
 // would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to the operands' 16 bits (2^-9 of a term
 // that enters sums, for bf16); for fp16 dh is scaled to a largest value in [1, 2) first, so that small gradients stay normal numbers; fp32
 // is split into planes.
-#include "ht_dense.cuh"
+#include "ht_dense_rows.cuh"
 
 namespace ht {
 namespace dense {
@@ -23,28 +23,43 @@ __device__ __forceinline__ float sigmoid(float a) {
   return EXACT ? 1.0f / (1.0f + expf(-a)) : __fdividef(1.0f, 1.0f + __expf(-a));
 }
 template <bool EXACT, bool SLOPE>
-__device__ __forceinline__ void activate(int act, const float (&a)[32], float (&g)[32], float (&d)[32]) {
-  if (act == HT_ACTIVATION_SILU || act == HT_ACTIVATION_SIGMOID) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float s = sigmoid<EXACT>(a[i]);
-      g[i] = act == HT_ACTIVATION_SILU ? a[i] * s : s;
-      if (SLOPE) d[i] = act == HT_ACTIVATION_SILU ? s * (1.0f + a[i] * (1.0f - s)) : s * (1.0f - s);
-    }
-  } else if (act == HT_ACTIVATION_GELU) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float phi = 0.5f * erfcf(a[i] * -0.70710678118654752f);  // the normal distribution function
-      g[i] = a[i] * phi;
-      if (SLOPE) d[i] = phi + a[i] * 0.39894228040143268f * (EXACT ? expf(-0.5f * a[i] * a[i]) : __expf(-0.5f * a[i] * a[i]));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      g[i] = a[i] < 0.0f ? 0.0f : a[i];  // (no number stays none)
-      if (SLOPE) d[i] = a[i] > 0.0f ? 1.0f : 0.0f;
-    }
+__device__ __forceinline__ float activate_one(int act, float a, float &slope) {
+  if (act == HT_ACTIVATION_SILU) {
+    const float s = sigmoid<EXACT>(a);
+    if (SLOPE) slope = s * (1.0f + a * (1.0f - s));
+    return a * s;
   }
+  if (act == HT_ACTIVATION_SIGMOID) {
+    const float s = sigmoid<EXACT>(a);
+    if (SLOPE) slope = s * (1.0f - s);
+    return s;
+  }
+  if (act == HT_ACTIVATION_GELU) {
+    const float phi = 0.5f * erfcf(a * -0.70710678118654752f);  // the normal distribution function
+    if (SLOPE) slope = phi + a * 0.39894228040143268f * (EXACT ? expf(-0.5f * a * a) : __expf(-0.5f * a * a));
+    return a * phi;
+  }
+  if (SLOPE) slope = a > 0.0f ? 1.0f : 0.0f;
+  return a < 0.0f ? 0.0f : a;  // (no number stays none)
+}
+template <bool EXACT, bool SLOPE>
+__device__ __forceinline__ void activate(int act, const float (&a)[32], float (&g)[32], float (&d)[32]) {
+  auto all = [&](int which) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float slope = 0.0f;
+      g[i] = activate_one<EXACT, SLOPE>(which, a[i], slope);
+      if (SLOPE) d[i] = slope;
+    }
+  };
+  if (act == HT_ACTIVATION_SILU)
+    all(HT_ACTIVATION_SILU);
+  else if (act == HT_ACTIVATION_GELU)
+    all(HT_ACTIVATION_GELU);
+  else if (act == HT_ACTIVATION_RELU)
+    all(HT_ACTIVATION_RELU);
+  else
+    all(HT_ACTIVATION_SIGMOID);
 }
 
 template <typename T>
@@ -79,6 +94,30 @@ struct GatedEpilogue {
     if (top < rows) store_box(w, h + (size_t)top * (size_t)cols + col, (size_t)cols, min(32, rows - top), min(32, n), align, g);
   }
   __device__ __forceinline__ void end(State &, const Where &) const {}
+};
+
+template <typename T>
+struct FewGatedEpilogue {
+  static constexpr bool kPair = true;
+  template <int NT>
+  struct State {};
+  int rows, cols, act;
+  const T *bg, *bv;
+  T *h;
+  template <typename S>
+  __device__ __forceinline__ void begin(S &) const {}
+  template <int NT>
+  __device__ __forceinline__ void values(State<NT> &, int, int row, int o, int outputs, const float (&c)[4]) const {
+    if (o >= outputs) return;
+    const float ba = bg != nullptr ? to_float(bg[o]) : 0.0f, bu = bv != nullptr ? to_float(bv[o]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float slope;
+      if (row + i < rows) h[(size_t)(row + i) * (size_t)cols + o] = from_float<T>(activate_one<sizeof(T) == 4, false>(act, c[i] + ba, slope) * (c[2 + i] + bu));
+    }
+  }
+  template <int NT>
+  __device__ __forceinline__ void end(State<NT> &, int, int) const {}
 };
 
 // The power of two at or below the largest |dh| (its bits in *top), 1 where there is none.
@@ -136,6 +175,7 @@ struct GatedGradEpilogue {
 
 // The bits of the largest |dh| (fp16) into *top, which starts as 0: bits of numbers without a sign order like the numbers.
 __global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__ v, int64_t n, uint32_t *top) {
+  after_previous_kernel();
   uint32_t most = 0;
   const int64_t quads = n / 8, step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   for (int64_t i = at; i < quads; i += step) {
@@ -149,7 +189,10 @@ __global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__
   most = __reduce_max_sync(0xffffffffu, most);
   if ((threadIdx.x & 31) == 0) atomicMax(top, __float_as_uint(__half2float(__ushort_as_half((unsigned short)most))));
 }
-__global__ void scale_kernel(const uint32_t *top, float *alpha) { *alpha = scale_of(top); }
+__global__ void scale_kernel(const uint32_t *top, float *alpha) {
+  after_previous_kernel();
+  *alpha = scale_of(top);
+}
 
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // da and du of one piece, unless the caller sets less
 
@@ -163,6 +206,8 @@ int screen(const ht_dense_problem *p) {
 
 template <typename T>
 struct Plan {
+  bool few = false;  // the forward
+  FewPlan few_plan;
   Operand<T> x, wg, wv;
   int64_t piece = 0, pitch = 0;
   typename Kind<T>::Operand *g = nullptr;
@@ -171,6 +216,8 @@ struct Plan {
   size_t bytes;
   Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, void *ws) {
     Arena arena(ws);
+    bytes = 0;
+    if ((few = !backward && few_rows<T>(p.rows, p.features, p.outputs, true, &few_plan))) return;
     x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
     wg.set(arena, static_cast<const T *>(wgp), p.outputs, p.features, p.features);
     wv.set(arena, static_cast<const T *>(wvp), p.outputs, p.features, p.features);
@@ -202,6 +249,12 @@ int forward(const ht_dense_problem &p, const void *x, const void *wg, const void
   Plan<T> plan(p, x, wg, wv, false, false, false, ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   int sms = 0, rc;
+  if (plan.few) {
+    const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(wg), static_cast<const T *>(wv)}, p.x_stride, (int)p.rows, (int)p.features,
+                          (int)p.outputs};
+    const FewGatedEpilogue<T> e = {(int)p.rows, (int)p.outputs, p.activation, static_cast<const T *>(bg), static_cast<const T *>(bv), static_cast<T *>(h)};
+    return launch_few(a, e, plan.few_plan, stream);
+  }
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
   if ((rc = plan.lay_out(stream)) != HT_OK) return rc;
   TileProblem t;
@@ -241,10 +294,8 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
   if (scaled) {
     const int64_t n = p.rows * p.outputs;
     HT_CUDA_TRY(cudaMemsetAsync(plan.top, 0, sizeof(uint32_t), stream));
-    largest_kernel<<<blocks_for(n, 256 * 32, 148 * 8), 256, 0, stream>>>(static_cast<const __half *>(dh), n, plan.top);
-    HT_CHECK_LAUNCH();
-    scale_kernel<<<1, 1, 0, stream>>>(plan.top, plan.alpha);
-    HT_CHECK_LAUNCH();
+    HT_TRY(launch_next(largest_kernel, dim3(blocks_for(n, 256 * 32, 148 * 8)), 256, 0, stream, 1, static_cast<const __half *>(dh), n, plan.top));
+    HT_TRY(launch_next(scale_kernel, dim3(1), 1, 0, stream, 1, plan.top, plan.alpha));
   }
   const float *alpha = scaled ? plan.alpha : nullptr;
   constexpr int kPlanes = Kind<T>::kPlanes;
