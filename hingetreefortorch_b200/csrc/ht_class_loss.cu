@@ -385,7 +385,7 @@ struct BackwardPlan {
   int64_t piece, pitch;  // classes of a piece, elements of a row of g
   typename Kind<T>::Operand *g;
   RowGrad *row_grad;
-  float *alpha, *sum, *row_sums;
+  float *alpha, *sum, *parts, *row_sums;
   size_t bytes;
   BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, void *ws) {
     Arena arena(ws);
@@ -394,14 +394,17 @@ struct BackwardPlan {
     w.set(arena, wp, p.outputs, p.features, p.features);
     const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
     const int64_t per_class = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 2;
-    // pieces of whole tiles; at least one tile, and all classes where they fit
-    piece = std::max<int64_t>(limit / per_class / 256 * 256, 256);
-    if (piece >= p.outputs) piece = p.outputs;
+    piece = piece_of(p.outputs, limit / per_class);
     pitch = round_up(piece, 64);
     g = arena.take<typename Kind<T>::Operand>(p.rows * pitch * Kind<T>::kPlanes);
     row_grad = arena.take<RowGrad>(p.rows);
     alpha = arena.take<float>(1);
     sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
+    parts = nullptr;
+    int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, p.outputs, Kind<T>::kPlanes);
+    for (const int64_t count : {piece, (p.outputs - 1) % piece + 1})
+      most = std::max(most, product_parts(count, p.features, std::max<int64_t>(p.rows, 1), Kind<T>::kPlanes));
+    if (most > 0) parts = arena.take<float>(most);
     row_sums = has_db ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * pitch) : nullptr;
     bytes = arena.used;
   }
@@ -460,7 +463,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
       store.rows = store.part = (int)p.rows;
       store.out = dx, store.align = row_alignment(dx, p.features * (int64_t)sizeof(T));
       store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
-      if ((rc = product_dx<T>(q, store, sms, stream)) != HT_OK) return rc;
+      if ((rc = product_dx<T>(q, store, plan.piece < p.outputs ? nullptr : plan.parts, sms, stream)) != HT_OK) return rc;
     }
     if (dw != nullptr) {
       TileProblem q = t;
@@ -470,7 +473,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
       store.rows = store.part = (int)count;
       store.out = dw + (size_t)first * (size_t)p.features, store.align = row_alignment(store.out, p.features * (int64_t)sizeof(T));
       store.sum = nullptr, store.keep = false;
-      if ((rc = product_dw<T>(q, store, sms, stream)) != HT_OK) return rc;
+      if ((rc = product_dw<T>(q, store, plan.parts, sms, stream)) != HT_OK) return rc;
     }
     if (db != nullptr && (rc = column_sums<T>(plan.row_sums, row_sum_count(p.rows, shape), plan.pitch, count, plan.alpha, db + first, stream)) != HT_OK)
       return rc;

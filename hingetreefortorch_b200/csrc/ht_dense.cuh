@@ -242,7 +242,56 @@ __device__ __forceinline__ void load_box(const Where &w, const T *first, size_t 
   }
   __syncwarp();
 }
-// The alignment of a matrix's rows for the two above.
+// load_box in two halves: begun early (cp.async, for rows on 4 bytes at least; others wait for the second half), and finished into
+// registers.  A box takes 1024 sizeof(T) bytes at `at`.
+template <typename T, int BYTES>
+__device__ __forceinline__ void fetch_box(uint32_t at, const T *first, size_t pitch, int rows, int cols, int lane) {
+  constexpr int kPerRow = 32 * (int)sizeof(T) / BYTES, kRows = 32 / kPerRow, kValues = BYTES / (int)sizeof(T);
+  const int piece = lane % kPerRow, c = piece * kValues;
+  if (c >= cols) return;
+  const int bytes = min(BYTES, (cols - c) * (int)sizeof(T));
+#pragma unroll 4
+  for (int r = lane / kPerRow; r < rows; r += kRows) {
+    const uint32_t to = at + box_offset<T>((uint32_t)r, (uint32_t)(piece * BYTES / 16)) + (uint32_t)(piece * BYTES % 16);
+    const T *from = first + (size_t)r * pitch + c;
+    if constexpr (BYTES == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(from), "r"(bytes), "n"(BYTES) : "memory");
+  }
+}
+template <typename T>
+__device__ __forceinline__ void begin_box(uint32_t at, const T *first, size_t pitch, int rows, int cols, int align, int lane) {
+  if (align >= 16)
+    fetch_box<T, 16>(at, first, pitch, rows, cols, lane);
+  else if (align == 8)
+    fetch_box<T, 8>(at, first, pitch, rows, cols, lane);
+  else if (align == 4)
+    fetch_box<T, 4>(at, first, pitch, rows, cols, lane);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <typename T>
+__device__ __forceinline__ void finish_box(uint32_t at, const T *first, size_t pitch, int rows, int cols, int align, int lane, float (&v)[32]) {
+  constexpr int kStep = 32 / (int)sizeof(T);
+  if (align >= 4)
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  else
+    move_box_by<T, false>(at, const_cast<T *>(first), pitch, rows, cols, align, lane);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 32; i += kStep) {
+    uint32_t q[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 t = lds_b128(at + box_offset<T>((uint32_t)lane, (uint32_t)(i / kStep * 2 + h)));
+      q[4 * h] = t.x, q[4 * h + 1] = t.y, q[4 * h + 2] = t.z, q[4 * h + 3] = t.w;
+    }
+    from_words<T>(q, i, v);
+  }
+  __syncwarp();
+}
+
+// The alignment of a matrix's rows for the functions above.
 inline int row_alignment(const void *data, int64_t row_bytes) {
   const uint64_t bits = (uint64_t)reinterpret_cast<uintptr_t>(data) | (uint64_t)row_bytes | 32u;
   return (int)(bits & (~bits + 1));
@@ -309,11 +358,17 @@ struct StoreEpilogue {
   float *sum;          // [rows, cols] or null
   bool begins, keep;   // the first piece of a sum, not the last one
   int align, sum_align;
+  float *parts;        // [parts of k][rows][pitch]: sums that another kernel adds, or null
+  int parts_pitch;
   __device__ __forceinline__ void begin(State &s, const Where &) const { s.alpha = alpha != nullptr ? __ldg(alpha) : 1.0f; }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
     const int top = w.row - w.lane, row = top < split ? top : top - split;
     const int m = min(32, min(part - row, rows - top)), n = min(32, cols - col);
     if (m <= 0 || n <= 0) return;
+    if (parts != nullptr) {  // rows of 32 bytes: whole boxes, in their pitch
+      store_box(w, parts + ((size_t)w.part * (size_t)rows + (size_t)top) * (size_t)parts_pitch + col, (size_t)parts_pitch, m, min(32, parts_pitch - col), 32, v);
+      return;
+    }
     if (sum != nullptr) {
       float *acc = sum + (size_t)top * (size_t)cols + col;
       if (!begins) {
@@ -333,6 +388,39 @@ struct StoreEpilogue {
   }
   __device__ __forceinline__ void end(State &, const Where &) const {}
 };
+
+// out = alpha sum_part parts[part], parts ascending; 4 columns a thread.  Reads 4 bytes a value and part, at the memory's or L2's speed.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const StoreEpilogue<T> e, int count) {
+  after_previous_kernel();
+  const float alpha = e.alpha != nullptr ? __ldg(e.alpha) : 1.0f;
+  const int quads = e.parts_pitch / 4;
+  const int64_t n = (int64_t)e.rows * quads, step = (int64_t)gridDim.x * 256;
+  const size_t plane = (size_t)e.rows * (size_t)e.parts_pitch;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const int r = (int)(i / quads), c = (int)(i - (int64_t)r * quads) * 4, row = r < e.split ? r : r - e.split;
+    if (c >= e.cols || row >= e.part) continue;
+    const float *from = e.parts + (size_t)r * (size_t)e.parts_pitch + c;
+    float4 sum = __ldg(reinterpret_cast<const float4 *>(from));
+#pragma unroll 4
+    for (int p = 1; p < count; ++p) {
+      const float4 q = __ldg(reinterpret_cast<const float4 *>(from + (size_t)p * plane));
+      sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+    }
+    T *to = (r < e.split ? e.out : e.out2) + (size_t)row * (size_t)e.cols + c;
+    const float v[4] = {alpha * sum.x, alpha * sum.y, alpha * sum.z, alpha * sum.w};
+    if (e.align >= 4 * (int)sizeof(T) && c + 4 <= e.cols) {
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+      else
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pack_pair(v[0], v[1], to), pack_pair(v[2], v[3], to));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < e.cols) to[j] = from_float<T>(v[j]);
+    }
+  }
+}
 
 // ---- operands ---------------------------------------------------------------------------------------------------------
 
@@ -463,11 +551,27 @@ int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols,
   return HT_OK;
 }
 
-// dx (+)= g w over a piece of outputs, dw = g^T x (ht_dense_products.cu).
+// Outputs of a piece where `most` fit the bound: all of them, or pieces of whole tiles, about equal, 256 at the least.
+inline int64_t piece_of(int64_t outputs, int64_t most) {
+  if (most >= outputs) return outputs;
+  const int64_t whole = std::max<int64_t>(most / 256 * 256, 256), pieces = (outputs + whole - 1) / whole;
+  return std::min(outputs, round_up((outputs + pieces - 1) / pieces, 256));
+}
+
+// The two products of a backward pass (ht_dense_products.cu): dx (+)= g w over a piece of the outputs, dw = g^T x.  `parts`: room for
+// product_parts() floats, or null; what a product with few tiles is cut into along k is summed there.
+constexpr int kMostParts = 16;
+inline TileShape product_shape(int64_t rows, int64_t cols, int64_t k, int planes, bool in_parts) {
+  return tile_shape(rows, cols, k, planes, false, in_parts ? kMostParts : 1);
+}
+inline int64_t product_parts(int64_t rows, int64_t cols, int64_t k, int planes) {
+  const int split = product_shape(rows, cols, k, planes, true).split;
+  return split > 1 ? split * rows * round_up(cols, 8) : 0;
+}
 template <typename T>
-int product_dx(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream);
+int product_dx(const TileProblem &p, StoreEpilogue<T> e, float *parts, int sms, cudaStream_t stream);
 template <typename T>
-int product_dw(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream);
+int product_dw(const TileProblem &p, StoreEpilogue<T> e, float *parts, int sms, cudaStream_t stream);
 
 }  // namespace dense
 }  // namespace ht

@@ -7,20 +7,31 @@
 namespace ht {
 namespace dense {
 
-template <typename T>
-int product_dx(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream) {
+namespace {
+template <typename T, bool A_MN>
+int product(const TileProblem &p, StoreEpilogue<T> &e, float *parts, int sms, cudaStream_t stream) {
   constexpr int kPlanes = Kind<T>::kPlanes;
-  return launch_tiles<kPlanes, false, true>(p, e, tile_shape(p.rows, p.cols, p.k * p.segments, kPlanes, false), sms, stream);
+  const TileShape shape = product_shape(p.rows, p.cols, p.k * p.segments, kPlanes, parts != nullptr);
+  if (shape.split == 1) return launch_tiles<kPlanes, A_MN, true>(p, e, shape, sms, stream);
+  e.parts = parts;
+  e.parts_pitch = (int)round_up(p.cols, 8);
+  HT_TRY((launch_tiles<kPlanes, A_MN, true>(p, e, shape, sms, stream)));
+  return launch_next(add_parts_kernel<T>, dim3(blocks_for(p.rows * (e.parts_pitch / 4), 256, 148 * 8)), 256, 0, stream, 1, e, parts_of(p, shape));
+}
+}  // namespace
+
+template <typename T>
+int product_dx(const TileProblem &p, StoreEpilogue<T> e, float *parts, int sms, cudaStream_t stream) {
+  return product<T, false>(p, e, parts, sms, stream);
 }
 template <typename T>
-int product_dw(const TileProblem &p, const StoreEpilogue<T> &e, int sms, cudaStream_t stream) {
-  constexpr int kPlanes = Kind<T>::kPlanes;
-  return launch_tiles<kPlanes, true, true>(p, e, tile_shape(p.rows, p.cols, p.k, kPlanes, false), sms, stream);
+int product_dw(const TileProblem &p, StoreEpilogue<T> e, float *parts, int sms, cudaStream_t stream) {
+  return product<T, true>(p, e, parts, sms, stream);
 }
 
-#define HT_DENSE_PRODUCTS(T)                                                                       \
-  template int product_dx<T>(const TileProblem &, const StoreEpilogue<T> &, int, cudaStream_t);    \
-  template int product_dw<T>(const TileProblem &, const StoreEpilogue<T> &, int, cudaStream_t);
+#define HT_DENSE_PRODUCTS(T)                                                                            \
+  template int product_dx<T>(const TileProblem &, StoreEpilogue<T>, float *, int, cudaStream_t);    \
+  template int product_dw<T>(const TileProblem &, StoreEpilogue<T>, float *, int, cudaStream_t);
 HT_DENSE_PRODUCTS(float)
 HT_DENSE_PRODUCTS(__nv_bfloat16)
 HT_DENSE_PRODUCTS(__half)

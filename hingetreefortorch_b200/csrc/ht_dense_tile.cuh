@@ -10,8 +10,9 @@
 // fp32 operands come as three bf16 planes (x = x0 + x1 + x2, each the rounding of what is left: 24 bits): the products x0 y0 in one
 // accumulator, and x0 y1, x1 y0, x1 y1, x0 y2, x2 y0 in a second; what is left out is below 2^-24 of a term.  The tensor core truncates
 // when it adds to an accumulator, always towards zero (measured: 32 instructions in a row lose about 9e-7 of the sum, which is more than an fp32
-// sum loses to rounding).  So the large products leave for registers every 8 instructions (128 values of k) and are added there in
-// fp32; the small ones are 2^-8 of those and stay to the end.
+// sum loses to rounding).  So the large products leave for registers every 16 instructions (256 values of k) and are added there in
+// fp32; the small ones are 2^-8 of those and stay to the end.  (Every 8 instructions lose half as much again, and leave the epilogue of a
+// tile no time beside the next one's products.)
 //
 // A persistent kernel of 320 threads a CTA, one CTA per SM, alone (CTAS = 1, tiles of 128 rows) or in clusters of two that share a
 // tile of 256 rows (CTAS = 2): tcgen05.mma.cta_group::2 reads each CTA's 128 rows of A and half of B's rows from that CTA's shared
@@ -50,7 +51,7 @@ using namespace tile;
 constexpr int kTileM = 128, kTileK = 64;
 constexpr int kTileThreads = 320;
 constexpr int kEpilogueWarps = 8;
-constexpr int kChunkBlocks = 2;  // blocks of 64 values of k between two visits of the registers (three planes)
+constexpr int kChunkBlocks = 4;  // blocks of 64 values of k between two visits of the registers (three planes)
 constexpr int kMostStages = 12;
 constexpr uint32_t kStageBudget = 192 * 1024;
 constexpr uint32_t kBoxBytes = 4096;  // of an epilogue warp: 32 rows of 32 columns on their way to or from memory
@@ -120,14 +121,16 @@ struct alignas(64) TileArgs {
   int bn;                  // columns of a tile: both halves of a pair together
   int k, k_blocks;         // of one segment
   int segments;            // 2: the sum over k goes on in a[1], b[1]
+  int part_blocks;         // blocks of 64 values of k, of both segments together, in a part; tiles are counted part by part
   int b_n0, b_k0;          // where B's rows / values of k begin
   int stages;
   uint32_t a_bytes, stage_bytes;  // of one CTA
 };
 
-// How a product is cut: CTAs that share a tile of 128 rows each, and its columns.
+// How a product is cut: CTAs that share a tile of 128 rows each, its columns, parts of k.
 struct TileShape {
   int ctas, bn;
+  int split = 1;  // parts of k, each with sums of its own
   int rows() const { return 128 * ctas; }
 };
 
@@ -136,7 +139,9 @@ struct Where {
   int row;       // of the output
   bool inside;   // row < rows of the output
   uint32_t box;  // shared memory of the warp
-  int m_block, n_block, half, quarter, lane;
+  int col;       // the first of this half's columns
+  int units;     // of 32 columns in this half
+  int m_block, n_block, part, half, quarter, lane;
 };
 
 __device__ __forceinline__ uint64_t k_major_descriptor(uint32_t address) {
@@ -283,7 +288,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
   const int first_tile = (int)blockIdx.x / CTAS, tile_step = (int)gridDim.x / CTAS;
-  const int blocks = a.segments * a.k_blocks;
   constexpr uint32_t kColumns = 512;
 
   if (threadIdx.x == 0) {
@@ -322,15 +326,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
   auto give_up = [&]() {
     if (a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_PIPELINE_TIMEOUT);
   };
-  // Tile -> (row block, column block): groups of 16 row blocks, the rows of a group fastest.
-  auto place = [&](int tile, int &mb, int &nb) {
+  // What one turn of the loops is: a tile, and a part of k.  Groups of 16 row blocks, the rows of a group fastest.
+  struct Turn {
+    int mb, nb, part, first, last;  // blocks of k: first .. last - 1
+  };
+  const int all_blocks = a.segments * a.k_blocks, per_part = a.m_blocks * a.n_blocks;
+  auto place = [&](int index) {
     constexpr int kGroup = 16;
+    Turn t;
+    t.part = index / per_part;
+    const int tile = index - t.part * per_part;
     const int per_group = kGroup * a.n_blocks, g = tile / per_group, in = tile - g * per_group;
     const int rows = min(kGroup, a.m_blocks - g * kGroup);
-    nb = in / rows;
-    mb = g * kGroup + (in - nb * rows);
+    t.nb = in / rows;
+    t.mb = g * kGroup + (in - t.nb * rows);
+    t.first = t.part * a.part_blocks;
+    t.last = min(all_blocks, t.first + a.part_blocks);
+    return t;
   };
-
   // A wait of the whole warp.
   auto arrived = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0; };
 
@@ -340,13 +353,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       uint32_t it = 0, s = 0, phase = 1;
       bool ok = true;
       for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
-        int mb, nb;
-        place(tile, mb, nb);
-        const int m0 = (mb * CTAS + rank) * kTileM;
+        const Turn turn = place(tile);
+        const int m0 = (turn.mb * CTAS + rank) * kTileM;
         const int half = a.bn / 2;
         // a pair of matrices: one each to the CTAs of a pair, both to one alone
-        const int n0 = a.b_n0 + nb * (kPair ? half : a.bn) + (CTAS == 2 && !kPair ? rank * half : 0);
-        for (int kb = 0; kb < blocks; ++kb, ++it) {
+        const int n0 = a.b_n0 + turn.nb * (kPair ? half : a.bn) + (CTAS == 2 && !kPair ? rank * half : 0);
+        for (int kb = turn.first; kb < turn.last; ++kb, ++it) {
           if (!arrived(&empty[s], phase)) {
             give_up();
             ok = false;
@@ -405,9 +417,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       constexpr uint32_t step_a = A_MN ? 128u : 2u, step_b = B_MN ? 128u : 2u;  // 16 values of k, in units of 16 bytes
       for (int tile = first_tile; tile < a.tiles; tile += tile_step, ++t) {
         uint32_t d = tmem_d;
-        for (int kb = 0; kb < blocks; ++kb) {
-          const bool first = kThree ? kb % kChunkBlocks == 0 : kb == 0;
-          if (kThree && kb == 0) wait_here(drained_small, (t & 1u) ^ 1u);
+        const Turn at_work = place(tile);
+        for (int kb = at_work.first; kb < at_work.last; ++kb) {
+          const int since = kb - at_work.first;
+          const bool first = kThree ? since % kChunkBlocks == 0 : since == 0;
+          if (kThree && since == 0) wait_here(drained_small, (t & 1u) ^ 1u);
           const uint32_t buffer = chunk % kBuffers;
           auto turn = [&]() {  // the accumulator's previous sum has been read
             if (!first) return;
@@ -435,7 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
               const uint64_t ak = da + (uint64_t)(step_a * (uint32_t)kk);
               const uint64_t bk = db + (uint64_t)part * (3u * b_plane) + (uint64_t)(step_b * (uint32_t)kk);
               const uint32_t to = tmem_d + 256u + (uint32_t)part * b_rows;
-              mma_f16<CTAS>(one, to, ak + 2 * a_plane, bk, a.instruction, kk > 0 || kb > 0);
+              mma_f16<CTAS>(one, to, ak + 2 * a_plane, bk, a.instruction, kk > 0 || since > 0);
               mma_f16<CTAS>(one, to, ak, bk + 2 * b_plane, a.instruction, 1u);
               mma_f16<CTAS>(one, to, ak + a_plane, bk + b_plane, a.instruction, 1u);
               mma_f16<CTAS>(one, to, ak + a_plane, bk, a.instruction, 1u);
@@ -458,7 +472,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
             s = 0;
             phase ^= 1u;
           }
-          if (kb == blocks - 1 || (kThree && kb % kChunkBlocks == kChunkBlocks - 1)) {
+          if (kb == at_work.last - 1 || (kThree && since % kChunkBlocks == kChunkBlocks - 1)) {
             mma_commit<CTAS>(one, smem_addr(&accumulated[buffer]));
             ++chunk;
           }
@@ -471,7 +485,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
     uint32_t chunk = 0;
     const int units = kPair ? a.bn / 128 : a.bn / 64;  // of 32 columns (a pair: 32 of each), for this half
     Where w;
-    w.half = half, w.quarter = quarter, w.lane = lane;
+    w.half = half, w.quarter = quarter, w.lane = lane, w.units = units;
     w.box = stages + kStageBudget + (uint32_t)(warp - 2) * kBoxBytes;
     auto wait_for = [&](uint32_t c) {
       bool there = mbar_wait(&accumulated[c % kBuffers], (c / kBuffers) & 1u);
@@ -491,15 +505,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       }
     };
     for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
-      int mb;
-      place(tile, mb, w.n_block);
-      w.m_block = mb * CTAS + rank;
+      const Turn turn = place(tile);
+      w.n_block = turn.nb, w.part = turn.part;
+      w.m_block = turn.mb * CTAS + rank;
       w.row = w.m_block * kTileM + quarter * 32 + lane;
       w.inside = w.row < epilogue.rows;
       typename Epilogue::State state;
       const int col0 = w.n_block * (kPair ? a.bn / 2 : a.bn);
+      w.col = col0 + half * units * 32;
+      epilogue.begin(state, w);  // under the tile's products
       if constexpr (!kThree) {
-        epilogue.begin(state, w);
         if (!wait_for(chunk)) break;
         const uint32_t acc = lanes + (chunk & 1u) * 256u;
 #pragma unroll 1
@@ -529,7 +544,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           for (int i = 0; i < 32; ++i) sum[u][i] = 0.0f;
         auto column = [&](int u) { return kPair ? (u & 1) * (a.bn / 2) + (half * units + (u >> 1)) * 32 : (half * units + u) * 32; };
         bool there = true;
-        const int chunks = (blocks + kChunkBlocks - 1) / kChunkBlocks;
+        const int chunks = (turn.last - turn.first + kChunkBlocks - 1) / kChunkBlocks;
         for (int c = 0; c <= chunks; ++c) {
           if (c < chunks && !(there = wait_for(chunk))) break;
           const uint32_t acc = lanes + (c < chunks ? 0u : 256u);
@@ -545,7 +560,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           release(c < chunks ? &drained[0] : drained_small);
         }
         if (!there) break;
-        epilogue.begin(state, w);
 #pragma unroll
         for (int u = 0; u < kMostUnits; ++u) {
           if (u >= parts) break;
@@ -605,29 +619,41 @@ inline int sm_count(int *sms) {
 // How to cut a product: the shape with which the SMs are done first.  Cycles of a step of 16 values of k, measured: a pair of CTAs with 256
 // columns 160, with 128 columns 110; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120 (three planes: 6 of those, of
 // 128 columns at the most alone).  A tile costs about 2500 cycles besides.  Against that, the operands have to come from memory once,
-// 23 bytes a cycle and SM where all read, twice that where few do.
-inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, bool pair) {
+// 23 bytes a cycle and SM where all read, twice that where few do.  Where `most_parts` allows it, k is cut as well: each part writes its
+// sums in fp32, and a kernel adds them (8 bytes a value and part, and about 6000 cycles).
+inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, bool pair, int most_parts = 1) {
   constexpr int kPlanSMs = 148;
   constexpr double kBytesPerCycle = 23.0;
   TileShape best = {1, 128};
   double least = 0.0;
-  for (int ctas = 2; ctas >= 1; --ctas)
-    for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 64) {
-      if (bn % (ctas == 2 || pair ? 128 : 64) != 0) continue;
-      const int64_t n = pair ? bn / 2 : bn;
-      const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n) * ctas, last = tiles % kPlanSMs;
-      const double rounds = (double)((tiles + kPlanSMs - 1) / kPlanSMs);
-      const double step = ctas == 2 ? (bn == 256 ? 160.0 : 110.0) : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
-      const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k + 15) / 16) * step + 2500.0);
-      const double bytes = 2.0 * planes * (double)k * (double)(rows + cols * (pair ? 2 : 1)) / (double)tiles;
-      const double memory = bytes / kBytesPerCycle * ((double)(tiles / kPlanSMs) + (last > 0 ? std::max(0.5, (double)last / kPlanSMs) : 0.0));
-      const double cycles = std::max(products, memory);
-      if (least == 0.0 || cycles < least * 0.999) {
-        best = {ctas, bn};
-        least = cycles;
+  for (int split = 1; split <= most_parts && (split == 1 || k / split >= 4 * kTileK); ++split)
+    for (int ctas = 2; ctas >= 1; --ctas)
+      for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 64) {
+        if (bn % (ctas == 2 || pair ? 128 : 64) != 0) continue;
+        const int64_t n = pair ? bn / 2 : bn;
+        const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n) * ctas * split, last = tiles % kPlanSMs;
+        const double rounds = (double)((tiles + kPlanSMs - 1) / kPlanSMs);
+        const double step = ctas == 2 ? (bn == 256 ? 160.0 : 110.0) : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
+        const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k / split + 15) / 16) * step + 2500.0);
+        const double bytes = 2.0 * planes * (double)k * (double)(rows + cols * (pair ? 2 : 1)) / (double)tiles;
+        const double memory = bytes / kBytesPerCycle * ((double)(tiles / kPlanSMs) + (last > 0 ? std::max(0.5, (double)last / kPlanSMs) : 0.0));
+        const double sums = split > 1 ? 6000.0 + 8.0 * split * (double)rows * (double)cols / (kBytesPerCycle * kPlanSMs) : 0.0;
+        const double cycles = std::max(products, memory) + sums;
+        if (least == 0.0 || cycles < least * 0.999) {
+          best = {ctas, bn, split};
+          least = cycles;
+        }
       }
-    }
   return best;
+}
+
+// Blocks of k in a part, and the parts that have any.
+inline int part_blocks_of(const TileProblem &p, const TileShape &shape) {
+  return (int)((p.segments * ((p.k + kTileK - 1) / kTileK) + shape.split - 1) / shape.split);
+}
+inline int parts_of(const TileProblem &p, const TileShape &shape) {
+  const int per = part_blocks_of(p, shape);
+  return (int)((p.segments * ((p.k + kTileK - 1) / kTileK) + per - 1) / per);
 }
 
 template <int PLANES, bool A_MN, bool B_MN, class Epilogue>
@@ -642,18 +668,19 @@ int launch_tiles(const TileProblem &p, const Epilogue &epilogue, const TileShape
     if (!encode_matrix_16(&a.b[s], p.b[s], B_MN ? kTileK : b_rows)) return HT_ERR_UNSUPPORTED;
   }
   const int64_t m_blocks = (p.rows + shape.rows() - 1) / shape.rows(), n_blocks = (p.cols + columns - 1) / columns;
-  if (m_blocks * n_blocks > 0x3fffffff || p.k > 0x3fffffff) return HT_ERR_UNSUPPORTED;
+  if (m_blocks * n_blocks * shape.split > 0x3fffffff || p.k > 0x3fffffff) return HT_ERR_UNSUPPORTED;
   a.status_word = p.status_word;
   const int n = PLANES == 3 && kPair && shape.ctas == 1 ? bn / 2 : bn;  // columns of one instruction
   a.instruction = (1u << 4) | ((p.f16 ? 0u : 1u) << 7) | ((p.f16 ? 0u : 1u) << 10) | ((A_MN ? 1u : 0u) << 15) |
                   ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(shape.rows() >> 4) << 24);
   a.m_blocks = (int)m_blocks;
   a.n_blocks = (int)n_blocks;
-  a.tiles = (int)(m_blocks * n_blocks);
+  a.tiles = (int)(m_blocks * n_blocks * parts_of(p, shape));
   a.bn = bn;
   a.k = (int)p.k;
   a.k_blocks = (int)((p.k + kTileK - 1) / kTileK);
   a.segments = p.segments;
+  a.part_blocks = part_blocks_of(p, shape);
   a.b_n0 = (int)p.b_n0;
   a.b_k0 = (int)p.b_k0;
   a.a_bytes = (uint32_t)kTileM * 128u * PLANES;

@@ -20,7 +20,7 @@ namespace {
 // The activation g and its derivative d at a.  EXACT: fp32 results; otherwise what is rounded to 16 bits afterwards.
 template <bool EXACT>
 __device__ __forceinline__ float sigmoid(float a) {
-  return EXACT ? 1.0f / (1.0f + expf(-a)) : __fdividef(1.0f, 1.0f + __expf(-a));
+  return __fdividef(1.0f, 1.0f + (EXACT ? expf(-a) : __expf(-a)));  // (a quotient of 2 ulp)
 }
 template <bool EXACT, bool SLOPE>
 __device__ __forceinline__ float activate_one(int act, float a, float &slope) {
@@ -131,8 +131,10 @@ template <typename T>
 struct GatedGradEpilogue {
   static constexpr bool kPair = true;
   static constexpr bool kExact = sizeof(T) == 4;
+  static constexpr int kBoxes = (int)kBoxBytes / (1024 * (int)sizeof(T));  // of dh that a warp's shared memory holds
   struct State {
     float scale;
+    int unit;
   };
   int rows, cols, act, first, outputs;  // the piece: outputs first .. first + cols - 1
   const T *bg, *bv;
@@ -143,7 +145,18 @@ struct GatedGradEpilogue {
   int pitch;
   size_t plane;
   float *row_sums;  // [row_sum_count][2 pitch] or null
-  __device__ __forceinline__ void begin(State &s, const Where &) const { s.scale = top != nullptr ? 1.0f / scale_of(top) : 1.0f; }
+  __device__ __forceinline__ void fetch(const Where &w, int unit) const {
+    const int r = w.row - w.lane, col = w.col + 32 * unit;
+    if (unit < w.units && r < rows && col < cols)
+      begin_box(w.box + (uint32_t)(unit % kBoxes) * 1024u * (uint32_t)sizeof(T), dh + (size_t)r * (size_t)outputs + first + col, (size_t)outputs,
+                min(32, rows - r), min(32, cols - col), align, w.lane);
+  }
+  __device__ __forceinline__ void begin(State &s, const Where &w) const {
+    s.scale = top != nullptr ? 1.0f / scale_of(top) : 1.0f;
+    s.unit = 0;
+#pragma unroll
+    for (int i = 0; i < kBoxes; ++i) fetch(w, i);  // (a tile has two units at the most)
+  }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
     const int n = cols - col;
     if (n <= 0) return;
@@ -151,8 +164,12 @@ struct GatedGradEpilogue {
     add_bias(bv, first + col, n, u);
     float act_a[32], slope[32], dh_[32];
     activate<kExact, true>(act, a, act_a, slope);
-    const int top = w.row - w.lane;
-    if (top < rows) load_box(w, dh + (size_t)top * (size_t)outputs + first + col, (size_t)outputs, min(32, rows - top), min(32, n), align, dh_);
+    const int r = w.row - w.lane;
+    if (r < rows)
+      finish_box(w.box + (uint32_t)(s.unit % kBoxes) * 1024u * (uint32_t)sizeof(T), dh + (size_t)r * (size_t)outputs + first + col, (size_t)outputs,
+                 min(32, rows - r), min(32, n), align, w.lane, dh_);
+    ++s.unit;
+    if (kBoxes == 1) fetch(w, s.unit);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float d = dh_[i] * s.scale;
@@ -212,7 +229,7 @@ struct Plan {
   int64_t piece = 0, pitch = 0;
   typename Kind<T>::Operand *g = nullptr;
   uint32_t *top = nullptr;
-  float *alpha = nullptr, *sum = nullptr, *row_sums = nullptr;
+  float *alpha = nullptr, *sum = nullptr, *parts = nullptr, *row_sums = nullptr;
   size_t bytes;
   Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, void *ws) {
     Arena arena(ws);
@@ -224,13 +241,17 @@ struct Plan {
     if (backward) {
       const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
       const int64_t per_output = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 4;
-      piece = std::max<int64_t>(limit / per_output / 256 * 256, 256);
-      if (piece >= p.outputs) piece = p.outputs;
+      piece = piece_of(p.outputs, limit / per_output);
       pitch = round_up(piece, 64);
       g = arena.template take<typename Kind<T>::Operand>(p.rows * 2 * pitch * Kind<T>::kPlanes);
       top = arena.take<uint32_t>(1);
       alpha = arena.take<float>(1);
       sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
+      int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, 2 * p.outputs, Kind<T>::kPlanes);
+      for (const int64_t count : {piece, (p.outputs - 1) % piece + 1})
+        for (const int64_t height : {count, pitch + count})  // one weight's gradient, both
+          most = std::max(most, product_parts(height, p.features, std::max<int64_t>(p.rows, 1), Kind<T>::kPlanes));
+      if (most > 0) parts = arena.take<float>(most);
       row_sums = has_bias ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * 2 * pitch) : nullptr;
     }
     bytes = arena.used;
@@ -334,7 +355,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
       store.rows = store.part = (int)p.rows;
       store.out = static_cast<T *>(out.dx), store.align = row_alignment(store.out, p.features * (int64_t)sizeof(T));
       store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
-      if ((rc = product_dx<T>(q, store, sms, stream)) != HT_OK) return rc;
+      if ((rc = product_dx<T>(q, store, plan.piece < p.outputs ? nullptr : plan.parts, sms, stream)) != HT_OK) return rc;
     }
     if (dwg != nullptr || dwv != nullptr) {
       // rows of the product: da's columns, then du's; one of the two weights alone takes its half
@@ -352,7 +373,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
       store.out2 = both ? dwv + (size_t)first * (size_t)p.features : nullptr;
       store.align = std::min(row_alignment(dwg, p.features * (int64_t)sizeof(T)), row_alignment(dwv, p.features * (int64_t)sizeof(T)));
       store.sum = nullptr, store.keep = false;
-      if ((rc = product_dw<T>(q, store, sms, stream)) != HT_OK) return rc;
+      if ((rc = product_dw<T>(q, store, plan.parts, sms, stream)) != HT_OK) return rc;
     }
     const int64_t blocks = row_sum_count(p.rows, shape);
     if (dbg != nullptr && (rc = column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, alpha, dbg + first, stream)) != HT_OK) return rc;
