@@ -55,7 +55,7 @@ struct LossEpilogue {
   float2 *partial;      // [rows][slots], slots = 2 n_blocks
   int slots;
   float *target_score;  // [rows]
-  __device__ __forceinline__ void begin(State &s, const Where &w) const {
+  __device__ __forceinline__ void begin(State &s, const Where &w, bool) const {
     s.m = -INFINITY, s.l = 0.0f, s.target = -1;
     if (w.inside) {
       const int64_t t = __ldg(target + w.row);
@@ -117,7 +117,7 @@ struct LossGradEpilogue {
   int pitch;
   size_t plane;
   float *row_sums;  // [row_sum_count][pitch] or null
-  __device__ __forceinline__ void begin(State &s, const Where &w) const {
+  __device__ __forceinline__ void begin(State &s, const Where &w, bool) const {
     s.r = {0.0f, 0.0f, 0.0f, -1};
     if (w.inside) {
       const float4 q = __ldg(reinterpret_cast<const float4 *>(row_grad + w.row));

@@ -243,7 +243,7 @@ __device__ __forceinline__ void load_box(const Where &w, const T *first, size_t 
   __syncwarp();
 }
 // load_box in two halves: begun early (cp.async, for rows on 4 bytes at least; others wait for the second half), and finished into
-// registers.  A box takes 1024 sizeof(T) bytes at `at`.
+// registers: `last`, or another box has been begun since.  A box takes 1024 sizeof(T) bytes at `at`.
 template <typename T, int BYTES>
 __device__ __forceinline__ void fetch_box(uint32_t at, const T *first, size_t pitch, int rows, int cols, int lane) {
   constexpr int kPerRow = 32 * (int)sizeof(T) / BYTES, kRows = 32 / kPerRow, kValues = BYTES / (int)sizeof(T);
@@ -271,11 +271,15 @@ __device__ __forceinline__ void begin_box(uint32_t at, const T *first, size_t pi
   asm volatile("cp.async.commit_group;" ::: "memory");
 }
 template <typename T>
-__device__ __forceinline__ void finish_box(uint32_t at, const T *first, size_t pitch, int rows, int cols, int align, int lane, float (&v)[32]) {
+__device__ __forceinline__ void finish_box(uint32_t at, const T *first, size_t pitch, int rows, int cols, int align, int lane, bool last, float (&v)[32]) {
   constexpr int kStep = 32 / (int)sizeof(T);
-  if (align >= 4)
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  else
+  if (align >= 4) {
+    if (last)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    else
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+  } else
+  
     move_box_by<T, false>(at, const_cast<T *>(first), pitch, rows, cols, align, lane);
   __syncwarp();
 #pragma unroll
@@ -360,7 +364,7 @@ struct StoreEpilogue {
   int align, sum_align;
   float *parts;        // [parts of k][rows][pitch]: sums that another kernel adds, or null
   int parts_pitch;
-  __device__ __forceinline__ void begin(State &s, const Where &) const { s.alpha = alpha != nullptr ? __ldg(alpha) : 1.0f; }
+  __device__ __forceinline__ void begin(State &s, const Where &, bool) const { s.alpha = alpha != nullptr ? __ldg(alpha) : 1.0f; }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
     const int top = w.row - w.lane, row = top < split ? top : top - split;
     const int m = min(32, min(part - row, rows - top)), n = min(32, cols - col);

@@ -141,6 +141,7 @@ struct Where {
   uint32_t box;  // shared memory of the warp
   int col;       // the first of this half's columns
   int units;     // of 32 columns in this half
+  int next_row, next_col;  // the same of this warp's next tile; beyond the matrix where there is none
   int m_block, n_block, part, half, quarter, lane;
 };
 
@@ -499,7 +500,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       __syncwarp();
       if (lane == 0) {
         if constexpr (CTAS == 2)
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(of_first_cta(bar)) : "memory");
+          // (relaxed: what is handed back is tensor memory that has been read; a release would wait for the stores of the tile before)
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(of_first_cta(bar)) : "memory");
         else
           mbar_arrive(bar);
       }
@@ -513,7 +515,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       typename Epilogue::State state;
       const int col0 = w.n_block * (kPair ? a.bn / 2 : a.bn);
       w.col = col0 + half * units * 32;
-      epilogue.begin(state, w);  // under the tile's products
+      w.next_row = 0x7fffffff, w.next_col = 0;
+      if (tile + tile_step < a.tiles) {
+        const Turn next = place(tile + tile_step);
+        w.next_row = (next.mb * CTAS + rank) * kTileM + quarter * 32 + lane;
+        w.next_col = next.nb * (kPair ? a.bn / 2 : a.bn) + half * units * 32;
+      }
+      epilogue.begin(state, w, tile == first_tile);  // under the tile's products
       if constexpr (!kThree) {
         if (!wait_for(chunk)) break;
         const uint32_t acc = lanes + (chunk & 1u) * 256u;

@@ -80,7 +80,7 @@ struct GatedEpilogue {
   const T *bg, *bv;
   T *h;  // [rows, cols]
   int align;
-  __device__ __forceinline__ void begin(State &, const Where &) const {}
+  __device__ __forceinline__ void begin(State &, const Where &, bool) const {}
   __device__ __forceinline__ void unit(State &, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
     const int n = cols - col;
     if (n <= 0) return;
@@ -145,31 +145,36 @@ struct GatedGradEpilogue {
   int pitch;
   size_t plane;
   float *row_sums;  // [row_sum_count][2 pitch] or null
-  __device__ __forceinline__ void fetch(const Where &w, int unit) const {
-    const int r = w.row - w.lane, col = w.col + 32 * unit;
-    if (unit < w.units && r < rows && col < cols)
-      begin_box(w.box + (uint32_t)(unit % kBoxes) * 1024u * (uint32_t)sizeof(T), dh + (size_t)r * (size_t)outputs + first + col, (size_t)outputs,
-                min(32, rows - r), min(32, cols - col), align, w.lane);
+  __device__ __forceinline__ void fetch(const Where &w, int slot, int row, int col) const {
+    const int r = row - w.lane;
+    const bool some = r < rows && col < cols;
+    begin_box(w.box + (uint32_t)slot * 1024u * (uint32_t)sizeof(T), dh + (some ? (size_t)r * (size_t)outputs + first + col : 0), (size_t)outputs,
+              some ? min(32, rows - r) : 0, min(32, cols - col), align, w.lane);
   }
-  __device__ __forceinline__ void begin(State &s, const Where &w) const {
+  __device__ __forceinline__ void begin(State &s, const Where &w, bool first_tile) const {
     s.scale = top != nullptr ? 1.0f / scale_of(top) : 1.0f;
     s.unit = 0;
-#pragma unroll
-    for (int i = 0; i < kBoxes; ++i) fetch(w, i);  // (a tile has two units at the most)
+    if (first_tile)  // later ones have been fetched under the tile before
+      for (int i = 0; i < min(kBoxes, w.units); ++i) fetch(w, i, w.row, w.col + 32 * i);
   }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&a)[32], float (&u)[32]) const {
     const int n = cols - col;
+    float dh_[32];
+    const int r = w.row - w.lane, boxes = min(kBoxes, w.units), slot = s.unit % kBoxes;
+    finish_box(w.box + (uint32_t)slot * 1024u * (uint32_t)sizeof(T), dh + (r < rows ? (size_t)r * (size_t)outputs + first + col : 0), (size_t)outputs,
+               r < rows ? min(32, rows - r) : 0, min(32, n), align, w.lane, boxes == 1, dh_);
+    // its place is free for the unit `boxes` further on, of this tile or the next
+    const int then = s.unit + boxes;
+    if (then < w.units)
+      fetch(w, slot, w.row, w.col + 32 * then);
+    else
+      fetch(w, slot, w.next_row, w.next_col + 32 * (then - w.units));
+    ++s.unit;
     if (n <= 0) return;
     add_bias(bg, first + col, n, a);
     add_bias(bv, first + col, n, u);
-    float act_a[32], slope[32], dh_[32];
+    float act_a[32], slope[32];
     activate<kExact, true>(act, a, act_a, slope);
-    const int r = w.row - w.lane;
-    if (r < rows)
-      finish_box(w.box + (uint32_t)(s.unit % kBoxes) * 1024u * (uint32_t)sizeof(T), dh + (size_t)r * (size_t)outputs + first + col, (size_t)outputs,
-                 min(32, rows - r), min(32, n), align, w.lane, dh_);
-    ++s.unit;
-    if (kBoxes == 1) fetch(w, s.unit);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float d = dh_[i] * s.scale;
