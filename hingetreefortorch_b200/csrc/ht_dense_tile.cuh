@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
             load_3d<CTAS>(one, at, am, k0, m0, bar);
           }
           if (B_MN) {
-            for (int g = 0; g < a.bn / (64 * CTAS); ++g) load_3d<CTAS>(one, bt + (uint32_t)g * (8192u * PLANES), bm, n0 + 64 * g, a.b_k0 + k0, bar);
+            for (int g = 0; g < (a.bn / CTAS + 63) / 64; ++g) load_3d<CTAS>(one, bt + (uint32_t)g * (8192u * PLANES), bm, n0 + 64 * g, a.b_k0 + k0, bar);
           } else if (kPair) {
             load_3d<CTAS>(one, bt, &a.b[rank], k0, n0, bar);
             if (CTAS == 1) load_3d<CTAS>(one, bt + (uint32_t)half * 128u * PLANES, &a.b[1], k0, n0, bar);
@@ -484,7 +484,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
     const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp may only touch the lanes 32 (warp % 4) ...
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     uint32_t chunk = 0;
-    const int units = kPair ? a.bn / 128 : a.bn / 64;  // of 32 columns (a pair: 32 of each), for this half
+    // of 32 columns (a pair: 32 of each), the first half of them, rounded up, for one of the two warps
+    const int all_units = kPair ? a.bn / 64 : a.bn / 32, unit0 = half * ((all_units + 1) / 2), units = (all_units + 1 - half) / 2;
     Where w;
     w.half = half, w.quarter = quarter, w.lane = lane, w.units = units;
     w.box = stages + kStageBudget + (uint32_t)(warp - 2) * kBoxBytes;
@@ -514,12 +515,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       w.inside = w.row < epilogue.rows;
       typename Epilogue::State state;
       const int col0 = w.n_block * (kPair ? a.bn / 2 : a.bn);
-      w.col = col0 + half * units * 32;
+      w.col = col0 + unit0 * 32;
       w.next_row = 0x7fffffff, w.next_col = 0;
       if (tile + tile_step < a.tiles) {
         const Turn next = place(tile + tile_step);
         w.next_row = (next.mb * CTAS + rank) * kTileM + quarter * 32 + lane;
-        w.next_col = next.nb * (kPair ? a.bn / 2 : a.bn) + half * units * 32;
+        w.next_col = next.nb * (kPair ? a.bn / 2 : a.bn) + unit0 * 32;
       }
       epilogue.begin(state, w, tile == first_tile);  // under the tile's products
       if constexpr (!kThree) {
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
         const uint32_t acc = lanes + (chunk & 1u) * 256u;
 #pragma unroll 1
         for (int u = 0; u < units; ++u) {
-          const int c = (half * units + u) * 32;
+          const int c = (unit0 + u) * 32;
           float v[32];
           tmem_load_32(acc + (uint32_t)c, v);
           if constexpr (kPair) {
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
         for (int u = 0; u < kMostUnits; ++u)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[u][i] = 0.0f;
-        auto column = [&](int u) { return kPair ? (u & 1) * (a.bn / 2) + (half * units + (u >> 1)) * 32 : (half * units + u) * 32; };
+        auto column = [&](int u) { return kPair ? (u & 1) * (a.bn / 2) + (unit0 + (u >> 1)) * 32 : (unit0 + u) * 32; };
         bool there = true;
         const int chunks = (turn.last - turn.first + kChunkBlocks - 1) / kChunkBlocks;
         for (int c = 0; c <= chunks; ++c) {
@@ -568,14 +569,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           release(c < chunks ? &drained[0] : drained_small);
         }
         if (!there) break;
+        // one copy of the epilogue's code, and the columns pass by: four copies did not stay in the instruction cache
+        constexpr int kAtOnce = kPair ? 2 : 1;
+#pragma unroll 1
+        for (int u = 0; u < parts; u += kAtOnce) {
+          if constexpr (kPair)
+            epilogue.unit(state, w, col0 + column(u), sum[0], sum[1]);
+          else
+            epilogue.unit(state, w, col0 + column(u), sum[0]);
 #pragma unroll
-        for (int u = 0; u < kMostUnits; ++u) {
-          if (u >= parts) break;
-          if constexpr (kPair) {
-            if ((u & 1) == 0) epilogue.unit(state, w, col0 + column(u), sum[u], sum[u + 1]);
-          } else {
-            epilogue.unit(state, w, col0 + column(u), sum[u]);
-          }
+          for (int q = 0; q + kAtOnce < kMostUnits; ++q)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[q][i] = sum[q + kAtOnce][i];
         }
       }
       epilogue.end(state, w);
@@ -625,7 +630,7 @@ inline int sm_count(int *sms) {
 }
 
 // How to cut a product: the shape with which the SMs are done first.  Cycles of a step of 16 values of k, measured: a pair of CTAs with 256
-// columns 160, with 128 columns 110; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120 (three planes: 6 of those, of
+// columns 160, with 128 columns 110, in steps of 32 between; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120 (three planes: 6 of those, of
 // 128 columns at the most alone).  A tile costs about 2500 cycles besides.  Against that, the operands have to come from memory once,
 // 23 bytes a cycle and SM where all read, twice that where few do.  Where `most_parts` allows it, k is cut as well: each part writes its
 // sums in fp32, and a kernel adds them (8 bytes a value and part, and about 6000 cycles).
@@ -636,12 +641,12 @@ inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, b
   double least = 0.0;
   for (int split = 1; split <= most_parts && (split == 1 || k / split >= 4 * kTileK); ++split)
     for (int ctas = 2; ctas >= 1; --ctas)
-      for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 64) {
-        if (bn % (ctas == 2 || pair ? 128 : 64) != 0) continue;
+      for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 32) {
+        if (bn % (ctas == 2 ? (pair ? 64 : 32) : pair ? 128 : 64) != 0) continue;
         const int64_t n = pair ? bn / 2 : bn;
         const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n) * ctas * split, last = tiles % kPlanSMs;
         const double rounds = (double)((tiles + kPlanSMs - 1) / kPlanSMs);
-        const double step = ctas == 2 ? (bn == 256 ? 160.0 : 110.0) : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
+        const double step = ctas == 2 ? 60.0 + 0.39 * bn : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
         const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k / split + 15) / 16) * step + 2500.0);
         const double bytes = 2.0 * planes * (double)k * (double)(rows + cols * (pair ? 2 : 1)) / (double)tiles;
         const double memory = bytes / kBytesPerCycle * ((double)(tiles / kPlanSMs) + (last > 0 ? std::max(0.5, (double)last / kPlanSMs) : 0.0));
@@ -654,6 +659,8 @@ inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, b
       }
   return best;
 }
+
+constexpr int round_up_to(int v, int to) { return (v + to - 1) / to * to; }
 
 // Blocks of k in a part, and the parts that have any.
 inline int part_blocks_of(const TileProblem &p, const TileShape &shape) {
@@ -692,7 +699,7 @@ int launch_tiles(const TileProblem &p, const Epilogue &epilogue, const TileShape
   a.b_n0 = (int)p.b_n0;
   a.b_k0 = (int)p.b_k0;
   a.a_bytes = (uint32_t)kTileM * 128u * PLANES;
-  a.stage_bytes = a.a_bytes + (uint32_t)(bn / shape.ctas) * 128u * PLANES;
+  a.stage_bytes = a.a_bytes + (uint32_t)(B_MN ? round_up_to(bn / shape.ctas, 64) : bn / shape.ctas) * 128u * PLANES;
   a.stages = (int)std::min<uint32_t>(kStageBudget / a.stage_bytes, kMostStages);
   const dim3 grid((unsigned)(shape.ctas * std::min(a.tiles, std::max(sms / shape.ctas, 1))));
   return shape.ctas == 2 ? launch_next(dense_tile_kernel<2, PLANES, A_MN, B_MN, Epilogue>, grid, kTileThreads, kTileSmem, stream, 2, a, epilogue)
