@@ -182,6 +182,19 @@ struct FewLossEpilogue {
       }
     }
   }
+  // rows that no other warp has
+  __device__ __forceinline__ void end_alone(State<1> &s, int row0, int lane) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, s.m[0][i], d), l = __shfl_xor_sync(0xffffffffu, s.l[0][i], d);
+        join(s.m[0][i], s.l[0][i], m, l);
+      }
+      const int row = row0 + 2 * lane + i;
+      if (lane < 4 && row < rows) partial[(size_t)row * (size_t)slots + blockIdx.x] = make_float2(s.m[0][i], s.l[0][i]);
+    }
+  }
   template <int NT>
   __device__ __forceinline__ void end(State<NT> &s, int row0, int lane) const {
     // the lanes with the same rows, then (each warp has its own outputs) the warps: a block's scores are one piece
@@ -330,7 +343,8 @@ struct ForwardPlan {
   size_t bytes;
   ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, void *ws) {
     Arena arena(ws);
-    few = few_rows<T>(p.rows, p.features, p.outputs, false, &few_plan);
+    few = few_rows<T>(p.rows, p.features, p.outputs, false, &few_plan) ||
+          some_rows<T>(p.rows, p.features, p.outputs, p.x_stride, false, &few_plan);
     if (!few) {
       x.set(arena, xp, p.rows, p.features, p.x_stride);
       w.set(arena, wp, p.outputs, p.features, p.features);
@@ -355,11 +369,10 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
     if (plan.few) {
       const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(w), nullptr}, p.x_stride, (int)p.rows, (int)p.features, (int)p.outputs};
       const FewLossEpilogue<T> e = {(int)p.rows, plan.slots, static_cast<const T *>(bias), target, plan.partial, plan.target_score};
-      if ((rc = launch_few(a, e, plan.few_plan, stream)) != HT_OK) return rc;
+      HT_TRY(launch_rows(a, e, plan.few_plan, stream));
     } else {
       if ((rc = sm_count(&sms)) != HT_OK) return rc;
-      if ((rc = plan.x.lay_out(stream)) != HT_OK) return rc;
-      if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
+      HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
       TileProblem t;
       t.a[0] = plan.x.m;
       t.b[0] = plan.w.m;
@@ -424,8 +437,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
   }
   int sms = 0, rc;
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  if ((rc = plan.x.lay_out(stream)) != HT_OK) return rc;
-  if ((rc = plan.w.lay_out(stream)) != HT_OK) return rc;
+  HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
   const float unit = p.dtype == HT_DTYPE_F16 ? 16384.0f : 1.0f;
   if (reduction == HT_REDUCTION_NONE) {
     HT_TRY(launch_next(row_scale_kernel, dim3(1), 1024, 0, stream, 1, grad, p.rows, unit, plan.alpha));
@@ -452,7 +464,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     Matrix g;
     g.data = plan.g, g.rows = p.rows, g.cols = count, g.pitch = plan.pitch, g.planes = kPlanes, g.plane = p.rows * plan.pitch;
     StoreEpilogue<T> store = {};
-    store.alpha = plan.alpha;
+    store.scale.number = plan.alpha;
     store.cols = (int)p.features;
     store.split = 0x7fffffff;
     store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));
@@ -475,8 +487,8 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
       store.sum = nullptr, store.keep = false;
       if ((rc = product_dw<T>(q, store, plan.parts, sms, stream)) != HT_OK) return rc;
     }
-    if (db != nullptr && (rc = column_sums<T>(plan.row_sums, row_sum_count(p.rows, shape), plan.pitch, count, plan.alpha, db + first, stream)) != HT_OK)
-      return rc;
+    if (db != nullptr)
+      HT_TRY(column_sums<T>(plan.row_sums, row_sum_count(p.rows, shape), plan.pitch, count, store.scale, db + first, nullptr, plan.pitch, stream));
   }
   return HT_OK;
 }

@@ -347,6 +347,20 @@ __device__ __forceinline__ float sum_rows(const float (&v)[32], int lane) {
   return h[0];
 }
 
+// What gradients are multiplied by when they leave: a number on the device, or the power of two at or below the number whose bits
+// are at `top` (1 where that is no normal number), or 1.
+struct Scale {
+  const float *number = nullptr;
+  const uint32_t *top = nullptr;
+  __device__ __forceinline__ float value() const {
+    if (top != nullptr) {
+      const uint32_t e = __ldg(top) & 0x7f800000u;
+      return e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
+    }
+    return number != nullptr ? __ldg(number) : 1.0f;
+  }
+};
+
 // ---- epilogue: the products themselves, scaled -----------------------------------------------------------------------
 // out = alpha (acc + products): `sum` holds what earlier pieces of k have given, in fp32; `keep`: the sum goes on (then all rows go to one matrix).
 template <typename T>
@@ -358,13 +372,13 @@ struct StoreEpilogue {
   int rows, cols;
   T *out, *out2;       // [part, cols] each: of the products' rows, those from `split` (a multiple of 32) on go to out2
   int split, part;
-  const float *alpha;  // on the device; null: 1
+  Scale scale;
   float *sum;          // [rows, cols] or null
   bool begins, keep;   // the first piece of a sum, not the last one
   int align, sum_align;
   float *parts;        // [parts of k][rows][pitch]: sums that another kernel adds, or null
   int parts_pitch;
-  __device__ __forceinline__ void begin(State &s, const Where &, bool) const { s.alpha = alpha != nullptr ? __ldg(alpha) : 1.0f; }
+  __device__ __forceinline__ void begin(State &s, const Where &, bool) const { s.alpha = scale.value(); }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
     const int top = w.row - w.lane, row = top < split ? top : top - split;
     const int m = min(32, min(part - row, rows - top)), n = min(32, cols - col);
@@ -397,7 +411,7 @@ struct StoreEpilogue {
 template <typename T>
 __global__ void __launch_bounds__(256) add_parts_kernel(const StoreEpilogue<T> e, int count) {
   after_previous_kernel();
-  const float alpha = e.alpha != nullptr ? __ldg(e.alpha) : 1.0f;
+  const float alpha = e.scale.value();
   const int quads = e.parts_pitch / 4;
   const int64_t n = (int64_t)e.rows * quads, step = (int64_t)gridDim.x * 256;
   const size_t plane = (size_t)e.rows * (size_t)e.parts_pitch;
@@ -466,24 +480,34 @@ struct Operand {
     copy = arena.template take<typename Kind<T>::Operand>(m.plane * m.planes);
     m.data = copy;
   }
-  int lay_out(cudaStream_t stream) const;
+};
+
+// The copies of a call's operands, all in one launch.
+template <typename T>
+struct LayOut {
+  struct Job {
+    const T *source;
+    typename Kind<T>::Operand *copy;
+    int64_t rows, cols, stride, pitch, plane, ignore;
+    const int64_t *target;
+    bool whole;  // rows of the source start on 16 bytes
+  } jobs[3];
 };
 
 // 8 columns a thread.  x is read once, the copy written once: 10 bytes a value from fp32, 4 from 16 bits.
 template <typename T>
-__global__ void __launch_bounds__(256) lay_out_kernel(const T *__restrict__ x, int64_t rows, int64_t cols, int64_t stride, int64_t pitch,
-                                                      int64_t plane, typename Kind<T>::Operand *__restrict__ copy,
-                                                      const int64_t *__restrict__ target, int64_t ignore, bool whole) {
+__global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ LayOut<T> all) {
   after_previous_kernel();
-  const int64_t per_row = pitch / 8, n = rows * per_row;
+  const typename LayOut<T>::Job &a = all.jobs[blockIdx.y];
+  const int64_t per_row = a.pitch / 8, n = a.rows * per_row;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / per_row, c = (i - r * per_row) * 8;
     float v[8];
-    const T *from = x + r * stride + c;
-    if (target != nullptr && __ldg(target + r) == ignore) {
+    const T *from = a.source + r * a.stride + c;
+    if (a.target != nullptr && __ldg(a.target + r) == a.ignore) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    } else if (whole && c + 8 <= cols) {
+    } else if (a.whole && c + 8 <= a.cols) {
       T t[8];
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(from));
@@ -495,9 +519,9 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const T *__restrict__ x, i
       for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_float(from[j]) : 0.0f;
+      for (int j = 0; j < 8; ++j) v[j] = c + j < a.cols ? to_float(from[j]) : 0.0f;
     }
-    typename Kind<T>::Operand *to = copy + r * pitch + c;
+    typename Kind<T>::Operand *to = a.copy + r * a.pitch + c;
     if constexpr (Kind<T>::kPlanes == 1) {
       *reinterpret_cast<uint4 *>(to) = make_uint4(pack_pair(v[0], v[1], to), pack_pair(v[2], v[3], to), pack_pair(v[4], v[5], to), pack_pair(v[6], v[7], to));
     } else {
@@ -506,53 +530,63 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const T *__restrict__ x, i
       for (int j = 0; j < 8; ++j) split_planes(v[j], p[0][j], p[1][j], p[2][j]);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
-        *reinterpret_cast<uint4 *>(to + q * plane) =
+        *reinterpret_cast<uint4 *>(to + q * a.plane) =
             make_uint4(pack_pair(p[q][0], p[q][1], to), pack_pair(p[q][2], p[q][3], to), pack_pair(p[q][4], p[q][5], to), pack_pair(p[q][6], p[q][7], to));
     }
   }
 }
-
-// Sums of 32 rows that an epilogue leaves for these rows: of every tile's, inside the matrix or not.
-inline int64_t row_sum_count(int64_t rows, const TileShape &shape) { return (rows + shape.rows() - 1) / shape.rows() * shape.rows() / 32; }
 
 inline unsigned blocks_for(int64_t work, int64_t per_block, int64_t most) {
   return (unsigned)std::min<int64_t>(std::max<int64_t>((work + per_block - 1) / per_block, 1), most);
 }
 
 template <typename T>
-int Operand<T>::lay_out(cudaStream_t stream) const {
-  if (copy == nullptr || m.rows == 0) return HT_OK;
-  const bool whole = (reinterpret_cast<uintptr_t>(source) & 15u) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
-  const int64_t work = m.rows * (m.pitch / 8);
-  HT_TRY(launch_next(lay_out_kernel<T>, dim3(blocks_for(work, 256, 148 * 16)), 256, 0, stream, 1, source, m.rows, m.cols, stride, m.pitch, m.plane, copy, target, ignore, whole));
-  return HT_OK;
+int lay_out(std::initializer_list<const Operand<T> *> operands, cudaStream_t stream) {
+  LayOut<T> all = {};
+  int64_t most = 0;
+  unsigned count = 0;
+  for (const Operand<T> *o : operands) {
+    if (o->copy == nullptr || o->m.rows == 0) continue;
+    const bool whole = (reinterpret_cast<uintptr_t>(o->source) & 15u) == 0 && o->stride * (int64_t)sizeof(T) % 16 == 0;
+    all.jobs[count++] = {o->source, o->copy, o->m.rows, o->m.cols, o->stride, o->m.pitch, o->m.plane, o->ignore, o->target, whole};
+    most = std::max(most, o->m.rows * (o->m.pitch / 8));
+  }
+  if (count == 0) return HT_OK;
+  return launch_next(lay_out_kernel<T>, dim3(blocks_for(most, 256, 148 * 16), count), 256, 0, stream, 1, all);
 }
 
-// Column sums from the sums of 32 rows each that the epilogues leave: out[c] = alpha sum_r partial[r, c], r ascending in 8
-// strands that are added in order.  32 columns a block.
+// Sums of 32 rows that an epilogue leaves for these rows: of every tile's, inside the matrix or not.
+inline int64_t row_sum_count(int64_t rows, const TileShape &shape) { return (rows + shape.rows() - 1) / shape.rows() * shape.rows() / 32; }
+
+// Column sums from the sums of 32 rows each that the epilogues leave: out[c] = alpha sum_r partial[r, c], r in 8 strands,
+// ascending in each, that are added in order.  32 columns a block; columns from `second` on go to out2.
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols,
-                                                          const float *__restrict__ alpha, T *__restrict__ out) {
+__global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols, int64_t second,
+                                                          Scale scale, T *__restrict__ out, T *__restrict__ out2) {
   after_previous_kernel();
   __shared__ float strand[8][33];
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane, part = c < second ? c : c - second;
+  T *const to = c < second ? out : out2;
+  const bool inside = part < cols && to != nullptr;
   float sum = 0.0f;
-  if (c < cols)
+  if (inside)
+#pragma unroll 4
     for (int64_t r = y; r < rows; r += 8) sum += __ldg(partial + r * pitch + c);
   strand[y][lane] = sum;
   __syncthreads();
-  if (y == 0 && c < cols) {
+  if (y == 0 && inside) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) sum += strand[i][lane];
-    out[c] = from_float<T>((alpha != nullptr ? __ldg(alpha) : 1.0f) * sum);
+    to[part] = from_float<T>(scale.value() * sum);
   }
 }
 
+// (out2: the sums from column `second` on; null, or one of the two null: those are not wanted)
 template <typename T>
-int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols, const float *alpha, T *out, cudaStream_t stream) {
-  HT_TRY(launch_next(column_sums_kernel<T>, dim3((unsigned)((cols + 31) / 32)), 256, 0, stream, 1, partial, rows, pitch, cols, alpha, out));
-  return HT_OK;
+int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols, const Scale &scale, T *out, T *out2, int64_t second, cudaStream_t stream) {
+  return launch_next(column_sums_kernel<T>, dim3((unsigned)(((out2 != nullptr ? second : 0) + cols + 31) / 32)), 256, 0, stream, 1, partial, rows, pitch, cols,
+                     second, scale, out, out2);
 }
 
 // Outputs of a piece where `most` fit the bound: all of them, or pieces of whole tiles, about equal, 256 at the least.

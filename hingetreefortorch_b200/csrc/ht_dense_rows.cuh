@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
   epilogue.template end<NT>(state, row0, lane);
 }
 
-// How few rows are computed: n-tiles of 8 rows, row groups, blocks.
+// How few rows are computed: tiles of 8 rows (0: by some_rows_kernel), blocks, bytes of a row of x, warps that share weights.
 struct FewPlan {
   int tiles, blocks, pitch, split;
 };
@@ -244,6 +244,107 @@ int launch_few(FewArgs<T> a, const Epilogue &e, const FewPlan &plan, cudaStream_
                              : run(few_rows_kernel<T, 4, kFull, Epilogue>);
   };
   return a.features * (int64_t)sizeof(T) % 16 == 0 ? by_tiles(std::true_type()) : by_tiles(std::false_type());
+}
+
+// ---- some more rows, few weights --------------------------------------------------------------------------------------
+// fp32, up to 128 rows: a tile of 128 rows would have a handful of SMs walk k through three planes (100 rows, 1000 to 2 x 700: 35 us).  Here a
+// block takes 16 rows of the weights (of a pair: 8 of each), its 16 warps take 64 rows of x each and share k, and x comes straight
+// from L2 in the instruction's layout, since no warp uses what another does.  A warp's chain of additions in the tensor core is
+// at most 96 long (k <= 2048), which loses 1e-6 of a sum at the worst; the warps' sums are added in fp32, 8 rows a warp.
+// What bounds it: rows x k from L2 for every 16 rows of the weights, and the latency of a few loads in a row.
+constexpr int kSomeTiles = 8;  // of 8 rows a warp
+
+template <typename T, class Epilogue>
+__global__ void __launch_bounds__(kFewThreads, 1) some_rows_kernel(const FewArgs<T> a, const Epilogue epilogue) {
+  constexpr bool kPair = Epilogue::kPair;
+  constexpr int kOutputs = kPair ? 8 : 16, kStep = 16;
+  static_assert(std::is_same<T, float>::value, "16-bit rows take the tiles");
+  extern __shared__ __align__(128) unsigned char few_smem[];
+  float4 *const sums = reinterpret_cast<float4 *>(few_smem);  // [warps][tiles][32]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  const int part = warp % a.split, row0 = warp / a.split * (8 * kSomeTiles);
+  const int steps = (a.features + kStep - 1) / kStep, groups = (a.outputs + kOutputs - 1) / kOutputs;
+  after_previous_kernel();
+  typename Epilogue::template State<1> state;
+  epilogue.begin(state);
+  for (int group = (int)blockIdx.x; group < groups; group += (int)gridDim.x) {
+    const int o = group * kOutputs + g;
+    const T *row_a = a.w[0] + (int64_t)min(o, a.outputs - 1) * a.features;
+    const T *row_b = kPair ? a.w[1] + (int64_t)min(o, a.outputs - 1) * a.features : a.w[0] + (int64_t)min(o + 8, a.outputs - 1) * a.features;
+    float c[kSomeTiles][4];
+#pragma unroll
+    for (int n = 0; n < kSomeTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[n][i] = 0.0f;
+    for (int s = part; s < steps; s += a.split) {
+      const int k = s * kStep + j * 4;
+      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+      const bool there = k < a.features;
+      const uint4 qa = there ? __ldg(reinterpret_cast<const uint4 *>(row_a + k)) : zero, qb = there ? __ldg(reinterpret_cast<const uint4 *>(row_b + k)) : zero;
+      uint4 q[kSomeTiles];
+#pragma unroll
+      for (int n = 0; n < kSomeTiles; ++n) {
+        const int r = row0 + 8 * n + g;
+        q[n] = there && r < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)r * a.x_stride + k)) : zero;
+      }
+      const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
+#pragma unroll
+      for (int h = 0; h < 4; h += 2) {
+        uint32_t high[4], low[4];
+        split_tf32(wa[h], high[0], low[0]);
+        split_tf32(wb[h], high[1], low[1]);
+        split_tf32(wa[h + 1], high[2], low[2]);
+        split_tf32(wb[h + 1], high[3], low[3]);
+#pragma unroll
+        for (int n = 0; n < kSomeTiles; ++n) {
+          const uint32_t x[4] = {q[n].x, q[n].y, q[n].z, q[n].w};
+          uint32_t h0, l0, h1, l1;
+          split_tf32(x[h], h0, l0);
+          split_tf32(x[h + 1], h1, l1);
+          mma_few<T>(c[n], low, h0, h1);
+          mma_few<T>(c[n], high, l0, l1);
+          mma_few<T>(c[n], high, h0, h1);
+        }
+      }
+    }
+    __syncthreads();  // the sums of the group before have been read
+#pragma unroll
+    for (int n = 0; n < kSomeTiles; ++n) sums[(warp * kSomeTiles + n) * 32 + lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+    __syncthreads();
+    if (part < kSomeTiles) {  // this warp: the tile `part` of its rows
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = 0; i < a.split; ++i) {
+        const float4 t = sums[((warp - part + i) * kSomeTiles + part) * 32 + lane];
+        v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+      }
+      epilogue.template values<1>(state, 0, row0 + 8 * part + 2 * j, o, a.outputs, v);
+    }
+  }
+  if (part < kSomeTiles) epilogue.end_alone(state, row0 + 8 * part, lane);
+}
+
+// Whether that is the way: more rows than the kernel above takes, and few enough groups of weights that every block has one or two.
+template <typename T>
+bool some_rows(int64_t rows, int64_t features, int64_t outputs, int64_t x_stride, bool pair, FewPlan *plan) {
+  const int64_t groups = (outputs + (pair ? 7 : 15)) / (pair ? 8 : 16);
+  if (sizeof(T) != 4 || rows < 1 || rows > 128 || features > 2048 || features % 4 != 0 || x_stride % 4 != 0 || groups > 2 * 148) return false;
+  plan->tiles = 0;
+  plan->split = rows > 64 ? 8 : 16;
+  plan->blocks = (int)std::min<int64_t>(groups, 148);
+  return true;
+}
+
+template <class Epilogue>
+int launch_some(FewArgs<float> a, const Epilogue &e, const FewPlan &plan, cudaStream_t stream) {
+  a.split = plan.split;
+  return launch_next(some_rows_kernel<float, Epilogue>, dim3((unsigned)plan.blocks), kFewThreads, sizeof(float4) * 32 * kSomeTiles * kFewWarps, stream, 1, a, e);
+}
+
+template <typename T, class Epilogue>
+int launch_rows(const FewArgs<T> &a, const Epilogue &e, const FewPlan &plan, cudaStream_t stream) {
+  if constexpr (std::is_same<T, float>::value)
+    if (plan.tiles == 0) return launch_some(a, e, plan, stream);
+  return launch_few(a, e, plan, stream);
 }
 
 }  // namespace dense

@@ -34,9 +34,18 @@ __device__ __forceinline__ float activate_one(int act, float a, float &slope) {
     if (SLOPE) slope = s * (1.0f - s);
     return s;
   }
-  if (act == HT_ACTIVATION_GELU) {
-    const float phi = 0.5f * erfcf(a * -0.70710678118654752f);  // the normal distribution function
-    if (SLOPE) slope = phi + a * 0.39894228040143268f * (EXACT ? expf(-0.5f * a * a) : __expf(-0.5f * a * a));
+  if (act == HT_ACTIVATION_GELU) {  // with the normal distribution function
+    float phi, e;
+    if (EXACT) {
+      phi = 0.5f * erfcf(a * -0.70710678118654752f);
+      e = SLOPE ? expf(-0.5f * a * a) : 0.0f;
+    } else {  // formula 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions: within 1.5e-7, and its exponential is the slope's
+      const float z = fabsf(a) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
+      e = __expf(-0.5f * a * a);
+      const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+      phi = a < 0.0f ? tail : 1.0f - tail;
+    }
+    if (SLOPE) slope = fmaf(a * 0.39894228040143268f, e, phi);
     return a * phi;
   }
   if (SLOPE) slope = a > 0.0f ? 1.0f : 0.0f;
@@ -116,15 +125,10 @@ struct FewGatedEpilogue {
       if (row + i < rows) h[(size_t)(row + i) * (size_t)cols + o] = from_float<T>(activate_one<sizeof(T) == 4, false>(act, c[i] + ba, slope) * (c[2 + i] + bu));
     }
   }
+  __device__ __forceinline__ void end_alone(State<1> &, int, int) const {}
   template <int NT>
   __device__ __forceinline__ void end(State<NT> &, int, int) const {}
 };
-
-// The power of two at or below the largest |dh| (its bits in *top), 1 where there is none.
-__device__ __forceinline__ float scale_of(const uint32_t *top) {
-  const uint32_t e = __ldg(top) & 0x7f800000u;
-  return e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
-}
 
 // da and du of a piece of the outputs, side by side in one operand, and their sums over 32 rows for the biases' gradients.
 template <typename T>
@@ -140,7 +144,7 @@ struct GatedGradEpilogue {
   const T *bg, *bv;
   const T *dh;          // [rows, outputs]
   int align;
-  const uint32_t *top;  // fp16: dh is divided by this power of two; else null
+  Scale scale;          // fp16: dh is divided by this power of two
   typename Kind<T>::Operand *g;  // [planes][rows][2 pitch]: da, then du
   int pitch;
   size_t plane;
@@ -152,7 +156,7 @@ struct GatedGradEpilogue {
               some ? min(32, rows - r) : 0, min(32, cols - col), align, w.lane);
   }
   __device__ __forceinline__ void begin(State &s, const Where &w, bool first_tile) const {
-    s.scale = top != nullptr ? 1.0f / scale_of(top) : 1.0f;
+    s.scale = 1.0f / scale.value();
     s.unit = 0;
     if (first_tile)  // later ones have been fetched under the tile before
       for (int i = 0; i < min(kBoxes, w.units); ++i) fetch(w, i, w.row, w.col + 32 * i);
@@ -211,10 +215,6 @@ __global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__
   most = __reduce_max_sync(0xffffffffu, most);
   if ((threadIdx.x & 31) == 0) atomicMax(top, __float_as_uint(__half2float(__ushort_as_half((unsigned short)most))));
 }
-__global__ void scale_kernel(const uint32_t *top, float *alpha) {
-  after_previous_kernel();
-  *alpha = scale_of(top);
-}
 
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // da and du of one piece, unless the caller sets less
 
@@ -234,12 +234,14 @@ struct Plan {
   int64_t piece = 0, pitch = 0;
   typename Kind<T>::Operand *g = nullptr;
   uint32_t *top = nullptr;
-  float *alpha = nullptr, *sum = nullptr, *parts = nullptr, *row_sums = nullptr;
+  float *sum = nullptr, *parts = nullptr, *row_sums = nullptr;
   size_t bytes;
   Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, void *ws) {
     Arena arena(ws);
     bytes = 0;
-    if ((few = !backward && few_rows<T>(p.rows, p.features, p.outputs, true, &few_plan))) return;
+    few = !backward && (few_rows<T>(p.rows, p.features, p.outputs, true, &few_plan) ||
+                        some_rows<T>(p.rows, p.features, p.outputs, p.x_stride, true, &few_plan));
+    if (few) return;
     x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
     wg.set(arena, static_cast<const T *>(wgp), p.outputs, p.features, p.features);
     wv.set(arena, static_cast<const T *>(wvp), p.outputs, p.features, p.features);
@@ -250,7 +252,6 @@ struct Plan {
       pitch = round_up(piece, 64);
       g = arena.template take<typename Kind<T>::Operand>(p.rows * 2 * pitch * Kind<T>::kPlanes);
       top = arena.take<uint32_t>(1);
-      alpha = arena.take<float>(1);
       sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
       int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, 2 * p.outputs, Kind<T>::kPlanes);
       for (const int64_t count : {piece, (p.outputs - 1) % piece + 1})
@@ -260,12 +261,6 @@ struct Plan {
       row_sums = has_bias ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * 2 * pitch) : nullptr;
     }
     bytes = arena.used;
-  }
-  int lay_out(cudaStream_t stream) const {
-    int rc = x.lay_out(stream);
-    if (rc == HT_OK) rc = wg.lay_out(stream);
-    if (rc == HT_OK) rc = wv.lay_out(stream);
-    return rc;
   }
 };
 
@@ -279,10 +274,10 @@ int forward(const ht_dense_problem &p, const void *x, const void *wg, const void
     const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(wg), static_cast<const T *>(wv)}, p.x_stride, (int)p.rows, (int)p.features,
                           (int)p.outputs};
     const FewGatedEpilogue<T> e = {(int)p.rows, (int)p.outputs, p.activation, static_cast<const T *>(bg), static_cast<const T *>(bv), static_cast<T *>(h)};
-    return launch_few(a, e, plan.few_plan, stream);
+    return launch_rows(a, e, plan.few_plan, stream);
   }
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  if ((rc = plan.lay_out(stream)) != HT_OK) return rc;
+  HT_TRY(lay_out<T>({&plan.x, &plan.wg, &plan.wv}, stream));
   TileProblem t;
   t.a[0] = plan.x.m;
   t.b[0] = plan.wg.m;
@@ -315,15 +310,15 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
   }
   int sms = 0, rc;
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  if ((rc = plan.lay_out(stream)) != HT_OK) return rc;
+  HT_TRY(lay_out<T>({&plan.x, &plan.wg, &plan.wv}, stream));
   const bool scaled = p.dtype == HT_DTYPE_F16;
   if (scaled) {
     const int64_t n = p.rows * p.outputs;
     HT_CUDA_TRY(cudaMemsetAsync(plan.top, 0, sizeof(uint32_t), stream));
     HT_TRY(launch_next(largest_kernel, dim3(blocks_for(n, 256 * 32, 148 * 8)), 256, 0, stream, 1, static_cast<const __half *>(dh), n, plan.top));
-    HT_TRY(launch_next(scale_kernel, dim3(1), 1, 0, stream, 1, plan.top, plan.alpha));
   }
-  const float *alpha = scaled ? plan.alpha : nullptr;
+  Scale scale;
+  if (scaled) scale.top = plan.top;
   constexpr int kPlanes = Kind<T>::kPlanes;
   const size_t plane = (size_t)(p.rows * 2 * plan.pitch);
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
@@ -339,12 +334,12 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
     e.rows = (int)p.rows, e.cols = (int)count, e.act = p.activation, e.first = (int)first, e.outputs = (int)p.outputs;
     e.bg = static_cast<const T *>(bg), e.bv = static_cast<const T *>(bv), e.dh = static_cast<const T *>(dh);
     e.align = row_alignment(e.dh, p.outputs * (int64_t)sizeof(T));
-    e.top = scaled ? plan.top : nullptr;
+    e.scale = scale;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = plane, e.row_sums = plan.row_sums;
     const TileShape shape = tile_shape(p.rows, count, p.features, kPlanes, true);
     if ((rc = launch_tiles<kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
     StoreEpilogue<T> store = {};
-    store.alpha = alpha;
+    store.scale = scale;
     store.cols = (int)p.features;
     store.split = 0x7fffffff;
     store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));
@@ -381,8 +376,9 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
       if ((rc = product_dw<T>(q, store, plan.parts, sms, stream)) != HT_OK) return rc;
     }
     const int64_t blocks = row_sum_count(p.rows, shape);
-    if (dbg != nullptr && (rc = column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, alpha, dbg + first, stream)) != HT_OK) return rc;
-    if (dbv != nullptr && (rc = column_sums<T>(plan.row_sums + plan.pitch, blocks, 2 * plan.pitch, count, alpha, dbv + first, stream)) != HT_OK) return rc;
+    if (has_bias)
+      HT_TRY(column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, scale, dbg == nullptr ? nullptr : dbg + first, dbv == nullptr ? nullptr : dbv + first,
+                            plan.pitch, stream));
   }
   return HT_OK;
 }
