@@ -36,12 +36,6 @@ __device__ __forceinline__ void join(float &m, float &l, float m2, float l2) {
   m = top;
 }
 
-// What a row's gradient is made of: exp((s - m)) scale - [v = target] factor.
-struct RowGrad {
-  float m, scale, factor;
-  int target;
-};
-
 template <typename T>
 struct LossEpilogue {
   static constexpr bool kPair = false;
@@ -55,7 +49,9 @@ struct LossEpilogue {
   float2 *partial;      // [rows][slots], slots = 2 n_blocks
   int slots;
   float *target_score;  // [rows]
+  unsigned *ended;      // set to 0 for the kernel that joins the pieces
   __device__ __forceinline__ void begin(State &s, const Where &w, bool) const {
+    if (w.m_block == 0 && w.n_block == 0 && w.half == 0 && w.quarter == 0 && w.lane == 0) *ended = 0u;
     s.m = -INFINITY, s.l = 0.0f, s.target = -1;
     if (w.inside) {
       const int64_t t = __ldg(target + w.row);
@@ -108,21 +104,31 @@ template <typename T>
 struct LossGradEpilogue {
   static constexpr bool kPair = false;
   struct State {
-    RowGrad r;
+    float m, scale, factor;  // g = exp(s - m) scale - [v = target] factor
+    int target;
   };
   int rows, cols, first;  // the piece: classes first .. first + cols - 1
   const T *bias;
-  const RowGrad *row_grad;
+  const float2 *stats;
+  const int64_t *target;
+  int64_t ignore, classes;
+  const float *grad;      // of single rows, or null: one for all, which leaves with the sums
+  float one;              // the factor of a row that counts, and of one whose gradient is the scale of all
+  Scale scale;
   typename Kind<T>::Operand *g;  // [planes][rows][pitch]
   int pitch;
   size_t plane;
   float *row_sums;  // [row_sum_count][pitch] or null
   __device__ __forceinline__ void begin(State &s, const Where &w, bool) const {
-    s.r = {0.0f, 0.0f, 0.0f, -1};
-    if (w.inside) {
-      const float4 q = __ldg(reinterpret_cast<const float4 *>(row_grad + w.row));
-      s.r = {q.x, q.y, q.z, __float_as_int(q.w)};
-    }
+    s.m = s.scale = s.factor = 0.0f, s.target = -1;
+    if (!w.inside) return;
+    const float2 q = __ldg(stats + w.row);
+    const int64_t t = __ldg(target + w.row);
+    const bool valid = t >= 0 && t < classes;
+    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? __ldg(grad + w.row) / scale.value() : one;
+    if (t != ignore && valid) s.target = (int)t;
+    s.m = q.x;
+    s.scale = s.factor / q.y;
   }
   __device__ __forceinline__ void unit(State &s, const Where &w, int col, float (&v)[32]) const {
     const int n = cols - col;
@@ -133,12 +139,12 @@ struct LossGradEpilogue {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += b[i];
     }
-    const int at = s.r.target - first - col;
-    const bool none = s.r.factor == 0.0f;  // a row that does not count, or is not there
+    const int at = s.target - first - col;
+    const bool none = s.factor == 0.0f;  // a row that does not count, or is not there
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float p = exp2_fast((v[i] - s.r.m) * kLog2e) * s.r.scale;
-      v[i] = none || i >= n ? 0.0f : i == at ? p - s.r.factor : p;
+      const float p = exp2_fast((v[i] - s.m) * kLog2e) * s.scale;
+      v[i] = none || i >= n ? 0.0f : i == at ? p - s.factor : p;
     }
     if (w.inside) store_operand<T>(g + (size_t)w.row * (size_t)pitch + col, plane, v);
     if (row_sums != nullptr) row_sums[(size_t)(w.m_block * 4 + w.quarter) * (size_t)pitch + col + w.lane] = sum_rows(v, w.lane);
@@ -159,8 +165,10 @@ struct FewLossEpilogue {
   const int64_t *target;
   float2 *partial;
   float *target_score;
+  unsigned *ended;
   template <typename S>
   __device__ __forceinline__ void begin(S &s) const {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *ended = 0u;
     for (auto &m : s.m) m[0] = m[1] = -INFINITY;
     for (auto &l : s.l) l[0] = l[1] = 0.0f;
   }
@@ -219,64 +227,81 @@ struct FewLossEpilogue {
 };
 
 // Joins the pieces of every row, a warp each, in a fixed order: stats[row] = (m, l), the row's loss to `loss`.  A row whose target is
-// no class: loss NaN and a flag.
-__global__ void __launch_bounds__(256) join_rows_kernel(const float2 *__restrict__ partial, int slots, const float *__restrict__ target_score,
-                                                        const int64_t *__restrict__ target, int64_t ignore, int64_t rows, int64_t classes,
-                                                        float2 *__restrict__ stats, float *__restrict__ loss, uint32_t *status_word) {
+// no class: loss NaN and a flag.  For a sum or mean the last block to end adds the rows' losses, in fp64 and in an order that
+// depends on the number of rows alone, and leaves the number of rows that count behind the statistics.
+struct JoinArgs {
+  const float2 *partial;
+  int slots;
+  const float *target_score;
+  const int64_t *target;
+  int64_t ignore, rows, classes;
+  float2 *stats;
+  float *row_loss;
+  float *total;         // null: single rows
+  bool mean;
+  unsigned *ended;      // blocks that have, 0 at the start
+  uint32_t *status_word;
+};
+__global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
   after_previous_kernel();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  float m = -INFINITY, l = 0.0f;
-  const float2 *pieces = partial + (size_t)row * (size_t)slots;
+  if (row < a.rows) {
+    float m = -INFINITY, l = 0.0f;
+    const float2 *pieces = a.partial + (size_t)row * (size_t)a.slots;
 #pragma unroll 4
-  for (int s = lane; s < slots; s += 32) {
-    const float2 q = __ldg(pieces + s);
-    join(m, l, q.x, q.y);
-  }
+    for (int s = lane; s < a.slots; s += 32) {
+      const float2 q = __ldg(pieces + s);
+      join(m, l, q.x, q.y);
+    }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
-    join(m, l, m2, l2);
-  }
-  if (lane != 0) return;
-  if (stats != nullptr) stats[row] = make_float2(m, l);
-  const int64_t t = target[row];
-  float result = 0.0f;
-  if (t != ignore) {
-    if (t >= 0 && t < classes) {
-      result = (float)((double)logf(l) + ((double)m - (double)target_score[row]));
-    } else {
-      result = NAN;
-      if (status_word != nullptr) atomicOr(status_word, HT_FLAG_TARGET_RANGE);
+    for (int d = 16; d > 0; d >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
+      join(m, l, m2, l2);
+    }
+    if (lane == 0) {
+      if (a.stats != nullptr) a.stats[row] = make_float2(m, l);
+      const int64_t t = a.target[row];
+      float result = 0.0f;
+      if (t != a.ignore) {
+        if (t >= 0 && t < a.classes) {
+          result = (float)((double)logf(l) + ((double)m - (double)a.target_score[row]));
+        } else {
+          result = NAN;
+          if (a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_TARGET_RANGE);
+        }
+      }
+      a.row_loss[row] = result;
     }
   }
-  loss[row] = result;
-}
-
-// Sum or mean of the rows' losses in fp64, strand by strand in a fixed order; summary = the number of rows that count.
-__global__ void __launch_bounds__(1024) reduce_loss_kernel(const float *__restrict__ row_loss, const int64_t *__restrict__ target, int64_t ignore,
-                                                           int64_t rows, int mean, float *__restrict__ loss, float *__restrict__ summary) {
-  after_previous_kernel();
-  __shared__ double sums[32];
-  __shared__ long long counts[32];
+  if (a.total == nullptr) return;
+  __shared__ bool last;
+  __threadfence();  // the row's loss, before the block counts as ended
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.ended, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  __shared__ double sums[8];
+  __shared__ long long counts[8];
   double sum = 0.0;
   long long count = 0;
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-    if (target[r] == ignore) continue;
-    sum += (double)row_loss[r];
+#pragma unroll 8
+  for (int64_t r = threadIdx.x; r < a.rows; r += 256) {
+    if (__ldg(a.target + r) == a.ignore) continue;
+    sum += (double)__ldcg(a.row_loss + r);
     ++count;
   }
   for (int s = 16; s > 0; s >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, s);
     count += __shfl_xor_sync(0xffffffffu, count, s);
   }
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum, counts[threadIdx.x >> 5] = count;
+  if (lane == 0) sums[threadIdx.x >> 5] = sum, counts[threadIdx.x >> 5] = count;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 32; ++i) sum += sums[i], count += counts[i];
-    loss[0] = (float)(mean ? sum / (double)count : sum);
-    if (summary != nullptr) summary[0] = (float)count;
+    for (int i = 1; i < 8; ++i) sum += sums[i], count += counts[i];
+    a.total[0] = (float)(a.mean ? sum / (double)count : sum);
+    if (a.stats != nullptr) a.stats[a.rows].x = (float)count;
   }
 }
 
@@ -297,31 +322,6 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict
   }
 }
 
-// One upstream gradient for all rows (sum, mean) or one each, as what the rows' epilogue multiplies by; alpha: what their sums are
-// multiplied by.  The factors are at most `unit`.
-__global__ void __launch_bounds__(256) row_grad_kernel(const float2 *__restrict__ stats, const float *__restrict__ summary, const int64_t *__restrict__ target,
-                                                       int64_t ignore, int64_t rows, int64_t classes, const float *__restrict__ grad, int reduction,
-                                                       float unit, RowGrad *__restrict__ row_grad, float *__restrict__ alpha) {
-  after_previous_kernel();
-  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (row == 0 && reduction != HT_REDUCTION_NONE) {
-    const float count = summary[0];
-    alpha[0] = reduction == HT_REDUCTION_SUM ? grad[0] / unit : count > 0.0f ? grad[0] / count / unit : 0.0f;
-  }
-  if (row >= rows) return;
-  const float2 q = stats[row];
-  const int64_t t = target[row];
-  const bool counts = t != ignore, valid = t >= 0 && t < classes;
-  float factor = 0.0f;
-  if (counts) factor = !valid ? NAN : reduction == HT_REDUCTION_NONE ? grad[row] / alpha[0] : unit;
-  float4 r;
-  r.x = q.x;
-  r.y = factor / q.y;
-  r.z = factor;
-  r.w = __int_as_float(valid && counts ? (int)t : -1);
-  reinterpret_cast<float4 *>(row_grad)[row] = r;
-}
-
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // g of one piece, unless the caller sets less
 
 int screen(const ht_dense_problem *p) {
@@ -340,6 +340,7 @@ struct ForwardPlan {
   int slots;
   float2 *partial;
   float *target_score, *row_loss;
+  unsigned *ended;
   size_t bytes;
   ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, void *ws) {
     Arena arena(ws);
@@ -354,6 +355,7 @@ struct ForwardPlan {
     partial = arena.take<float2>((int64_t)slots * p.rows);
     target_score = arena.take<float>(p.rows);
     row_loss = arena.take<float>(p.rows);
+    ended = arena.take<unsigned>(1);
     bytes = arena.used;
   }
 };
@@ -368,7 +370,7 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
   if (p.rows > 0) {
     if (plan.few) {
       const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(w), nullptr}, p.x_stride, (int)p.rows, (int)p.features, (int)p.outputs};
-      const FewLossEpilogue<T> e = {(int)p.rows, plan.slots, static_cast<const T *>(bias), target, plan.partial, plan.target_score};
+      const FewLossEpilogue<T> e = {(int)p.rows, plan.slots, static_cast<const T *>(bias), target, plan.partial, plan.target_score, plan.ended};
       HT_TRY(launch_rows(a, e, plan.few_plan, stream));
     } else {
       if ((rc = sm_count(&sms)) != HT_OK) return rc;
@@ -379,17 +381,16 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
       t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
       t.f16 = p.dtype == HT_DTYPE_F16;
       t.status_word = status_word;
-      const LossEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), target, plan.partial, plan.slots, plan.target_score};
+      const LossEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), target, plan.partial, plan.slots, plan.target_score, plan.ended};
       if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, plan.shape, sms, stream)) != HT_OK) return rc;
     }
-    HT_TRY(launch_next(join_rows_kernel, dim3((unsigned)((p.rows + 7) / 8)), 256, 0, stream, 1, plan.partial, plan.slots, plan.target_score, target, ignore, p.rows,
-                                                                       p.outputs, reinterpret_cast<float2 *>(stats), row_loss, status_word));
   }
-  if (reduction != HT_REDUCTION_NONE) {
-    HT_TRY(launch_next(reduce_loss_kernel, dim3(1), 1024, 0, stream, 1, row_loss, target, ignore, p.rows, reduction == HT_REDUCTION_MEAN, loss,
-                                               stats == nullptr ? nullptr : stats + 2 * p.rows));
-  }
-  return HT_OK;
+  // (no rows: a sum of nothing)
+  JoinArgs j = {plan.partial, plan.slots, plan.target_score, target, ignore, p.rows, p.outputs, reinterpret_cast<float2 *>(stats), row_loss, nullptr,
+                reduction == HT_REDUCTION_MEAN, plan.ended, status_word};
+  if (reduction != HT_REDUCTION_NONE) j.total = loss;
+  if (p.rows == 0) HT_CUDA_TRY(cudaMemsetAsync(plan.ended, 0, sizeof(unsigned), stream));
+  return launch_next(join_rows_kernel, dim3((unsigned)std::max<int64_t>((p.rows + 7) / 8, 1)), 256, 0, stream, 1, j);
 }
 
 template <typename T>
@@ -397,7 +398,6 @@ struct BackwardPlan {
   Operand<T> x, w;
   int64_t piece, pitch;  // classes of a piece, elements of a row of g
   typename Kind<T>::Operand *g;
-  RowGrad *row_grad;
   float *alpha, *sum, *parts, *row_sums;
   size_t bytes;
   BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, void *ws) {
@@ -410,7 +410,6 @@ struct BackwardPlan {
     piece = piece_of(p.outputs, limit / per_class);
     pitch = round_up(piece, 64);
     g = arena.take<typename Kind<T>::Operand>(p.rows * pitch * Kind<T>::kPlanes);
-    row_grad = arena.take<RowGrad>(p.rows);
     alpha = arena.take<float>(1);
     sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
     parts = nullptr;
@@ -442,8 +441,10 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
   if (reduction == HT_REDUCTION_NONE) {
     HT_TRY(launch_next(row_scale_kernel, dim3(1), 1024, 0, stream, 1, grad, p.rows, unit, plan.alpha));
   }
-  HT_TRY(launch_next(row_grad_kernel, dim3((unsigned)((p.rows + 255) / 256)), 256, 0, stream, 1, reinterpret_cast<const float2 *>(stats), stats + 2 * p.rows, target, ignore,
-                                                                       p.rows, p.outputs, grad, reduction, unit, plan.row_grad, plan.alpha));
+  Scale scale;
+  scale.number = reduction == HT_REDUCTION_NONE ? plan.alpha : grad;
+  if (reduction == HT_REDUCTION_MEAN) scale.count = stats + 2 * p.rows;
+  if (reduction != HT_REDUCTION_NONE) scale.unit = unit;
   constexpr int kPlanes = Kind<T>::kPlanes;
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
     const int64_t count = std::min(plan.piece, p.outputs - first);
@@ -456,7 +457,10 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     LossGradEpilogue<T> e = {};
     e.rows = (int)p.rows, e.cols = (int)count, e.first = (int)first;
     e.bias = static_cast<const T *>(bias);
-    e.row_grad = plan.row_grad;
+    e.stats = reinterpret_cast<const float2 *>(stats);
+    e.target = target, e.ignore = ignore, e.classes = p.outputs;
+    e.grad = reduction == HT_REDUCTION_NONE ? grad : nullptr;
+    e.one = unit, e.scale = scale;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = (size_t)(p.rows * plan.pitch);
     e.row_sums = plan.row_sums;
     const TileShape shape = tile_shape(p.rows, count, p.features, kPlanes, false);
@@ -464,7 +468,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     Matrix g;
     g.data = plan.g, g.rows = p.rows, g.cols = count, g.pitch = plan.pitch, g.planes = kPlanes, g.plane = p.rows * plan.pitch;
     StoreEpilogue<T> store = {};
-    store.scale.number = plan.alpha;
+    store.scale = scale;
     store.cols = (int)p.features;
     store.split = 0x7fffffff;
     store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));

@@ -347,17 +347,20 @@ __device__ __forceinline__ float sum_rows(const float (&v)[32], int lane) {
   return h[0];
 }
 
-// What gradients are multiplied by when they leave: a number on the device, or the power of two at or below the number whose bits
-// are at `top` (1 where that is no normal number), or 1.
+// What gradients are multiplied by when they leave: a number on the device (over a count that is there as well, 0 for none, and over
+// `unit`), or the power of two at or below the number whose bits are at `top` (1 where that is no normal number), or 1.
 struct Scale {
-  const float *number = nullptr;
+  const float *number = nullptr, *count = nullptr;
+  float unit = 1.0f;
   const uint32_t *top = nullptr;
   __device__ __forceinline__ float value() const {
     if (top != nullptr) {
       const uint32_t e = __ldg(top) & 0x7f800000u;
       return e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
     }
-    return number != nullptr ? __ldg(number) : 1.0f;
+    if (number == nullptr) return 1.0f;
+    const float n = __ldg(number) / unit, c = count != nullptr ? __ldg(count) : 1.0f;
+    return c > 0.0f ? n / c : 0.0f;
   }
 };
 
@@ -558,13 +561,13 @@ int lay_out(std::initializer_list<const Operand<T> *> operands, cudaStream_t str
 // Sums of 32 rows that an epilogue leaves for these rows: of every tile's, inside the matrix or not.
 inline int64_t row_sum_count(int64_t rows, const TileShape &shape) { return (rows + shape.rows() - 1) / shape.rows() * shape.rows() / 32; }
 
-// Column sums from the sums of 32 rows each that the epilogues leave: out[c] = alpha sum_r partial[r, c], r in 8 strands,
+// Column sums from the sums of 32 rows each that the epilogues leave: out[c] = alpha sum_r partial[r, c], r in 32 strands,
 // ascending in each, that are added in order.  32 columns a block; columns from `second` on go to out2.
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols, int64_t second,
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols, int64_t second,
                                                           Scale scale, T *__restrict__ out, T *__restrict__ out2) {
   after_previous_kernel();
-  __shared__ float strand[8][33];
+  __shared__ float strand[32][33];
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane, part = c < second ? c : c - second;
   T *const to = c < second ? out : out2;
@@ -572,12 +575,12 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float *__restric
   float sum = 0.0f;
   if (inside)
 #pragma unroll 4
-    for (int64_t r = y; r < rows; r += 8) sum += __ldg(partial + r * pitch + c);
+    for (int64_t r = y; r < rows; r += 32) sum += __ldg(partial + r * pitch + c);
   strand[y][lane] = sum;
   __syncthreads();
   if (y == 0 && inside) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += strand[i][lane];
+    for (int i = 1; i < 32; ++i) sum += strand[i][lane];
     to[part] = from_float<T>(scale.value() * sum);
   }
 }
@@ -585,7 +588,7 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float *__restric
 // (out2: the sums from column `second` on; null, or one of the two null: those are not wanted)
 template <typename T>
 int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols, const Scale &scale, T *out, T *out2, int64_t second, cudaStream_t stream) {
-  return launch_next(column_sums_kernel<T>, dim3((unsigned)(((out2 != nullptr ? second : 0) + cols + 31) / 32)), 256, 0, stream, 1, partial, rows, pitch, cols,
+  return launch_next(column_sums_kernel<T>, dim3((unsigned)(((out2 != nullptr ? second : 0) + cols + 31) / 32)), 1024, 0, stream, 1, partial, rows, pitch, cols,
                      second, scale, out, out2);
 }
 
