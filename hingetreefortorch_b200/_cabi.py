@@ -38,7 +38,7 @@ SYMBOLS = [
     "ht_forest_normalised_workspace_bytes", "ht_forest_normalised_forward_f32", "ht_forest_normalised_backward_f32",
     "ht_batchnorm_input_grad_f32", "ht_batchnorm_statistics_f32", "ht_batchnorm_running_f32",
     "ht_init_medians_workspace_bytes", "ht_init_medians_f32", "ht_init_medians_f64", "ht_thresholds_f32", "ht_thresholds_f64",
-    "ht_gated_linear_workspace_bytes", "ht_gated_linear_forward", "ht_gated_linear_backward",
+    "ht_gated_linear_workspace_bytes", "ht_gated_linear_kept_bytes", "ht_linear_class_loss_kept_bytes", "ht_gated_linear_forward", "ht_gated_linear_backward",
     "ht_linear_class_loss_workspace_bytes", "ht_linear_class_loss_forward", "ht_linear_class_loss_backward",
 ]
 

@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include "hingetree_cpp_autograd.h"
 
@@ -75,6 +76,24 @@ torch::Tensor backward_workspace(ht_dense_problem &p, const torch::Tensor &like,
   }
 }
 
+// Room for the copies that a forward leaves for its backward, where the caller's settings and the device's memory admit it.
+torch::Tensor room_to_keep(size_t bytes, const torch::Tensor &like) {
+  if (bytes == 0 || !may_keep((int64_t)bytes)) return torch::Tensor();
+  try {
+    return fresh({(int64_t)bytes}, like, torch::kUInt8);
+  } catch (const c10::OutOfMemoryError &) {
+    return torch::Tensor();
+  }
+}
+// The copies of a node's forward; they go with the graph's buffers.
+torch::Tensor take_kept(AutogradContext *ctx) {
+  const auto at = ctx->saved_data.find("kept");
+  if (at == ctx->saved_data.end()) return torch::Tensor();
+  const torch::Tensor kept = at->second.toTensor();
+  if (!torch::autograd::get_current_graph_task_keep_graph()) ctx->saved_data.erase(at);
+  return kept;
+}
+
 // ---- gated projection ------------------------------------------------------------------------------------------------
 
 int activation_code(const std::string &name) {
@@ -86,13 +105,14 @@ int activation_code(const std::string &name) {
 }
 
 torch::Tensor gated_forward(const torch::Tensor &x, const torch::Tensor &wg, const torch::Tensor &wv, const torch::Tensor &bg,
-                            const torch::Tensor &bv, int activation) {
+                            const torch::Tensor &bv, int activation, torch::Tensor *kept = nullptr) {
   c10::DeviceGuard guard(x.device());
   const ht_dense_problem p = problem_of(x, wg, activation);
+  if (kept != nullptr) *kept = room_to_keep(ht_gated_linear_kept_bytes(&p), x);
   torch::Tensor h = fresh({p.rows, p.outputs}, x);
   const torch::Tensor ws = make_workspace(ht_gated_linear_workspace_bytes(&p, 0), x);
-  raise_status(ht_gated_linear_forward(&p, pointer(x), pointer(wg), pointer(wv), pointer(bg), pointer(bv), h.data_ptr(), ws.data_ptr(), ws.numel(),
-                                       long_lived_word(x), current_stream(x)),
+  raise_status(ht_gated_linear_forward(&p, pointer(x), pointer(wg), pointer(wv), pointer(bg), pointer(bv), h.data_ptr(),
+                                       kept != nullptr && kept->defined() ? kept->data_ptr() : nullptr, ws.data_ptr(), ws.numel(), long_lived_word(x), current_stream(x)),
                "gated linear");
   return h;
 }
@@ -102,7 +122,10 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
                                const OptionalTensor &bg, const OptionalTensor &bv, int64_t activation) {
     ctx->save_for_backward({x, wg, wv, given(bg), given(bv)});
     ctx->saved_data["activation"] = activation;
-    return gated_forward(x, wg, wv, given(bg), given(bv), (int)activation);
+    torch::Tensor kept;
+    const torch::Tensor h = gated_forward(x, wg, wv, given(bg), given(bv), (int)activation, &kept);
+    if (kept.defined()) ctx->saved_data["kept"] = kept;
+    return h;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     refuse_second_derivative("gated_linear");
@@ -114,9 +137,9 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
     variable_list out(6);
     for (int i = 0, edge = 0; i < 5; ++i)  // a bias that is not there has no edge
       if (s[i].defined() && ctx->needs_input_grad(edge++)) out[i] = fresh(s[i].sizes(), s[i]);
-    const torch::Tensor ws = backward_workspace(p, x, ht_gated_linear_workspace_bytes);
+    const torch::Tensor kept = take_kept(ctx), ws = backward_workspace(p, x, ht_gated_linear_workspace_bytes);
     auto to = [](const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
-    raise_status(ht_gated_linear_backward(&p, pointer(x), pointer(s[1]), pointer(s[2]), pointer(s[3]), pointer(s[4]), pointer(dh), to(out[0]),
+    raise_status(ht_gated_linear_backward(&p, pointer(x), pointer(s[1]), pointer(s[2]), pointer(s[3]), pointer(s[4]), pointer(dh), pointer(kept), to(out[0]),
                                           to(out[1]), to(out[2]), to(out[3]), to(out[4]), ws.data_ptr(), ws.numel(), long_lived_word(x),
                                           current_stream(x)),
                  "gated linear backward");
@@ -153,15 +176,17 @@ int reduction_code(const std::string &name) {
 
 // {loss, what the backward needs of the softmax (with `keep`)}
 std::pair<torch::Tensor, torch::Tensor> loss_forward(const torch::Tensor &x, const torch::Tensor &w, const torch::Tensor &bias,
-                                                     const torch::Tensor &target, int64_t ignore, int reduction, bool keep) {
+                                                     const torch::Tensor &target, int64_t ignore, int reduction, bool keep,
+                                                     torch::Tensor *kept = nullptr) {
   c10::DeviceGuard guard(x.device());
   const ht_dense_problem p = problem_of(x, w, 0);
+  if (kept != nullptr) *kept = room_to_keep(ht_linear_class_loss_kept_bytes(&p), x);
   torch::Tensor loss = reduction == HT_REDUCTION_NONE ? fresh({p.rows}, x, torch::kFloat32) : fresh({}, x, torch::kFloat32);
   torch::Tensor stats = keep ? fresh({2 * p.rows + 2}, x, torch::kFloat32) : torch::Tensor();
   const torch::Tensor ws = make_workspace(ht_linear_class_loss_workspace_bytes(&p, 0), x);
   raise_status(ht_linear_class_loss_forward(&p, pointer(x), pointer(w), pointer(bias), target.const_data_ptr<int64_t>(), ignore, reduction,
-                                            loss.data_ptr<float>(), keep ? stats.data_ptr<float>() : nullptr, ws.data_ptr(), ws.numel(),
-                                            long_lived_word(x), current_stream(x)),
+                                            loss.data_ptr<float>(), keep ? stats.data_ptr<float>() : nullptr,
+                                            kept != nullptr && kept->defined() ? kept->data_ptr() : nullptr, ws.data_ptr(), ws.numel(), long_lived_word(x), current_stream(x)),
                "class loss");
   return {loss, stats};
 }
@@ -169,7 +194,9 @@ std::pair<torch::Tensor, torch::Tensor> loss_forward(const torch::Tensor &x, con
 struct ClassLossNode : public torch::autograd::Function<ClassLossNode> {
   static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &w, const OptionalTensor &bias,
                                const torch::Tensor &target, int64_t ignore, int64_t reduction) {
-    const auto result = loss_forward(x, w, given(bias), target, ignore, (int)reduction, true);
+    torch::Tensor kept;
+    const auto result = loss_forward(x, w, given(bias), target, ignore, (int)reduction, true, &kept);
+    if (kept.defined()) ctx->saved_data["kept"] = kept;
     ctx->save_for_backward({x, w, given(bias), target, result.second});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
@@ -185,11 +212,11 @@ struct ClassLossNode : public torch::autograd::Function<ClassLossNode> {
     variable_list out(6);
     for (int i = 0, edge = 0; i < 3; ++i)  // a bias that is not there has no edge
       if (s[i].defined() && ctx->needs_input_grad(edge++)) out[i] = fresh(s[i].sizes(), s[i]);
-    const torch::Tensor ws = backward_workspace(p, x, ht_linear_class_loss_workspace_bytes);
+    const torch::Tensor kept = take_kept(ctx), ws = backward_workspace(p, x, ht_linear_class_loss_workspace_bytes);
     auto to = [](const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
     raise_status(ht_linear_class_loss_backward(&p, pointer(x), pointer(s[1]), pointer(s[2]), s[3].const_data_ptr<int64_t>(),
                                                ctx->saved_data["ignore"].toInt(), (int)ctx->saved_data["reduction"].toInt(),
-                                               grad.const_data_ptr<float>(), s[4].const_data_ptr<float>(), to(out[0]), to(out[1]), to(out[2]),
+                                               grad.const_data_ptr<float>(), s[4].const_data_ptr<float>(), pointer(kept), to(out[0]), to(out[1]), to(out[2]),
                                                ws.data_ptr(), ws.numel(), long_lived_word(x), current_stream(x)),
                  "class loss backward");
     return out;

@@ -249,6 +249,8 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
   if (row < a.rows) {
     float m = -INFINITY, l = 0.0f;
     const float2 *pieces = a.partial + (size_t)row * (size_t)a.slots;
+    const int64_t t = __ldg(a.target + row);
+    const float score = __ldg(a.target_score + row);  // (nothing of use where the row has no target)
 #pragma unroll 4
     for (int s = lane; s < a.slots; s += 32) {
       const float2 q = __ldg(pieces + s);
@@ -261,11 +263,10 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
     }
     if (lane == 0) {
       if (a.stats != nullptr) a.stats[row] = make_float2(m, l);
-      const int64_t t = a.target[row];
       float result = 0.0f;
       if (t != a.ignore) {
         if (t >= 0 && t < a.classes) {
-          result = (float)((double)logf(l) + ((double)m - (double)a.target_score[row]));
+          result = (float)((double)logf(l) + ((double)m - (double)score));
         } else {
           result = NAN;
           if (a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_TARGET_RANGE);
@@ -331,6 +332,16 @@ int screen(const ht_dense_problem *p) {
   return HT_OK;
 }
 
+// The copies that a forward leaves for its backward: of what cannot be read as it is, with the rows that do not count as zeros.
+template <typename T>
+size_t keep(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, void *kept, Operand<T> &x, Operand<T> &w) {
+  Arena arena(kept);
+  const bool copied = !Operand<T>::direct(p.x_stride);
+  x.set(arena, xp, p.rows, p.features, p.x_stride, copied, copied ? target : nullptr, ignore);
+  w.set(arena, wp, p.outputs, p.features, p.features);
+  return arena.used;
+}
+
 template <typename T>
 struct ForwardPlan {
   bool few;
@@ -342,11 +353,13 @@ struct ForwardPlan {
   float *target_score, *row_loss;
   unsigned *ended;
   size_t bytes;
-  ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, void *ws) {
+  ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, void *kept, void *ws) {
     Arena arena(ws);
     few = few_rows<T>(p.rows, p.features, p.outputs, false, &few_plan) ||
           some_rows<T>(p.rows, p.features, p.outputs, p.x_stride, false, &few_plan);
-    if (!few) {
+    if (kept != nullptr) {
+      keep(p, xp, wp, target, ignore, kept, x, w);
+    } else if (!few) {
       x.set(arena, xp, p.rows, p.features, p.x_stride);
       w.set(arena, wp, p.outputs, p.features, p.features);
     }
@@ -362,19 +375,20 @@ struct ForwardPlan {
 
 template <typename T>
 int forward(const ht_dense_problem &p, const void *x, const void *w, const void *bias, const int64_t *target, int64_t ignore, int reduction,
-            float *loss, float *stats, void *ws, size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
-  ForwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), ws);
+            float *loss, float *stats, void *kept, void *ws, size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
+  ForwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), target, ignore, kept, ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   int sms = 0, rc;
   float *row_loss = reduction == HT_REDUCTION_NONE ? loss : plan.row_loss;
   if (p.rows > 0) {
+    // (copies that are left for the backward are made whichever kernel runs)
+    if (kept != nullptr || !plan.few) HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
     if (plan.few) {
       const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(w), nullptr}, p.x_stride, (int)p.rows, (int)p.features, (int)p.outputs};
       const FewLossEpilogue<T> e = {(int)p.rows, plan.slots, static_cast<const T *>(bias), target, plan.partial, plan.target_score, plan.ended};
       HT_TRY(launch_rows(a, e, plan.few_plan, stream));
     } else {
       if ((rc = sm_count(&sms)) != HT_OK) return rc;
-      HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
       TileProblem t;
       t.a[0] = plan.x.m;
       t.b[0] = plan.w.m;
@@ -400,11 +414,15 @@ struct BackwardPlan {
   typename Kind<T>::Operand *g;
   float *alpha, *sum, *parts, *row_sums;
   size_t bytes;
-  BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, void *ws) {
+  BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, const void *kept,
+               void *ws) {
     Arena arena(ws);
-    static const int64_t some = 0;
-    x.set(arena, xp, p.rows, p.features, p.x_stride, target != nullptr ? target : &some, ignore);
-    w.set(arena, wp, p.outputs, p.features, p.features);
+    if (kept != nullptr) {
+      keep(p, xp, wp, target, ignore, const_cast<void *>(kept), x, w);
+      x.ready = w.ready = true;
+    }
+    if (kept == nullptr || x.copy == nullptr) x.set(arena, xp, p.rows, p.features, p.x_stride, true, target, ignore), x.ready = false;
+    if (kept == nullptr) w.set(arena, wp, p.outputs, p.features, p.features);
     const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
     const int64_t per_class = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 2;
     piece = piece_of(p.outputs, limit / per_class);
@@ -424,10 +442,10 @@ struct BackwardPlan {
 
 template <typename T>
 int backward(const ht_dense_problem &p, const void *x, const void *w, const void *bias, const int64_t *target, int64_t ignore, int reduction,
-             const float *grad, const float *stats, void *dx_, void *dw_, void *db_, void *ws, size_t ws_bytes, uint32_t *status_word,
+             const float *grad, const float *stats, const void *kept, void *dx_, void *dw_, void *db_, void *ws, size_t ws_bytes, uint32_t *status_word,
              cudaStream_t stream) {
   T *dx = static_cast<T *>(dx_), *dw = static_cast<T *>(dw_), *db = static_cast<T *>(db_);
-  BackwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), target, ignore, dx != nullptr, db != nullptr, ws);
+  BackwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), target, ignore, dx != nullptr, db != nullptr, kept, ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   if (p.rows == 0) {
     if (dw != nullptr) HT_CUDA_TRY(cudaMemsetAsync(dw, 0, sizeof(T) * (size_t)(p.outputs * p.features), stream));
@@ -513,13 +531,22 @@ extern "C" size_t ht_linear_class_loss_workspace_bytes(const ht_dense_problem *p
   if (screen(p) != HT_OK) return 0;
   return by_type(p->dtype, [&](auto zero) -> size_t {
     typedef decltype(zero) T;
-    return backward != 0 ? BackwardPlan<T>(*p, nullptr, nullptr, nullptr, 0, true, true, nullptr).bytes
-                         : ForwardPlan<T>(*p, nullptr, nullptr, nullptr).bytes;
+    return backward != 0 ? BackwardPlan<T>(*p, nullptr, nullptr, nullptr, 0, true, true, nullptr, nullptr).bytes
+                         : ForwardPlan<T>(*p, nullptr, nullptr, nullptr, 0, nullptr, nullptr).bytes;
+  });
+}
+
+extern "C" size_t ht_linear_class_loss_kept_bytes(const ht_dense_problem *p) {
+  if (screen(p) != HT_OK || p->rows == 0) return 0;
+  return by_type(p->dtype, [&](auto zero) -> size_t {
+    typedef decltype(zero) T;
+    Operand<T> x, w;
+    return keep<T>(*p, nullptr, nullptr, nullptr, 0, nullptr, x, w);
   });
 }
 
 extern "C" int ht_linear_class_loss_forward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
-                                            int64_t ignore_index, int reduction, float *loss, float *stats, void *workspace,
+                                            int64_t ignore_index, int reduction, float *loss, float *stats, void *kept, void *workspace,
                                             size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream) {
   int rc = screen(p);
   if (rc != HT_OK) return rc;
@@ -527,26 +554,27 @@ extern "C" int ht_linear_class_loss_forward(const ht_dense_problem *p, const voi
   if (p->rows == 0 && reduction == HT_REDUCTION_NONE) return HT_OK;
   if (loss == nullptr || (p->rows > 0 && (x == nullptr || w == nullptr || target == nullptr))) return HT_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(stats) |
-        reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+        reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
     return HT_ERR_UNSUPPORTED;
   return by_type(p->dtype, [&](auto zero) -> int {
-    return forward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, loss, stats, workspace, workspace_bytes, status_word,
+    return forward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, loss, stats, kept, workspace, workspace_bytes, status_word,
                                    reinterpret_cast<cudaStream_t>(stream));
   });
 }
 
 extern "C" int ht_linear_class_loss_backward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
-                                             int64_t ignore_index, int reduction, const float *grad, const float *stats, void *dx, void *dw,
+                                             int64_t ignore_index, int reduction, const float *grad, const float *stats, const void *kept, void *dx, void *dw,
                                              void *dbias, void *workspace, size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream) {
   int rc = screen(p);
   if (rc != HT_OK) return rc;
   if (reduction != HT_REDUCTION_NONE && reduction != HT_REDUCTION_MEAN && reduction != HT_REDUCTION_SUM) return HT_ERR_INVALID_ARGUMENT;
   if (p->rows > 0 && (x == nullptr || w == nullptr || target == nullptr || grad == nullptr || stats == nullptr)) return HT_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(stats) |
-        reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+        reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw) |
+        reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
     return HT_ERR_UNSUPPORTED;
   return by_type(p->dtype, [&](auto zero) -> int {
-    return backward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, grad, stats, dx, dw, dbias, workspace, workspace_bytes,
+    return backward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, grad, stats, kept, dx, dw, dbias, workspace, workspace_bytes,
                                     status_word, reinterpret_cast<cudaStream_t>(stream));
   });
 }

@@ -148,6 +148,25 @@ __device__ __forceinline__ void move_box(uint32_t box, T *first, size_t pitch, i
     }
   }
 }
+// Whole boxes of 16-bit rows that start on 2 bytes, to memory: two values at a time from the first even address on, out of two words of the
+// box where the row starts on an odd one, whose first and last value go alone.
+template <typename T>
+__device__ __forceinline__ void store_odd_box(uint32_t box, T *first, size_t pitch, int rows, int lane) {
+  auto word = [&](uint32_t r, uint32_t i) { return lds_b32(box + box_offset<T>(r, i >> 2) + (i & 3u) * 4u); };
+  const uint32_t i = (uint32_t)lane & 15u;
+#pragma unroll 4
+  for (uint32_t r = (uint32_t)lane >> 4; r < 32u; r += 2u) {
+    T *const row = first + (size_t)r * pitch;
+    const bool odd = (reinterpret_cast<uintptr_t>(row) & 2u) != 0;
+    const uint32_t low = word(r, i), high = word(r, min(i + 1u, 15u));
+    if ((int)r < rows && !(odd && i == 15u)) *reinterpret_cast<uint32_t *>(row + 2 * i + (odd ? 1 : 0)) = odd ? __funnelshift_r(low, high, 16) : low;
+  }
+  T *const own = first + (size_t)lane * pitch;
+  if (lane < rows && (reinterpret_cast<uintptr_t>(own) & 2u) != 0) {
+    *reinterpret_cast<uint16_t *>(own) = (uint16_t)word((uint32_t)lane, 0u);
+    *reinterpret_cast<uint16_t *>(own + 31) = (uint16_t)(word((uint32_t)lane, 15u) >> 16);
+  }
+}
 template <typename T, bool STORE>
 __device__ __forceinline__ void move_box_by(uint32_t box, T *first, size_t pitch, int rows, int cols, int align, int lane) {
   if (align >= 16)
@@ -156,8 +175,12 @@ __device__ __forceinline__ void move_box_by(uint32_t box, T *first, size_t pitch
     move_box<T, 8, STORE>(box, first, pitch, rows, cols, lane);
   else if (align == 4 || sizeof(T) == 4)
     move_box<T, 4, STORE>(box, first, pitch, rows, cols, lane);
-  else if constexpr (sizeof(T) == 2)
-    move_box<T, 2, STORE>(box, first, pitch, rows, cols, lane);
+  else if constexpr (sizeof(T) == 2) {
+    if (STORE && cols >= 32)
+      store_odd_box<T>(box, first, pitch, rows, lane);
+    else
+      move_box<T, 2, STORE>(box, first, pitch, rows, cols, lane);
+  }
 }
 
 template <typename T>
@@ -471,10 +494,13 @@ struct Operand {
   const int64_t *target = nullptr;
   int64_t ignore = 0;
   static bool direct(int64_t stride) { return Kind<T>::kPlanes == 1 && stride % 8 == 0; }
-  void set(Arena &arena, const T *data, int64_t rows, int64_t cols, int64_t row_stride, const int64_t *skip = nullptr, int64_t skipped = 0) {
+  bool ready = false;  // the copy has been made by an earlier call
+  // `skips`: rows whose target is the ignored one come as zeros, in a copy.
+  void set(Arena &arena, const T *data, int64_t rows, int64_t cols, int64_t row_stride, bool skips = false, const int64_t *skip = nullptr,
+           int64_t skipped = 0) {
     source = data, stride = row_stride, target = skip, ignore = skipped;
     m.rows = rows, m.cols = cols, m.planes = Kind<T>::kPlanes;
-    if (direct(row_stride) && skip == nullptr) {
+    if (direct(row_stride) && !skips) {
       m.data = data, m.pitch = row_stride;
       return;
     }
@@ -549,7 +575,7 @@ int lay_out(std::initializer_list<const Operand<T> *> operands, cudaStream_t str
   int64_t most = 0;
   unsigned count = 0;
   for (const Operand<T> *o : operands) {
-    if (o->copy == nullptr || o->m.rows == 0) continue;
+    if (o->copy == nullptr || o->ready || o->m.rows == 0) continue;
     const bool whole = (reinterpret_cast<uintptr_t>(o->source) & 15u) == 0 && o->stride * (int64_t)sizeof(T) % 16 == 0;
     all.jobs[count++] = {o->source, o->copy, o->m.rows, o->m.cols, o->stride, o->m.pitch, o->m.plane, o->ignore, o->target, whole};
     most = std::max(most, o->m.rows * (o->m.pitch / 8));

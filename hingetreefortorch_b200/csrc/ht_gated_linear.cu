@@ -5,7 +5,7 @@
 //
 // Forward: one tile product over the rows of both weights side by side, 64 or 128 columns of each; the epilogue has the two products
 // of an element in one thread and writes h alone.
-// Backward: nothing but x is kept.  The projections are formed again, the epilogue reads dh and writes da and du in the operands' type,
+// Backward: of the forward nothing is kept but copies of operands that cannot be read as they are.  The projections are formed again, the epilogue reads dh and writes da and du in the operands' type,
 // and those enter the products of ht_dense_products.cu: dx as one sum over both, dwg and dwv as one product.  16 N K H
 // operations for a training step where 12 N K H are needed; keeping a and u in fp32, which the gradient's accuracy asks for,
 // would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to the operands' 16 bits (2^-9 of a term
@@ -235,16 +235,24 @@ struct Plan {
   typename Kind<T>::Operand *g = nullptr;
   uint32_t *top = nullptr;
   float *sum = nullptr, *parts = nullptr, *row_sums = nullptr;
-  size_t bytes;
-  Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, void *ws) {
+  size_t bytes = 0, kept_bytes = 0;
+  Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, bool keeps, void *kept,
+       void *ws) {
     Arena arena(ws);
-    bytes = 0;
     few = !backward && (few_rows<T>(p.rows, p.features, p.outputs, true, &few_plan) ||
                         some_rows<T>(p.rows, p.features, p.outputs, p.x_stride, true, &few_plan));
+    // the copies of what cannot be read as it is: made by the forward for both where they are kept
+    Arena keeping(kept);
+    Arena &copies = keeps ? keeping : arena;
+    if (!few || keeps) {
+      x.set(copies, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
+      wg.set(copies, static_cast<const T *>(wgp), p.outputs, p.features, p.features);
+      wv.set(copies, static_cast<const T *>(wvp), p.outputs, p.features, p.features);
+      x.ready = wg.ready = wv.ready = backward && keeps;
+    }
+    kept_bytes = keeping.used;
+    bytes = arena.used;
     if (few) return;
-    x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
-    wg.set(arena, static_cast<const T *>(wgp), p.outputs, p.features, p.features);
-    wv.set(arena, static_cast<const T *>(wvp), p.outputs, p.features, p.features);
     if (backward) {
       const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
       const int64_t per_output = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 4;
@@ -265,11 +273,12 @@ struct Plan {
 };
 
 template <typename T>
-int forward(const ht_dense_problem &p, const void *x, const void *wg, const void *wv, const void *bg, const void *bv, void *h, void *ws,
+int forward(const ht_dense_problem &p, const void *x, const void *wg, const void *wv, const void *bg, const void *bv, void *h, void *kept, void *ws,
             size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
-  Plan<T> plan(p, x, wg, wv, false, false, false, ws);
+  Plan<T> plan(p, x, wg, wv, false, false, false, kept != nullptr, kept, ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   int sms = 0, rc;
+  HT_TRY(lay_out<T>({&plan.x, &plan.wg, &plan.wv}, stream));
   if (plan.few) {
     const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(wg), static_cast<const T *>(wv)}, p.x_stride, (int)p.rows, (int)p.features,
                           (int)p.outputs};
@@ -277,7 +286,6 @@ int forward(const ht_dense_problem &p, const void *x, const void *wg, const void
     return launch_rows(a, e, plan.few_plan, stream);
   }
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  HT_TRY(lay_out<T>({&plan.x, &plan.wg, &plan.wv}, stream));
   TileProblem t;
   t.a[0] = plan.x.m;
   t.b[0] = plan.wg.m;
@@ -296,9 +304,9 @@ struct Gradients {
 
 template <typename T>
 int backward(const ht_dense_problem &p, const void *x, const void *wg, const void *wv, const void *bg, const void *bv, const void *dh,
-             const Gradients &out, void *ws, size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
+             const void *kept, const Gradients &out, void *ws, size_t ws_bytes, uint32_t *status_word, cudaStream_t stream) {
   const bool has_bias = out.dbg != nullptr || out.dbv != nullptr;
-  Plan<T> plan(p, x, wg, wv, true, out.dx != nullptr, has_bias, ws);
+  Plan<T> plan(p, x, wg, wv, true, out.dx != nullptr, has_bias, kept != nullptr, const_cast<void *>(kept), ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   T *dwg = static_cast<T *>(out.dwg), *dwv = static_cast<T *>(out.dwv), *dbg = static_cast<T *>(out.dbg), *dbv = static_cast<T *>(out.dbv);
   if (p.rows == 0) {
@@ -404,35 +412,42 @@ using namespace ht::dense;
 extern "C" size_t ht_gated_linear_workspace_bytes(const ht_dense_problem *p, int backward) {
   if (screen(p) != HT_OK) return 0;
   return by_type(p->dtype, [&](auto zero) -> size_t {
-    return Plan<decltype(zero)>(*p, nullptr, nullptr, nullptr, backward != 0, true, true, nullptr).bytes;
+    return Plan<decltype(zero)>(*p, nullptr, nullptr, nullptr, backward != 0, true, true, false, nullptr, nullptr).bytes;
+  });
+}
+
+extern "C" size_t ht_gated_linear_kept_bytes(const ht_dense_problem *p) {
+  if (screen(p) != HT_OK || p->rows == 0) return 0;
+  return by_type(p->dtype, [&](auto zero) -> size_t {
+    return Plan<decltype(zero)>(*p, nullptr, nullptr, nullptr, false, false, false, true, nullptr, nullptr).kept_bytes;
   });
 }
 
 extern "C" int ht_gated_linear_forward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
-                                       const void *gate_bias, const void *value_bias, void *h, void *workspace, size_t workspace_bytes,
+                                       const void *gate_bias, const void *value_bias, void *h, void *kept, void *workspace, size_t workspace_bytes,
                                        uint32_t *status_word, ht_stream_t stream) {
   const int rc = screen(p);
   if (rc != HT_OK) return rc;
   if (p->rows == 0) return HT_OK;
   if (x == nullptr || gate_weight == nullptr || value_weight == nullptr || h == nullptr) return HT_ERR_INVALID_ARGUMENT;
-  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, h, workspace})) return HT_ERR_UNSUPPORTED;
+  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, h, kept, workspace})) return HT_ERR_UNSUPPORTED;
   return by_type(p->dtype, [&](auto zero) -> int {
-    return forward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, h, workspace, workspace_bytes, status_word,
+    return forward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, h, kept, workspace, workspace_bytes, status_word,
                                    reinterpret_cast<cudaStream_t>(stream));
   });
 }
 
 extern "C" int ht_gated_linear_backward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
-                                        const void *gate_bias, const void *value_bias, const void *dh, void *dx, void *dgate_weight,
+                                        const void *gate_bias, const void *value_bias, const void *dh, const void *kept, void *dx, void *dgate_weight,
                                         void *dvalue_weight, void *dgate_bias, void *dvalue_bias, void *workspace, size_t workspace_bytes,
                                         uint32_t *status_word, ht_stream_t stream) {
   const int rc = screen(p);
   if (rc != HT_OK) return rc;
   if (p->rows > 0 && (x == nullptr || gate_weight == nullptr || value_weight == nullptr || dh == nullptr)) return HT_ERR_INVALID_ARGUMENT;
-  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, dh, dx, dgate_weight, dvalue_weight, workspace})) return HT_ERR_UNSUPPORTED;
+  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, dh, kept, dx, dgate_weight, dvalue_weight, workspace})) return HT_ERR_UNSUPPORTED;
   const Gradients out = {dx, dgate_weight, dvalue_weight, dgate_bias, dvalue_bias};
   return by_type(p->dtype, [&](auto zero) -> int {
-    return backward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, dh, out, workspace, workspace_bytes, status_word,
+    return backward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, dh, kept, out, workspace, workspace_bytes, status_word,
                                     reinterpret_cast<cudaStream_t>(stream));
   });
 }

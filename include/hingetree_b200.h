@@ -426,7 +426,9 @@ int ht_thresholds_f64(int fix, double *thr, const int64_t *ord, int64_t T, int d
  * from row to row, weights [outputs, features], biases [outputs] or NULL, gradients like what they belong to.  Sums, softmax statistics and
  * losses are fp32; fp32 products are as accurate as fp32 ones (three bf16 planes a value).  Pointers to matrices, biases,
  * statistics and workspaces start on 16 bytes (HT_ERR_UNSUPPORTED otherwise).  No atomics: the same call gives the same bits.
- * Workspaces: the matching *_workspace_bytes (0 for a bad problem). */
+ * Workspaces: the matching *_workspace_bytes (0 for a bad problem).  kept (may be NULL, in both calls): *_kept_bytes that a forward fills and
+ * the backward of the same tensors is given, copies of operands that cannot be read as they are (fp32, and 16-bit rows that do not start on
+ * 16 bytes); otherwise the backward makes them again. */
 #define HT_DTYPE_F32 0
 #define HT_DTYPE_BF16 1
 #define HT_DTYPE_F16 2
@@ -450,25 +452,27 @@ typedef struct ht_dense_problem {
 /* h[n, o] = act(x[n] . gate_weight[o] + gate_bias[o]) * (x[n] . value_weight[o] + value_bias[o]).  The backward forms the projections
  * again; gradients that are NULL are not computed.  rows = 0: nothing to write, or zeros for the weights. */
 size_t ht_gated_linear_workspace_bytes(const ht_dense_problem *p, int backward);
+size_t ht_gated_linear_kept_bytes(const ht_dense_problem *p);
 int ht_gated_linear_forward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
-                            const void *gate_bias, const void *value_bias, void *h, void *workspace, size_t workspace_bytes,
-                            uint32_t *status_word, ht_stream_t stream);
+                            const void *gate_bias, const void *value_bias, void *h, void *kept, void *workspace,
+                            size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
 int ht_gated_linear_backward(const ht_dense_problem *p, const void *x, const void *gate_weight, const void *value_weight,
-                             const void *gate_bias, const void *value_bias, const void *dh, void *dx, void *dgate_weight,
-                             void *dvalue_weight, void *dgate_bias, void *dvalue_bias, void *workspace, size_t workspace_bytes,
-                             uint32_t *status_word, ht_stream_t stream);
+                             const void *gate_bias, const void *value_bias, const void *dh, const void *kept, void *dx,
+                             void *dgate_weight, void *dvalue_weight, void *dgate_bias, void *dvalue_bias, void *workspace,
+                             size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
 
 /* loss[n] = log sum_o exp(s[n, o]) - s[n, target[n]] with s = x w^T + bias, never in memory; a row whose target is ignore_index has loss
  * and gradients 0 whatever it holds; a target outside [0, outputs) makes the row's loss (and gradients that it enters) NaN and
  * sets HT_FLAG_TARGET_RANGE.  loss: [rows] floats, or one for a sum or mean.  stats (may be NULL: no backward follows):
  * 2 rows + 2 floats that the backward is given.  grad: the upstream gradient, shaped like loss. */
 size_t ht_linear_class_loss_workspace_bytes(const ht_dense_problem *p, int backward);
+size_t ht_linear_class_loss_kept_bytes(const ht_dense_problem *p);
 int ht_linear_class_loss_forward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
-                                 int64_t ignore_index, int reduction, float *loss, float *stats, void *workspace,
+                                 int64_t ignore_index, int reduction, float *loss, float *stats, void *kept, void *workspace,
                                  size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
 int ht_linear_class_loss_backward(const ht_dense_problem *p, const void *x, const void *w, const void *bias, const int64_t *target,
-                                  int64_t ignore_index, int reduction, const float *grad, const float *stats, void *dx, void *dw,
-                                  void *dbias, void *workspace, size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
+                                  int64_t ignore_index, int reduction, const float *grad, const float *stats, const void *kept,
+                                  void *dx, void *dw, void *dbias, void *workspace, size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -67,21 +67,21 @@ def test_entries_screen_before_they_touch_a_device():
         for backward in (0, 1):
             assert lib.ht_gated_linear_workspace_bytes(ctypes.byref(p), backward) == 0
             assert lib.ht_linear_class_loss_workspace_bytes(ctypes.byref(p), backward) == 0
-        assert lib.ht_gated_linear_forward(ctypes.byref(p), null, null, null, null, null, null, null, size(0), null, null) == -1
-        assert lib.ht_linear_class_loss_forward(ctypes.byref(p), null, null, null, null, ctypes.c_int64(-100), 1, null, null, null, size(0), null, null) == -1
+        assert lib.ht_gated_linear_forward(ctypes.byref(p), null, null, null, null, null, null, null, null, size(0), null, null) == -1
+        assert lib.ht_linear_class_loss_forward(ctypes.byref(p), null, null, null, null, ctypes.c_int64(-100), 1, null, null, null, null, size(0), null, null) == -1
     p = DenseProblem(1, 4, 8, 16, 32, 16, 0)
-    assert lib.ht_gated_linear_forward(ctypes.byref(p), null, null, null, null, null, null, null, size(0), null, null) == -1
+    assert lib.ht_gated_linear_forward(ctypes.byref(p), null, null, null, null, null, null, null, null, size(0), null, null) == -1
     host = (ctypes.c_char * 4096)()
     at = (ctypes.addressof(host) + 255) // 256 * 256
     ptr, odd = ctypes.c_void_p(at), ctypes.c_void_p(at + 2)
     g = ctypes.byref(good)
     # a pointer that does not start on 16 bytes; no room for a workspace; a reduction that there is not; nothing to write to
-    assert lib.ht_gated_linear_forward(g, odd, ptr, ptr, null, null, ptr, ptr, size(1 << 20), null, null) == -5
-    assert lib.ht_gated_linear_backward(g, ptr, ptr, ptr, null, null, ptr, ptr, ptr, ptr, null, null, ptr, size(16), null, null) == -4
-    assert lib.ht_linear_class_loss_forward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 3, ptr, null, ptr, size(1 << 20), null, null) == -1
-    assert lib.ht_linear_class_loss_forward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 1, null, null, ptr, size(1 << 20), null, null) == -1
-    assert lib.ht_linear_class_loss_forward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 1, ptr, null, null, size(0), null, null) == -4
-    assert lib.ht_linear_class_loss_backward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 1, ptr, null, ptr, ptr, null, ptr, size(1 << 20), null, null) == -1
+    assert lib.ht_gated_linear_forward(g, odd, ptr, ptr, null, null, ptr, null, ptr, size(1 << 20), null, null) == -5
+    assert lib.ht_gated_linear_backward(g, ptr, ptr, ptr, null, null, ptr, null, ptr, ptr, ptr, null, null, ptr, size(16), null, null) == -4
+    assert lib.ht_linear_class_loss_forward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 3, ptr, null, null, ptr, size(1 << 20), null, null) == -1
+    assert lib.ht_linear_class_loss_forward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 1, null, null, null, ptr, size(1 << 20), null, null) == -1
+    assert lib.ht_linear_class_loss_forward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 1, ptr, null, null, null, size(0), null, null) == -4
+    assert lib.ht_linear_class_loss_backward(g, ptr, ptr, null, ptr, ctypes.c_int64(-100), 1, ptr, null, null, ptr, ptr, null, ptr, size(1 << 20), null, null) == -1
 
 
 @pytest.mark.parametrize("dtype,planes", [(0, 3), (1, 1), (2, 1)])
