@@ -19,7 +19,8 @@ namespace dense {
 constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;
 constexpr int kFewRing = 8;  // steps of k in flight
 constexpr uint32_t kFewRingBytes = kFewWarps * kFewRing * 1024;
-constexpr int64_t kFewMostBytes = 224 * 1024 - (int64_t)kFewRingBytes;  // of x in shared memory, and of the warps' sums
+// of x in shared memory and of the warps' sums: what the rings and an epilogue's own 4 KB leave
+constexpr int64_t kFewMostBytes = 222 * 1024 - (int64_t)kFewRingBytes;
 
 template <typename T>
 struct FewArgs {

@@ -122,6 +122,30 @@ def test_class_loss(kind, rows, features, classes, reduction):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,features,classes", [
+    (8, 200, 40000),      # few rows, a warp for every 16 classes
+    (8, 2700, 50), (8, 5400, 50), (8, 2660, 50), (7, 2900, 40), (14, 2500, 40), (30, 1240, 40), (29, 1300, 30),  # x about fills shared memory
+    (16, 1030, 6000), (20, 500, 300), (32, 2050, 90), (24, 4096, 100), (31, 70, 5000),
+    (33, 4, 17), (64, 1024, 2300), (65, 100, 4700), (100, 2048, 31), (128, 36, 1000), (77, 2052, 130), (90, 99, 600),
+    (6000, 33, 70),       # few tiles of the weights' gradient, long sums over the rows
+    (150, 48, 9000),      # and of the features'
+    (2500, 300, 300), (1100, 65, 1500), (700, 520, 225)])
+def test_class_loss_by_size(kind, rows, features, classes):
+    """Sizes at which other kernels, tile shapes and cuts of the sums are taken."""
+    x, w, b, t = loss_inputs(kind, rows, features, classes, bias=features % 2 == 0, ignored=rows % 2 == 1, seed=rows)
+    check_loss(x, w, b, t, "mean")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("act,rows,features,outputs", [
+    ("silu", 8, 200, 20000), ("gelu", 16, 1030, 3000), ("relu", 20, 500, 150), ("sigmoid", 32, 2050, 45), ("gelu", 24, 4096, 50),
+    ("silu", 33, 4, 9), ("gelu", 64, 1024, 1150), ("sigmoid", 65, 100, 2350), ("silu", 100, 2048, 16), ("relu", 128, 36, 500), ("gelu", 77, 2052, 65),
+    ("silu", 90, 99, 300), ("gelu", 6000, 33, 35), ("silu", 150, 48, 5000), ("gelu", 2500, 300, 150), ("sigmoid", 1100, 65, 900), ("silu", 700, 520, 97)])
+def test_gated_linear_by_size(kind, act, rows, features, outputs):
+    check_gated(*gated_inputs(kind, rows, features, outputs, bias=features % 2 == 0, seed=rows), act)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_rows_that_do_not_count(kind):
     """Whatever an ignored row holds, nothing of it enters; none at all: NaN for a mean, and no gradient."""
     x, w, b, t = loss_inputs(kind, 200, 72, 300, ignored=True)
@@ -307,22 +331,27 @@ def both(x, w, b, t, reduction="mean", **options):
 @pytest.mark.parametrize("kind", TYPES)
 def test_strides_and_alignment(kind):
     """Rows apart, columns apart, an odd start, more dimensions, one row for all: the values count, not where they lie."""
+    for rows in (3, 20, 200):
+        x, w, b, t = loss_inputs(kind, rows, 40, 70)
+        want = both(x, w, b, t)
+        wide = torch.zeros(rows, 48, device="cuda", dtype=kind)
+        wide[:, :40] = x
+        odd = torch.zeros(rows * 40 + 1, device="cuda", dtype=kind)
+        odd[1:] = x.flatten()
+        ragged = torch.zeros(rows, 41, device="cuda", dtype=kind)
+        ragged[:, 1:] = x
+        narrow = torch.zeros(rows, 41, device="cuda", dtype=kind)  # rows apart by an odd number of values, the first one aligned
+        narrow[:, :40] = x
+        for view in (wide[:, :40], odd[1:].view(rows, 40), ragged[:, 1:], narrow[:, :40], x.t().contiguous().t()):
+            assert torch.equal(view, x)
+            for got, value in zip(both(view, w, b, t), want):
+                assert torch.equal(got, value)
     x, w, b, t = loss_inputs(kind, 60, 40, 70)
     want = both(x, w, b, t)
-    wide = torch.zeros(60, 48, device="cuda", dtype=kind)
-    wide[:, :40] = x
-    odd = torch.zeros(60 * 40 + 1, device="cuda", dtype=kind)
-    odd[1:] = x.flatten()
-    ragged = torch.zeros(60, 41, device="cuda", dtype=kind)
-    ragged[:, 1:] = x
     odd_w = torch.zeros(70 * 40 + 1, device="cuda", dtype=kind)
     odd_w[1:] = w.flatten()
     odd_b = torch.zeros(71, device="cuda", dtype=kind)
     odd_b[1:] = b
-    for view in (wide[:, :40], odd[1:].view(60, 40), ragged[:, 1:], x.t().contiguous().t()):
-        assert torch.equal(view, x)
-        for got, value in zip(both(view, w, b, t), want):
-            assert torch.equal(got, value)
     for got, value in zip(both(x, odd_w[1:].view(70, 40), odd_b[1:], t), want):
         assert torch.equal(got, value)
     for got, value in zip(both(x, w.t().contiguous().t(), b, t), want):
@@ -405,6 +434,76 @@ def test_other_streams_and_captured_graphs():
         for k in order:
             assert all(torch.equal(a, c) for a, c in zip(graphs[k][2], both(*fresh[k], t)))
     assert hingetree_cpp.pipeline_status() == 0
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_what_is_kept_for_the_backward_does_not_change_it(kind):
+    """Copies of operands that a forward leaves (fp32, and rows that do not start on 16 bytes): kept, made again, used twice."""
+    x, w, b, t = loss_inputs(kind, 150, 75, 300, ignored=True)
+    dh = normal(generator(4), 150, 300, kind=kind)
+
+    def run(times):
+        leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+        out = [F.linear_class_loss(*leaves, t), F.gated_linear(leaves[0], leaves[1], leaves[1], leaves[2], leaves[2])]
+        return [[torch.autograd.grad(o, leaves, d, retain_graph=k + 1 < times) for k in range(times)] for o, d in zip(out, (None, dh))]
+
+    kept = run(3)
+    hingetree_cpp.set_save_forward(False)
+    try:
+        again = run(1)
+    finally:
+        hingetree_cpp.set_save_forward(True)
+    for a, c in zip(kept, again):
+        for grads in a:
+            assert all(torch.equal(g, v) for g, v in zip(grads, c[0]))
+
+
+def test_calls_on_two_streams_at_once():
+    """Large and small calls of either operator on two streams, alternately: nothing is shared that they could meet in."""
+    cases = [loss_inputs(kind, rows, 136, 900, ignored=True, seed=rows) for kind in TYPES for rows in (5, 100, 900)]
+    want = [both(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = {}
+    for turn in range(3):
+        for k, c in enumerate(cases):
+            with torch.cuda.stream(streams[(k + turn) % 2]):
+                got[turn, k] = both(*c)
+    torch.cuda.synchronize()
+    for (_, k), values in got.items():
+        assert all(torch.equal(a, v) for a, v in zip(values, want[k]))
+    assert hingetree_cpp.pipeline_status() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_captured_answers(rows):
+    """Few rows, captured and replayed on new data, in inference mode too."""
+    for kind in TYPES:
+        x, w, b, t = loss_inputs(kind, rows, 72, 500)
+        y, _, _, s = loss_inputs(kind, rows, 72, 500, seed=9)
+
+        def answer():
+            return F.linear_class_loss(x, w, b, t, reduction="none"), F.gated_linear(x, w, w, b, b), F.linear_class_loss(x, w, b, t)
+
+        with torch.inference_mode():
+            first = answer()
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(graph):
+            out = answer()
+        graph.replay()
+        assert all(torch.equal(a, c) for a, c in zip(out, first))
+        x.copy_(y)
+        t.copy_(s)
+        graph.replay()
+        assert all(torch.equal(a, c) for a, c in zip(out, answer()))
+
+
+def test_transforms_are_refused():
+    x, w, b, t = loss_inputs(torch.float32, 20, 8, 9)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: F.gated_linear(v, w, w))(x.view(4, 5, 8))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda v: F.linear_class_loss(v, w, b, t), (x,), (torch.ones_like(x),))
 
 
 def test_no_second_derivative():
