@@ -5,7 +5,7 @@
 // of a row, not what the instruction's layout spreads over it: whole sectors are read, and a lane fetches what it uses itself, into a ring of 8
 // steps of its own in shared memory (cp.async), across the ends of rows.  128 KB an SM are then in flight; with the loads of 4 steps in registers
 // instead, 205 MB of fp32 weights took 73 us.
-// fp32 values are taken as two TF32 numbers (x = x0 + x1, 22 bits and a sign) and the products x0 w0 + x0 w1 + x1 w0, summed 4 steps at a time
+// fp32 values are taken as two TF32 numbers (x = x0 + x1, 22 bits and a sign) and the products x0 w0 + x0 w1 + x1 w0, summed 2 steps at a time
 // in a fresh accumulator and in fp32 from there on (the tensor core truncates when it adds).
 // With few weights several warps of a block share 16 rows and take k in turn.
 // What bounds it: the weights' bytes; the launch with few of them.
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
           }
         }
       }
-      if (kFloat && ((i & 3) == 3 || i == own - 1)) {
+      if (kFloat && ((i & 1) == 1 || i == own - 1)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -250,8 +250,8 @@ int launch_few(FewArgs<T> a, const Epilogue &e, const FewPlan &plan, cudaStream_
 // ---- some more rows, few weights --------------------------------------------------------------------------------------
 // fp32, up to 128 rows: a tile of 128 rows would have a handful of SMs walk k through three planes (100 rows, 1000 to 2 x 700: 35 us).  Here a
 // block takes 16 rows of the weights (of a pair: 8 of each), its 16 warps take 64 rows of x each and share k, and x comes straight
-// from L2 in the instruction's layout, since no warp uses what another does.  A warp's chain of additions in the tensor core is
-// at most 96 long (k <= 2048), which loses 1e-6 of a sum at the worst; the warps' sums are added in fp32, 8 rows a warp.
+// from L2 in the instruction's layout, since no warp uses what another does.  Every step's sum starts afresh and is added in fp32 (chains of 48
+// additions in the tensor core lost 1.5e-6 of the sums); the warps' sums are added last, 8 rows a warp.
 // What bounds it: rows x k from L2 for every 16 rows of the weights, and the latency of a few loads in a row.
 constexpr int kSomeTiles = 8;  // of 8 rows a warp
 
@@ -289,23 +289,29 @@ __global__ void __launch_bounds__(kFewThreads, 1) some_rows_kernel(const FewArgs
         q[n] = there && r < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)r * a.x_stride + k)) : zero;
       }
       const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
+      uint32_t high[2][4], low[2][4];
 #pragma unroll
-      for (int h = 0; h < 4; h += 2) {
-        uint32_t high[4], low[4];
-        split_tf32(wa[h], high[0], low[0]);
-        split_tf32(wb[h], high[1], low[1]);
-        split_tf32(wa[h + 1], high[2], low[2]);
-        split_tf32(wb[h + 1], high[3], low[3]);
+      for (int h = 0; h < 2; ++h) {
+        split_tf32(wa[2 * h], high[h][0], low[h][0]);
+        split_tf32(wb[2 * h], high[h][1], low[h][1]);
+        split_tf32(wa[2 * h + 1], high[h][2], low[h][2]);
+        split_tf32(wb[2 * h + 1], high[h][3], low[h][3]);
+      }
 #pragma unroll
-        for (int n = 0; n < kSomeTiles; ++n) {
-          const uint32_t x[4] = {q[n].x, q[n].y, q[n].z, q[n].w};
+      for (int n = 0; n < kSomeTiles; ++n) {
+        const uint32_t x[4] = {q[n].x, q[n].y, q[n].z, q[n].w};
+        float fresh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           uint32_t h0, l0, h1, l1;
-          split_tf32(x[h], h0, l0);
-          split_tf32(x[h + 1], h1, l1);
-          mma_few<T>(c[n], low, h0, h1);
-          mma_few<T>(c[n], high, l0, l1);
-          mma_few<T>(c[n], high, h0, h1);
+          split_tf32(x[2 * h], h0, l0);
+          split_tf32(x[2 * h + 1], h1, l1);
+          mma_few<T>(fresh, low[h], h0, h1);
+          mma_few<T>(fresh, high[h], l0, l1);
+          mma_few<T>(fresh, high[h], h0, h1);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[n][i] += fresh[i];
       }
     }
     __syncthreads();  // the sums of the group before have been read

@@ -630,10 +630,12 @@ inline int sm_count(int *sms) {
 }
 
 // How to cut a product: the shape with which the SMs are done first.  Cycles of a step of 16 values of k, measured: a pair of CTAs with 256
-// columns 160, with 128 columns 118, in steps of 32 between; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120 (three planes: 6 of those, of
-// 128 columns at the most alone).  A tile costs about 2500 cycles besides.  Against that, the operands have to come from memory once,
-// 23 bytes a cycle and SM where all read, twice that where few do.  Where `most_parts` allows it, k is cut as well: each part writes its
-// sums in fp32, and a kernel adds them (8 bytes a value and part, and about 6000 cycles).
+// columns 160, with 128 columns 118, in steps of 32 between; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120
+// (three planes: 6 of those, of 128 columns at the most alone).  A tile costs about 1300 cycles besides, a launch in pairs 1200.  Against
+// that, the operands have to come from memory once, 23 bytes a cycle and SM where all read, twice that where few do.  Where `most_parts`
+// allows it, k is cut as well: each part writes its sums in fp32, and a kernel adds them (8 bytes a value and part, about 6000 cycles).
+// Measured against the other shapes, us: 1555 x 336 to 2 x 1008, bf16: 7.5 with what is taken, alone and 256, 8.1 to 8.9 with others; 1003 x
+// 776 x 10008: 24.5 in pairs, 30.8 and 33.6 alone; 600 x 2048 to 2 x 300, fp32: 39 with 128 columns, 67 with 256.
 inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, bool pair, int most_parts = 1) {
   constexpr int kPlanSMs = 148;
   constexpr double kBytesPerCycle = 23.0;
@@ -647,7 +649,7 @@ inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, b
         const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n) * ctas * split, last = tiles % kPlanSMs;
         const double rounds = (double)((tiles + kPlanSMs - 1) / kPlanSMs);
         const double step = ctas == 2 ? 75.0 + 0.335 * bn : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
-        const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k / split + 15) / 16) * step + 2500.0);
+        const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k / split + 15) / 16) * step + 1300.0) + (ctas == 2 ? 1200.0 : 0.0);
         const double bytes = 2.0 * planes * (double)k * (double)(rows + cols * (pair ? 2 : 1)) / (double)tiles;
         const double memory = bytes / kBytesPerCycle * ((double)(tiles / kPlanSMs) + (last > 0 ? std::max(0.5, (double)last / kPlanSMs) : 0.0));
         const double sums = split > 1 ? 6000.0 + 8.0 * split * (double)rows * (double)cols / (kBytesPerCycle * kPlanSMs) : 0.0;
