@@ -13,7 +13,9 @@ def gated_linear(x, gate_weight, value_weight, gate_bias=None, value_bias=None, 
 
     x: [..., features]; weights: [outputs, features]; biases: [outputs] or None; all torch.float32, bfloat16 or float16, one type for all.
     activation: 'silu', 'gelu' (with the normal distribution function), 'relu' or 'sigmoid'.  Sums are fp32 whatever the type, and
-    fp32 results are as accurate as fp32 products.  Nothing but the inputs is kept for the backward, which forms the projections again."""
+    fp32 results are as accurate as fp32 products (of finite numbers: an infinity gives NaN).  The backward forms the projections again; of
+    the forward it keeps the inputs and, for fp32 and for 16-bit rows that do not start on 16 bytes, their copies in the tensor
+    cores' layout (6 or 2 bytes a number; hingetree_cpp.set_save_forward(False): none).  No second derivative."""
     return hingetree_cpp.gated_linear(x, gate_weight, value_weight, gate_bias, value_bias, activation)
 
 
@@ -27,5 +29,5 @@ def linear_class_loss(x, weight, bias, target, ignore_index=-100, reduction="mea
     A row whose target is ignore_index has loss and gradient 0 whatever it holds.  A target that is neither a class nor ignore_index
     makes the loss NaN, and the next call that reads the device's status word (hingetree_cpp.pipeline_status(), or the first call on new
     ordinals) raises RuntimeError.  The backward holds the gradient of the scores in pieces of 512 MiB at the most, less with
-    hingetree_cpp.set_backward_scratch_limit(bytes)."""
+    hingetree_cpp.set_backward_scratch_limit(bytes), and what gated_linear keeps of its inputs.  No second derivative."""
     return hingetree_cpp.linear_class_loss(x, weight, bias, target, ignore_index, reduction)

@@ -118,13 +118,16 @@ class Expand(torch.nn.Module):
         return _Patches.apply(inData, None, self.padding)
 
 
+_SAVED = object()  # in the place of a tensor (an operator's argument may be None)
+
+
 class _Traced(torch.autograd.Function):
     """One of the extension's `*_apply` as torch.jit.trace records it: a Python operation, which calls it again whenever the
     trace runs.  The backward differentiates another such call."""
 
     @staticmethod
     def forward(ctx, name, *args):
-        ctx.name, ctx.others = name, [None if isinstance(a, torch.Tensor) else a for a in args]
+        ctx.name, ctx.others = name, [_SAVED if isinstance(a, torch.Tensor) else a for a in args]
         ctx.save_for_backward(*[a for a in args if isinstance(a, torch.Tensor)])
         return _op(name)(*args)
 
@@ -132,7 +135,7 @@ class _Traced(torch.autograd.Function):
     def backward(ctx, grad):
         tensors, needs = iter(ctx.saved_tensors), ctx.needs_input_grad[1:]
         with torch.enable_grad():
-            args = [next(tensors).detach().requires_grad_(need) if a is None else a for a, need in zip(ctx.others, needs)]
+            args = [next(tensors).detach().requires_grad_(need) if a is _SAVED else a for a, need in zip(ctx.others, needs)]
             out = _op(ctx.name)(*args)
         grads = iter(torch.autograd.grad(out, [a for a, need in zip(args, needs) if need], grad))
         return (None, *[next(grads) if need else None for need in needs])

@@ -35,9 +35,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <utility>
 
 #include "ht_common.cuh"
 #include "ht_tile_common.cuh"
@@ -74,18 +71,7 @@ __device__ __forceinline__ void after_previous_kernel() {
 // Launches a kernel that begins with after_previous_kernel(), in clusters of `ctas`.
 template <typename... Parameters, typename... Arguments>
 int launch_next(void (*kernel)(Parameters...), dim3 grid, int threads, size_t shared, cudaStream_t stream, int ctas, const Arguments &...arguments) {
-  if (shared > 48 * 1024) {  // asked for once a kernel and device; more than is asked for does no harm
-    int device = 0;
-    HT_CUDA_TRY(cudaGetDevice(&device));
-    static std::mutex mutex;
-    static std::map<std::pair<const void *, int>, size_t> granted;
-    std::lock_guard<std::mutex> lock(mutex);
-    size_t &most = granted[{reinterpret_cast<const void *>(kernel), device}];
-    if (shared > most) {
-      HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
-      most = shared;
-    }
-  }
+  if (shared > 48 * 1024) HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
   cudaLaunchAttribute attributes[2] = {};
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[0].val.programmaticStreamSerializationAllowed = 1;
@@ -284,7 +270,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
   uint64_t *accumulated = empty + kMostStages;                         // [2] an accumulator is complete
   uint64_t *drained = accumulated + 2;                                 // [2] ... and has been read out
   uint64_t *drained_small = drained + 2;                               // the small products' accumulator
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained_small + 1);
+  uint64_t *settled = drained_small + 1;                               // every product issued has ended
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(settled + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
@@ -301,6 +288,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
       mbar_init(&drained[b], kEpilogueWarps * CTAS);
     }
     mbar_init(drained_small, kEpilogueWarps * CTAS);
+    mbar_init(settled, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -479,6 +467,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           }
         }
       }
+      // whatever became of the waits: tensor memory is not freed under a product
+      mma_commit<CTAS>(one, smem_addr(settled));
+      mbar_wait(settled, 0u);
     }
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2;  // a warp may only touch the lanes 32 (warp % 4) ...

@@ -601,6 +601,17 @@ def test_a_traced_front_and_loss_compute_on_new_data():
     assert torch.equal(traced(y, s), Net()(y, s))
 
 
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_traced_front_is_differentiated(bias):
+    front = R.GatedLinear(12, 20, bias=bias, activation="gelu").cuda()
+    gen = generator()
+    x, y = normal(gen, 30, 12), normal(gen, 30, 12)
+    traced = torch.jit.trace(front, (x,), check_trace=False)
+    params = list(front.parameters())
+    for got, want in zip(torch.autograd.grad(traced(y).square().sum(), params), torch.autograd.grad(front(y).square().sum(), params)):
+        assert torch.equal(got, want)
+
+
 def test_half_a_million_rows_of_few_features():
     """Row counts far beyond a tile, and products of sizes beyond 2^31: offsets are 64 bits wide."""
     rows, features, classes = 530000, 8, 4100  # 2.2e9 scores
