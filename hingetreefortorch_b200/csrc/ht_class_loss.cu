@@ -227,8 +227,8 @@ struct FewLossEpilogue {
 };
 
 // Joins the pieces of every row, a warp each, in a fixed order: stats[row] = (m, l), the row's loss to `loss`.  A row whose target is
-// no class: loss NaN and a flag.  For a sum or mean the last block to end adds the rows' losses, in fp64 and in an order that
-// depends on the number of rows alone, and leaves the number of rows that count behind the statistics.
+// no class: loss NaN and a flag.  For a sum or mean every block adds its rows' losses in fp64, and the last one to end the blocks' sums,
+// in an order that depends on the number of rows alone; it leaves the number of rows that count behind the statistics.
 struct JoinArgs {
   const float2 *partial;
   int slots;
@@ -236,9 +236,9 @@ struct JoinArgs {
   const int64_t *target;
   int64_t ignore, rows, classes;
   float2 *stats;
-  float *row_loss;
-  float *total;         // null: single rows
+  float *row_loss, *total;  // one of them, the other null: single rows, or their sum or mean
   bool mean;
+  double2 *block_sums;  // [blocks]: sum of losses, rows that count
   unsigned *ended;      // blocks that have, 0 at the start
   uint32_t *status_word;
 };
@@ -246,6 +246,8 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
   after_previous_kernel();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  float result = 0.0f;
+  bool counts = false;
   if (row < a.rows) {
     float m = -INFINITY, l = 0.0f;
     const float2 *pieces = a.partial + (size_t)row * (size_t)a.slots;
@@ -261,48 +263,47 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
       const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
       join(m, l, m2, l2);
     }
+    counts = t != a.ignore;
+    const bool valid = t >= 0 && t < a.classes;
+    if (counts) result = valid ? (float)((double)logf(l) + ((double)m - (double)score)) : NAN;
     if (lane == 0) {
       if (a.stats != nullptr) a.stats[row] = make_float2(m, l);
-      float result = 0.0f;
-      if (t != a.ignore) {
-        if (t >= 0 && t < a.classes) {
-          result = (float)((double)logf(l) + ((double)m - (double)score));
-        } else {
-          result = NAN;
-          if (a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_TARGET_RANGE);
-        }
-      }
-      a.row_loss[row] = result;
+      if (a.row_loss != nullptr) a.row_loss[row] = result;
+      if (counts && !valid && a.status_word != nullptr) atomicOr(a.status_word, HT_FLAG_TARGET_RANGE);
     }
   }
   if (a.total == nullptr) return;
+  __shared__ double2 sums[8];
   __shared__ bool last;
-  __threadfence();  // the row's loss, before the block counts as ended
+  if (lane == 0) sums[threadIdx.x >> 5] = make_double2((double)result, counts ? 1.0 : 0.0);
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.ended, 1u) == gridDim.x - 1;
+  if (threadIdx.x == 0) {
+    double2 sum = sums[0];
+    for (int i = 1; i < 8; ++i) sum.x += sums[i].x, sum.y += sums[i].y;
+    a.block_sums[blockIdx.x] = sum;
+    __threadfence();  // the block's sum, before it counts as ended
+    last = atomicAdd(a.ended, 1u) == gridDim.x - 1;
+  }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  __shared__ double sums[8];
-  __shared__ long long counts[8];
-  double sum = 0.0;
-  long long count = 0;
-#pragma unroll 8
-  for (int64_t r = threadIdx.x; r < a.rows; r += 256) {
-    if (__ldg(a.target + r) == a.ignore) continue;
-    sum += (double)__ldcg(a.row_loss + r);
-    ++count;
+  double2 sum = make_double2(0.0, 0.0);
+#pragma unroll 4
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += 256) {
+    const double2 q = __ldcg(a.block_sums + i);
+    sum.x += q.x, sum.y += q.y;
   }
-  for (int s = 16; s > 0; s >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    count += __shfl_xor_sync(0xffffffffu, count, s);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    sum.x += __shfl_xor_sync(0xffffffffu, sum.x, d);
+    sum.y += __shfl_xor_sync(0xffffffffu, sum.y, d);
   }
-  if (lane == 0) sums[threadIdx.x >> 5] = sum, counts[threadIdx.x >> 5] = count;
+  if (lane == 0) sums[threadIdx.x >> 5] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) sum += sums[i], count += counts[i];
-    a.total[0] = (float)(a.mean ? sum / (double)count : sum);
-    if (a.stats != nullptr) a.stats[a.rows].x = (float)count;
+    for (int i = 1; i < 8; ++i) sum.x += sums[i].x, sum.y += sums[i].y;
+    a.total[0] = (float)(a.mean ? sum.x / sum.y : sum.x);
+    if (a.stats != nullptr) a.stats[a.rows].x = (float)sum.y;
   }
 }
 
@@ -350,7 +351,8 @@ struct ForwardPlan {
   TileShape shape;
   int slots;
   float2 *partial;
-  float *target_score, *row_loss;
+  float *target_score;
+  double2 *block_sums;
   unsigned *ended;
   size_t bytes;
   ForwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, void *kept, void *ws) {
@@ -367,7 +369,7 @@ struct ForwardPlan {
     slots = few ? few_plan.blocks : (int)(2 * ((p.outputs + shape.bn - 1) / shape.bn));
     partial = arena.take<float2>((int64_t)slots * p.rows);
     target_score = arena.take<float>(p.rows);
-    row_loss = arena.take<float>(p.rows);
+    block_sums = arena.take<double2>(p.rows / 8 + 1);
     ended = arena.take<unsigned>(1);
     bytes = arena.used;
   }
@@ -379,7 +381,6 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
   ForwardPlan<T> plan(p, static_cast<const T *>(x), static_cast<const T *>(w), target, ignore, kept, ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   int sms = 0, rc;
-  float *row_loss = reduction == HT_REDUCTION_NONE ? loss : plan.row_loss;
   if (p.rows > 0) {
     // (copies that are left for the backward are made whichever kernel runs)
     if (kept != nullptr || !plan.few) HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
@@ -400,9 +401,9 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
     }
   }
   // (no rows: a sum of nothing)
-  JoinArgs j = {plan.partial, plan.slots, plan.target_score, target, ignore, p.rows, p.outputs, reinterpret_cast<float2 *>(stats), row_loss, nullptr,
-                reduction == HT_REDUCTION_MEAN, plan.ended, status_word};
-  if (reduction != HT_REDUCTION_NONE) j.total = loss;
+  JoinArgs j = {plan.partial, plan.slots, plan.target_score, target, ignore, p.rows, p.outputs, reinterpret_cast<float2 *>(stats), nullptr, nullptr,
+                reduction == HT_REDUCTION_MEAN, plan.block_sums, plan.ended, status_word};
+  (reduction == HT_REDUCTION_NONE ? j.row_loss : j.total) = loss;
   if (p.rows == 0) HT_CUDA_TRY(cudaMemsetAsync(plan.ended, 0, sizeof(unsigned), stream));
   return launch_next(join_rows_kernel, dim3((unsigned)std::max<int64_t>((p.rows + 7) / 8, 1)), 256, 0, stream, 1, j);
 }

@@ -225,7 +225,7 @@ bool few_rows(int64_t rows, int64_t features, int64_t outputs, bool pair, FewPla
   plan->pitch = (int)pitch;
   plan->split = 1;
   while (plan->split < kFewWarps && groups * plan->split * 2 <= most * kFewWarps) plan->split *= 2;
-  plan->blocks = (int)std::min<int64_t>((groups * plan->split + kFewWarps - 1) / kFewWarps, most);
+  plan->blocks = (int)std::min<int64_t>(groups, most);  // (every SM has its share of the groups, even if some of its warps have none)
   return true;
 }
 
