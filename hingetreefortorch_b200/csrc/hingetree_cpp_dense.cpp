@@ -85,13 +85,19 @@ torch::Tensor room_to_keep(size_t bytes, const torch::Tensor &like) {
     return torch::Tensor();
   }
 }
-// The copies of a node's forward; they go with the graph's buffers.
-torch::Tensor take_kept(AutogradContext *ctx) {
+// Leaves a forward's copies to its node, with the distance of x's rows that their layout goes by.
+void leave_kept(AutogradContext *ctx, const torch::Tensor &kept, const torch::Tensor &x) {
+  if (!kept.defined()) return;
+  ctx->saved_data["kept"] = kept;
+  ctx->saved_data["kept_stride"] = problem_of(x, x, 0).x_stride;
+}
+// The copies of a node's forward; they go with the graph's buffers.  Not taken where a hook has given x other strides since.
+torch::Tensor take_kept(AutogradContext *ctx, const ht_dense_problem &p) {
   const auto at = ctx->saved_data.find("kept");
   if (at == ctx->saved_data.end()) return torch::Tensor();
   const torch::Tensor kept = at->second.toTensor();
   if (!torch::autograd::get_current_graph_task_keep_graph()) ctx->saved_data.erase(at);
-  return kept;
+  return ctx->saved_data["kept_stride"].toInt() == p.x_stride ? kept : torch::Tensor();
 }
 
 // ---- gated projection ------------------------------------------------------------------------------------------------
@@ -124,20 +130,21 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
     ctx->saved_data["activation"] = activation;
     torch::Tensor kept;
     const torch::Tensor h = gated_forward(x, wg, wv, given(bg), given(bv), (int)activation, &kept);
-    if (kept.defined()) ctx->saved_data["kept"] = kept;
+    leave_kept(ctx, kept, x);
     return h;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     refuse_second_derivative("gated_linear");
-    const variable_list s = ctx->get_saved_variables();
-    const torch::Tensor &x = s[0];
-    c10::DeviceGuard guard(x.device());
+    variable_list s = ctx->get_saved_variables();
+    c10::DeviceGuard guard(s[0].device());
+    const torch::Tensor x = as_rows(s[0]);  // (a hook on what is saved may have laid it out anew)
+    for (int i = 1; i < 5; ++i) s[i] = as_whole(s[i]);
     ht_dense_problem p = problem_of(x, s[1], (int)ctx->saved_data["activation"].toInt());
     const torch::Tensor dh = as_whole(grads[0]);
     variable_list out(6);
     for (int i = 0, edge = 0; i < 5; ++i)  // a bias that is not there has no edge
       if (s[i].defined() && ctx->needs_input_grad(edge++)) out[i] = fresh(s[i].sizes(), s[i]);
-    const torch::Tensor kept = take_kept(ctx), ws = backward_workspace(p, x, ht_gated_linear_workspace_bytes);
+    const torch::Tensor kept = take_kept(ctx, p), ws = backward_workspace(p, x, ht_gated_linear_workspace_bytes);
     auto to = [](const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
     raise_status(ht_gated_linear_backward(&p, pointer(x), pointer(s[1]), pointer(s[2]), pointer(s[3]), pointer(s[4]), pointer(dh), pointer(kept), to(out[0]),
                                           to(out[1]), to(out[2]), to(out[3]), to(out[4]), ws.data_ptr(), ws.numel(), long_lived_word(x),
@@ -196,7 +203,7 @@ struct ClassLossNode : public torch::autograd::Function<ClassLossNode> {
                                const torch::Tensor &target, int64_t ignore, int64_t reduction) {
     torch::Tensor kept;
     const auto result = loss_forward(x, w, given(bias), target, ignore, (int)reduction, true, &kept);
-    if (kept.defined()) ctx->saved_data["kept"] = kept;
+    leave_kept(ctx, kept, x);
     ctx->save_for_backward({x, w, given(bias), target, result.second});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["reduction"] = reduction;
@@ -204,15 +211,16 @@ struct ClassLossNode : public torch::autograd::Function<ClassLossNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     refuse_second_derivative("linear_class_loss");
-    const variable_list s = ctx->get_saved_variables();
-    const torch::Tensor &x = s[0];
-    c10::DeviceGuard guard(x.device());
+    variable_list s = ctx->get_saved_variables();
+    c10::DeviceGuard guard(s[0].device());
+    const torch::Tensor x = as_rows(s[0]);  // (a hook on what is saved may have laid it out anew)
+    for (int i = 1; i < 5; ++i) s[i] = as_whole(s[i]);
     ht_dense_problem p = problem_of(x, s[1], 0);
     const torch::Tensor grad = grads[0].contiguous();
     variable_list out(6);
     for (int i = 0, edge = 0; i < 3; ++i)  // a bias that is not there has no edge
       if (s[i].defined() && ctx->needs_input_grad(edge++)) out[i] = fresh(s[i].sizes(), s[i]);
-    const torch::Tensor kept = take_kept(ctx), ws = backward_workspace(p, x, ht_linear_class_loss_workspace_bytes);
+    const torch::Tensor kept = take_kept(ctx, p), ws = backward_workspace(p, x, ht_linear_class_loss_workspace_bytes);
     auto to = [](const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
     raise_status(ht_linear_class_loss_backward(&p, pointer(x), pointer(s[1]), pointer(s[2]), s[3].const_data_ptr<int64_t>(),
                                                ctx->saved_data["ignore"].toInt(), (int)ctx->saved_data["reduction"].toInt(),

@@ -11,13 +11,13 @@
 // accumulator, and x0 y1, x1 y0, x1 y1, x0 y2, x2 y0 in a second; what is left out is below 2^-24 of a term.  The tensor core truncates
 // when it adds to an accumulator, always towards zero (measured: 32 instructions in a row lose about 9e-7 of the sum, which is more than an fp32
 // sum loses to rounding).  So the large products leave for registers every 16 instructions (256 values of k) and are added there in
-// fp32; the small ones are 2^-8 of those and stay to the end.  (Every 8 instructions lose half as much again, and leave the epilogue of a
-// tile no time beside the next one's products.)
+// fp32; the small ones are 2^-8 of those and stay to the end.  (Every 8 instructions would lose half of that, 2e-7 instead of 4e-7, but leave the
+// epilogue of a tile no time beside the next one's products.)
 //
 // A persistent kernel of 320 threads a CTA, one CTA per SM, alone (CTAS = 1, tiles of 128 rows) or in clusters of two that share a
 // tile of 256 rows (CTAS = 2): tcgen05.mma.cta_group::2 reads each CTA's 128 rows of A and half of B's rows from that CTA's shared
 // memory, which halves what a product moves of B into and out of shared memory, the resource that bounds the single form
-// (16384 x 16384 x 1024, bf16: 1110 TFLOP/s alone).
+// (16384 x 16384 x 1024, bf16: 1110 TFLOP/s alone, 1280 in pairs; 8192 cubed 1200 and 1520).
 //   warp 0      one lane issues the TMA loads (cp.async.bulk.tensor, 128-byte swizzle, no multicast) into a ring of stages of 64 values of
 //               k; in a pair both CTAs load their part and their bytes arrive at the first CTA's barrier;
 //   warp 1      allocates tensor memory, and one lane (of the first CTA) issues tcgen05.mma.kind::f16 (M 128 or 256, N up to 256,

@@ -458,6 +458,37 @@ def test_what_is_kept_for_the_backward_does_not_change_it(kind):
             assert all(torch.equal(g, v) for g, v in zip(grads, c[0]))
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("apart", [75, 80, 83])
+def test_hooks_may_lay_out_what_is_saved_anew(kind, apart):
+    """Saved tensors that come back with other strides, from the host or in columns: the backward goes by what it is given."""
+    x, w, b, t = loss_inputs(kind, 150, 75, 300, ignored=True)
+    dh = normal(generator(4), 150, 300, kind=kind)
+    wide = torch.zeros(150, apart, device="cuda", dtype=kind)
+    wide[:, :75] = x
+
+    def strided(v):
+        if v.dim() != 2:
+            return v
+        home = torch.zeros(v.shape[0], 75 + (-apart) % 16, device="cuda", dtype=v.dtype)
+        home[:, :75] = v
+        return home[:, :75]
+
+    def run():
+        leaves = [wide.detach().requires_grad_(), w.detach().requires_grad_(), b.detach().requires_grad_()]
+        rows = leaves[0][:, :75]
+        out = [F.linear_class_loss(rows, leaves[1], leaves[2], t), F.gated_linear(rows, leaves[1], leaves[1], leaves[2], leaves[2])]
+        return leaves, out
+
+    leaves, out = run()
+    want = [torch.autograd.grad(o, leaves, d) for o, d in zip(out, (None, dh))]
+    for pack, unpack in ((lambda v: v.cpu(), lambda v: v.cuda()), (strided, lambda v: v), (lambda v: v.t().contiguous().t() if v.dim() == 2 else v, lambda v: v)):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            leaves, out = run()
+        for o, d, grads in zip(out, (None, dh), want):
+            assert all(torch.equal(g, v) for g, v in zip(torch.autograd.grad(o, leaves, d), grads))
+
+
 def test_calls_on_two_streams_at_once():
     """Large and small calls of either operator on two streams, alternately: nothing is shared that they could meet in."""
     cases = [loss_inputs(kind, rows, 136, 900, ignored=True, seed=rows) for kind in TYPES for rows in (5, 100, 900)]
