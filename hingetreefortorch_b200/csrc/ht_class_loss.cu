@@ -405,7 +405,7 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
                 reduction == HT_REDUCTION_MEAN, plan.block_sums, plan.ended, status_word};
   (reduction == HT_REDUCTION_NONE ? j.row_loss : j.total) = loss;
   if (p.rows == 0) HT_CUDA_TRY(cudaMemsetAsync(plan.ended, 0, sizeof(unsigned), stream));
-  return launch_next(join_rows_kernel, dim3((unsigned)std::max<int64_t>((p.rows + 7) / 8, 1)), 256, 0, stream, 1, j);
+  return launch_next<join_rows_kernel>(dim3((unsigned)std::max<int64_t>((p.rows + 7) / 8, 1)), 256, 0, 0, stream, 1, j);
 }
 
 template <typename T>
@@ -458,7 +458,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
   HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
   const float unit = p.dtype == HT_DTYPE_F16 ? 16384.0f : 1.0f;
   if (reduction == HT_REDUCTION_NONE) {
-    HT_TRY(launch_next(row_scale_kernel, dim3(1), 1024, 0, stream, 1, grad, p.rows, unit, plan.alpha));
+    HT_TRY(launch_next<row_scale_kernel>(dim3(1), 1024, 0, 0, stream, 1, grad, p.rows, unit, plan.alpha));
   }
   Scale scale;
   scale.number = reduction == HT_REDUCTION_NONE ? plan.alpha : grad;

@@ -581,7 +581,7 @@ int lay_out(std::initializer_list<const Operand<T> *> operands, cudaStream_t str
     most = std::max(most, o->m.rows * (o->m.pitch / 8));
   }
   if (count == 0) return HT_OK;
-  return launch_next(lay_out_kernel<T>, dim3(blocks_for(most, 256, 148 * 16), count), 256, 0, stream, 1, all);
+  return launch_next<lay_out_kernel<T>>(dim3(blocks_for(most, 256, 148 * 16), count), 256, 0, 0, stream, 1, all);
 }
 
 // Sums of 32 rows that an epilogue leaves for these rows: of every tile's, inside the matrix or not.
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restri
 // (out2: the sums from column `second` on; null, or one of the two null: those are not wanted)
 template <typename T>
 int column_sums(const float *partial, int64_t rows, int64_t pitch, int64_t cols, const Scale &scale, T *out, T *out2, int64_t second, cudaStream_t stream) {
-  return launch_next(column_sums_kernel<T>, dim3((unsigned)(((out2 != nullptr ? second : 0) + cols + 31) / 32)), 1024, 0, stream, 1, partial, rows, pitch, cols,
+  return launch_next<column_sums_kernel<T>>(dim3((unsigned)(((out2 != nullptr ? second : 0) + cols + 31) / 32)), 1024, 0, 0, stream, 1, partial, rows, pitch, cols,
                      second, scale, out, out2);
 }
 

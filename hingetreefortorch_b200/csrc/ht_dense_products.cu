@@ -16,7 +16,7 @@ int product(const TileProblem &p, StoreEpilogue<T> &e, float *parts, int sms, cu
   e.parts = parts;
   e.parts_pitch = (int)round_up(p.cols, 8);
   HT_TRY((launch_tiles<kPlanes, A_MN, true>(p, e, shape, sms, stream)));
-  return launch_next(add_parts_kernel<T>, dim3(blocks_for(p.rows * (e.parts_pitch / 4), 256, 148 * 8)), 256, 0, stream, 1, e, parts_of(p, shape));
+  return launch_next<add_parts_kernel<T>>(dim3(blocks_for(p.rows * (e.parts_pitch / 4), 256, 148 * 8)), 256, 0, 0, stream, 1, e, parts_of(p, shape));
 }
 }  // namespace
 

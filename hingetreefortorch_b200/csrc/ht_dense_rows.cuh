@@ -237,12 +237,12 @@ int launch_few(FewArgs<T> a, const Epilogue &e, const FewPlan &plan, cudaStream_
   const size_t x_bytes = (size_t)std::min(a.rows, 8 * plan.tiles) * (size_t)plan.pitch;
   const size_t bytes = kFewRingBytes + x_bytes + (plan.split > 1 ? sizeof(float4) * 32 * kFewWarps * (size_t)plan.tiles : 0);
   const dim3 grid((unsigned)plan.blocks, (unsigned)((a.rows + 8 * plan.tiles - 1) / (8 * plan.tiles)));
-  auto run = [&](auto kernel) { return launch_next(kernel, grid, kFewThreads, bytes, stream, 1, a, e); };
+  constexpr size_t kMost = (size_t)kFewRingBytes + (size_t)kFewMostBytes;
   auto by_tiles = [&](auto full) -> int {
     constexpr bool kFull = decltype(full)::value;
-    return plan.tiles == 1   ? run(few_rows_kernel<T, 1, kFull, Epilogue>)
-           : plan.tiles == 2 ? run(few_rows_kernel<T, 2, kFull, Epilogue>)
-                             : run(few_rows_kernel<T, 4, kFull, Epilogue>);
+    return plan.tiles == 1   ? launch_next<few_rows_kernel<T, 1, kFull, Epilogue>>(grid, kFewThreads, bytes, kMost, stream, 1, a, e)
+           : plan.tiles == 2 ? launch_next<few_rows_kernel<T, 2, kFull, Epilogue>>(grid, kFewThreads, bytes, kMost, stream, 1, a, e)
+                             : launch_next<few_rows_kernel<T, 4, kFull, Epilogue>>(grid, kFewThreads, bytes, kMost, stream, 1, a, e);
   };
   return a.features * (int64_t)sizeof(T) % 16 == 0 ? by_tiles(std::true_type()) : by_tiles(std::false_type());
 }
@@ -344,7 +344,8 @@ bool some_rows(int64_t rows, int64_t features, int64_t outputs, int64_t x_stride
 template <class Epilogue>
 int launch_some(FewArgs<float> a, const Epilogue &e, const FewPlan &plan, cudaStream_t stream) {
   a.split = plan.split;
-  return launch_next(some_rows_kernel<float, Epilogue>, dim3((unsigned)plan.blocks), kFewThreads, sizeof(float4) * 32 * kSomeTiles * kFewWarps, stream, 1, a, e);
+  constexpr size_t kBytes = sizeof(float4) * 32 * kSomeTiles * kFewWarps;
+  return launch_next<some_rows_kernel<float, Epilogue>>(dim3((unsigned)plan.blocks), kFewThreads, kBytes, kBytes, stream, 1, a, e);
 }
 
 template <typename T, class Epilogue>

@@ -35,6 +35,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "ht_common.cuh"
 #include "ht_tile_common.cuh"
@@ -68,10 +69,25 @@ __device__ __forceinline__ void after_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Launches a kernel that begins with after_previous_kernel(), in clusters of `ctas`.
 template <typename... Parameters, typename... Arguments>
-int launch_next(void (*kernel)(Parameters...), dim3 grid, int threads, size_t shared, cudaStream_t stream, int ctas, const Arguments &...arguments) {
-  if (shared > 48 * 1024) HT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+cudaError_t launch_with(const cudaLaunchConfig_t &config, void (*kernel)(Parameters...), const Arguments &...arguments) {
+  return cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
+}
+
+// Launches a kernel that begins with after_previous_kernel(), in clusters of `ctas`.  `most`: of shared memory in any of the kernel's launches,
+// asked for once on a device.
+template <auto KERNEL, typename... Arguments>
+int launch_next(dim3 grid, int threads, size_t shared, size_t most, cudaStream_t stream, int ctas, const Arguments &...arguments) {
+  if (shared > 48 * 1024) {
+    static std::atomic<uint64_t> granted{0};  // devices, by number
+    int device = 0;
+    HT_CUDA_TRY(cudaGetDevice(&device));
+    const uint64_t bit = device < 64 ? (uint64_t)1 << device : 0;
+    if ((granted.load(std::memory_order_relaxed) & bit) == 0) {
+      HT_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+      granted.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchAttribute attributes[2] = {};
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[0].val.programmaticStreamSerializationAllowed = 1;
@@ -85,7 +101,7 @@ int launch_next(void (*kernel)(Parameters...), dim3 grid, int threads, size_t sh
   config.stream = stream;
   config.attrs = attributes;
   config.numAttrs = ctas > 1 ? 2 : 1;
-  HT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...));
+  HT_CUDA_TRY(launch_with(config, KERNEL, arguments...));
   HT_CHECK_LAUNCH();
   return HT_OK;
 }
@@ -695,8 +711,8 @@ int launch_tiles(const TileProblem &p, const Epilogue &epilogue, const TileShape
   a.stage_bytes = a.a_bytes + (uint32_t)(B_MN ? round_up_to(bn / shape.ctas, 64) : bn / shape.ctas) * 128u * PLANES;
   a.stages = (int)std::min<uint32_t>(kStageBudget / a.stage_bytes, kMostStages);
   const dim3 grid((unsigned)(shape.ctas * std::min(a.tiles, std::max(sms / shape.ctas, 1))));
-  return shape.ctas == 2 ? launch_next(dense_tile_kernel<2, PLANES, A_MN, B_MN, Epilogue>, grid, kTileThreads, kTileSmem, stream, 2, a, epilogue)
-                         : launch_next(dense_tile_kernel<1, PLANES, A_MN, B_MN, Epilogue>, grid, kTileThreads, kTileSmem, stream, 1, a, epilogue);
+  return shape.ctas == 2 ? launch_next<dense_tile_kernel<2, PLANES, A_MN, B_MN, Epilogue>>(grid, kTileThreads, kTileSmem, kTileSmem, stream, 2, a, epilogue)
+                         : launch_next<dense_tile_kernel<1, PLANES, A_MN, B_MN, Epilogue>>(grid, kTileThreads, kTileSmem, kTileSmem, stream, 1, a, epilogue);
 }
 
 }  // namespace dense

@@ -323,7 +323,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
   if (scaled) {
     const int64_t n = p.rows * p.outputs;
     HT_CUDA_TRY(cudaMemsetAsync(plan.top, 0, sizeof(uint32_t), stream));
-    HT_TRY(launch_next(largest_kernel, dim3(blocks_for(n, 256 * 32, 148 * 8)), 256, 0, stream, 1, static_cast<const __half *>(dh), n, plan.top));
+    HT_TRY(launch_next<largest_kernel>(dim3(blocks_for(n, 256 * 32, 148 * 8)), 256, 0, 0, stream, 1, static_cast<const __half *>(dh), n, plan.top));
   }
   Scale scale;
   if (scaled) scale.top = plan.top;
