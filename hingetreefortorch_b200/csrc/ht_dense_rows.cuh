@@ -8,7 +8,8 @@
 // fp32 values are taken as two TF32 numbers (x = x0 + x1, 22 bits and a sign) and the products x0 w0 + x0 w1 + x1 w0, summed 2 steps at a time
 // in a fresh accumulator and in fp32 from there on (the tensor core truncates when it adds).
 // With few weights several warps of a block share 16 rows and take k in turn.
-// What bounds it: the weights' bytes; the launch with few of them.
+// What bounds it: the weights' bytes; the launch with few of them.  Measured, 1 row of bf16: 205 MB of weights 38 us (5.4 TB/s), 40 MB 7.5 us; 16
+// rows 41 and 8.7.
 #pragma once
 
 #include "ht_dense.cuh"
@@ -252,7 +253,7 @@ int launch_few(FewArgs<T> a, const Epilogue &e, const FewPlan &plan, cudaStream_
 // block takes 16 rows of the weights (of a pair: 8 of each), its 16 warps take 64 rows of x each and share k, and x comes straight
 // from L2 in the instruction's layout, since no warp uses what another does.  Every step's sum starts afresh and is added in fp32 (chains of 48
 // additions in the tensor core lost 1.5e-6 of the sums); the warps' sums are added last, 8 rows a warp.
-// What bounds it: rows x k from L2 for every 16 rows of the weights, and the latency of a few loads in a row.
+// What bounds it: rows x k from L2 for every 16 rows of the weights, and the latency of a few loads in a row (100 rows, 1000 to 2 x 700: 14.5 us).
 constexpr int kSomeTiles = 8;  // of 8 rows a warp
 
 template <typename T, class Epilogue>

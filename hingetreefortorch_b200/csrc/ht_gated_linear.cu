@@ -5,12 +5,15 @@
 //
 // Forward: one tile product over the rows of both weights side by side, 64 or 128 columns of each; the epilogue has the two products
 // of an element in one thread and writes h alone.
-// Backward: of the forward nothing is kept but copies of operands that cannot be read as they are.  The projections are formed again, the epilogue reads dh and writes da and du in the operands' type,
-// and those enter the products of ht_dense_products.cu: dx as one sum over both, dwg and dwv as one product.  16 N K H
-// operations for a training step where 12 N K H are needed; keeping a and u in fp32, which the gradient's accuracy asks for,
-// would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to the operands' 16 bits (2^-9 of a term
-// that enters sums, for bf16); for fp16 dh is scaled to a largest value in [1, 2) first, so that small gradients stay normal numbers; fp32
-// is split into planes.
+// Backward: of the forward nothing is kept but copies of operands that cannot be read as they are.  The projections are formed again, the
+// epilogue reads dh and writes da and du in the operands' type, and those enter the products of ht_dense_products.cu: dx as one sum over
+// both, dwg and dwv as one product.  16 N K H operations for a training step where 12 N K H are needed; keeping a and u in fp32, which
+// the gradient's accuracy asks for, would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to the operands' 16 bits
+// (2^-9 of a term that enters sums, for bf16); for fp16 dh is scaled to a largest value in [1, 2) first, so that small gradients stay
+// normal numbers; fp32 is split into planes.
+// Measured, 8192 x 784 to 12700 in bf16: forward 262 us (1245 TFLOP/s, tensor pipe 66 %: power and clock), projections again with da and du
+// 318 us (1027, 54 %: 208 MB of dh in and 416 MB out beside the products), dx 274 and both weights 282 us; 4096 x 784 to 2048 in fp32: 123,
+// 189, 133 and 132 us.
 #include "ht_dense_rows.cuh"
 
 namespace ht {
@@ -199,7 +202,8 @@ struct GatedGradEpilogue {
   __device__ __forceinline__ void end(State &, const Where &) const {}
 };
 
-// The bits of the largest |dh| (fp16) into *top, which starts as 0: bits of numbers without a sign order like the numbers.
+// The bits of the largest |dh| (fp16) into *top, which starts as 0: bits of numbers without a sign order like the numbers.  One read of dh, 2 bytes
+// a value; 5 us for 1555 x 1001, which the launch bounds.
 __global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__ v, int64_t n, uint32_t *top) {
   after_previous_kernel();
   uint32_t most = 0;
