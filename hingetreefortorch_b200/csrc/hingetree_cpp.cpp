@@ -901,6 +901,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_backward_scratch_limit", &set_backward_scratch_limit,
         "Upper bound in bytes on the scratch a backward allocates for what it keeps per tree evaluation (forest: 6 to 12 bytes, in "
         "fixed-order mode 22 to 28; convolution: 2) and a forward keeps for it; above it slower kernels give the same results. "
+        "The dense layers around a forest hold the gradient of scores or projections in pieces within it (512 MiB at the most). "
         "Default: no bound.");
   m.def("batchnorm_statistics", &batchnorm_statistics,
         "[mean, biased variance, 1 / sqrt(variance + eps)] per column from the columns' sums and sums of squares over `rows` rows.");
