@@ -12,9 +12,8 @@
 // Backward: a piece of the classes at a time (so that g of a piece, in the operands' type, stays within a bound), the scores are
 // formed again, turned into g in the epilogue, and g enters the two products of ht_dense_products.cu.  That is 8 N V K
 // operations for a training step where 6 N V K are needed; keeping the scores would cost 4 N V bytes and their traffic.
-// g is rounded to the operands' 16 bits: 2^-9 (bf16) of a term that enters sums, below what rounding the sums themselves
-// costs; for fp16 it is scaled by 2^14 first, so that probabilities down to 4e-9 are normal numbers; for fp32 it is split
-// into planes like x and w.
+// g is rounded to bf16 for bf16: 2^-9 of a term that enters sums, below what rounding the sums themselves costs.  For fp16 it is held as two
+// bf16 numbers and for fp32 as three, like x and w beside it (GradKind).
 // Measured, 16384 x 1024, 50000 classes in bf16: forward 1092 us (1537 TFLOP/s; tensor pipe 77 %), per piece of 12544 classes the gradient of the
 // scores 304 us (1384), dx 289 and dw 285 us; a step takes 5.5 ms where those add up to 4.75, power bounds it.
 #include "ht_dense_rows.cuh"
@@ -115,9 +114,8 @@ struct LossGradEpilogue {
   const int64_t *target;
   int64_t ignore, classes;
   const float *grad;      // of single rows, or null: one for all, which leaves with the sums
-  float one;              // the factor of a row that counts, and of one whose gradient is the scale of all
   Scale scale;
-  typename Kind<T>::Operand *g;  // [planes][rows][pitch]
+  typename GradKind<T>::Operand *g;  // [planes][rows][pitch]
   int pitch;
   size_t plane;
   float *row_sums;  // [row_sum_count][pitch] or null
@@ -127,7 +125,7 @@ struct LossGradEpilogue {
     const float2 q = __ldg(stats + w.row);
     const int64_t t = __ldg(target + w.row);
     const bool valid = t >= 0 && t < classes;
-    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? __ldg(grad + w.row) / scale.value() : one;
+    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? __ldg(grad + w.row) / scale.value() : 1.0f;
     if (t != ignore && valid) s.target = (int)t;
     s.m = q.x;
     s.scale = s.factor / q.y;
@@ -310,8 +308,8 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
   }
 }
 
-// The power of two at or below the largest |g|, over `unit`: what gradients of single rows are scaled by.
-__global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict__ grad, int64_t rows, float unit, float *__restrict__ alpha) {
+// The power of two at or below the largest |g|: what gradients of single rows are scaled by.
+__global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict__ grad, int64_t rows, float *__restrict__ alpha) {
   after_previous_kernel();
   __shared__ uint32_t tops[32];
   uint32_t top = 0;
@@ -322,8 +320,8 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict
   if (threadIdx.x == 0) {
     for (int i = 1; i < 32; ++i) top = max(top, tops[i]);
     const uint32_t e = top & 0x7f800000u;
-    // (the quotient stays a normal number; an infinity or no number is left to the rows)
-    alpha[0] = (e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e)) / unit;
+    // (an infinity or no number is left to the rows)
+    alpha[0] = e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
   }
 }
 
@@ -386,7 +384,7 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
   int sms = 0, rc;
   if (p.rows > 0) {
     // (copies that are left for the backward are made whichever kernel runs)
-    if (kept != nullptr || !plan.few) HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
+    if (kept != nullptr || !plan.few) HT_TRY(lay_out<T>(stream, plan.x, plan.w));
     if (plan.few) {
       const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(w), nullptr}, p.x_stride, (int)p.rows, (int)p.features, (int)p.outputs};
       const FewLossEpilogue<T> e = {(int)p.rows, plan.slots, static_cast<const T *>(bias), target, plan.partial, plan.target_score, plan.ended};
@@ -413,9 +411,10 @@ int forward(const ht_dense_problem &p, const void *x, const void *w, const void 
 
 template <typename T>
 struct BackwardPlan {
-  Operand<T> x, w;
+  Operand<T> x, w;         // of the scores
+  GradOperand<T> gx, gw;   // of the products that g enters; fp16: copies of their own, of w a piece at a time
   int64_t piece, pitch;  // classes of a piece, elements of a row of g
-  typename Kind<T>::Operand *g;
+  typename GradKind<T>::Operand *g;
   float *alpha, *sum, *parts, *row_sums;
   size_t bytes;
   BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, const void *kept,
@@ -425,19 +424,26 @@ struct BackwardPlan {
       keep(p, xp, wp, target, ignore, const_cast<void *>(kept), x, w);
       x.ready = w.ready = true;
     }
-    if (kept == nullptr || x.copy == nullptr) x.set(arena, xp, p.rows, p.features, p.x_stride, true, target, ignore), x.ready = false;
+    // (rows that do not count are zeros in the products' copy of x)
+    if (kept == nullptr || (kSameOperands<T> && x.copy == nullptr))
+      x.set(arena, xp, p.rows, p.features, p.x_stride, kSameOperands<T>, kSameOperands<T> ? target : nullptr, ignore), x.ready = false;
     if (kept == nullptr) w.set(arena, wp, p.outputs, p.features, p.features);
+    constexpr int kPlanes = GradKind<T>::kPlanes;
     const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
-    const int64_t per_class = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 2;
+    const int64_t per_class = std::max<int64_t>(p.rows, 1) * kPlanes * 2;
     piece = piece_of(p.outputs, limit / per_class);
     pitch = round_up(piece, 64);
-    g = arena.take<typename Kind<T>::Operand>(p.rows * pitch * Kind<T>::kPlanes);
+    if constexpr (!kSameOperands<T>) {
+      gx.set(arena, xp, p.rows, p.features, p.x_stride, true, target, ignore);
+      if (has_dx) gw.set(arena, wp, piece, p.features, p.features);
+    }
+    g = arena.take<typename GradKind<T>::Operand>(p.rows * pitch * kPlanes);
     alpha = arena.take<float>(1);
     sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
     parts = nullptr;
-    int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, p.outputs, Kind<T>::kPlanes);
+    int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, p.outputs, kPlanes);
     for (const int64_t count : {piece, (p.outputs - 1) % piece + 1})
-      most = std::max(most, product_parts(count, p.features, std::max<int64_t>(p.rows, 1), Kind<T>::kPlanes));
+      most = std::max(most, product_parts(count, p.features, std::max<int64_t>(p.rows, 1), kPlanes));
     if (most > 0) parts = arena.take<float>(most);
     row_sums = has_db ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * pitch) : nullptr;
     bytes = arena.used;
@@ -458,18 +464,18 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
   }
   int sms = 0, rc;
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  HT_TRY(lay_out<T>({&plan.x, &plan.w}, stream));
-  const float unit = p.dtype == HT_DTYPE_F16 ? 16384.0f : 1.0f;
-  if (reduction == HT_REDUCTION_NONE) {
-    HT_TRY(launch_next<row_scale_kernel>(dim3(1), 1024, 0, 0, stream, 1, grad, p.rows, unit, plan.alpha));
-  }
+  if (reduction == HT_REDUCTION_NONE) HT_TRY(launch_next<row_scale_kernel>(dim3(1), 1024, 0, 0, stream, 1, grad, p.rows, plan.alpha));
   Scale scale;
   scale.number = reduction == HT_REDUCTION_NONE ? plan.alpha : grad;
   if (reduction == HT_REDUCTION_MEAN) scale.count = stats + 2 * p.rows;
-  if (reduction != HT_REDUCTION_NONE) scale.unit = unit;
-  constexpr int kPlanes = Kind<T>::kPlanes;
+  constexpr int kPlanes = GradKind<T>::kPlanes;
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
     const int64_t count = std::min(plan.piece, p.outputs - first);
+    LayOut<T> copies = {};
+    if constexpr (!kSameOperands<T>) plan.gx.from(plan.x, 0, p.rows), plan.gw.from(plan.w, first, count);
+    if (first == 0) copies.add(plan.x), copies.add(plan.w), copies.add(plan.gx);
+    copies.add(plan.gw);
+    HT_TRY(lay_out<T>(copies, stream));
     TileProblem t;
     t.f16 = p.dtype == HT_DTYPE_F16;
     t.status_word = status_word;
@@ -482,11 +488,11 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     e.stats = reinterpret_cast<const float2 *>(stats);
     e.target = target, e.ignore = ignore, e.classes = p.outputs;
     e.grad = reduction == HT_REDUCTION_NONE ? grad : nullptr;
-    e.one = unit, e.scale = scale;
+    e.scale = scale;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = (size_t)(p.rows * plan.pitch);
     e.row_sums = plan.row_sums;
-    const TileShape shape = tile_shape(p.rows, count, p.features, kPlanes, false);
-    if ((rc = launch_tiles<kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
+    const TileShape shape = tile_shape(p.rows, count, p.features, Kind<T>::kPlanes, false);
+    if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
     Matrix g;
     g.data = plan.g, g.rows = p.rows, g.cols = count, g.pitch = plan.pitch, g.planes = kPlanes, g.plane = p.rows * plan.pitch;
     StoreEpilogue<T> store = {};
@@ -496,8 +502,10 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));
     if (dx != nullptr) {
       TileProblem q = t;
+      q.f16 = false;
       q.a[0] = g;
-      q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = first;
+      q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = kSameOperands<T> ? first : 0;
+      if (!kSameOperands<T>) q.b[0] = plan.gw.m;
       store.rows = store.part = (int)p.rows;
       store.out = dx, store.align = row_alignment(dx, p.features * (int64_t)sizeof(T));
       store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
@@ -505,8 +513,9 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     }
     if (dw != nullptr) {
       TileProblem q = t;
+      q.f16 = false;
       q.a[0] = g;
-      q.b[0] = plan.x.m;
+      q.b[0] = kSameOperands<T> ? plan.x.m : plan.gx.m;
       q.rows = count, q.cols = p.features, q.k = p.rows, q.b_n0 = 0;
       store.rows = store.part = (int)count;
       store.out = dw + (size_t)first * (size_t)p.features, store.align = row_alignment(store.out, p.features * (int64_t)sizeof(T));

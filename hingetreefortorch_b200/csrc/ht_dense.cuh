@@ -26,6 +26,18 @@ struct Kind<__half> {
   typedef __half Operand;
 };
 
+// What gradients of scores or projections are held as, and the other operand of the products that they enter.  fp16 has neither the range nor,
+// by one scale for all, room for rows of different sizes (u act'(a) beyond 65504, one row a million times the next): two bf16
+// numbers, 2^-17 of a value of any size, with x and the weights, 11 bits each, exact in two as well.  Three products for one: 8192 x 784 to
+// 12700 takes 2.4 ms a training step where bf16 takes 1.3.
+template <typename T>
+struct GradKind : Kind<T> {};
+template <>
+struct GradKind<__half> {
+  static constexpr int kPlanes = 2;
+  typedef __nv_bfloat16 Operand;
+};
+
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -326,12 +338,12 @@ inline int row_alignment(const void *data, int64_t row_bytes) {
 
 // The same as operands of a later product: [planes][rows][pitch], rows of a multiple of 64 elements; a lane's row.
 template <typename T>
-__device__ __forceinline__ void store_operand(typename Kind<T>::Operand *out, size_t plane, const float (&v)[32]) {
-  typedef typename Kind<T>::Operand O;
+__device__ __forceinline__ void store_operand(typename GradKind<T>::Operand *out, size_t plane, const float (&v)[32]) {
+  typedef typename GradKind<T>::Operand O;
 #pragma unroll
   for (int i = 0; i < 32; i += 16) {
     uint32_t q[8];
-    if constexpr (Kind<T>::kPlanes == 1) {
+    if constexpr (GradKind<T>::kPlanes == 1) {
       to_words<O>(v, i, q);
       store_32_bytes(out + i, q);
     } else {
@@ -347,7 +359,7 @@ __device__ __forceinline__ void store_operand(typename Kind<T>::Operand *out, si
       }
       store_32_bytes(out + i, q);
       store_32_bytes(out + plane + i, q1);
-      store_32_bytes(out + 2 * plane + i, q2);
+      if constexpr (GradKind<T>::kPlanes == 3) store_32_bytes(out + 2 * plane + i, q2);
     }
   }
 }
@@ -370,19 +382,12 @@ __device__ __forceinline__ float sum_rows(const float (&v)[32], int lane) {
   return h[0];
 }
 
-// What gradients are multiplied by when they leave: a number on the device (over a count that is there as well, 0 for none, and over
-// `unit`), or the power of two at or below the number whose bits are at `top` (1 where that is no normal number), or 1.
+// What gradients are multiplied by when they leave: a number on the device (over a count that is there as well, 0 for none), or 1.
 struct Scale {
   const float *number = nullptr, *count = nullptr;
-  float unit = 1.0f;
-  const uint32_t *top = nullptr;
   __device__ __forceinline__ float value() const {
-    if (top != nullptr) {
-      const uint32_t e = __ldg(top) & 0x7f800000u;
-      return e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
-    }
     if (number == nullptr) return 1.0f;
-    const float n = __ldg(number) / unit, c = count != nullptr ? __ldg(count) : 1.0f;
+    const float n = __ldg(number), c = count != nullptr ? __ldg(count) : 1.0f;
     return c > 0.0f ? n / c : 0.0f;
   }
 };
@@ -483,44 +488,65 @@ struct Arena {
   }
 };
 
-// A matrix as the tile product reads it: itself, or laid out anew (`copy`).  fp32 is split into planes, 16-bit rows that do not start on 16
-// bytes are padded, and rows whose target is `ignore` come as zeros where `target` is given.
-template <typename T>
+// A matrix as the tile product reads it, K = Kind or GradKind of its type: itself, or laid out anew (`copy`).  What K splits is split into
+// planes, 16-bit rows that do not start on 16 bytes are padded, and rows whose target is `ignore` come as zeros where `target` is given.
+template <typename T, typename K = Kind<T>>
 struct Operand {
   Matrix m;
-  typename Kind<T>::Operand *copy = nullptr;
+  typename K::Operand *copy = nullptr;
   const T *source = nullptr;
   int64_t stride = 0;
   const int64_t *target = nullptr;
   int64_t ignore = 0;
-  static bool direct(int64_t stride) { return Kind<T>::kPlanes == 1 && stride % 8 == 0; }
+  static bool direct(int64_t stride) { return K::kPlanes == 1 && stride % 8 == 0; }
   bool ready = false;  // the copy has been made by an earlier call
   // `skips`: rows whose target is the ignored one come as zeros, in a copy.
   void set(Arena &arena, const T *data, int64_t rows, int64_t cols, int64_t row_stride, bool skips = false, const int64_t *skip = nullptr,
            int64_t skipped = 0) {
     source = data, stride = row_stride, target = skip, ignore = skipped;
-    m.rows = rows, m.cols = cols, m.planes = Kind<T>::kPlanes;
+    m.rows = rows, m.cols = cols, m.planes = K::kPlanes;
     if (direct(row_stride) && !skips) {
       m.data = data, m.pitch = row_stride;
       return;
     }
     m.pitch = round_up(cols, 8);
     m.plane = rows * m.pitch;
-    copy = arena.template take<typename Kind<T>::Operand>(m.plane * m.planes);
+    copy = arena.template take<typename K::Operand>(m.plane * m.planes);
     m.data = copy;
   }
 };
+// The other operand of the products that a gradient enters, where that is not what the forward reads.
+template <typename T>
+struct GradOperand : Operand<T, GradKind<T>> {
+  // `rows` rows from `first` on, out of the matrix, or out of its copy where an earlier call has made one (whose rows start on 16 bytes).
+  void from(const Operand<T> &o, int64_t first, int64_t rows) {
+    const bool again = o.copy != nullptr && o.ready;
+    this->source = (again ? reinterpret_cast<const T *>(o.copy) : o.source) + first * (again ? o.m.pitch : o.stride);
+    this->stride = again ? o.m.pitch : o.stride;
+    this->m.rows = rows;
+  }
+};
+template <typename T>
+constexpr bool kSameOperands = Kind<T>::kPlanes == GradKind<T>::kPlanes;
 
 // The copies of a call's operands, all in one launch.
 template <typename T>
 struct LayOut {
   struct Job {
     const T *source;
-    typename Kind<T>::Operand *copy;
+    void *copy;
     int64_t rows, cols, stride, pitch, plane, ignore;
     const int64_t *target;
+    int planes;
     bool whole;  // rows of the source start on 16 bytes
-  } jobs[3];
+  } jobs[6];
+  unsigned count;
+  template <typename K>
+  void add(const Operand<T, K> &o) {
+    if (o.copy == nullptr || o.ready || o.m.rows == 0) return;
+    const bool whole = (reinterpret_cast<uintptr_t>(o.source) & 15u) == 0 && o.stride * (int64_t)sizeof(T) % 16 == 0;
+    jobs[count++] = {o.source, o.copy, o.m.rows, o.m.cols, o.stride, o.m.pitch, o.m.plane, o.ignore, o.target, o.m.planes, whole};
+  }
 };
 
 // 8 columns a thread.  x is read once, the copy written once: 10 bytes a value from fp32, 4 from 16 bits; 8192 x 1024 of fp32 in 13 us
@@ -551,15 +577,17 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ La
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = c + j < a.cols ? to_float(from[j]) : 0.0f;
     }
-    typename Kind<T>::Operand *to = a.copy + r * a.pitch + c;
-    if constexpr (Kind<T>::kPlanes == 1) {
+    if (Kind<T>::kPlanes == 1 && a.planes == 1) {
+      typename Kind<T>::Operand *to = static_cast<typename Kind<T>::Operand *>(a.copy) + r * a.pitch + c;
       *reinterpret_cast<uint4 *>(to) = make_uint4(pack_pair(v[0], v[1], to), pack_pair(v[2], v[3], to), pack_pair(v[4], v[5], to), pack_pair(v[6], v[7], to));
-    } else {
+    } else if constexpr (GradKind<T>::kPlanes > 1) {
+      constexpr int kPlanes = GradKind<T>::kPlanes;  // (two: the third one of 11 bits is 0)
+      __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(a.copy) + r * a.pitch + c;
       float p[3][8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) split_planes(v[j], p[0][j], p[1][j], p[2][j]);
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
+      for (int q = 0; q < kPlanes; ++q)
         *reinterpret_cast<uint4 *>(to + q * a.plane) =
             make_uint4(pack_pair(p[q][0], p[q][1], to), pack_pair(p[q][2], p[q][3], to), pack_pair(p[q][4], p[q][5], to), pack_pair(p[q][6], p[q][7], to));
     }
@@ -571,18 +599,17 @@ inline unsigned blocks_for(int64_t work, int64_t per_block, int64_t most) {
 }
 
 template <typename T>
-int lay_out(std::initializer_list<const Operand<T> *> operands, cudaStream_t stream) {
-  LayOut<T> all = {};
+int lay_out(const LayOut<T> &all, cudaStream_t stream) {
+  if (all.count == 0) return HT_OK;
   int64_t most = 0;
-  unsigned count = 0;
-  for (const Operand<T> *o : operands) {
-    if (o->copy == nullptr || o->ready || o->m.rows == 0) continue;
-    const bool whole = (reinterpret_cast<uintptr_t>(o->source) & 15u) == 0 && o->stride * (int64_t)sizeof(T) % 16 == 0;
-    all.jobs[count++] = {o->source, o->copy, o->m.rows, o->m.cols, o->stride, o->m.pitch, o->m.plane, o->ignore, o->target, whole};
-    most = std::max(most, o->m.rows * (o->m.pitch / 8));
-  }
-  if (count == 0) return HT_OK;
-  return launch_next<lay_out_kernel<T>>(dim3(blocks_for(most, 256, 148 * 16), count), 256, 0, 0, stream, 1, all);
+  for (unsigned i = 0; i < all.count; ++i) most = std::max(most, all.jobs[i].rows * (all.jobs[i].pitch / 8));
+  return launch_next<lay_out_kernel<T>>(dim3(blocks_for(most, 256, 148 * 16), all.count), 256, 0, 0, stream, 1, all);
+}
+template <typename T, typename... Operands>
+int lay_out(cudaStream_t stream, const Operands &...operands) {
+  LayOut<T> all = {};
+  (all.add(operands), ...);
+  return lay_out(all, stream);
 }
 
 // Sums of 32 rows that an epilogue leaves for these rows: of every tile's, inside the matrix or not.

@@ -10,7 +10,7 @@ namespace dense {
 namespace {
 template <typename T, bool A_MN>
 int product(const TileProblem &p, StoreEpilogue<T> &e, float *parts, int sms, cudaStream_t stream) {
-  constexpr int kPlanes = Kind<T>::kPlanes;
+  constexpr int kPlanes = GradKind<T>::kPlanes;
   const TileShape shape = product_shape(p.rows, p.cols, p.k * p.segments, kPlanes, parts != nullptr);
   if (shape.split == 1) return launch_tiles<kPlanes, A_MN, true>(p, e, shape, sms, stream);
   e.parts = parts;

@@ -13,6 +13,7 @@
 // sum loses to rounding).  So the large products leave for registers every 16 instructions (256 values of k) and are added there in
 // fp32; the small ones are 2^-8 of those and stay to the end.  (Every 8 instructions would lose half of that, 2e-7 instead of 4e-7, but leave the
 // epilogue of a tile no time beside the next one's products.)
+// The gradients of an fp16 layer and what they are multiplied by come as two planes: x0 y0, and x0 y1, x1 y0.
 //
 // A persistent kernel of 320 threads a CTA, one CTA per SM, alone (CTAS = 1, tiles of 128 rows) or in clusters of two that share a
 // tile of 256 rows (CTAS = 2): tcgen05.mma.cta_group::2 reads each CTA's 128 rows of A and half of B's rows from that CTA's shared
@@ -24,7 +25,7 @@
 //               K 16) and commits each stage back to the loads and each finished accumulator to the epilogue, of both CTAs;
 //   warps 2-9   the epilogue, under the main loop of the next tile: two warps per quarter of the CTA's 128 lanes, each with one half
 //               of the columns.
-// Tensor memory: two accumulators of 256 columns, used in turn; with three planes one for the large and one for the small products,
+// Tensor memory: two accumulators of 256 columns, used in turn; with two or three planes one for the large and one for the small products,
 // and the small ones of a block are issued first, so that the large ones' accumulator is read out meanwhile.
 // Tiles are walked in groups of 16 row blocks, rows fastest, so that what the SMs read at one time is shared in L2.
 // Every wait is bounded: when one runs out the kernel flags HT_FLAG_PIPELINE_TIMEOUT, every role stops at its own next wait, the
@@ -49,7 +50,10 @@ using namespace tile;
 constexpr int kTileM = 128, kTileK = 64;
 constexpr int kTileThreads = 320;
 constexpr int kEpilogueWarps = 8;
-constexpr int kChunkBlocks = 4;  // blocks of 64 values of k between two visits of the registers (three planes)
+// Blocks of 64 values of k between two visits of the registers: with three planes, for fp32 results; with two, for fp16 ones, 64 instructions lose
+// 2e-6 of a sum.
+template <int PLANES>
+constexpr int kChunkBlocks = PLANES == 3 ? 4 : 16;
 constexpr int kMostStages = 12;
 constexpr uint32_t kStageBudget = 192 * 1024;
 constexpr uint32_t kBoxBytes = 4096;  // of an epilogue warp: 32 rows of 32 columns on their way to or from memory
@@ -107,7 +111,7 @@ int launch_next(dim3 grid, int threads, size_t shared, size_t most, cudaStream_t
 }
 
 // A 16-bit matrix in device memory, row-major, `pitch` elements from row to row (a multiple of 8, base on 16 bytes); with
-// three planes, `plane` elements apart.
+// several planes, `plane` elements apart.
 struct Matrix {
   const void *data = nullptr;
   int64_t rows = 0, cols = 0, pitch = 0;
@@ -276,8 +280,8 @@ template <int CTAS, int PLANES, bool A_MN, bool B_MN, class Epilogue>
 __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __grid_constant__ TileArgs a, const __grid_constant__ Epilogue epilogue) {
   constexpr bool kPair = Epilogue::kPair;  // the tile's columns are those of two matrices, half and half
   static_assert(!kPair || !B_MN, "a pair's weights have k contiguous");
-  constexpr bool kThree = PLANES == 3;
-  constexpr int kBuffers = kThree ? 1 : 2;  // accumulators that are used in turn
+  constexpr bool kSplit = PLANES > 1;
+  constexpr int kBuffers = kSplit ? 1 : 2;  // accumulators that are used in turn
   extern __shared__ __align__(1024) unsigned char tile_smem[];
   unsigned char *base = tile_smem + ((1024u - (smem_addr(tile_smem) & 1023u)) & 1023u);
   const uint32_t stages = smem_addr(base);
@@ -425,15 +429,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
         const Turn at_work = place(tile);
         for (int kb = at_work.first; kb < at_work.last; ++kb) {
           const int since = kb - at_work.first;
-          const bool first = kThree ? since % kChunkBlocks == 0 : since == 0;
-          if (kThree && since == 0) wait_here(drained_small, (t & 1u) ^ 1u);
+          const bool first = kSplit ? since % kChunkBlocks<PLANES> == 0 : since == 0;
+          if (kSplit && since == 0) wait_here(drained_small, (t & 1u) ^ 1u);
           const uint32_t buffer = chunk % kBuffers;
           auto turn = [&]() {  // the accumulator's previous sum has been read
             if (!first) return;
             d = tmem_d + buffer * 256u;
             wait_here(&drained[buffer], ((chunk / kBuffers) & 1u) ^ 1u);
           };
-          if (!kThree) turn();
+          if (!kSplit) turn();
           wait_here(&full[s], phase);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const int left = a.k - (kb >= a.k_blocks ? kb - a.k_blocks : kb) * kTileK;
@@ -441,27 +445,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           const uint32_t at = stages + s * a.stage_bytes, bt = at + a.a_bytes;
           const uint64_t da = A_MN ? mn_major_descriptor(at, 8192u * PLANES) : k_major_descriptor(at);
           const uint64_t db = B_MN ? mn_major_descriptor(bt, 8192u * PLANES) : k_major_descriptor(bt);
-          constexpr int kParts = kThree && kPair && CTAS == 1 ? 2 : 1;  // two matrices in one CTA, three planes: an instruction each
+          constexpr int kParts = kSplit && kPair && CTAS == 1 ? 2 : 1;  // two matrices in one CTA, several planes: an instruction each
           auto large = [&](int kk) {
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
               mma_f16<CTAS>(one, d + (uint32_t)part * b_rows, da + (uint64_t)(step_a * (uint32_t)kk),
-                            db + (uint64_t)part * (3u * b_plane) + (uint64_t)(step_b * (uint32_t)kk), a.instruction, kk > 0 || !first);
+                            db + (uint64_t)part * (PLANES * b_plane) + (uint64_t)(step_b * (uint32_t)kk), a.instruction, kk > 0 || !first);
           };
           auto small = [&](int kk) {
 #pragma unroll
             for (int part = 0; part < kParts; ++part) {
               const uint64_t ak = da + (uint64_t)(step_a * (uint32_t)kk);
-              const uint64_t bk = db + (uint64_t)part * (3u * b_plane) + (uint64_t)(step_b * (uint32_t)kk);
+              const uint64_t bk = db + (uint64_t)part * (PLANES * b_plane) + (uint64_t)(step_b * (uint32_t)kk);
               const uint32_t to = tmem_d + 256u + (uint32_t)part * b_rows;
-              mma_f16<CTAS>(one, to, ak + 2 * a_plane, bk, a.instruction, kk > 0 || since > 0);
-              mma_f16<CTAS>(one, to, ak, bk + 2 * b_plane, a.instruction, 1u);
-              mma_f16<CTAS>(one, to, ak + a_plane, bk + b_plane, a.instruction, 1u);
-              mma_f16<CTAS>(one, to, ak + a_plane, bk, a.instruction, 1u);
+              if constexpr (PLANES == 3) {
+                mma_f16<CTAS>(one, to, ak + 2 * a_plane, bk, a.instruction, kk > 0 || since > 0);
+                mma_f16<CTAS>(one, to, ak, bk + 2 * b_plane, a.instruction, 1u);
+                mma_f16<CTAS>(one, to, ak + a_plane, bk + b_plane, a.instruction, 1u);
+              }
+              mma_f16<CTAS>(one, to, ak + a_plane, bk, a.instruction, PLANES == 3 || kk > 0 || since > 0);
               mma_f16<CTAS>(one, to, ak, bk + b_plane, a.instruction, 1u);
             }
           };
-          if (kThree) {
+          if (kSplit) {
             for (int kk = 0; kk < steps; ++kk) small(kk);
             turn();
             if (first) asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
             s = 0;
             phase ^= 1u;
           }
-          if (kb == at_work.last - 1 || (kThree && since % kChunkBlocks == kChunkBlocks - 1)) {
+          if (kb == at_work.last - 1 || (kSplit && since % kChunkBlocks<PLANES> == kChunkBlocks<PLANES> - 1)) {
             mma_commit<CTAS>(one, smem_addr(&accumulated[buffer]));
             ++chunk;
           }
@@ -530,7 +536,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
         w.next_col = next.nb * (kPair ? a.bn / 2 : a.bn) + unit0 * 32;
       }
       epilogue.begin(state, w, tile == first_tile);  // under the tile's products
-      if constexpr (!kThree) {
+      if constexpr (!kSplit) {
         if (!wait_for(chunk)) break;
         const uint32_t acc = lanes + (chunk & 1u) * 256u;
 #pragma unroll 1
@@ -560,7 +566,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) dense_tile_kernel(const __gri
           for (int i = 0; i < 32; ++i) sum[u][i] = 0.0f;
         auto column = [&](int u) { return kPair ? (u & 1) * (a.bn / 2) + (unit0 + (u >> 1)) * 32 : (unit0 + u) * 32; };
         bool there = true;
-        const int chunks = (turn.last - turn.first + kChunkBlocks - 1) / kChunkBlocks;
+        const int chunks = (turn.last - turn.first + kChunkBlocks<PLANES> - 1) / kChunkBlocks<PLANES>;
         for (int c = 0; c <= chunks; ++c) {
           if (c < chunks && !(there = wait_for(chunk))) break;
           const uint32_t acc = lanes + (c < chunks ? 0u : 256u);
@@ -638,7 +644,7 @@ inline int sm_count(int *sms) {
 
 // How to cut a product: the shape with which the SMs are done first.  Cycles of a step of 16 values of k, measured: a pair of CTAs with 256
 // columns 160, with 128 columns 118, in steps of 32 between; one CTA with 256 columns 170, with 192 150, with 128 125, with 64 120
-// (three planes: 6 of those, of 128 columns at the most alone).  A tile costs about 1300 cycles besides, a launch in pairs 1200.  Against
+// (three planes: 6 of those, two: 3, of 128 columns at the most alone).  A tile costs about 1300 cycles besides, a launch in pairs 1200.  Against
 // that, the operands have to come from memory once, 23 bytes a cycle and SM where all read, twice that where few do.  Where `most_parts`
 // allows it, k is cut as well: each part writes its sums in fp32, and a kernel adds them (8 bytes a value and part, about 6000 cycles).
 // Measured against the other shapes, us: 1555 x 336 to 2 x 1008, bf16: 7.5 with what is taken, alone and 256, 8.1 to 8.9 with others; 1003 x
@@ -650,13 +656,13 @@ inline TileShape tile_shape(int64_t rows, int64_t cols, int64_t k, int planes, b
   double least = 0.0;
   for (int split = 1; split <= most_parts && (split == 1 || k / split >= 4 * kTileK); ++split)
     for (int ctas = 2; ctas >= 1; --ctas)
-      for (int bn = ctas == 1 && planes == 3 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 32) {
+      for (int bn = ctas == 1 && planes > 1 ? 128 : 256; bn >= (ctas == 2 || pair ? 128 : 64); bn -= 32) {
         if (bn % (ctas == 2 ? (pair ? 64 : 32) : pair ? 128 : 64) != 0) continue;
         const int64_t n = pair ? bn / 2 : bn;
         const int64_t tiles = ((rows + 128 * ctas - 1) / (128 * ctas)) * ((cols + n - 1) / n) * ctas * split, last = tiles % kPlanSMs;
         const double rounds = (double)((tiles + kPlanSMs - 1) / kPlanSMs);
         const double step = ctas == 2 ? 75.0 + 0.335 * bn : bn == 256 ? 170.0 : bn == 192 ? 150.0 : bn == 128 ? 125.0 : 120.0;
-        const double products = rounds * ((planes == 3 ? 6.0 : 1.0) * (double)((k / split + 15) / 16) * step + 1300.0) + (ctas == 2 ? 1200.0 : 0.0);
+        const double products = rounds * ((planes == 3 ? 6.0 : planes == 2 ? 3.0 : 1.0) * (double)((k / split + 15) / 16) * step + 1300.0) + (ctas == 2 ? 1200.0 : 0.0);
         const double bytes = 2.0 * planes * (double)k * (double)(rows + cols * (pair ? 2 : 1)) / (double)tiles;
         const double memory = bytes / kBytesPerCycle * ((double)(tiles / kPlanSMs) + (last > 0 ? std::max(0.5, (double)last / kPlanSMs) : 0.0));
         const double sums = split > 1 ? 6000.0 + 8.0 * split * (double)rows * (double)cols / (kBytesPerCycle * kPlanSMs) : 0.0;
@@ -694,7 +700,7 @@ int launch_tiles(const TileProblem &p, const Epilogue &epilogue, const TileShape
   const int64_t m_blocks = (p.rows + shape.rows() - 1) / shape.rows(), n_blocks = (p.cols + columns - 1) / columns;
   if (m_blocks * n_blocks * shape.split > 0x3fffffff || p.k > 0x3fffffff) return HT_ERR_UNSUPPORTED;
   a.status_word = p.status_word;
-  const int n = PLANES == 3 && kPair && shape.ctas == 1 ? bn / 2 : bn;  // columns of one instruction
+  const int n = PLANES > 1 && kPair && shape.ctas == 1 ? bn / 2 : bn;  // columns of one instruction
   a.instruction = (1u << 4) | ((p.f16 ? 0u : 1u) << 7) | ((p.f16 ? 0u : 1u) << 10) | ((A_MN ? 1u : 0u) << 15) |
                   ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(shape.rows() >> 4) << 24);
   a.m_blocks = (int)m_blocks;

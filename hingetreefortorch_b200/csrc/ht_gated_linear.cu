@@ -8,9 +8,8 @@
 // Backward: of the forward nothing is kept but copies of operands that cannot be read as they are.  The projections are formed again, the
 // epilogue reads dh and writes da and du in the operands' type, and those enter the products of ht_dense_products.cu: dx as one sum over
 // both, dwg and dwv as one product.  16 N K H operations for a training step where 12 N K H are needed; keeping a and u in fp32, which
-// the gradient's accuracy asks for, would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to the operands' 16 bits
-// (2^-9 of a term that enters sums, for bf16); for fp16 dh is scaled to a largest value in [1, 2) first, so that small gradients stay
-// normal numbers; fp32 is split into planes.
+// the gradient's accuracy asks for, would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to bf16 for bf16 (2^-9 of a term that
+// enters sums); for fp16 they are held as two bf16 numbers and for fp32 as three, like x and the weights beside them (GradKind).
 // Measured, 8192 x 784 to 12700 in bf16: forward 262 us (1245 TFLOP/s, tensor pipe 66 %: power and clock), projections again with da and du
 // 318 us (1027, 54 %: 208 MB of dh in and 416 MB out beside the products), dx 274 and both weights 282 us; 4096 x 784 to 2048 in fp32: 123,
 // 189, 133 and 132 us.
@@ -140,15 +139,13 @@ struct GatedGradEpilogue {
   static constexpr bool kExact = sizeof(T) == 4;
   static constexpr int kBoxes = (int)kBoxBytes / (1024 * (int)sizeof(T));  // of dh that a warp's shared memory holds
   struct State {
-    float scale;
     int unit;
   };
   int rows, cols, act, first, outputs;  // the piece: outputs first .. first + cols - 1
   const T *bg, *bv;
   const T *dh;          // [rows, outputs]
   int align;
-  Scale scale;          // fp16: dh is divided by this power of two
-  typename Kind<T>::Operand *g;  // [planes][rows][2 pitch]: da, then du
+  typename GradKind<T>::Operand *g;  // [planes][rows][2 pitch]: da, then du
   int pitch;
   size_t plane;
   float *row_sums;  // [row_sum_count][2 pitch] or null
@@ -159,7 +156,6 @@ struct GatedGradEpilogue {
               some ? min(32, rows - r) : 0, min(32, cols - col), align, w.lane);
   }
   __device__ __forceinline__ void begin(State &s, const Where &w, bool first_tile) const {
-    s.scale = 1.0f / scale.value();
     s.unit = 0;
     if (first_tile)  // later ones have been fetched under the tile before
       for (int i = 0; i < min(kBoxes, w.units); ++i) fetch(w, i, w.row, w.col + 32 * i);
@@ -184,11 +180,11 @@ struct GatedGradEpilogue {
     activate<kExact, true>(act, a, act_a, slope);
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const float d = dh_[i] * s.scale;
+      const float d = dh_[i];
       a[i] = w.inside && i < n ? d * u[i] * slope[i] : 0.0f;
       u[i] = w.inside && i < n ? d * act_a[i] : 0.0f;
     }
-    typename Kind<T>::Operand *to = g + (size_t)w.row * (size_t)(2 * pitch) + col;
+    typename GradKind<T>::Operand *to = g + (size_t)w.row * (size_t)(2 * pitch) + col;
     if (w.inside) {
       store_operand<T>(to, plane, a);
       store_operand<T>(to + pitch, plane, u);
@@ -201,24 +197,6 @@ struct GatedGradEpilogue {
   }
   __device__ __forceinline__ void end(State &, const Where &) const {}
 };
-
-// The bits of the largest |dh| (fp16) into *top, which starts as 0: bits of numbers without a sign order like the numbers.  One read of dh, 2 bytes
-// a value; 5 us for 1555 x 1001, which the launch bounds.
-__global__ void __launch_bounds__(256) largest_kernel(const __half *__restrict__ v, int64_t n, uint32_t *top) {
-  after_previous_kernel();
-  uint32_t most = 0;
-  const int64_t quads = n / 8, step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  for (int64_t i = at; i < quads; i += step) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(v) + i);
-    const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) most = max(most, max(words[j] & 0x7fffu, (words[j] >> 16) & 0x7fffu));
-  }
-  if (at == 0)
-    for (int64_t i = quads * 8; i < n; ++i) most = max(most, (uint32_t)__half_as_ushort(v[i]) & 0x7fffu);
-  most = __reduce_max_sync(0xffffffffu, most);
-  if ((threadIdx.x & 31) == 0) atomicMax(top, __float_as_uint(__half2float(__ushort_as_half((unsigned short)most))));
-}
 
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // da and du of one piece, unless the caller sets less
 
@@ -234,10 +212,10 @@ template <typename T>
 struct Plan {
   bool few = false;  // the forward
   FewPlan few_plan;
-  Operand<T> x, wg, wv;
+  Operand<T> x, wg, wv;         // of the projections
+  GradOperand<T> gx, gwg, gwv;  // of the products that da and du enter; fp16: copies of their own, of the weights a piece at a time
   int64_t piece = 0, pitch = 0;
-  typename Kind<T>::Operand *g = nullptr;
-  uint32_t *top = nullptr;
+  typename GradKind<T>::Operand *g = nullptr;
   float *sum = nullptr, *parts = nullptr, *row_sums = nullptr;
   size_t bytes = 0, kept_bytes = 0;
   Plan(const ht_dense_problem &p, const void *xp, const void *wgp, const void *wvp, bool backward, bool has_dx, bool has_bias, bool keeps, void *kept,
@@ -259,16 +237,21 @@ struct Plan {
     if (few) return;
     if (backward) {
       const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kPieceBytes) : kPieceBytes;
-      const int64_t per_output = std::max<int64_t>(p.rows, 1) * Kind<T>::kPlanes * 4;
+      constexpr int kPlanes = GradKind<T>::kPlanes;
+      const int64_t per_output = std::max<int64_t>(p.rows, 1) * kPlanes * 4;
       piece = piece_of(p.outputs, limit / per_output);
       pitch = round_up(piece, 64);
-      g = arena.template take<typename Kind<T>::Operand>(p.rows * 2 * pitch * Kind<T>::kPlanes);
-      top = arena.take<uint32_t>(1);
+      if constexpr (!kSameOperands<T>) {
+        gx.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
+        if (has_dx) gwg.set(arena, static_cast<const T *>(wgp), piece, p.features, p.features);
+        if (has_dx) gwv.set(arena, static_cast<const T *>(wvp), piece, p.features, p.features);
+      }
+      g = arena.template take<typename GradKind<T>::Operand>(p.rows * 2 * pitch * kPlanes);
       sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
-      int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, 2 * p.outputs, Kind<T>::kPlanes);
+      int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, 2 * p.outputs, kPlanes);
       for (const int64_t count : {piece, (p.outputs - 1) % piece + 1})
         for (const int64_t height : {count, pitch + count})  // one weight's gradient, both
-          most = std::max(most, product_parts(height, p.features, std::max<int64_t>(p.rows, 1), Kind<T>::kPlanes));
+          most = std::max(most, product_parts(height, p.features, std::max<int64_t>(p.rows, 1), kPlanes));
       if (most > 0) parts = arena.take<float>(most);
       row_sums = has_bias ? arena.take<float>(row_sum_count(p.rows, {2, 0}) * 2 * pitch) : nullptr;
     }
@@ -282,7 +265,7 @@ int forward(const ht_dense_problem &p, const void *x, const void *wg, const void
   Plan<T> plan(p, x, wg, wv, false, false, false, kept != nullptr, kept, ws);
   if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
   int sms = 0, rc;
-  HT_TRY(lay_out<T>({&plan.x, &plan.wg, &plan.wv}, stream));
+  HT_TRY(lay_out<T>(stream, plan.x, plan.wg, plan.wv));
   if (plan.few) {
     const FewArgs<T> a = {static_cast<const T *>(x), {static_cast<const T *>(wg), static_cast<const T *>(wv)}, p.x_stride, (int)p.rows, (int)p.features,
                           (int)p.outputs};
@@ -322,21 +305,17 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
   }
   int sms = 0, rc;
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  HT_TRY(lay_out<T>({&plan.x, &plan.wg, &plan.wv}, stream));
-  const bool scaled = p.dtype == HT_DTYPE_F16;
-  if (scaled) {
-    const int64_t n = p.rows * p.outputs;
-    HT_CUDA_TRY(cudaMemsetAsync(plan.top, 0, sizeof(uint32_t), stream));
-    HT_TRY(launch_next<largest_kernel>(dim3(blocks_for(n, 256 * 32, 148 * 8)), 256, 0, 0, stream, 1, static_cast<const __half *>(dh), n, plan.top));
-  }
-  Scale scale;
-  if (scaled) scale.top = plan.top;
-  constexpr int kPlanes = Kind<T>::kPlanes;
+  constexpr int kPlanes = GradKind<T>::kPlanes;
   const size_t plane = (size_t)(p.rows * 2 * plan.pitch);
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
     const int64_t count = std::min(plan.piece, p.outputs - first);
+    LayOut<T> copies = {};
+    if constexpr (!kSameOperands<T>) plan.gx.from(plan.x, 0, p.rows), plan.gwg.from(plan.wg, first, count), plan.gwv.from(plan.wv, first, count);
+    if (first == 0) copies.add(plan.x), copies.add(plan.wg), copies.add(plan.wv), copies.add(plan.gx);
+    copies.add(plan.gwg), copies.add(plan.gwv);
+    HT_TRY(lay_out<T>(copies, stream));
     TileProblem t;
-    t.f16 = scaled;
+    t.f16 = p.dtype == HT_DTYPE_F16;
     t.status_word = status_word;
     t.a[0] = plan.x.m;
     t.b[0] = plan.wg.m;
@@ -346,12 +325,10 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
     e.rows = (int)p.rows, e.cols = (int)count, e.act = p.activation, e.first = (int)first, e.outputs = (int)p.outputs;
     e.bg = static_cast<const T *>(bg), e.bv = static_cast<const T *>(bv), e.dh = static_cast<const T *>(dh);
     e.align = row_alignment(e.dh, p.outputs * (int64_t)sizeof(T));
-    e.scale = scale;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = plane, e.row_sums = plan.row_sums;
-    const TileShape shape = tile_shape(p.rows, count, p.features, kPlanes, true);
-    if ((rc = launch_tiles<kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
+    const TileShape shape = tile_shape(p.rows, count, p.features, Kind<T>::kPlanes, true);
+    if ((rc = launch_tiles<Kind<T>::kPlanes, false, false>(t, e, shape, sms, stream)) != HT_OK) return rc;
     StoreEpilogue<T> store = {};
-    store.scale = scale;
     store.cols = (int)p.features;
     store.split = 0x7fffffff;
     store.sum_align = row_alignment(plan.sum, p.features * (int64_t)sizeof(float));
@@ -359,11 +336,13 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
     g.rows = p.rows, g.pitch = 2 * plan.pitch, g.planes = kPlanes, g.plane = (int64_t)plane;
     if (out.dx != nullptr) {
       TileProblem q = t;
+      q.f16 = false;
+      if (!kSameOperands<T>) q.b[0] = plan.gwg.m, q.b[1] = plan.gwv.m;
       g.cols = count;
       g.data = plan.g, q.a[0] = g;
       g.data = plan.g + plan.pitch, q.a[1] = g;
       q.segments = 2;
-      q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = first;
+      q.rows = p.rows, q.cols = p.features, q.k = count, q.b_n0 = 0, q.b_k0 = kSameOperands<T> ? first : 0;
       store.rows = store.part = (int)p.rows;
       store.out = static_cast<T *>(out.dx), store.align = row_alignment(store.out, p.features * (int64_t)sizeof(T));
       store.sum = plan.sum, store.begins = first == 0, store.keep = first + count < p.outputs;
@@ -372,11 +351,12 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
     if (dwg != nullptr || dwv != nullptr) {
       // rows of the product: da's columns, then du's; one of the two weights alone takes its half
       TileProblem q = t;
+      q.f16 = false;
       const bool both = dwg != nullptr && dwv != nullptr;
       g.data = dwg != nullptr ? plan.g : plan.g + plan.pitch;
       g.cols = both ? plan.pitch + count : count;
       q.a[0] = g;
-      q.b[0] = plan.x.m;
+      q.b[0] = kSameOperands<T> ? plan.x.m : plan.gx.m;
       q.rows = g.cols, q.cols = p.features, q.k = p.rows, q.b_n0 = 0;
       store.rows = (int)g.cols;
       store.part = (int)count;
@@ -389,7 +369,7 @@ int backward(const ht_dense_problem &p, const void *x, const void *wg, const voi
     }
     const int64_t blocks = row_sum_count(p.rows, shape);
     if (has_bias)
-      HT_TRY(column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, scale, dbg == nullptr ? nullptr : dbg + first, dbv == nullptr ? nullptr : dbv + first,
+      HT_TRY(column_sums<T>(plan.row_sums, blocks, 2 * plan.pitch, count, Scale(), dbg == nullptr ? nullptr : dbg + first, dbv == nullptr ? nullptr : dbv + first,
                             plan.pitch, stream));
   }
   return HT_OK;

@@ -1,0 +1,87 @@
+"""The dense layers around a forest over the range of their types.
+
+Bounds are an element's own: what another row, output or feature holds does not widen them.  u: half a step of a type.  A sum of K
+products loses at most (K + 16) 2^-23 of the sum of their magnitudes (the tensor core truncates when it adds).  fp16 gradients are held as
+two bf16 numbers, 2^-17 of their size; one more factor of two is for the products of the two second ones, which are left out.
+"""
+import pytest
+import torch
+
+from hingetreefortorch_b200 import HingeTree as F
+from test_dense_gpu import TYPES, gate, gated_inputs, generator, lost, loss_inputs, normal, within
+
+pytestmark = pytest.mark.gpu
+
+HELD = {torch.float32: 2.0 ** -22, torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -16}
+
+
+# ---- gradients of every size -------------------------------------------------------------------------------------------
+
+def check_gated_gradients(x, wg, wv, dh, act):
+    kind = x.dtype
+    leaves = [v.detach().requires_grad_() for v in (x, wg, wv)]
+    grads = torch.autograd.grad(F.gated_linear(*leaves, activation=act), leaves, dh)
+    X, G, V, D = (v.detach().double() for v in (x, wg, wv, dh))
+    a, u = X @ G.t(), X @ V.t()
+    da, du = (lost(X.shape[1]) * (X.abs() @ M.abs().t()) for M in (G, V))
+    g, slope = gate(a, act)
+    eps = (2.0 ** -21 if kind == torch.float32 else 2.0 ** -17) * (1 + a.abs()) + 1.2 * da
+    ga, gu = D * u * slope, D * g
+    Ea = HELD[kind] * ga.abs() + D.abs() * (du + u.abs() * eps)
+    Eu = HELD[kind] * gu.abs() + D.abs() * eps
+    k = lost(2 * dh.shape[1]) + HELD[kind]
+    within(grads[0], ga @ G + gu @ V, Ea @ G.abs() + Eu @ V.abs() + k * (ga.abs() @ G.abs() + gu.abs() @ V.abs()), kind)
+    k = lost(dh.shape[0]) + HELD[kind]
+    within(grads[1], ga.t() @ X, Ea.t() @ X.abs() + k * (ga.abs().t() @ X.abs()), kind)
+    within(grads[2], gu.t() @ X, Eu.t() @ X.abs() + k * (gu.abs().t() @ X.abs()), kind)
+    return grads
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_large_projections_with_small_gradients(kind, act):
+    """u act'(a) or act(a) far beyond 65504 / 2, where h and every gradient are numbers of the type (three rows: a
+    weight's gradient is below 3 x 200 x 0.0019 x 40000 x 1.09 = 49704)."""
+    x = torch.full((3, 1), 200.0, device="cuda", dtype=kind)
+    grads = check_gated_gradients(x, torch.full((3, 1), 1 / 200, device="cuda", dtype=kind), torch.full((3, 1), 200.0, device="cuda", dtype=kind),
+                                  torch.full((3, 3), 0.0019, device="cuda", dtype=kind), act)
+    assert all(torch.isfinite(g).all() for g in grads)
+    # act(a) itself: 60000 with a value of one in 32
+    grads = check_gated_gradients(x, torch.full((3, 1), 300.0, device="cuda", dtype=kind), torch.full((3, 1), 1 / 6400, device="cuda", dtype=kind),
+                                  torch.full((3, 3), 2.0 ** -12, device="cuda", dtype=kind), act)
+    assert all(torch.isfinite(g).all() for g in grads)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,features,outputs", [(64, 64, 90), (300, 72, 200), (9, 75, 33)])
+def test_rows_whose_gradients_differ_in_size(kind, rows, features, outputs):
+    """One row's gradients are a million times the others': each row's result is as exact as it would be alone."""
+    x, wg, wv, _, _, dh = gated_inputs(kind, rows, features, outputs, bias=False)
+    dh = dh.float() * 1e-2
+    dh[rows // 2] *= 1e6
+    for act in ("silu", "relu"):
+        check_gated_gradients(x, wg, wv, dh.to(kind), act)
+
+
+def check_loss_gradients(x, w, t, grad, ignore=-100):
+    kind = x.dtype
+    leaves = [v.detach().requires_grad_() for v in (x, w)]
+    grads = torch.autograd.grad(F.linear_class_loss(*leaves, None, t, ignore_index=ignore, reduction="none"), leaves, grad)
+    X, W = (v.detach().double() for v in (x, w))
+    s = X @ W.t()
+    ds = lost(X.shape[1]) * (X.abs() @ W.abs().t()).amax(1, keepdim=True)
+    r = torch.where(t != ignore, grad.double(), 0.0)[:, None]
+    p = torch.softmax(s, 1)
+    g = p.scatter_add(1, torch.where(t != ignore, t, 0)[:, None], torch.full_like(r, -1.0)) * r
+    E = HELD[kind] * g.abs() + r.abs() * (p * (2 * ds + 2.0 ** -20) + 2.0 ** -24)
+    within(grads[0], g @ W, E @ W.abs() + (lost(W.shape[0]) + HELD[kind]) * (g.abs() @ W.abs()), kind)
+    within(grads[1], g.t() @ X, E.t() @ X.abs() + (lost(X.shape[0]) + HELD[kind]) * (g.abs().t() @ X.abs()), kind)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,features,classes", [(64, 64, 300), (200, 75, 1000)])
+def test_losses_whose_gradients_differ_in_size(kind, rows, features, classes):
+    x, w, _, t = loss_inputs(kind, rows, features, classes, bias=False)
+    grad = normal(generator(2), rows).abs() * 1e-2 + 1e-3
+    grad[::7] *= 1e6
+    check_loss_gradients(x, w, t, grad)
