@@ -114,7 +114,6 @@ struct LossGradEpilogue {
   const int64_t *target;
   int64_t ignore, classes;
   const float *grad;      // of single rows, or null: one for all, which leaves with the sums
-  Scale scale;
   typename GradKind<T>::Operand *g;  // [planes][rows][pitch]
   int pitch;
   size_t plane;
@@ -125,7 +124,7 @@ struct LossGradEpilogue {
     const float2 q = __ldg(stats + w.row);
     const int64_t t = __ldg(target + w.row);
     const bool valid = t >= 0 && t < classes;
-    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? __ldg(grad + w.row) / scale.value() : 1.0f;
+    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? __ldg(grad + w.row) : 1.0f;
     if (t != ignore && valid) s.target = (int)t;
     s.m = q.x;
     s.scale = s.factor / q.y;
@@ -308,23 +307,6 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
   }
 }
 
-// The power of two at or below the largest |g|: what gradients of single rows are scaled by.
-__global__ void __launch_bounds__(1024) row_scale_kernel(const float *__restrict__ grad, int64_t rows, float *__restrict__ alpha) {
-  after_previous_kernel();
-  __shared__ uint32_t tops[32];
-  uint32_t top = 0;
-  for (int64_t r = threadIdx.x; r < rows; r += 1024) top = max(top, __float_as_uint(fabsf(grad[r])));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 32; ++i) top = max(top, tops[i]);
-    const uint32_t e = top & 0x7f800000u;
-    // (an infinity or no number is left to the rows)
-    alpha[0] = e < 0x10000000u || e == 0x7f800000u ? 1.0f : __uint_as_float(e);
-  }
-}
-
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;  // g of one piece, unless the caller sets less
 
 int screen(const ht_dense_problem *p) {
@@ -415,7 +397,7 @@ struct BackwardPlan {
   GradOperand<T> gx, gw;   // of the products that g enters; fp16: copies of their own, of w a piece at a time
   int64_t piece, pitch;  // classes of a piece, elements of a row of g
   typename GradKind<T>::Operand *g;
-  float *alpha, *sum, *parts, *row_sums;
+  float *sum, *parts, *row_sums;
   size_t bytes;
   BackwardPlan(const ht_dense_problem &p, const T *xp, const T *wp, const int64_t *target, int64_t ignore, bool has_dx, bool has_db, const void *kept,
                void *ws) {
@@ -438,7 +420,6 @@ struct BackwardPlan {
       if (has_dx) gw.set(arena, wp, piece, p.features, p.features);
     }
     g = arena.take<typename GradKind<T>::Operand>(p.rows * pitch * kPlanes);
-    alpha = arena.take<float>(1);
     sum = has_dx && piece < p.outputs ? arena.take<float>(p.rows * p.features) : nullptr;
     parts = nullptr;
     int64_t most = piece < p.outputs ? 0 : product_parts(p.rows, p.features, p.outputs, kPlanes);
@@ -464,9 +445,8 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
   }
   int sms = 0, rc;
   if ((rc = sm_count(&sms)) != HT_OK) return rc;
-  if (reduction == HT_REDUCTION_NONE) HT_TRY(launch_next<row_scale_kernel>(dim3(1), 1024, 0, 0, stream, 1, grad, p.rows, plan.alpha));
   Scale scale;
-  scale.number = reduction == HT_REDUCTION_NONE ? plan.alpha : grad;
+  if (reduction != HT_REDUCTION_NONE) scale.number = grad;
   if (reduction == HT_REDUCTION_MEAN) scale.count = stats + 2 * p.rows;
   constexpr int kPlanes = GradKind<T>::kPlanes;
   for (int64_t first = 0; first < p.outputs; first += plan.piece) {
@@ -488,7 +468,6 @@ int backward(const ht_dense_problem &p, const void *x, const void *w, const void
     e.stats = reinterpret_cast<const float2 *>(stats);
     e.target = target, e.ignore = ignore, e.classes = p.outputs;
     e.grad = reduction == HT_REDUCTION_NONE ? grad : nullptr;
-    e.scale = scale;
     e.g = plan.g, e.pitch = (int)plan.pitch, e.plane = (size_t)(p.rows * plan.pitch);
     e.row_sums = plan.row_sums;
     const TileShape shape = tile_shape(p.rows, count, p.features, Kind<T>::kPlanes, false);

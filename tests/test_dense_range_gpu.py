@@ -4,6 +4,8 @@ Bounds are an element's own: what another row, output or feature holds does not 
 products loses at most (K + 16) 2^-23 of the sum of their magnitudes (the tensor core truncates when it adds).  fp16 gradients are held as
 two bf16 numbers, 2^-17 of their size; one more factor of two is for the products of the two second ones, which are left out.
 """
+import math
+
 import pytest
 import torch
 
@@ -85,3 +87,17 @@ def test_losses_whose_gradients_differ_in_size(kind, rows, features, classes):
     grad = normal(generator(2), rows).abs() * 1e-2 + 1e-3
     grad[::7] *= 1e6
     check_loss_gradients(x, w, t, grad)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("junk", [3e38, math.inf, math.nan])
+def test_the_upstream_gradient_of_a_row_that_does_not_count(kind, junk):
+    x, w, _, t = loss_inputs(kind, 100, 72, 300, bias=False, ignored=True)
+    grad = torch.where(t == -100, torch.full((100,), junk, device="cuda"), torch.full((100,), 1e-3, device="cuda"))
+    clean = torch.where(t == -100, torch.zeros_like(grad), grad)
+    leaves = [v.detach().requires_grad_() for v in (x, w)]
+    loss = F.linear_class_loss(*leaves, None, t, reduction="none")
+    want = torch.autograd.grad(loss, leaves, clean, retain_graph=True)
+    for got, value in zip(torch.autograd.grad(loss, leaves, grad), want):
+        assert torch.equal(got, value)
+    check_loss_gradients(x, w, t, clean)
