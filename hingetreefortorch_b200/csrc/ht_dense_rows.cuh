@@ -49,9 +49,11 @@ __device__ __forceinline__ void mma_few(float (&c)[4], const uint32_t (&a)[4], u
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // v = high + low: high is v rounded to 11 bits (in integers: the conversion instruction runs at an eighth of their rate and bound the kernel,
-// 70 us for 205 MB of weights), low the rest, of which the tensor core drops what is below 2^-23 of v.
+// 70 us for 205 MB of weights), low the rest, of which the tensor core drops what is below 2^-23 of v.  A number that rounds to infinity is
+// truncated instead.
 __device__ __forceinline__ void split_tf32(uint32_t v, uint32_t &high, uint32_t &low) {
   high = (v + 0x1000u) & 0xffffe000u;
+  if ((high & 0x7f800000u) == 0x7f800000u) high = v & 0xffffe000u;
   low = __float_as_uint(__uint_as_float(v) - __uint_as_float(high));
 }
 

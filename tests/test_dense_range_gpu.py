@@ -101,3 +101,23 @@ def test_the_upstream_gradient_of_a_row_that_does_not_count(kind, junk):
     for got, value in zip(torch.autograd.grad(loss, leaves, grad), want):
         assert torch.equal(got, value)
     check_loss_gradients(x, w, t, clean)
+
+
+# ---- values of every size ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 20, 100, 300])
+@pytest.mark.parametrize("features", [33, 64])
+def test_the_largest_numbers(rows, features):
+    """The largest fp32 numbers are numbers, however many rows there are: as a feature beside small weights, and as a weight."""
+    top = torch.finfo(torch.float32).max
+    gen = generator(rows)
+    x, w = normal(gen, rows, features), normal(gen, 70, features, scale=1e-29)
+    x[:, 3], x[0, 5], x[rows // 2, 7] = top, -top, float.fromhex("0x1.ffep127")  # (the last one: the first that rounds to infinity at 11 bits)
+    zero, one = torch.zeros_like(w), torch.ones(70, device="cuda")
+    s, ds = x.double() @ w.double().t(), lost(features) * (x.double().abs() @ w.double().abs().t())
+    within(F.gated_linear(x, w, zero, None, one, "relu"), s.clamp_min(0), ds, torch.float32)
+    t = torch.arange(rows, device="cuda") % 70
+    loss = F.linear_class_loss(x, w, None, t, reduction="none")
+    within(loss, torch.logsumexp(s, 1) - s.gather(1, t[:, None])[:, 0], 2 * ds.amax(1) + 2.0 ** -20, torch.float32)
+    swapped = F.gated_linear(w[:rows % 70], x[:70], torch.zeros_like(x[:70]), None, one[:min(rows, 70)], "relu")  # weights and features change places
+    within(swapped, s[:70, :rows % 70].t().clamp_min(0), ds[:70, :rows % 70].t(), torch.float32)
