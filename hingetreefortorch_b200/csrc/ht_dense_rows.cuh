@@ -5,11 +5,12 @@
 // of a row, not what the instruction's layout spreads over it: whole sectors are read, and a lane fetches what it uses itself, into a ring of 8
 // steps of its own in shared memory (cp.async), across the ends of rows.  128 KB an SM are then in flight; with the loads of 4 steps in registers
 // instead, 205 MB of fp32 weights took 73 us.
-// fp32 values are taken as two TF32 numbers (x = x0 + x1, 22 bits and a sign) and the products x0 w0 + x0 w1 + x1 w0, summed 2 steps at a time
-// in a fresh accumulator and in fp32 from there on (the tensor core truncates when it adds).
+// fp32 values are taken as three bf16 numbers like in the tiles, six products; those of a step (16 values of k) start in a fresh accumulator, the
+// small ones first, and are added in fp32 from there on (the tensor core truncates when it adds).  Off by 1.0e-7 in norm at 1024 values of k,
+// cuBLAS's fp32 products by 1.5e-7 to 2.7e-7.
 // With few weights several warps of a block share 16 rows and take k in turn.
 // What bounds it: the weights' bytes; the launch with few of them.  Measured, 1 row of bf16: 205 MB of weights 38 us (5.4 TB/s), 40 MB 7.5 us; 16
-// rows 41 and 8.7.
+// rows 41 and 8.7.  1 row of fp32, 205 MB: 49 us with the loss's second kernel, 32 rows 121 (the splits of x, which every warp makes again).
 #pragma once
 
 #include "ht_dense.cuh"
@@ -35,11 +36,7 @@ struct FewArgs {
 
 template <typename T>
 __device__ __forceinline__ void mma_few(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, float>::value)
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else if constexpr (std::is_same<T, __half>::value)
+  if constexpr (std::is_same<T, __half>::value)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -48,13 +45,36 @@ __device__ __forceinline__ void mma_few(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// v = high + low: high is v rounded to 11 bits (in integers: the conversion instruction runs at an eighth of their rate and bound the kernel,
-// 70 us for 205 MB of weights), low the rest, of which the tensor core drops what is below 2^-23 of v.  A number that rounds to infinity is
-// truncated instead.
-__device__ __forceinline__ void split_tf32(uint32_t v, uint32_t &high, uint32_t &low) {
-  high = (v + 0x1000u) & 0xffffe000u;
-  if ((high & 0x7f800000u) == 0x7f800000u) high = v & 0xffffe000u;
-  low = __float_as_uint(__uint_as_float(v) - __uint_as_float(high));
+// Four values as three bf16 numbers each, two to a word (split_planes, two values an instruction).  The first rounding does not leave the finite
+// numbers; of an infinity the rest is one as well, and the third number none.
+struct Planes {
+  uint32_t p[3][2];
+};
+__device__ __forceinline__ Planes split_four(const uint4 &q) {
+  Planes r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float a = __uint_as_float(i == 0 ? q.x : q.z), b = __uint_as_float(i == 0 ? q.y : q.w);
+    uint32_t top;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(top) : "f"(b), "f"(a));
+    const float rest_a = a - __uint_as_float(top << 16), rest_b = b - __uint_as_float(top & 0xffff0000u);
+    const uint32_t middle = pack_pair(rest_a, rest_b, static_cast<const __nv_bfloat16 *>(nullptr));
+    r.p[0][i] = top;
+    r.p[1][i] = middle;
+    r.p[2][i] = pack_pair(rest_a - __uint_as_float(middle << 16), rest_b - __uint_as_float(middle & 0xffff0000u), static_cast<const __nv_bfloat16 *>(nullptr));
+  }
+  return r;
+}
+// sum += the products of 16 values of k of the rows a and b of the weights with those of x.
+__device__ __forceinline__ void mma_planes(float (&sum)[4], const Planes &a, const Planes &b, const Planes &x) {
+  float fresh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto product = [&](int w, int of_x) {
+    const uint32_t rows[4] = {a.p[w][0], b.p[w][0], a.p[w][1], b.p[w][1]};
+    mma_few<__nv_bfloat16>(fresh, rows, x.p[of_x][0], x.p[of_x][1]);
+  };
+  product(2, 0), product(0, 2), product(1, 1), product(1, 0), product(0, 1), product(0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] += fresh[i];
 }
 
 // A lane's 16 bytes of a row from place `k` on, zeros behind its end, value by value.
@@ -138,53 +158,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
   uint32_t slot = 0;
   for (int base = 0; base < groups; base += stride) {  // (as often in every warp)
     const int group = base + first;
-    float c[NT][4], fresh[NT][4];
+    float c[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[n][i] = fresh[n][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) c[n][i] = 0.0f;
     for (int i = 0; i < (group < groups ? own : 0); ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kFewRing - 2) : "memory");
       const uint4 qa = lds_b128(ring + slot * 1024u), qb = lds_b128(ring + slot * 1024u + 512u);
       slot = (slot + 1) % kFewRing;
       const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
-      uint32_t ha[4], la[4], hb[4], lb[4];
-      if constexpr (kFloat) {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          split_tf32(wa[h], ha[h], la[h]);
-          split_tf32(wb[h], hb[h], lb[h]);
-        }
-      }
+      Planes pa, pb;
+      if constexpr (kFloat) pa = split_four(qa), pb = split_four(qb);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         uint4 q = make_uint4(0u, 0u, 0u, 0u);
         if (8 * n + g < held) q = lds_b128(x_lane + (uint32_t)(8 * n * a.pitch + 64 * (part + i * a.split)));
-        const uint32_t x[4] = {q.x, q.y, q.z, q.w};
+        if constexpr (kFloat) {
+          mma_planes(c[n], pa, pb, split_four(q));
+        } else {
+          const uint32_t x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int h = 0; h < 4; h += 2) {
-          if constexpr (kFloat) {
-            uint32_t h0, l0, h1, l1;
-            split_tf32(x[h], h0, l0);
-            split_tf32(x[h + 1], h1, l1);
-            const uint32_t high[4] = {ha[h], hb[h], ha[h + 1], hb[h + 1]}, low[4] = {la[h], lb[h], la[h + 1], lb[h + 1]};
-            mma_few<T>(fresh[n], low, h0, h1);
-            mma_few<T>(fresh[n], high, l0, l1);
-            mma_few<T>(fresh[n], high, h0, h1);
-          } else {
+          for (int h = 0; h < 4; h += 2) {
             const uint32_t w[4] = {wa[h], wb[h], wa[h + 1], wb[h + 1]};
             mma_few<T>(c[n], w, x[h], x[h + 1]);
           }
         }
-      }
-      if (kFloat && ((i & 1) == 1 || i == own - 1)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            c[n][h] += fresh[n][h];
-            fresh[n][h] = 0.0f;
-          }
       }
       fetch();
     }
@@ -291,31 +290,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) some_rows_kernel(const FewArgs
         const int r = row0 + 8 * n + g;
         q[n] = there && r < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)r * a.x_stride + k)) : zero;
       }
-      const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
-      uint32_t high[2][4], low[2][4];
+      const Planes pa = split_four(qa), pb = split_four(qb);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        split_tf32(wa[2 * h], high[h][0], low[h][0]);
-        split_tf32(wb[2 * h], high[h][1], low[h][1]);
-        split_tf32(wa[2 * h + 1], high[h][2], low[h][2]);
-        split_tf32(wb[2 * h + 1], high[h][3], low[h][3]);
-      }
-#pragma unroll
-      for (int n = 0; n < kSomeTiles; ++n) {
-        const uint32_t x[4] = {q[n].x, q[n].y, q[n].z, q[n].w};
-        float fresh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t h0, l0, h1, l1;
-          split_tf32(x[2 * h], h0, l0);
-          split_tf32(x[2 * h + 1], h1, l1);
-          mma_few<T>(fresh, low[h], h0, h1);
-          mma_few<T>(fresh, high[h], l0, l1);
-          mma_few<T>(fresh, high[h], h0, h1);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[n][i] += fresh[i];
-      }
+      for (int n = 0; n < kSomeTiles; ++n) mma_planes(c[n], pa, pb, split_four(q[n]));
     }
     __syncthreads();  // the sums of the group before have been read
 #pragma unroll

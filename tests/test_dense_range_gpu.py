@@ -121,3 +121,55 @@ def test_the_largest_numbers(rows, features):
     within(loss, torch.logsumexp(s, 1) - s.gather(1, t[:, None])[:, 0], 2 * ds.amax(1) + 2.0 ** -20, torch.float32)
     swapped = F.gated_linear(w[:rows % 70], x[:70], torch.zeros_like(x[:70]), None, one[:min(rows, 70)], "relu")  # weights and features change places
     within(swapped, s[:70, :rows % 70].t().clamp_min(0), ds[:70, :rows % 70].t(), torch.float32)
+
+
+# ---- fp32 as exact as fp32 ---------------------------------------------------------------------------------------------
+# In norm, for random numbers.  Three bf16 numbers a value and six products leave 2^-24 of a term.  The kernels for few rows add every 16 terms
+# in fp32: a truncation of 2^-23 at the most, a rounding of 2^-24 at each of K / 16 additions in several strands; a sum of K fp32 products loses as much.
+# Bound 2^-22.  The tiles add 16 times in the tensor core, which truncates each time, up to 2^-23 of half the sum on average: 2^-20, and
+# 2^-22 for the rest.  (Two bf16 numbers and three products would be off by 4e-6, two TF32 numbers and three products by 2.6e-7.)
+
+def off(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.parametrize("rows,bound", [(1, 2.0 ** -22), (5, 2.0 ** -22), (13, 2.0 ** -22), (30, 2.0 ** -22), (64, 2.0 ** -22), (128, 2.0 ** -22),
+                                        (129, 1.25 * 2.0 ** -20), (700, 1.25 * 2.0 ** -20)])
+@pytest.mark.parametrize("features", [64, 336, 1024, 2048])
+@pytest.mark.parametrize("one_sign", [False, True])
+def test_fp32_products_in_norm(rows, bound, features, one_sign):
+    gen = generator(rows + features)
+    x, w = normal(gen, rows, features), normal(gen, 600, features, scale=features ** -0.5)
+    if one_sign:
+        x, w = x.abs(), w.abs()
+    s = x.double() @ w.double().t()
+    h = F.gated_linear(x, w, torch.zeros_like(w), None, torch.ones(600, device="cuda"), "relu")
+    assert off(h, s.clamp_min(0)) <= bound
+    # a loss of scores with that error: the score's own, and 2^-23 of rounding and exponentials
+    t = torch.randint(0, 600, (rows,), generator=gen, device="cuda")
+    want = torch.logsumexp(s, 1) - s.gather(1, t[:, None])[:, 0]
+    error = (F.linear_class_loss(x, w, None, t, reduction="none").double() - want).norm() / (s.norm() / 600 ** 0.5 + want.norm())
+    assert error <= 2 * bound
+
+
+@pytest.mark.parametrize("rows,features,outputs", [(8, 1024, 1000), (100, 336, 500), (300, 200, 513), (1024, 784, 2048), (5000, 333, 700)])
+def test_fp32_gradients_in_norm(rows, features, outputs):
+    """Two products one after the other, each as above, and the activation's 2^-21."""
+    x, wg, wv, bg, bv, dh = gated_inputs(torch.float32, rows, features, outputs)
+
+    def gradients(*given):
+        leaves = [v.detach().requires_grad_() for v in given[:-1]]
+        x, wg, wv, bg, bv = leaves
+        h = F.gated_linear(*leaves) if x.dtype == torch.float32 else torch.nn.functional.silu(x @ wg.t() + bg) * (x @ wv.t() + bv)
+        return torch.autograd.grad(h, leaves, given[-1])
+
+    for got, want in zip(gradients(x, wg, wv, bg, bv, dh), gradients(*(v.double() for v in (x, wg, wv, bg, bv, dh)))):
+        assert off(got, want) <= 2.5 * 2.0 ** -20 + 2.0 ** -21
+    x, w, b, t = loss_inputs(torch.float32, rows, features, outputs)
+    grads = []
+    for kind in (torch.float32, torch.float64):
+        leaves = [v.detach().to(kind).requires_grad_() for v in (x, w, b)]
+        loss = F.linear_class_loss(*leaves, t) if kind == torch.float32 else torch.nn.functional.cross_entropy(leaves[0] @ leaves[1].t() + leaves[2], t)
+        grads.append(torch.autograd.grad(loss, leaves))
+    for got, want in zip(*grads):  # (scores of some units: their error enters as it is)
+        assert off(got, want) <= 4 * 1.25 * 2.0 ** -20
