@@ -55,7 +55,7 @@ struct LossEpilogue {
     if (w.m_block == 0 && w.n_block == 0 && w.half == 0 && w.quarter == 0 && w.lane == 0) *ended = 0u;
     s.m = -INFINITY, s.l = 0.0f, s.target = -1;
     if (w.inside) {
-      const int64_t t = __ldg(target + w.row);
+      const int64_t t = load_plain(target + w.row);
       if (t >= 0 && t < cols) s.target = (int)t;
     }
   }
@@ -121,10 +121,10 @@ struct LossGradEpilogue {
   __device__ __forceinline__ void begin(State &s, const Where &w, bool) const {
     s.m = s.scale = s.factor = 0.0f, s.target = -1;
     if (!w.inside) return;
-    const float2 q = __ldg(stats + w.row);
-    const int64_t t = __ldg(target + w.row);
+    const float2 q = load_plain(stats + w.row);
+    const int64_t t = load_plain(target + w.row);
     const bool valid = t >= 0 && t < classes;
-    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? __ldg(grad + w.row) : 1.0f;
+    if (t != ignore) s.factor = !valid ? NAN : grad != nullptr ? load_plain(grad + w.row) : 1.0f;
     if (t != ignore && valid) s.target = (int)t;
     s.m = q.x;
     s.scale = s.factor / q.y;
@@ -176,7 +176,7 @@ struct FewLossEpilogue {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (row + i >= rows) continue;
-      const int64_t t = __ldg(target + row + i);
+      const int64_t t = load_plain(target + row + i);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = o + 8 * h;
@@ -251,11 +251,11 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const JoinArgs a) {
   if (row < a.rows) {
     float m = -INFINITY, l = 0.0f;
     const float2 *pieces = a.partial + (size_t)row * (size_t)a.slots;
-    const int64_t t = __ldg(a.target + row);
-    const float score = __ldg(a.target_score + row);  // (nothing of use where the row has no target)
+    const int64_t t = load_plain(a.target + row);
+    const float score = load_plain(a.target_score + row);  // (nothing of use where the row has no target)
 #pragma unroll 4
     for (int s = lane; s < a.slots; s += 32) {
-      const float2 q = __ldg(pieces + s);
+      const float2 q = load_plain(pieces + s);
       join(m, l, q.x, q.y);
     }
 #pragma unroll

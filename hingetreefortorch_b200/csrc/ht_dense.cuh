@@ -83,7 +83,7 @@ __device__ __forceinline__ void load_columns(const T *in, float (&v)[32], int n)
 #pragma unroll
     for (int i = 0; i < 32; i += kPer) {
       T t[kPer];
-      *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(in + i));
+      *reinterpret_cast<uint4 *>(t) = load_plain(reinterpret_cast<const uint4 *>(in + i));
 #pragma unroll
       for (int j = 0; j < kPer; ++j) v[i + j] = to_float(t[j]);
     }
@@ -148,7 +148,7 @@ __device__ __forceinline__ void move_box(uint32_t box, T *first, size_t pitch, i
       if (STORE)
         *reinterpret_cast<W *>(global) = *shared;
       else
-        *shared = __ldg(reinterpret_cast<const W *>(global));
+        *shared = load_plain(reinterpret_cast<const W *>(global));
     } else {
       T *const each = reinterpret_cast<T *>(shared);
       for (int j = 0; j < cols - c; ++j) {
@@ -387,7 +387,7 @@ struct Scale {
   const float *number = nullptr, *count = nullptr;
   __device__ __forceinline__ float value() const {
     if (number == nullptr) return 1.0f;
-    const float n = __ldg(number), c = count != nullptr ? __ldg(count) : 1.0f;
+    const float n = load_plain(number), c = count != nullptr ? load_plain(count) : 1.0f;
     return c > 0.0f ? n / c : 0.0f;
   }
 };
@@ -450,10 +450,10 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const StoreEpilogue<T> e
     const int r = (int)(i / quads), c = (int)(i - (int64_t)r * quads) * 4, row = r < e.split ? r : r - e.split;
     if (c >= e.cols || row >= e.part) continue;
     const float *from = e.parts + (size_t)r * (size_t)e.parts_pitch + c;
-    float4 sum = __ldg(reinterpret_cast<const float4 *>(from));
+    float4 sum = load_plain(reinterpret_cast<const float4 *>(from));
 #pragma unroll 4
     for (int p = 1; p < count; ++p) {
-      const float4 q = __ldg(reinterpret_cast<const float4 *>(from + (size_t)p * plane));
+      const float4 q = load_plain(reinterpret_cast<const float4 *>(from + (size_t)p * plane));
       sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
     }
     T *to = (r < e.split ? e.out : e.out2) + (size_t)row * (size_t)e.cols + c;
@@ -560,16 +560,16 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ La
     const int64_t r = i / per_row, c = (i - r * per_row) * 8;
     float v[8];
     const T *from = a.source + r * a.stride + c;
-    if (a.target != nullptr && __ldg(a.target + r) == a.ignore) {
+    if (a.target != nullptr && load_plain(a.target + r) == a.ignore) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.0f;
     } else if (a.whole && c + 8 <= a.cols) {
       T t[8];
       if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(from));
-        *reinterpret_cast<uint4 *>(t + 4) = __ldg(reinterpret_cast<const uint4 *>(from + 4));
+        *reinterpret_cast<uint4 *>(t) = load_plain(reinterpret_cast<const uint4 *>(from));
+        *reinterpret_cast<uint4 *>(t + 4) = load_plain(reinterpret_cast<const uint4 *>(from + 4));
       } else {
-        *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(from));
+        *reinterpret_cast<uint4 *>(t) = load_plain(reinterpret_cast<const uint4 *>(from));
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
@@ -618,8 +618,8 @@ inline int64_t row_sum_count(int64_t rows, const TileShape &shape) { return (row
 // Column sums from the sums of 32 rows each that the epilogues leave: out[c] = alpha sum_r partial[r, c], r in 32 strands,
 // ascending in each, that are added in order.  32 columns a block; columns from `second` on go to out2.  256 sums of 1000 columns 6 us, latency.
 template <typename T>
-__global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restrict__ partial, int64_t rows, int64_t pitch, int64_t cols, int64_t second,
-                                                          Scale scale, T *__restrict__ out, T *__restrict__ out2) {
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float *partial, int64_t rows, int64_t pitch, int64_t cols, int64_t second,
+                                                          Scale scale, T *out, T *out2) {
   after_previous_kernel();
   __shared__ float strand[32][33];
   const int lane = threadIdx.x & 31, y = threadIdx.x >> 5;
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float *__restri
   float sum = 0.0f;
   if (inside)
 #pragma unroll 4
-    for (int64_t r = y; r < rows; r += 32) sum += __ldg(partial + r * pitch + c);
+    for (int64_t r = y; r < rows; r += 32) sum += load_plain(partial + r * pitch + c);
   strand[y][lane] = sum;
   __syncthreads();
   if (y == 0 && inside) {

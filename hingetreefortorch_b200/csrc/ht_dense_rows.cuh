@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
     const T *from = a.x + (int64_t)(row0 + r) * a.x_stride;
     for (int i = lane; i < steps * 4; i += 32)
       *reinterpret_cast<uint4 *>(xs + (size_t)r * (size_t)a.pitch + 16 * i) =
-          a.x_whole && (i + 1) * kValues <= a.features ? __ldg(reinterpret_cast<const uint4 *>(from) + i) : load_values(from, i * kValues, a.features);
+          a.x_whole && (i + 1) * kValues <= a.features ? load_plain(reinterpret_cast<const uint4 *>(from) + i) : load_values(from, i * kValues, a.features);
   }
   __syncthreads();
   const uint32_t x_lane = smem_addr(xs) + (uint32_t)(g * a.pitch + 16 * j);
@@ -283,12 +283,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) some_rows_kernel(const FewArgs
       const int k = s * kStep + j * 4;
       const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
       const bool there = k < a.features;
-      const uint4 qa = there ? __ldg(reinterpret_cast<const uint4 *>(row_a + k)) : zero, qb = there ? __ldg(reinterpret_cast<const uint4 *>(row_b + k)) : zero;
+      const uint4 qa = there ? load_plain(reinterpret_cast<const uint4 *>(row_a + k)) : zero, qb = there ? load_plain(reinterpret_cast<const uint4 *>(row_b + k)) : zero;
       uint4 q[kSomeTiles];
 #pragma unroll
       for (int n = 0; n < kSomeTiles; ++n) {
         const int r = row0 + 8 * n + g;
-        q[n] = there && r < a.rows ? __ldg(reinterpret_cast<const uint4 *>(a.x + (int64_t)r * a.x_stride + k)) : zero;
+        q[n] = there && r < a.rows ? load_plain(reinterpret_cast<const uint4 *>(a.x + (int64_t)r * a.x_stride + k)) : zero;
       }
       const Planes pa = split_four(qa), pb = split_four(qb);
 #pragma unroll

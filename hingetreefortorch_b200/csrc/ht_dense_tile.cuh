@@ -73,6 +73,13 @@ __device__ __forceinline__ void after_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// What these kernels read may have been written while they were resident already, by the kernel before: all of it, a call's inputs too, by plain
+// loads.  (__ldg, and pointers that are const and __restrict__, are for what nothing writes as long as the kernel lives.)
+template <typename V>
+__device__ __forceinline__ V load_plain(const V *p) {
+  return *p;
+}
+
 template <typename... Parameters, typename... Arguments>
 cudaError_t launch_with(const cudaLaunchConfig_t &config, void (*kernel)(Parameters...), const Arguments &...arguments) {
   return cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
