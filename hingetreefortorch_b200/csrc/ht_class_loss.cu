@@ -546,8 +546,9 @@ extern "C" int ht_linear_class_loss_forward(const ht_dense_problem *p, const voi
   if (p->rows == 0 && reduction == HT_REDUCTION_NONE) return HT_OK;
   if (loss == nullptr || (p->rows > 0 && (x == nullptr || w == nullptr || target == nullptr))) return HT_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(stats) |
-        reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+        reinterpret_cast<uintptr_t>(kept)) & 15u) != 0)
     return HT_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return HT_ERR_WORKSPACE;
   return by_type(p->dtype, [&](auto zero) -> int {
     return forward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, loss, stats, kept, workspace, workspace_bytes, status_word,
                                    reinterpret_cast<cudaStream_t>(stream));
@@ -562,9 +563,9 @@ extern "C" int ht_linear_class_loss_backward(const ht_dense_problem *p, const vo
   if (reduction != HT_REDUCTION_NONE && reduction != HT_REDUCTION_MEAN && reduction != HT_REDUCTION_SUM) return HT_ERR_INVALID_ARGUMENT;
   if (p->rows > 0 && (x == nullptr || w == nullptr || target == nullptr || grad == nullptr || stats == nullptr)) return HT_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(stats) |
-        reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw) |
-        reinterpret_cast<uintptr_t>(workspace)) & 15u) != 0)
+        reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15u) != 0)
     return HT_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return HT_ERR_WORKSPACE;
   return by_type(p->dtype, [&](auto zero) -> int {
     return backward<decltype(zero)>(*p, x, w, bias, target, ignore_index, reduction, grad, stats, kept, dx, dw, dbias, workspace, workspace_bytes,
                                     status_word, reinterpret_cast<cudaStream_t>(stream));

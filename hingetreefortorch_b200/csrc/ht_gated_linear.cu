@@ -414,7 +414,8 @@ extern "C" int ht_gated_linear_forward(const ht_dense_problem *p, const void *x,
   if (rc != HT_OK) return rc;
   if (p->rows == 0) return HT_OK;
   if (x == nullptr || gate_weight == nullptr || value_weight == nullptr || h == nullptr) return HT_ERR_INVALID_ARGUMENT;
-  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, h, kept, workspace})) return HT_ERR_UNSUPPORTED;
+  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, h, kept})) return HT_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return HT_ERR_WORKSPACE;
   return by_type(p->dtype, [&](auto zero) -> int {
     return forward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, h, kept, workspace, workspace_bytes, status_word,
                                    reinterpret_cast<cudaStream_t>(stream));
@@ -428,7 +429,8 @@ extern "C" int ht_gated_linear_backward(const ht_dense_problem *p, const void *x
   const int rc = screen(p);
   if (rc != HT_OK) return rc;
   if (p->rows > 0 && (x == nullptr || gate_weight == nullptr || value_weight == nullptr || dh == nullptr)) return HT_ERR_INVALID_ARGUMENT;
-  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, dh, kept, dx, dgate_weight, dvalue_weight, workspace})) return HT_ERR_UNSUPPORTED;
+  if (!aligned({x, gate_weight, value_weight, gate_bias, value_bias, dh, kept, dx, dgate_weight, dvalue_weight})) return HT_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return HT_ERR_WORKSPACE;
   const Gradients out = {dx, dgate_weight, dvalue_weight, dgate_bias, dvalue_bias};
   return by_type(p->dtype, [&](auto zero) -> int {
     return backward<decltype(zero)>(*p, x, gate_weight, value_weight, gate_bias, value_bias, dh, kept, out, workspace, workspace_bytes, status_word,
