@@ -70,8 +70,10 @@ torch::Tensor backward_workspace(ht_dense_problem &p, const torch::Tensor &like,
     try {
       return make_workspace(need, like);
     } catch (const c10::OutOfMemoryError &) {
-      p.scratch_limit /= 4;
-      if (p.scratch_limit < 1 || bytes(&p, 1) == need) throw;
+      do {  // (a limit that changes nothing yet is no other attempt)
+        if (p.scratch_limit <= 1) throw;
+        p.scratch_limit = std::max<int64_t>(p.scratch_limit / 4, 1);
+      } while (bytes(&p, 1) >= need);
     }
   }
 }

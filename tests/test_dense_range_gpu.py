@@ -173,3 +173,25 @@ def test_fp32_gradients_in_norm(rows, features, outputs):
         grads.append(torch.autograd.grad(loss, leaves))
     for got, want in zip(*grads):  # (scores of some units: their error enters as it is)
         assert off(got, want) <= 4 * 1.25 * 2.0 ** -20
+
+
+# ---- little memory -----------------------------------------------------------------------------------------------------
+
+def test_a_backward_without_room_for_the_whole_gradient_takes_pieces():
+    """105 MB of score gradients, 60 MB to be had: pieces, although the bound on the scratch would admit all."""
+    x, w, _, t = loss_inputs(torch.bfloat16, 4096, 64, 12800, bias=False)
+    leaves = [v.requires_grad_() for v in (x, w)]
+    want = torch.autograd.grad(F.linear_class_loss(*leaves, None, t), leaves)
+    loss = F.linear_class_loss(*leaves, None, t)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (60 << 20)) / total)
+    try:
+        got = torch.autograd.grad(loss, leaves)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    # the same products, added in fp32 in another order (dx piece by piece, dw by how many tiles a piece has): either is off by half a step
+    # of bf16, 2^-9, and by far less in its sums, so they differ by 2^-8 at the most
+    for a, b in zip(got, want):
+        assert (a.float() - b.float()).norm() <= 2.0 ** -8 * b.float().norm()
