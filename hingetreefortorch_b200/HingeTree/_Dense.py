@@ -27,7 +27,6 @@ def linear_class_loss(x, weight, bias, target, ignore_index=-100, reduction="mea
     does) and 'sum', one per row for 'none'.
 
     A row whose target is ignore_index has loss and gradient 0 whatever it holds.  A target that is neither a class nor ignore_index
-    makes the loss NaN, and the next call that reads the device's status word (hingetree_cpp.pipeline_status(), or the first call on new
-    ordinals) raises RuntimeError.  The backward holds the gradient of the scores in pieces of 512 MiB at the most, less with
+    makes the loss NaN, and the next hingetree_cpp.pipeline_status() raises RuntimeError.  The backward holds the gradient of the scores in pieces of 512 MiB at the most, less with
     hingetree_cpp.set_backward_scratch_limit(bytes), and what gated_linear keeps of its inputs.  No second derivative."""
     return hingetree_cpp.linear_class_loss(x, weight, bias, target, ignore_index, reduction)

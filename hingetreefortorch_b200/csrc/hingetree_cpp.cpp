@@ -128,7 +128,8 @@ void remember_valid(const torch::Tensor &ord, int64_t channels) {
 // Calls whose ordinals are already known to be valid do not read anything back (no synchronisation), but their
 // kernels still get a status word: one long-lived word per device that collects HT_FLAG_PIPELINE_TIMEOUT (a
 // bounded wait inside a kernel ran out: outputs incomplete).  It is read together with the next call that
-// synchronises anyway, and by pipeline_status().
+// synchronises anyway, and by pipeline_status().  HT_FLAG_TARGET_RANGE in it is pipeline_status()'s alone: a class loss's bad
+// target is no reason for another call to fail.
 namespace {
 std::mutex g_sticky_mutex;
 std::vector<torch::Tensor> g_sticky_words;
@@ -178,9 +179,8 @@ void OrdinalGuard::finish() {
   if (!check_) return;
   const torch::Tensor both = torch::cat({word_, sticky_}).cpu();  // one blocking copy for both words
   const int32_t flags = both.data_ptr<int32_t>()[0], earlier = both.data_ptr<int32_t>()[1];
-  if (earlier != 0) sticky_.zero_();
+  if (((uint32_t)earlier & ~HT_FLAG_TARGET_RANGE) != 0) sticky_.bitwise_and_((int64_t)HT_FLAG_TARGET_RANGE);
   if (((uint32_t)flags | (uint32_t)earlier) & HT_FLAG_PIPELINE_TIMEOUT) raise_pipeline_timeout();
-  if ((uint32_t)earlier & HT_FLAG_TARGET_RANGE) raise_target_range();
   if (flags & (int32_t)HT_FLAG_ORDINAL_RANGE)
     bad_runtime("Error: An ordinal value is either negative or larger than or equal to the number of channels.");
   remember_valid(ord_, channels_);

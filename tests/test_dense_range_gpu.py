@@ -9,7 +9,8 @@ import math
 import pytest
 import torch
 
-from hingetreefortorch_b200 import HingeTree as F
+from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R
+from hingetreefortorch_b200._ext import hingetree_cpp
 from test_dense_gpu import TYPES, gate, gated_inputs, generator, lost, loss_inputs, normal, within
 
 pytestmark = pytest.mark.gpu
@@ -195,3 +196,20 @@ def test_a_backward_without_room_for_the_whole_gradient_takes_pieces():
     # of bf16, 2^-9, and by far less in its sums, so they differ by 2^-8 at the most
     for a, b in zip(got, want):
         assert (a.float() - b.float()).norm() <= 2.0 ** -8 * b.float().norm()
+
+
+# ---- targets that are no class -----------------------------------------------------------------------------------------
+
+def test_a_bad_target_leaves_other_operators_alone():
+    """A forest's first call on its ordinals reads the status word: it has its own result, and the flag waits for pipeline_status()."""
+    x, w, _, t = loss_inputs(torch.float32, 20, 8, 9, bias=False)
+    t[4] = 9
+    assert hingetree_cpp.pipeline_status() == 0
+    assert torch.isnan(F.linear_class_loss(x, w, None, t))
+    forest = R.RandomHingeForest(8, 5, 3).cuda()
+    first = forest(x)
+    forest.ordinals.copy_(forest.ordinals.clone())  # (a new version: looked at again)
+    assert torch.equal(forest(x), first)
+    with pytest.raises(RuntimeError, match="neither a class"):
+        hingetree_cpp.pipeline_status()
+    assert hingetree_cpp.pipeline_status() == 0
