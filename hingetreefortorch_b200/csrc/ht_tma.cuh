@@ -34,6 +34,16 @@ inline EncodeTiledFn encode_tiled_fn() {
       return nullptr;
     return reinterpret_cast<EncodeTiledFn>(p);
   }();
+  // Encoding wants the device's context current in the calling thread, and a thread whose first CUDA call this is (an autograd
+  // worker's backward) has none yet: an event makes it so, inside stream captures as well.
+  static thread_local int bound = -1;
+  int device = 0;
+  if (cudaGetDevice(&device) == cudaSuccess && device != bound) {
+    cudaEvent_t event;
+    if (cudaEventCreateWithFlags(&event, cudaEventDisableTiming) != cudaSuccess) return nullptr;
+    cudaEventDestroy(event);
+    bound = device;
+  }
   return fn;
 }
 

@@ -4,14 +4,17 @@ Bounds are an element's own: what another row, output or feature holds does not 
 products loses at most (K + 16) 2^-23 of the sum of their magnitudes (the tensor core truncates when it adds).  fp16 gradients are held as
 two bf16 numbers, 2^-17 of their size; one more factor of two is for the products of the two second ones, which are left out.
 """
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 
-from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R
+from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R, _cabi
 from hingetreefortorch_b200._ext import hingetree_cpp
 from test_dense_gpu import TYPES, gate, gated_inputs, generator, lost, loss_inputs, normal, within
+from test_dense_host import DenseProblem
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +216,28 @@ def test_a_bad_target_leaves_other_operators_alone():
     with pytest.raises(RuntimeError, match="neither a class"):
         hingetree_cpp.pipeline_status()
     assert hingetree_cpp.pipeline_status() == 0
+
+
+# ---- threads -----------------------------------------------------------------------------------------------------------
+
+def test_the_first_call_of_a_thread():
+    """An entry of the library is the first that a thread asks of CUDA: nothing has made the device's context current there."""
+    lib = _cabi.library()
+    lib.ht_linear_class_loss_workspace_bytes.restype = ctypes.c_size_t
+    x, w, _, t = loss_inputs(torch.bfloat16, 300, 64, 500, bias=False)
+    p = DenseProblem(1, 0, 300, 64, 500, 64, 0)
+    ws = torch.empty(lib.ht_linear_class_loss_workspace_bytes(ctypes.byref(p), 0), dtype=torch.uint8, device="cuda")
+    loss = torch.zeros(300, device="cuda")
+    torch.cuda.synchronize()
+    status = []
+
+    def call():
+        at = [ctypes.c_void_p(v.data_ptr()) for v in (x, w, t, loss, ws)]
+        status.append(lib.ht_linear_class_loss_forward(ctypes.byref(p), at[0], at[1], None, at[2], ctypes.c_int64(-100), 0, at[3], None, None, at[4],
+                                                       ctypes.c_size_t(ws.numel()), None, None))
+
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert status == [0] and torch.equal(loss, F.linear_class_loss(x, w, None, t, reduction="none"))
