@@ -138,8 +138,22 @@ torch::Tensor sticky_word(const c10::Device &device, bool create) {
   std::lock_guard<std::mutex> lock(g_sticky_mutex);
   const size_t index = device.has_index() ? (size_t)device.index() : (size_t)c10::cuda::current_device();
   if (g_sticky_words.size() <= index) g_sticky_words.resize(index + 1);
-  if (!g_sticky_words[index].defined() && create)
-    g_sticky_words[index] = torch::zeros({1}, torch::TensorOptions().dtype(torch::kInt32).device(device));
+  if (!g_sticky_words[index].defined() && create) {
+    // memory of its own, cleared before anything is launched on it: the first call may stand in a stream capture, whose allocations and
+    // launches go with the graph, in inference mode, whose tensors nobody else may clear, or on any stream
+    const c10::InferenceMode not_here(false);
+    const c10::DeviceGuard guard(c10::Device(c10::kCUDA, (c10::DeviceIndex)index));
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed{cudaStreamCaptureModeRelaxed};
+    void *word = nullptr;
+    cudaStream_t own = nullptr;
+    C10_CUDA_CHECK(cudaMalloc(&word, sizeof(int32_t)));
+    C10_CUDA_CHECK(cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking));
+    C10_CUDA_CHECK(cudaMemsetAsync(word, 0, sizeof(int32_t), own));
+    C10_CUDA_CHECK(cudaStreamSynchronize(own));
+    C10_CUDA_CHECK(cudaStreamDestroy(own));
+    g_sticky_words[index] =
+        torch::from_blob(word, {1}, torch::TensorOptions().dtype(torch::kInt32).device(c10::Device(c10::kCUDA, (c10::DeviceIndex)index)));
+  }
   return g_sticky_words[index];
 }
 
@@ -154,9 +168,7 @@ torch::Tensor sticky_word(const c10::Device &device, bool create) {
 }  // namespace
 
 uint32_t *long_lived_word(const torch::Tensor &like) {
-  const bool capturing = c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
-  const torch::Tensor word = sticky_word(like.device(), !capturing);
-  return word.defined() ? reinterpret_cast<uint32_t *>(word.data_ptr<int32_t>()) : nullptr;
+  return reinterpret_cast<uint32_t *>(sticky_word(like.device(), true).data_ptr<int32_t>());
 }
 
 OrdinalGuard::OrdinalGuard(const torch::Tensor &ord, int64_t channels) : ord_(ord), channels_(channels) {

@@ -31,7 +31,7 @@ bool may_keep(int64_t bytes);                  // from a forward to its backward
 bool may_keep(const torch::Tensor &scratch);
 void set_ordinal_check(const std::string &mode);
 int64_t pipeline_status();
-// The device's long-lived status word (null while a stream capture runs that would have to create it).
+// The device's long-lived status word.
 uint32_t *long_lived_word(const torch::Tensor &like);
 
 // Owns the device status word of one call and turns a flagged ordinal into the reference's

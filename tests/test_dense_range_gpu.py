@@ -6,6 +6,9 @@ two bf16 numbers, 2^-17 of their size; one more factor of two is for the product
 """
 import ctypes
 import math
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -216,6 +219,34 @@ def test_a_bad_target_leaves_other_operators_alone():
     with pytest.raises(RuntimeError, match="neither a class"):
         hingetree_cpp.pipeline_status()
     assert hingetree_cpp.pipeline_status() == 0
+
+
+FIRST_CALL = """
+import torch
+from hingetreefortorch_b200 import HingeTree as F
+from hingetreefortorch_b200._ext import hingetree_cpp
+x, w, t = torch.randn(200, 8, device="cuda"), torch.randn(9, 8, device="cuda"), torch.full((200,), 9, device="cuda")
+torch.cuda.synchronize()
+%s
+torch.cuda.synchronize()
+for _ in range(2):
+    try:
+        print("status", hingetree_cpp.pipeline_status())
+    except RuntimeError as e:
+        print("raised", "neither a class" in str(e))
+"""
+
+
+@pytest.mark.parametrize("call", [
+    "graph = torch.cuda.CUDAGraph()\nwith torch.no_grad(), torch.cuda.graph(graph):\n    F.linear_class_loss(x, w, None, t)\ngraph.replay()",
+    "with torch.inference_mode():\n    F.linear_class_loss(x, w, None, t)",
+    "with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):\n    F.linear_class_loss(x, w, None, t)"])
+def test_a_bad_target_in_the_first_call_of_a_process(call):
+    """Captured, in inference mode, on another stream: the flag is there afterwards, once."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL % call], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+    assert run.stdout.split("\n")[:2] == ["raised True", "status 0"]
 
 
 # ---- threads -----------------------------------------------------------------------------------------------------------
