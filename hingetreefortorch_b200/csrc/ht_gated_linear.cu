@@ -41,10 +41,15 @@ __device__ __forceinline__ float activate_one(int act, float a, float &slope) {
     if (EXACT) {
       phi = 0.5f * erfcf(a * -0.70710678118654752f);
       e = SLOPE ? expf(-0.5f * a * a) : 0.0f;
-    } else {  // formula 7.1.26 of Abramowitz and Stegun, Handbook of Mathematical Functions: within 1.5e-7, and its exponential is the slope's
-      const float z = fabsf(a) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
+    } else {
+      // erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + 0.425 z), the form of 7.1.26 in Abramowitz and Stegun, Handbook of Mathematical Functions; here P is
+      // fitted to the least relative error over z in [0, 10], 8e-6, so that the tail is as exact as the rest (7.1.26 itself is off by 1.5e-7 of 1,
+      // 0.16 % of the tail at -5).  The exponential is the slope's too.
+      const float z = fabsf(a) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.425f, z, 1.0f));
       e = __expf(-0.5f * a * a);
-      const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+      const float tail =
+          0.5f * e * t *
+          fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.153831834f, 0.427965646f), -0.0298281749f), 0.286887415f), 0.228281937f), 0.240533059f);
       phi = a < 0.0f ? tail : 1.0f - tail;
     }
     if (SLOPE) slope = fmaf(a * 0.39894228040143268f, e, phi);

@@ -130,6 +130,21 @@ def test_the_largest_numbers(rows, features):
     within(swapped, s[:70, :rows % 70].t().clamp_min(0), ds[:70, :rows % 70].t(), torch.float32)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [20, 400])
+def test_the_tails_of_gelu(kind, rows):
+    """The normal distribution function far out is as exact as in the middle: within 2^-15 of itself (its fit 2^-16.9, the exponential of up to 84,
+    rounded as fp32, 2^-17.5, a quotient), then the type's rounding.  A value of 1024 lifts what fp16 would lose among its smallest numbers."""
+    x = torch.linspace(-12.9, 12.9, rows, device="cuda").to(kind)[:, None].requires_grad_()
+    one, zero = torch.ones(8, 1, device="cuda", dtype=kind), torch.zeros(8, 1, device="cuda", dtype=kind)
+    h = F.gated_linear(x, one, zero, None, torch.full((8,), 1024.0, device="cuda", dtype=kind), "gelu")
+    a = x.detach().double()
+    phi, density = 0.5 * torch.erfc(-a / math.sqrt(2)), torch.exp(-a * a / 2) / math.sqrt(2 * math.pi)
+    within(h, (1024 * a * phi).expand(-1, 8), 2.0 ** -15 * 1024 * a.abs() * phi, kind)
+    dx, = torch.autograd.grad(h, x, torch.eye(8, device="cuda", dtype=kind)[:1].expand(rows, 8))
+    within(dx, 1024 * (phi + a * density), (2.0 ** -15 + HELD[kind]) * 1024 * (phi + a.abs() * density), kind)
+
+
 # ---- fp32 as exact as fp32 ---------------------------------------------------------------------------------------------
 # In norm, for random numbers.  Three bf16 numbers a value and six products leave 2^-24 of a term.  The kernels for few rows add every 16 terms
 # in fp32: a truncation of 2^-23 at the most, a rounding of 2^-24 at each of K / 16 additions in several strands; a sum of K fp32 products loses as much.
