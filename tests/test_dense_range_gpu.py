@@ -7,6 +7,7 @@ two bf16 numbers, 2^-17 of their size; one more factor of two is for the product
 import ctypes
 import math
 import os
+import random
 import subprocess
 import sys
 import threading
@@ -16,7 +17,7 @@ import torch
 
 from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R, _cabi
 from hingetreefortorch_b200._ext import hingetree_cpp
-from test_dense_gpu import TYPES, gate, gated_inputs, generator, lost, loss_inputs, normal, within
+from test_dense_gpu import TYPES, check_gated, check_loss, gate, gated_inputs, generator, lost, loss_inputs, normal, within
 from test_dense_host import DenseProblem
 
 pytestmark = pytest.mark.gpu
@@ -287,3 +288,44 @@ def test_the_first_call_of_a_thread():
     thread.join()
     torch.cuda.synchronize()
     assert status == [0] and torch.equal(loss, F.linear_class_loss(x, w, None, t, reduction="none"))
+
+
+# ---- long sums ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_gradients_summed_over_many_rows_of_one_sign(kind):
+    """400000 rows, every term positive and exact in the type: a weight's and a bias's gradient within one step of the sum."""
+    rows = 400000
+    x = (torch.randint(128, 256, (rows, 40), generator=generator(), device="cuda").float() / 128).to(kind)
+    wg, bg = torch.zeros(64, 40, device="cuda", dtype=kind), torch.ones(64, device="cuda", dtype=kind)
+    leaves = [v.clone().requires_grad_() for v in (wg, wg, bg, bg)]
+    h = F.gated_linear(x, *leaves, "relu")
+    grads = torch.autograd.grad(h, leaves, torch.full_like(h, 2.0 ** -14))
+    step = 2.0 ** -19 if kind == torch.float32 else torch.finfo(kind).eps  # (fp32: 2^-23 of half of 256 terms' sums, 32 times: 2^-20)
+    for got, want in zip(grads, [2.0 ** -14 * x.double().sum(0)] * 2 + [torch.full((), 2.0 ** -14 * rows, device="cuda", dtype=torch.float64)] * 2):
+        assert ((got.double() - want).abs() <= step * want).all()
+
+
+# ---- calls at random ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("seed", range(24))
+def test_calls_at_random(seed):
+    """Sizes, types, reductions, biases and strides drawn at random, against the formulas in 64 bits."""
+    rng = random.Random(seed)
+
+    def size(low, high):
+        return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+    rows, features, outputs, kind = size(1, 3000), size(1, 1500), size(1, 3000), rng.choice(TYPES)
+    bias, act, reduction = rng.random() < 0.5, rng.choice(["silu", "gelu", "relu", "sigmoid"]), rng.choice(["none", "mean", "sum"])
+
+    def strided(v):  # rows apart by a few more values than they have, or as they are
+        home = torch.zeros(v.shape[0], v.shape[1] + rng.choice([0, 1, 3, 8]), device="cuda", dtype=kind)
+        home[:, :v.shape[1]] = v
+        return home[:, :v.shape[1]]
+
+    x, wg, wv, bg, bv, dh = gated_inputs(kind, rows, features, outputs, bias=bias, seed=seed)
+    check_gated(strided(x), wg, strided(wv), bg, bv, dh, act)
+    x, w, b, t = loss_inputs(kind, rows, features, outputs, bias=bias, ignored=rows > 2 and rng.random() < 0.5, seed=seed)
+    grad = normal(generator(seed), rows, scale=2.0) if reduction == "none" else torch.tensor(1.7, device="cuda")
+    check_loss(strided(x), strided(w), b, t, reduction, grad)
