@@ -231,10 +231,12 @@ class RandomHingeFernFusedLinear(_FusedLinearMixin, RandomHingeFern):
 
 
 class SparseRandomHingeForestFusedLinear(RandomHingeForestFusedLinear):
+    _function = _F.SparseHingeTree
     _linear_function = _F.SparseHingeTreeFusedLinear
 
 
 class SparseRandomHingeFernFusedLinear(RandomHingeFernFusedLinear):
+    _function = _F.SparseHingeFern
     _linear_function = _F.SparseHingeFernFusedLinear
 
 

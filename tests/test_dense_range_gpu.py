@@ -329,3 +329,27 @@ def test_calls_at_random(seed):
     x, w, b, t = loss_inputs(kind, rows, features, outputs, bias=bias, ignored=rows > 2 and rng.random() < 0.5, seed=seed)
     grad = normal(generator(seed), rows, scale=2.0) if reduction == "none" else torch.tensor(1.7, device="cuda")
     check_loss(strided(x), strided(w), b, t, reduction, grad)
+
+
+# ---- forests with sparse gradients -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("sparse,dense", [(R.SparseRandomHingeForestFusedLinear, R.RandomHingeForestFusedLinear),
+                                          (R.SparseRandomHingeFernFusedLinear, R.RandomHingeFernFusedLinear)])
+def test_the_class_loss_of_a_sparse_forest_keeps_its_gradients_sparse(sparse, dense):
+    """As forward() does: thresholds and leaf weights sparse, the linear layer's and x's dense, with the dense forest's values."""
+    torch.manual_seed(1)
+    forests = [sparse(10, 30, 6, 4).cuda(), dense(10, 30, 6, 4).cuda()]
+    forests[1].load_state_dict(forests[0].state_dict())
+    x, t = torch.randn(50, 10, device="cuda"), torch.randint(0, 6, (50,), device="cuda")
+    inputs = [x.clone().requires_grad_() for _ in range(2)]
+    losses = [f.class_loss(v, t) for f, v in zip(forests, inputs)]
+    assert torch.equal(*losses)
+    for loss in losses:
+        loss.backward()
+    for name, p in forests[0].named_parameters():
+        if p.requires_grad:
+            other = dict(forests[1].named_parameters())[name].grad
+            assert p.grad.is_sparse == (name in ("thresholds", "weights")), name
+            # the same terms, added in an order that is free
+            assert torch.allclose(p.grad.to_dense(), other, rtol=1e-5, atol=1e-6 * other.abs().max().item())
+    assert not inputs[0].grad.is_sparse and torch.allclose(inputs[0].grad, inputs[1].grad, rtol=1e-5, atol=1e-6)
