@@ -59,20 +59,13 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b, const __half *) 
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// v = p0 + p1 + p2, each the rounding to bf16 of what the ones before leave: 24 bits.  A value that rounds to infinity without being
-// it is truncated instead; an infinity or no number stays in the first plane alone.
-__device__ __forceinline__ void split_planes(float v, float &p0, float &p1, float &p2) {
-  p0 = __bfloat162float(__float2bfloat16_rn(v));
-  if (!(fabsf(p0) < INFINITY)) {
-    p0 = fabsf(v) < INFINITY ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : v;
-    if (!(fabsf(v) < INFINITY)) {
-      p1 = p2 = 0.0f;
-      return;
-    }
-  }
-  const float r = v - p0;
-  p1 = __bfloat162float(__float2bfloat16_rn(r));
-  p2 = r - p1;
+// v = p0 + p1 + p2, each the rounding to bf16 of what the ones before leave: 24 bits; two values at a time, to a word each.  The first rounding
+// does not leave the finite numbers; of an infinity the rest is one as well, and the third number none.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+  asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(p0) : "f"(b), "f"(a));
+  const float rest_a = a - __uint_as_float(p0 << 16), rest_b = b - __uint_as_float(p0 & 0xffff0000u);
+  p1 = pack_pair(rest_a, rest_b, static_cast<const __nv_bfloat16 *>(nullptr));
+  p2 = pack_pair(rest_a - __uint_as_float(p1 << 16), rest_b - __uint_as_float(p1 & 0xffff0000u), static_cast<const __nv_bfloat16 *>(nullptr));
 }
 
 // n numbers of one row, contiguous; all lanes read the same ones.
@@ -349,14 +342,7 @@ __device__ __forceinline__ void store_operand(typename GradKind<T>::Operand *out
     } else {
       uint32_t q1[8], q2[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float a[3], b[3];
-        split_planes(v[i + 2 * j], a[0], a[1], a[2]);
-        split_planes(v[i + 2 * j + 1], b[0], b[1], b[2]);
-        q[j] = pack_pair(a[0], b[0], out);
-        q1[j] = pack_pair(a[1], b[1], out);
-        q2[j] = pack_pair(a[2], b[2], out);
-      }
+      for (int j = 0; j < 8; ++j) split_pair(v[i + 2 * j], v[i + 2 * j + 1], q[j], q1[j], q2[j]);
       store_32_bytes(out + i, q);
       store_32_bytes(out + plane + i, q1);
       if constexpr (GradKind<T>::kPlanes == 3) store_32_bytes(out + 2 * plane + i, q2);
@@ -583,13 +569,11 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ La
     } else if constexpr (GradKind<T>::kPlanes > 1) {
       constexpr int kPlanes = GradKind<T>::kPlanes;  // (two: the third one of 11 bits is 0)
       __nv_bfloat16 *to = static_cast<__nv_bfloat16 *>(a.copy) + r * a.pitch + c;
-      float p[3][8];
+      uint32_t p[3][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) split_planes(v[j], p[0][j], p[1][j], p[2][j]);
+      for (int j = 0; j < 4; ++j) split_pair(v[2 * j], v[2 * j + 1], p[0][j], p[1][j], p[2][j]);
 #pragma unroll
-      for (int q = 0; q < kPlanes; ++q)
-        *reinterpret_cast<uint4 *>(to + q * a.plane) =
-            make_uint4(pack_pair(p[q][0], p[q][1], to), pack_pair(p[q][2], p[q][3], to), pack_pair(p[q][4], p[q][5], to), pack_pair(p[q][6], p[q][7], to));
+      for (int q = 0; q < kPlanes; ++q) *reinterpret_cast<uint4 *>(to + q * a.plane) = make_uint4(p[q][0], p[q][1], p[q][2], p[q][3]);
     }
   }
 }

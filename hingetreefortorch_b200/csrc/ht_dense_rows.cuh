@@ -45,24 +45,14 @@ __device__ __forceinline__ void mma_few(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Four values as three bf16 numbers each, two to a word (split_planes, two values an instruction).  The first rounding does not leave the finite
-// numbers; of an infinity the rest is one as well, and the third number none.
+// Four values as three bf16 numbers each, two to a word.
 struct Planes {
   uint32_t p[3][2];
 };
 __device__ __forceinline__ Planes split_four(const uint4 &q) {
   Planes r;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float a = __uint_as_float(i == 0 ? q.x : q.z), b = __uint_as_float(i == 0 ? q.y : q.w);
-    uint32_t top;
-    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(top) : "f"(b), "f"(a));
-    const float rest_a = a - __uint_as_float(top << 16), rest_b = b - __uint_as_float(top & 0xffff0000u);
-    const uint32_t middle = pack_pair(rest_a, rest_b, static_cast<const __nv_bfloat16 *>(nullptr));
-    r.p[0][i] = top;
-    r.p[1][i] = middle;
-    r.p[2][i] = pack_pair(rest_a - __uint_as_float(middle << 16), rest_b - __uint_as_float(middle & 0xffff0000u), static_cast<const __nv_bfloat16 *>(nullptr));
-  }
+  split_pair(__uint_as_float(q.x), __uint_as_float(q.y), r.p[0][0], r.p[1][0], r.p[2][0]);
+  split_pair(__uint_as_float(q.z), __uint_as_float(q.w), r.p[0][1], r.p[1][1], r.p[2][1]);
   return r;
 }
 // sum += the products of 16 values of k of the rows a and b of the weights with those of x.
