@@ -29,7 +29,7 @@ struct Kind<__half> {
 // What gradients of scores or projections are held as, and the other operand of the products that they enter.  fp16 has neither the range nor,
 // by one scale for all, room for rows of different sizes (u act'(a) beyond 65504, one row a million times the next): two bf16
 // numbers, 2^-17 of a value of any size, with x and the weights, 11 bits each, exact in two as well.  Three products for one: 8192 x 784 to
-// 12700 takes 2.4 ms a training step where bf16 takes 1.3.
+// 12700 takes 2.3 ms a training step where bf16 takes 1.3.
 template <typename T>
 struct GradKind : Kind<T> {};
 template <>
@@ -535,7 +535,7 @@ struct LayOut {
   }
 };
 
-// 8 columns a thread.  x is read once, the copy written once: 10 bytes a value from fp32, 4 from 16 bits; 8192 x 1024 of fp32 in 13 us
+// 8 columns a thread.  x is read once, the copy written once: 10 bytes a value from fp32, 4 from 16 bits (6 into two planes); 8192 x 1024 of fp32 in 13 us
 // (6.3 TB/s), 10007 x 771 of fp16, whose rows start on odd addresses, in 9 (3.4 TB/s: loads of single values).
 template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(const __grid_constant__ LayOut<T> all) {

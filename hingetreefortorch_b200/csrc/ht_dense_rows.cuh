@@ -3,7 +3,7 @@
 // A warp takes 16 rows of the weights (of a pair: 8 of each matrix) as one operand of mma.sync and up to 8 NT rows of x, which lie in shared
 // memory, as the other.  A sum of products does not mind in which order its terms come, so a lane's share of k is 16 contiguous bytes
 // of a row, not what the instruction's layout spreads over it: whole sectors are read, and a lane fetches what it uses itself, into a ring of 8
-// steps of its own in shared memory (cp.async), across the ends of rows.  128 KB an SM are then in flight; with the loads of 4 steps in registers
+// steps of its own in shared memory (cp.async), 7 of them in flight, across the ends of rows: 112 KB an SM; with the loads of 4 steps in registers
 // instead, 205 MB of fp32 weights took 73 us.
 // fp32 values are taken as three bf16 numbers like in the tiles, six products; those of a step (16 values of k) start in a fresh accumulator, the
 // small ones first, and are added in fp32 from there on (the tensor core truncates when it adds).  Off by 1.0e-7 in norm at 1024 values of k,
@@ -244,7 +244,8 @@ int launch_few(FewArgs<T> a, const Epilogue &e, const FewPlan &plan, cudaStream_
 // block takes 16 rows of the weights (of a pair: 8 of each), its 16 warps take 64 rows of x each and share k, and x comes straight
 // from L2 in the instruction's layout, since no warp uses what another does.  Every step's sum starts afresh and is added in fp32 (chains of 48
 // additions in the tensor core lost 1.5e-6 of the sums); the warps' sums are added last, 8 rows a warp.
-// What bounds it: rows x k from L2 for every 16 rows of the weights, and the latency of a few loads in a row (100 rows, 1000 to 2 x 700: 14.5 us).
+// What bounds it: rows x k from L2 for every 16 rows of the weights, and the latency of a few loads in a row (100 rows, 1000 to 2 x 700: 17 us;
+// 14.5 with two TF32 numbers a value, which the largest finite numbers did not survive).
 constexpr int kSomeTiles = 8;  // of 8 rows a warp
 
 template <typename T, class Epilogue>

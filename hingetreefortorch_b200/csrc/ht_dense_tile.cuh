@@ -177,8 +177,8 @@ __device__ __forceinline__ uint64_t mn_major_descriptor(uint32_t address, uint32
 }
 
 // The warps that issue loads and products run as a whole, and `one` (set in one lane, by elect.sync) predicates the instruction itself:
-// descriptors, addresses and coordinates stay in uniform registers.  In a branch that one lane takes they are moved there for
-// every instruction, and a product of 16 values of k took 240 cycles, whatever its columns, where 256 columns need 128.
+// descriptors, addresses and coordinates are then the same in every lane.  In a branch that one lane takes a product of 16 values of k took 240
+// cycles, whatever its columns, where 256 columns need 128; that they were moved to uniform registers for every instruction is inferred from that.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t one;
   asm volatile(

@@ -11,8 +11,8 @@
 // the gradient's accuracy asks for, would cost 8 N H bytes and 16 N H of traffic.  da and du are rounded to bf16 for bf16 (2^-9 of a term that
 // enters sums); for fp16 they are held as two bf16 numbers and for fp32 as three, like x and the weights beside them (GradKind).
 // Measured, 8192 x 784 to 12700 in bf16: forward 262 us (1245 TFLOP/s, tensor pipe 66 %: power and clock), projections again with da and du
-// 318 us (1027, 54 %: 208 MB of dh in and 416 MB out beside the products), dx 274 and both weights 282 us; 4096 x 784 to 2048 in fp32: 123,
-// 189, 133 and 132 us.
+// 318 us (1027, 54 %: 208 MB of dh in and 416 MB out beside the products), dx 274 and both weights 282 us; 4096 x 784 to 2048 in fp32: 120,
+// 174, 129 and 129 us.
 #include "ht_dense_rows.cuh"
 
 namespace ht {

@@ -424,8 +424,10 @@ int ht_thresholds_f64(int fix, double *thr, const int64_t *ord, int64_t T, int d
  * neither (its pipelines put torch.nn modules there, README.md:110-129); they stand beside ht_linear_tf32_stats_f32 and the fused
  * linear forests.  All matrices are row-major in the problem's type: x [rows, features] with x_stride >= features elements
  * from row to row, weights [outputs, features], biases [outputs] or NULL, gradients like what they belong to.  Sums, softmax statistics and
- * losses are fp32; fp32 products are as accurate as fp32 ones (three bf16 planes a value).  Pointers to matrices, biases and
- * statistics start on 16 bytes (HT_ERR_UNSUPPORTED otherwise), workspaces on 256 (HT_ERR_WORKSPACE).  No atomics: the same call gives the same bits.
+ * losses are fp32; fp32 products are as accurate as fp32 ones (three bf16 planes a value).  Gradients of scores and projections are held in bf16 for
+ * bf16, in two bf16 numbers for fp16.  Pointers to matrices, biases and
+ * statistics start on 16 bytes (HT_ERR_UNSUPPORTED otherwise), workspaces on 256 (HT_ERR_WORKSPACE).  No result is summed by atomics: the
+ * same call with the same scratch_limit gives the same bits.
  * Workspaces: the matching *_workspace_bytes (0 for a bad problem).  kept (may be NULL, in both calls): *_kept_bytes that a forward fills and
  * the backward of the same tensors is given, copies of operands that cannot be read as they are (fp32, and 16-bit rows that do not start on
  * 16 bytes); otherwise the backward makes them again. */
