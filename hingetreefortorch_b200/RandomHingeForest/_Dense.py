@@ -9,6 +9,7 @@ import torch
 import torch.nn as nn
 
 from .. import HingeTree as _F
+from ._Answers import PackedClasses
 
 
 def _linear_parameters(outputs, inputs, bias):
@@ -59,6 +60,15 @@ class LinearClassLoss(nn.Module):
 
     def scores(self, x):
         return nn.functional.linear(x, self.weight, self.bias)
+
+    @torch.no_grad()
+    def sample(self, x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """A class drawn from the scores of each row, and the logarithm of its share (HingeTree.sample_classes)."""
+        return _F.sample_classes(self.scores(x), uniform, temperature, top_k, top_p, min_p)
+
+    def packed(self):
+        """The same scores under weights in 4 bits, for answers (PackedClasses)."""
+        return PackedClasses.of(self.weight, self.bias)
 
     def extra_repr(self):
         return "in_features=%d, classes=%d, bias=%s, ignore_index=%d, reduction=%s" % (

@@ -13,6 +13,7 @@ import torch.nn as nn
 import torch.nn.init as init
 
 from .. import HingeTree as _F
+from ._Answers import PackedClasses
 
 
 def _thresholds(out_channels, decisions):
@@ -194,12 +195,27 @@ class RandomHingeForestFusedLinear(_FusedLinearMixin, RandomHingeForest):
     def class_loss(self, x, target, ignore_index: int = -100, reduction: str = "mean"):
         """Softmax cross entropy of forward(x) as class scores against target (int64, [B] or [B, *inner]), which takes the trees'
         outputs and the linear layer as they are and never writes the scores (HingeTree.linear_class_loss)."""
+        return _F.linear_class_loss(self._features("class_loss", x), self.linear_weights, self.linear_bias, target, ignore_index, reduction)
+
+    def packed_classes(self):
+        """The linear layer with its weights in 4 bits, for answers (PackedClasses, whose rows are the trees' outputs)."""
+        return PackedClasses.of(self.linear_weights, self.linear_bias)
+
+    @torch.no_grad()
+    def sample(self, x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, packed=None):
+        """A class drawn from forward(x) as class scores with uniform ([B] or [B, *inner], float32), and the logarithm of its share
+        (HingeTree.sample_classes).  packed: what packed_classes() gave, whose scores are drawn from instead."""
+        if packed is not None:
+            return packed.sample(self._features("sample", x), uniform, temperature, top_k, top_p, min_p)
+        scores = self(x)
+        return _F.sample_classes(scores.movedim(1, -1) if scores.dim() > 2 else scores, uniform, temperature, top_k, top_p, min_p)
+
+    def _features(self, name, x):
+        """The trees' outputs, trees last."""
         if self.weights.dim() != 2:
-            raise RuntimeError("class_loss takes forests without extra_outputs: a leaf holds one number.")
+            raise RuntimeError(name + " takes forests without extra_outputs: a leaf holds one number.")
         features = self._function.apply(x, *self._tree_params())
-        if features.dim() > 2:  # trees last
-            features = features.movedim(1, -1)
-        return _F.linear_class_loss(features, self.linear_weights, self.linear_bias, target, ignore_index, reduction)
+        return features.movedim(1, -1) if features.dim() > 2 else features
 
     def _tree_params(self):
         return self.thresholds, self.ordinals, self.weights
@@ -224,6 +240,9 @@ class RandomHingeFernFusedLinear(_FusedLinearMixin, RandomHingeFern):
 
     forward = RandomHingeForestFusedLinear.forward
     class_loss = RandomHingeForestFusedLinear.class_loss
+    packed_classes = RandomHingeForestFusedLinear.packed_classes
+    sample = RandomHingeForestFusedLinear.sample
+    _features = RandomHingeForestFusedLinear._features
     _tree_params = RandomHingeForestFusedLinear._tree_params
     reachability = RandomHingeForestFusedLinear.reachability
     leafmap = RandomHingeForestFusedLinear.leafmap

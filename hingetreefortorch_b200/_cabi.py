@@ -40,6 +40,7 @@ SYMBOLS = [
     "ht_init_medians_workspace_bytes", "ht_init_medians_f32", "ht_init_medians_f64", "ht_thresholds_f32", "ht_thresholds_f64",
     "ht_gated_linear_workspace_bytes", "ht_gated_linear_kept_bytes", "ht_linear_class_loss_kept_bytes", "ht_gated_linear_forward", "ht_gated_linear_backward",
     "ht_linear_class_loss_workspace_bytes", "ht_linear_class_loss_forward", "ht_linear_class_loss_backward",
+    "ht_mx4_pack", "ht_mx4_unpack", "ht_linear_mx4_workspace_bytes", "ht_linear_mx4", "ht_sample_classes",
 ]
 
 

@@ -936,4 +936,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   htx::bind_more_ops(m);
   htx::bind_autograd(m);
   htx::bind_dense(m);
+  htx::bind_answers(m);
 }

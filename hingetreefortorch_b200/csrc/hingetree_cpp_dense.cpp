@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/graph_task.h>
 
 #include "hingetree_cpp_autograd.h"
+#include "hingetree_cpp_dense.h"
 
 namespace htx {
 
@@ -13,44 +14,15 @@ namespace {
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-using OptionalTensor = std::optional<torch::Tensor>;
-
-torch::Tensor given(const OptionalTensor &t) { return t.has_value() ? *t : torch::Tensor(); }
-OptionalTensor optional(const torch::Tensor &t) { return t.defined() ? OptionalTensor(t) : std::nullopt; }
-const void *pointer(const torch::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-
-void check_types(const torch::Tensor &x, std::initializer_list<const torch::Tensor *> others) {
-  if (x.scalar_type() != torch::kFloat32 && x.scalar_type() != torch::kBFloat16 && x.scalar_type() != torch::kFloat16)
-    bad_argument("Error: Unsupported data type. Only torch.float32, torch.bfloat16 and torch.float16 are supported.");
-  for (const torch::Tensor *t : others) {
-    if (!t->defined()) continue;
-    if (t->scalar_type() != x.scalar_type()) bad_argument("Error: x, the weights and the biases are expected to have the same type.");
-    if (t->device() != x.device()) bad_argument("Error: All tensors are expected to be on the same device.");
-  }
-}
 void check_weight(const torch::Tensor &x, const torch::Tensor &w, const torch::Tensor &bias) {
   if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1) || w.size(0) < 1 || w.size(1) < 1)
     bad_argument("Error: x must be [..., features] and a weight [outputs, features], with one feature and one output at least.");
   if (bias.defined() && (bias.dim() != 1 || bias.size(0) != w.size(0))) bad_argument("Error: a bias must be [outputs].");
 }
 
-// Rows of contiguous features, the first on 16 bytes; differentiable.
-torch::Tensor as_rows(const torch::Tensor &x) {
-  torch::Tensor rows = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  const bool contiguous = rows.is_contiguous();
-  if (!contiguous && (rows.stride(1) != 1 || rows.stride(0) < rows.size(1))) rows = rows.contiguous();
-  if (reinterpret_cast<uintptr_t>(rows.const_data_ptr()) % 16 != 0) rows = rows.clone(at::MemoryFormat::Contiguous);
-  return rows;
-}
-torch::Tensor as_whole(const torch::Tensor &t) {
-  if (!t.defined()) return t;
-  const torch::Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 != 0 ? c.clone(at::MemoryFormat::Contiguous) : c;
-}
-
 ht_dense_problem problem_of(const torch::Tensor &x, const torch::Tensor &w, int activation) {
   ht_dense_problem p = {};
-  p.dtype = x.scalar_type() == torch::kFloat32 ? HT_DTYPE_F32 : x.scalar_type() == torch::kBFloat16 ? HT_DTYPE_BF16 : HT_DTYPE_F16;
+  p.dtype = type_code(x);
   p.activation = activation;
   p.rows = x.size(0), p.features = x.size(1), p.outputs = w.size(0);
   p.x_stride = x.size(0) > 1 ? x.stride(0) : x.size(1);

@@ -101,6 +101,9 @@ void bind_autograd(pybind11::module_ &m);
 // Registers the dense layers around a forest (hingetree_cpp_dense.cpp).
 void bind_dense(pybind11::module_ &m);
 
+// Registers packed weights, class scores under them and the draw of a class (hingetree_cpp_answers.cpp).
+void bind_answers(pybind11::module_ &m);
+
 // Registers the convolution, fused-linear, fusion, sparse, trie and contract/expand operators.
 void bind_more_ops(pybind11::module_ &m);
 

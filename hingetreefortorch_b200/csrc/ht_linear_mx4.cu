@@ -1,0 +1,265 @@
+// y = x W^T + bias under weights held as microscaled 4-bit numbers (ht_mx4.cuh).
+//
+// A weight is exact in bf16, so that x alone decides the products: one of bf16 values, two of fp16 (two bf16 numbers a value, exact), three of
+// fp32 (three numbers, 24 bits), summed in fp32.
+#include "ht_mx4.cuh"
+
+namespace ht {
+namespace mx4 {
+namespace {
+
+using dense::after_previous_kernel;
+using dense::load_plain;
+using dense::to_float;
+
+// x's bf16 numbers a value.
+template <typename T>
+constexpr int kNumbers = std::is_same<T, __nv_bfloat16>::value ? 1 : std::is_same<T, __half>::value ? 2 : 3;
+
+// ---- few rows ---------------------------------------------------------------------------------------------------------
+// A warp takes 16 outputs (the 16 rows of mma.sync's first operand) and 128 features, of which a lane has a block of 32 of two outputs: their codes are 16
+// contiguous bytes each, read straight into registers, some groups of outputs ahead.  x, the other operand, is in registers for good where one
+// warp's share of the features never changes: up to 16 warps share a group of outputs, and their sums meet in shared memory.
+constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;
+
+template <typename T>
+struct FewArgs {
+  const T *x, *bias;
+  const uint8_t *codes, *scales;
+  T *y;
+  int64_t x_stride;
+  int rows, features, outputs, blocks;
+  int chunks;  // of 4 blocks of features
+  int sharing; // warps that share a group of outputs
+  bool whole;  // rows of x start on 16 bytes
+};
+
+// A lane's 32 features of one row of x as pairs (i, i + 4) of every 8, number by number.
+template <typename T>
+__device__ __forceinline__ void load_x(const FewArgs<T> &a, int row, int k, uint32_t (&x)[kNumbers<T>][16]) {
+  constexpr int kPer = 16 / (int)sizeof(T);
+  const T *from = a.x + (int64_t)row * a.x_stride + k;
+  const bool there = row < a.rows;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float v[8];
+    if (there && a.whole && k + 8 * q + 8 <= a.features) {
+#pragma unroll
+      for (int j = 0; j < 8; j += kPer) {
+        T t[kPer];
+        *reinterpret_cast<uint4 *>(t) = load_plain(reinterpret_cast<const uint4 *>(from + 8 * q + j));
+#pragma unroll
+        for (int n = 0; n < kPer; ++n) v[j + n] = to_float(t[n]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = there && k + 8 * q + j < a.features ? to_float(from[8 * q + j]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kNumbers<T> == 1) {
+        x[0][4 * q + i] = dense::pack_pair(v[i], v[i + 4], static_cast<const __nv_bfloat16 *>(nullptr));
+      } else {
+        uint32_t third;
+        dense::split_pair(v[i], v[i + 4], x[0][4 * q + i], x[1][4 * q + i], third);
+        if constexpr (kNumbers<T> == 3) x[2][4 * q + i] = third;
+      }
+    }
+  }
+}
+
+struct Codes {  // a lane's of two outputs
+  uint4 a, b;
+  uint32_t scales;  // a's in the low byte, b's in the next
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T, int NT, int AHEAD>
+__global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<T> a) {
+  constexpr int P = kNumbers<T>;
+  extern __shared__ __align__(16) float few_sums[];  // [2][warps][NT][32][4]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  const int team = warp / a.sharing, part = warp - team * a.sharing, teams = kFewWarps / a.sharing;
+  const int row0 = (int)blockIdx.y * (8 * NT);
+  const int groups = (a.outputs + 15) / 16, first = team * (int)gridDim.x + (int)blockIdx.x, stride = teams * (int)gridDim.x;
+  after_previous_kernel();
+  if (team >= teams) return;
+
+  uint32_t x[NT][P][16];
+  auto fragments = [&](int chunk) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) load_x(a, row0 + 8 * n + g, (4 * chunk + j) * kBlock, x[n]);
+  };
+  auto fetch = [&](int group, int chunk) {
+    Codes c = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u), 0x7f7fu};
+    const int block = 4 * chunk + j, o = group * 16 + g;
+    if (group < groups && block < a.blocks) {
+      const int64_t at = (int64_t)min(o, a.outputs - 1) * a.blocks + block, bt = (int64_t)min(o + 8, a.outputs - 1) * a.blocks + block;
+      c.a = load_plain(reinterpret_cast<const uint4 *>(a.codes) + at);
+      c.b = load_plain(reinterpret_cast<const uint4 *>(a.codes) + bt);
+      c.scales = (uint32_t)load_plain(a.scales + at) | (uint32_t)load_plain(a.scales + bt) << 8;
+    }
+    return c;
+  };
+  auto multiply = [&](const Codes &c, float (&sum)[NT][4]) {
+    const Scale sa = scale_of(c.scales & 255u), sb = scale_of(c.scales >> 8);
+    const bool beyond = __any_sync(0xffffffffu, sa.beyond || sb.beyond);
+    const uint32_t wa[4] = {c.a.x, c.a.y, c.a.z, c.a.w}, wb[4] = {c.b.x, c.b.y, c.b.z, c.b.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t va[4], vb[4];
+      numbers_of(wa[q], va);
+      numbers_of(wb[q], vb);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) va[i] = times(va[i], sa.first), vb[i] = times(vb[i], sb.first);
+      if (beyond) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) va[i] = times(va[i], sa.more), vb[i] = times(vb[i], sb.more);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (P == 1) {
+#pragma unroll
+          for (int h = 0; h < 4; h += 2) mma_bf16(sum[n], va[h], vb[h], va[h + 1], vb[h + 1], x[n][0][4 * q + h], x[n][0][4 * q + h + 1]);
+        } else {  // the tensor core truncates what it adds to: short sums, the small ones first, added in fp32
+          float fresh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+            for (int h = 0; h < 4; h += 2) mma_bf16(fresh, va[h], vb[h], va[h + 1], vb[h + 1], x[n][p][4 * q + h], x[n][p][4 * q + h + 1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[n][i] += fresh[i];
+        }
+      }
+    }
+  };
+  uint32_t buffer = 0;
+  auto finish = [&](int group, const float (&sum)[NT][4]) {
+    float4 *const own = reinterpret_cast<float4 *>(few_sums) + (size_t)(buffer * kFewWarps) * (NT * 32);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) own[(warp * NT + n) * 32 + lane] = make_float4(sum[n][0], sum[n][1], sum[n][2], sum[n][3]);
+    if (a.sharing > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(a.sharing * 32) : "memory");
+    else
+      __syncwarp();
+    // lane's number i is output g + 8 (i / 2) and row 2 j + i % 2
+    const float *sums = reinterpret_cast<const float *>(own) + (size_t)(team * a.sharing) * (NT * 128);
+    for (int f = part * 32 + lane; f < NT * 128; f += a.sharing * 32) {
+      float v = sums[f];
+      for (int p = 1; p < a.sharing; ++p) v += sums[p * (NT * 128) + f];
+      const int n = f >> 7, of = (f >> 2) & 31, i = f & 3;
+      const int o = group * 16 + (of >> 2) + 8 * (i >> 1), r = row0 + 8 * n + 2 * (of & 3) + (i & 1);
+      if (r < a.rows && o < a.outputs) {
+        v *= kHeld;
+        if (a.bias != nullptr) v += to_float(a.bias[o]);
+        a.y[(int64_t)r * a.outputs + o] = dense::from_float<T>(v);
+      }
+    }
+    buffer ^= 1u;  // (the next sums go to the other half, and those after them come after the next barrier)
+  };
+
+  if (a.chunks <= a.sharing) {
+    Codes ahead[AHEAD];
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) ahead[d] = fetch(first + d * stride, part);
+    fragments(part);
+    for (int base = first; base < groups; base += AHEAD * stride) {
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        const int group = base + d * stride;
+        if (group >= groups) break;
+        const Codes c = ahead[d];
+        ahead[d] = fetch(group + AHEAD * stride, part);
+        float sum[NT][4] = {};
+        multiply(c, sum);
+        finish(group, sum);
+      }
+    }
+  } else {
+    for (int group = first; group < groups; group += stride) {
+      float sum[NT][4] = {};
+      Codes next = fetch(group, part);
+      for (int chunk = part; chunk < a.chunks; chunk += a.sharing) {
+        const Codes c = next;
+        if (chunk + a.sharing < a.chunks) next = fetch(group, chunk + a.sharing);
+        fragments(chunk);
+        multiply(c, sum);
+      }
+      finish(group, sum);
+    }
+  }
+}
+
+int screen(const ht_dense_problem *p) {
+  if (p == nullptr || p->rows < 0 || p->features < 1 || p->outputs < 1 || p->x_stride < p->features) return HT_ERR_INVALID_ARGUMENT;
+  if (p->dtype != HT_DTYPE_F32 && p->dtype != HT_DTYPE_BF16 && p->dtype != HT_DTYPE_F16) return HT_ERR_INVALID_ARGUMENT;
+  if (p->rows > 0x7fffff00 || p->features > 0x3fffff00 || p->outputs > 0x3fffff00) return HT_ERR_UNSUPPORTED;
+  return HT_OK;
+}
+
+template <typename T, int NT, int AHEAD>
+int launch_few(const FewArgs<T> &a, cudaStream_t stream) {
+  const int groups = (a.outputs + 15) / 16;
+  constexpr size_t kBytes = sizeof(float) * 2 * kFewWarps * NT * 128;
+  const dim3 grid((unsigned)std::min(groups, 148), (unsigned)((a.rows + 8 * NT - 1) / (8 * NT)));
+  return dense::launch_next<few_rows_kernel<T, NT, AHEAD>>(grid, kFewThreads, kBytes, kBytes, stream, 1, a);
+}
+
+template <typename T>
+int forward(const ht_dense_problem &p, const void *x, const void *codes, const void *scales, const void *bias, void *y, void *ws, size_t ws_bytes,
+            uint32_t *status_word, cudaStream_t stream) {
+  FewArgs<T> a = {};
+  a.x = static_cast<const T *>(x), a.bias = static_cast<const T *>(bias), a.y = static_cast<T *>(y);
+  a.codes = static_cast<const uint8_t *>(codes), a.scales = static_cast<const uint8_t *>(scales);
+  a.x_stride = p.x_stride;
+  a.rows = (int)p.rows, a.features = (int)p.features, a.outputs = (int)p.outputs, a.blocks = (int)blocks_of(p.features);
+  a.chunks = (a.blocks + 3) / 4;
+  a.sharing = std::min(a.chunks, kFewWarps);
+  a.whole = p.x_stride * (int64_t)sizeof(T) % 16 == 0 || p.rows == 1;
+  if constexpr (kNumbers<T> == 1) {
+    return p.rows <= 8 ? launch_few<T, 1, 4>(a, stream) : launch_few<T, 2, 4>(a, stream);
+  } else {
+    return launch_few<T, 1, 4>(a, stream);
+  }
+}
+
+template <typename F>
+int by_type(int dtype, F &&f) {
+  return dtype == HT_DTYPE_F32 ? f(float()) : dtype == HT_DTYPE_BF16 ? f(__nv_bfloat16()) : f(__half());
+}
+
+bool aligned(std::initializer_list<const void *> pointers) {
+  uintptr_t all = 0;
+  for (const void *p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & 15u) == 0;
+}
+
+}  // namespace
+}  // namespace mx4
+}  // namespace ht
+
+using namespace ht;
+using namespace ht::mx4;
+
+extern "C" size_t ht_linear_mx4_workspace_bytes(const ht_dense_problem *p) {
+  if (screen(p) != HT_OK) return 0;
+  return 0;
+}
+
+extern "C" int ht_linear_mx4(const ht_dense_problem *p, const void *x, const void *codes, const void *scales, const void *bias, void *y, void *workspace,
+                             size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream) {
+  const int rc = screen(p);
+  if (rc != HT_OK) return rc;
+  if (p->rows == 0) return HT_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr || y == nullptr) return HT_ERR_INVALID_ARGUMENT;
+  if (!aligned({x, codes, scales, bias, y})) return HT_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return HT_ERR_WORKSPACE;
+  return by_type(p->dtype, [&](auto zero) -> int {
+    return forward<decltype(zero)>(*p, x, codes, scales, bias, y, workspace, workspace_bytes, status_word, reinterpret_cast<cudaStream_t>(stream));
+  });
+}

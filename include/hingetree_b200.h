@@ -476,6 +476,46 @@ int ht_linear_class_loss_backward(const ht_dense_problem *p, const void *x, cons
                                   int64_t ignore_index, int reduction, const float *grad, const float *stats, const void *kept,
                                   void *dx, void *dw, void *dbias, void *workspace, size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
 
+/* ---- answers of a linear layer with many classes ------------------------------------------------------------------
+ * A class head's weights as microscaled 4-bit numbers, class scores under them, and a class drawn from a row of scores.  No counterpart in
+ * the reference.
+ *
+ * MXFP4 of the Open Compute Project's Microscaling Formats specification v1.0: 32 neighbouring features share a power of two, byte b for
+ * 2^(b - 127), 255 for no number; codes are 4 bits (sign, 2 of exponent, 1 of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte,
+ * the first in the low half.  With blocks = features / 32, rounded up:  codes [outputs, 16 blocks], scales [outputs, blocks] bytes, both on
+ * 16 bytes, codes behind the last feature 0.
+ * ht_mx4_pack: b = max(floor(log2 max|w|) - 2, -127) + 127 (255 for a block with an infinity or no number, whose codes are 0), codes to the
+ * nearest number, of two as near the one with the even code, 6 at the most.  w [outputs, features], w_stride from row to row.
+ * ht_mx4_unpack: the values, rounded to the type (exact in bf16 and fp32, infinite beyond their range). */
+int ht_mx4_pack(int dtype, const void *w, int64_t w_stride, int64_t outputs, int64_t features, void *codes, void *scales, ht_stream_t stream);
+int ht_mx4_unpack(int dtype, const void *codes, const void *scales, int64_t outputs, int64_t features, void *w, int64_t w_stride, ht_stream_t stream);
+
+/* y[n, o] = x[n] . W[o] + bias[o] with W the values of codes and scales; x, bias (may be NULL) and y in the problem's type, sums fp32.  The problem's
+ * activation and scratch_limit are not read.  x, bias and y start on 16 bytes (HT_ERR_UNSUPPORTED), the workspace on 256. */
+size_t ht_linear_mx4_workspace_bytes(const ht_dense_problem *p);
+int ht_linear_mx4(const ht_dense_problem *p, const void *x, const void *codes, const void *scales, const void *bias, void *y, void *workspace,
+                  size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);
+
+/* A class drawn from each row of scores s [rows, classes] (stride elements from row to row) with the row's number u of uniform [rows]:
+ *   m = max s;  w_i = exp((s_i - m) / T), and with T = 0 the first class of the largest score alone;
+ *   in the order of falling scores, of equal ones the lower class first, the shortest of these prefixes counts, the first class always:
+ *   top_k classes (0: all), the shortest whose weight reaches top_p times that of the first top_k (1: all of them), the classes with w >= min_p;
+ *   drawn: the first class, in the order of classes, up to which what counts weighs more than u of all that counts (u = 1: the last one);
+ *   log_prob: the logarithm of its share.
+ * Weights and sums are held in 64 bits.  Each bound is one number, or one a row where the pointer is not
+ * NULL (row_top_k below 1, row_top_p from 1 on: all).  A row without an answer (its largest score not finite, a score or bound that is no
+ * number, T negative or infinite, u outside [0, 1]) has drawn = -1 and log_prob no number. */
+typedef struct ht_sample_problem {
+  int32_t dtype;
+  int32_t reserved;
+  int64_t rows, classes, stride;
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float *row_temperature, *row_top_p, *row_min_p;
+  const int64_t *row_top_k;
+} ht_sample_problem;
+int ht_sample_classes(const ht_sample_problem *p, const void *scores, const float *uniform, int64_t *drawn, float *log_probs, ht_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
