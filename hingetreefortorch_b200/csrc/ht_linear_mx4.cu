@@ -2,14 +2,13 @@
 //
 // A weight is exact in bf16, so that x alone decides the products: one of bf16 values, two of fp16 (two bf16 numbers a value, exact), three of
 // fp32 (three numbers, 24 bits), summed in fp32.
-#include "ht_mx4.cuh"
+#include "ht_mx4_tile.cuh"
 
 namespace ht {
 namespace mx4 {
 namespace {
 
 using dense::after_previous_kernel;
-using dense::load_plain;
 using dense::to_float;
 
 // x's bf16 numbers a value.
@@ -210,9 +209,36 @@ int launch_few(const FewArgs<T> &a, cudaStream_t stream) {
   return dense::launch_next<few_rows_kernel<T, NT, AHEAD>>(grid, kFewThreads, kBytes, kBytes, stream, 1, a);
 }
 
+// Whether the rows are few enough for the kernel above.
+template <typename T>
+bool few_rows(int64_t rows) {
+  return rows <= (kNumbers<T> == 1 ? 16 : 8);
+}
+
+template <typename T>
+struct Plan {
+  dense::Operand<T, dense::GradKind<T>> x;
+  size_t bytes = 0;
+  Plan(const ht_dense_problem &p, const void *xp, void *ws) {
+    dense::Arena arena(ws);
+    if (!few_rows<T>(p.rows)) x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
+    bytes = arena.used;
+  }
+};
+
 template <typename T>
 int forward(const ht_dense_problem &p, const void *x, const void *codes, const void *scales, const void *bias, void *y, void *ws, size_t ws_bytes,
             uint32_t *status_word, cudaStream_t stream) {
+  static_assert(kNumbers<T> == dense::GradKind<T>::kPlanes, "the operand's planes are x's numbers");
+  if (!few_rows<T>(p.rows)) {
+    Plan<T> plan(p, x, ws);
+    if (plan.bytes > ws_bytes || (plan.bytes > 0 && ws == nullptr)) return HT_ERR_WORKSPACE;
+    int sms = 0;
+    HT_TRY(dense::sm_count(&sms));
+    HT_TRY(dense::lay_out<T>(stream, plan.x));
+    return launch_tiles<T, kNumbers<T>>(plan.x.m, codes, static_cast<const uint8_t *>(scales), static_cast<const T *>(bias), static_cast<T *>(y), p.rows,
+                                        p.features, p.outputs, status_word, sms, stream);
+  }
   FewArgs<T> a = {};
   a.x = static_cast<const T *>(x), a.bias = static_cast<const T *>(bias), a.y = static_cast<T *>(y);
   a.codes = static_cast<const uint8_t *>(codes), a.scales = static_cast<const uint8_t *>(scales);
@@ -247,8 +273,13 @@ using namespace ht;
 using namespace ht::mx4;
 
 extern "C" size_t ht_linear_mx4_workspace_bytes(const ht_dense_problem *p) {
-  if (screen(p) != HT_OK) return 0;
-  return 0;
+  if (screen(p) != HT_OK || p->rows == 0) return 0;
+  size_t bytes = 0;
+  by_type(p->dtype, [&](auto zero) -> int {
+    bytes = Plan<decltype(zero)>(*p, nullptr, nullptr).bytes;
+    return HT_OK;
+  });
+  return bytes;
 }
 
 extern "C" int ht_linear_mx4(const ht_dense_problem *p, const void *x, const void *codes, const void *scales, const void *bias, void *y, void *workspace,
