@@ -33,7 +33,7 @@ struct FewArgs {
   bool whole;  // rows of x start on 16 bytes
 };
 
-// A lane's 32 features of one row of x as pairs (i, i + 4) of every 8, number by number.
+// A lane's 32 features of one row of x as pairs of neighbours, number by number.
 template <typename T>
 __device__ __forceinline__ void load_x(const FewArgs<T> &a, int row, int k, uint32_t (&x)[kNumbers<T>][16]) {
   constexpr int kPer = 16 / (int)sizeof(T);
@@ -57,10 +57,10 @@ __device__ __forceinline__ void load_x(const FewArgs<T> &a, int row, int k, uint
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (kNumbers<T> == 1) {
-        x[0][4 * q + i] = dense::pack_pair(v[i], v[i + 4], static_cast<const __nv_bfloat16 *>(nullptr));
+        x[0][4 * q + i] = dense::pack_pair(v[2 * i], v[2 * i + 1], static_cast<const __nv_bfloat16 *>(nullptr));
       } else {
         uint32_t third;
-        dense::split_pair(v[i], v[i + 4], x[0][4 * q + i], x[1][4 * q + i], third);
+        dense::split_pair(v[2 * i], v[2 * i + 1], x[0][4 * q + i], x[1][4 * q + i], third);
         if constexpr (kNumbers<T> == 3) x[2][4 * q + i] = third;
       }
     }
@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
   after_previous_kernel();
   if (team >= teams) return;
 
+  const uint32_t number = opaque_one();
   uint32_t x[NT][P][16];
   auto fragments = [&](int chunk) {
 #pragma unroll
@@ -107,19 +108,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
   };
   auto multiply = [&](const Codes &c, float (&sum)[NT][4]) {
     const Scale sa = scale_of(c.scales & 255u), sb = scale_of(c.scales >> 8);
-    const bool beyond = __any_sync(0xffffffffu, sa.beyond || sb.beyond);
     const uint32_t wa[4] = {c.a.x, c.a.y, c.a.z, c.a.w}, wb[4] = {c.b.x, c.b.y, c.b.z, c.b.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       uint32_t va[4], vb[4];
-      numbers_of(wa[q], va);
-      numbers_of(wb[q], vb);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) va[i] = times(va[i], sa.first), vb[i] = times(vb[i], sb.first);
-      if (beyond) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) va[i] = times(va[i], sa.more), vb[i] = times(vb[i], sb.more);
-      }
+      weights_of(wa[q], sa, number, va);
+      weights_of(wb[q], sb, number, vb);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if constexpr (P == 1) {

@@ -12,35 +12,45 @@ namespace mx4 {
 constexpr int kBlock = 32;
 __host__ __device__ inline int64_t blocks_of(int64_t features) { return (features + kBlock - 1) / kBlock; }
 
-// 8 codes of a word as bf16: word i of the four has codes i and i + 4.  The 3 bits of a magnitude in the lowest bits of the exponent and the
-// highest of the mantissa are the number times 2^-126, subnormal ones too, so one multiplication gives number and scale.  Operands are held as
-// 2^-4 of their values: from 2^-132, a subnormal number of bf16, up to 6 2^123 all are exact, where 6 2^127 is beyond it; what they are summed to is
-// multiplied by kHeld.
-//   first: 2^126 2^(b - 127) / kHeld, for b up to 132;  more: what is missing beyond (1 otherwise)
-constexpr float kHeld = 16.0f;
+// Codes as bf16 numbers.  A byte permutation whose selectors are the codes looks up 4 of them at a time: its fourth selector bit, the sign, turns
+// a byte whose highest bit is 0 into 0, so one look-up gives the positive numbers, another, with the signs inverted, the negative ones, and
+// their sum is 32 + 4 v.  Behind 0x42 that is the bf16 number 40 + v, and (40 + v) s - 40 s is v s without rounding.  s = 2^(b - 127) / kHeld: from
+// 2^-133, the smallest subnormal number of bf16, up to 40 2^122 all of it is in bf16's range, where 6 2^127 is not; what operands
+// are summed to is multiplied by kHeld.
+// Permutations, shifts and logic run at half the rate of the rest: 11 of them for 8 codes, where moving sign and magnitude to their places
+// by shifts took 19 (8192 x 1024 to 50000: HT_MX4_MEASURED).
+constexpr float kHeld = 32.0f;
 struct Scale {
-  uint32_t first, more;  // twice the same bf16
-  bool beyond;
+  uint32_t s, offset;  // twice the same bf16: s and -40 s
 };
 __device__ __forceinline__ Scale scale_of(uint32_t b) {
-  Scale s;
-  const uint32_t f = b == 255u ? 0x7fc0u : min(b + 122u, 254u) << 7, m = b > 132u && b != 255u ? (b - 5u) << 7 : 0x3f80u;
-  s.first = f | f << 16;
-  s.more = m | m << 16;
-  s.beyond = b > 132u;
-  return s;
+  uint32_t s = b < 6u ? 2u << b : (b - 5u) << 7, offset = b == 0u ? 0x8050u : 0x8020u | b << 7;
+  if (b == 255u) s = 0x7fc0u;
+  return {s | s << 16, offset | offset << 16};
 }
-__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t permute(uint32_t a, uint32_t b, uint32_t selectors) {
   uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(selectors));
   return r;
 }
-__device__ __forceinline__ void numbers_of(uint32_t w, uint32_t (&v)[4]) {
-  constexpr uint32_t kMagnitude = 0x01c001c0u, kSign = 0x80008000u;
-  v[0] = ((w << 6) & kMagnitude) | ((w << 12) & kSign);
-  v[1] = ((w << 2) & kMagnitude) | ((w << 8) & kSign);
-  v[2] = ((w >> 2) & kMagnitude) | ((w << 4) & kSign);
-  v[3] = ((w >> 6) & kMagnitude) | (w & kSign);
+// 8 codes of a word as 4 words of two neighbours.  `one` is 1 in a register: a sum by multiplication, which runs at the full rate.
+__device__ __forceinline__ void weights_of(uint32_t w, const Scale &scale, uint32_t one, uint32_t *out) {
+  const uint32_t n = w ^ 0x88888888u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t positive = permute(0x26242220u, 0x38302c28u, h == 0 ? w : w >> 16), negative = permute(0x1a1c1e20u, 0x08101418u, h == 0 ? n : n >> 16);
+    uint32_t bytes;
+    asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(bytes) : "r"(positive), "r"(one), "r"(negative));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(out[2 * h + i]) : "r"(__byte_perm(bytes, 0x42424242u, i == 0 ? 0x4140u : 0x4342u)), "r"(scale.s), "r"(scale.offset));
+  }
+}
+// 1 where the compiler does not know it.
+__device__ __forceinline__ uint32_t opaque_one() {
+  uint32_t one;
+  asm volatile("mov.u32 %0, 1;" : "=r"(one));
+  return one;
 }
 
 }  // namespace mx4

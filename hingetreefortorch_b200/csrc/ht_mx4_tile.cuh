@@ -52,14 +52,47 @@ struct alignas(64) TileArgs {
   int m_blocks, n_blocks, tiles, k_blocks;
 };
 
-__device__ __forceinline__ void mma_weights(uint32_t one, uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t instruction, uint32_t accumulate) {
+// The instructions of the warp that issues the products are few and follow one another closely: with a wait for x, one for weights and calls
+// of general helpers a stage of 64 columns took 730 cycles of it, twice what 192 columns need of the tensor core.
+__device__ __forceinline__ void mma_weights(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t instruction, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       :
-      : "r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(instruction), "r"(accumulate), "r"(one)
+      : "r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(instruction), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Whether a barrier's phase has passed, without waiting.
+__device__ __forceinline__ bool passed(uint64_t *bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Waits for it, `tries` times at the most; 0 is left when they ran out, and no wait after that tries more than once.
+__device__ __forceinline__ void wait_for_phase(uint64_t *bar, uint32_t parity, uint32_t &tries) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, %0;\n\t"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "@p bra DONE;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.gt.s32 q, n, 0;\n\t"
+      "@q bra AGAIN;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "DONE:\n\t}"
+      : "+r"(tries)
+      : "r"(smem_addr(bar)), "r"(parity), "n"(kTryNanoseconds)
       : "memory");
 }
 __device__ __forceinline__ void load_2d(uint32_t one, uint32_t dst, const CUtensorMap *map, int col, int row, uint32_t bar) {
@@ -83,35 +116,14 @@ __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t (&r
       : "memory");
 }
 
-// 32 codes of a block, 16 bytes, as 16 words of two neighbours.
-__device__ __forceinline__ void weights_of(const uint4 &codes, const Scale &scale, bool beyond, uint32_t *out) {
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t v[4];
-    numbers_of(w[q], v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = times(v[i], scale.first);
-    if (beyond) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = times(v[i], scale.more);
-    }
-    out[4 * q] = __byte_perm(v[0], v[1], 0x5410);
-    out[4 * q + 1] = __byte_perm(v[2], v[3], 0x5410);
-    out[4 * q + 2] = __byte_perm(v[0], v[1], 0x7632);
-    out[4 * q + 3] = __byte_perm(v[2], v[3], 0x7632);
-  }
-}
-
 template <typename T, int P>
 __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_constant__ TileArgs a, const T *bias, T *y) {
   extern __shared__ __align__(1024) unsigned char mx4_smem[];
   unsigned char *base = mx4_smem + ((1024u - (smem_addr(mx4_smem) & 1023u)) & 1023u);
   const uint32_t stage_bytes = (uint32_t)(P * a.bn) * 128u;
   const uint32_t boxes = smem_addr(base), stages = boxes + kBoxes * kBoxBytes;
-  uint64_t *full = reinterpret_cast<uint64_t *>(base + kBoxes * kBoxBytes + (size_t)kStages * P * kMostRows<P> * 128);  // x
-  uint64_t *weighted = full + kStages;        // the weights are in tensor memory
-  uint64_t *empty = weighted + kStages;       // of both
+  uint64_t *full = reinterpret_cast<uint64_t *>(base + kBoxes * kBoxBytes + (size_t)kStages * P * kMostRows<P> * 128);  // x and weights are there
+  uint64_t *empty = full + kStages;           // of both
   uint64_t *box_full = empty + kStages;       // codes
   uint64_t *box_empty = box_full + kBoxes;
   uint64_t *accumulated = box_empty + kBoxes; // [2] an accumulator is complete
@@ -123,8 +135,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
   constexpr uint32_t kColumns = 512;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&weighted[s], kSetWarps);
+      mbar_init(&full[s], 1 + kSetWarps);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < kBoxes; ++b) {
@@ -191,53 +202,59 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
       mbar_wait(ok ? &empty[s] : &full[s], (i / kStages) & 1u, ok ? kMaxSpins : 4096);
     }
   } else if (warp == 1) {
-    const uint32_t one = dense::elect_one();
     const uint32_t tmem_d = __reduce_or_sync(0xffffffffu, tmem);  // the same in a uniform register
-    uint32_t it = 0, chunk = 0;
-    // A lane whose wait ran out waits no more, and the warp goes on: no branch depends on a wait.
-    bool ok = true;
-    auto wait_here = [&](uint64_t *bar, uint32_t parity) {
-      if (ok && !mbar_wait(bar, parity)) {
-        ok = false;
-        give_up();
-      }
-    };
-    const uint64_t plane = (uint64_t)((uint32_t)a.bn * 128u >> 4);
-    for (int tile = (int)blockIdx.x; tile < a.tiles; tile += (int)gridDim.x) {
-      for (int kb = 0; kb < a.k_blocks; ++kb, ++it) {
-        const int in_chunk = kb % kChunk<P>;
-        const uint32_t buffer = chunk & 1u, d = tmem_d + buffer * (kWeightColumn / 2);
-        if (in_chunk == 0) wait_here(&drained[buffer], ((chunk >> 1) & 1u) ^ 1u);
-        const uint32_t s = it % kStages, parity = (it / kStages) & 1u;
-        wait_here(&full[s], parity);
-        wait_here(&weighted[s], parity);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int left = a.k - kb * kTileK;
-        const int steps = left >= kTileK ? 4 : (left + 15) / 16;
-        const uint64_t db = dense::k_major_descriptor(stages + s * stage_bytes);
-        const uint32_t wa = tmem_d + kWeightColumn + s * 32u;
+    uint32_t chunk = 0, tries = kMaxSpins;
+    const uint32_t plane = (uint32_t)a.bn * 128u >> 4;
+    const int own = (int)blockIdx.x < a.tiles ? (a.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0, total = own * a.k_blocks;
+    const int last_steps = (a.k - (a.k_blocks - 1) * kTileK + 15) / 16;
+    int kb = 0, in_chunk = 0;
+    bool there = passed(&full[0], 0u);
+    for (int base_it = 0; base_it < total; base_it += kStages) {
+      const uint32_t parity = (uint32_t)(base_it / kStages) & 1u;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if (kk >= steps) break;
-          const uint32_t more = kk > 0 || in_chunk > 0;
-          if constexpr (P == 3) {
-            const uint32_t small = d + kMostRows<3>;
-            mma_weights(one, small, wa + 8u * kk, db + 2 * plane + 2u * kk, a.instruction, more);
-            mma_weights(one, small, wa + 8u * kk, db + plane + 2u * kk, a.instruction, 1u);
-          } else if constexpr (P == 2) {
-            mma_weights(one, d, wa + 8u * kk, db + plane + 2u * kk, a.instruction, more);
+      for (int s = 0; s < kStages; ++s) {
+        if (base_it + s >= total) break;
+        const uint32_t buffer = chunk & 1u, d = tmem_d + buffer * (kWeightColumn / 2);
+        if (in_chunk == 0) wait_for_phase(&drained[buffer], ((chunk >> 1) & 1u) ^ 1u, tries);
+        if (!there) wait_for_phase(&full[s], parity, tries);
+        // the next stage's barrier is looked at under this stage's products
+        there = passed(&full[(s + 1) % kStages], s + 1 == kStages ? parity ^ 1u : parity);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const bool last = kb == a.k_blocks - 1;
+        const int steps = last ? last_steps : 4;
+        const uint64_t db = dense::k_major_descriptor(stages + (uint32_t)s * stage_bytes);
+        const uint32_t wa = tmem_d + kWeightColumn + (uint32_t)s * 32u;
+        if (dense::elect_one()) {
+          auto products = [&](int kk) {
+            const uint32_t more = kk > 0 || in_chunk > 0;
+            if constexpr (P == 3) {
+              const uint32_t small = d + kMostRows<3>;
+              mma_weights(small, wa + 8u * kk, db + 2 * plane + 2u * kk, a.instruction, more);
+              mma_weights(small, wa + 8u * kk, db + plane + 2u * kk, a.instruction, 1u);
+            } else if constexpr (P == 2) {
+              mma_weights(d, wa + 8u * kk, db + plane + 2u * kk, a.instruction, more);
+            }
+            mma_weights(d, wa + 8u * kk, db + 2u * kk, a.instruction, P == 2 ? 1u : more);
+          };
+          if (steps == 4) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) products(kk);
+          } else {
+            for (int kk = 0; kk < steps; ++kk) products(kk);
           }
-          mma_weights(one, d, wa + 8u * kk, db + 2u * kk, a.instruction, P == 2 ? 1u : more);
+          commit(&empty[s]);
+          if (last || in_chunk == kChunk<P> - 1) commit(&accumulated[buffer]);
         }
-        dense::mma_commit<1>(one, smem_addr(&empty[s]));
-        if (kb == a.k_blocks - 1 || in_chunk == kChunk<P> - 1) {
-          dense::mma_commit<1>(one, smem_addr(&accumulated[buffer]));
-          ++chunk;
-        }
+        __syncwarp();
+        if (last || in_chunk == kChunk<P> - 1) ++chunk;
+        in_chunk = last || in_chunk == kChunk<P> - 1 ? 0 : in_chunk + 1;
+        kb = last ? 0 : kb + 1;
       }
     }
+    if (tries == 0) give_up();
     // whatever became of the waits: tensor memory is not freed under a product
-    dense::mma_commit<1>(one, smem_addr(settled));
+    if (dense::elect_one()) commit(settled);
+    __syncwarp();
     mbar_wait(settled, 0u);
   } else if (warp < 2 + kEpilogueWarps) {
     const int quarter = warp & 3;  // a warp may only touch the lanes 32 (warp % 4) ...
@@ -262,10 +279,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
       auto store = [&](int unit, const float (&v)[32]) {
         const int row = turn.nb * a.bn + 32 * unit, count = a.rows - row;
         if (o >= a.outputs) return;
-        T *to = y + (int64_t)row * a.outputs + o;
+        T *const to = y + (int64_t)row * a.outputs + o;
+        if (count >= 32) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c, to += a.outputs)
-          if (c < count) *to = dense::from_float<T>(fmaf(v[c], kHeld, add));
+          for (int c = 0; c < 32; ++c) to[(uint64_t)(uint32_t)a.outputs * (uint32_t)c] = dense::from_float<T>(fmaf(v[c], kHeld, add));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (c < count) to[(uint64_t)(uint32_t)a.outputs * (uint32_t)c] = dense::from_float<T>(fmaf(v[c], kHeld, add));
+        }
       };
       if constexpr (P < 3) {
         if (!wait_for(chunk)) break;
@@ -330,29 +352,34 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
   } else {
     const int quarter = warp & 3, set = (warp - 2 - kEpilogueWarps) / kSetWarps;
     const int at = quarter * 32 + lane;  // this thread's output in a tile
+    const uint32_t number = opaque_one();
     const uint32_t weights = tmem + ((uint32_t)(quarter * 32) << 16) + kWeightColumn;
-    // The scales of this thread's stages of a box: two stages of two blocks, a byte each.
-    auto fetch_scales = [&](int tile, int q, uint32_t it) {
-      if (tile >= a.tiles) return 0u;
-      const uint8_t *from = a.scales + (int64_t)min(place(tile).mb * kTileM + at, a.outputs - 1) * a.blocks;
-      uint32_t r = 0;
+    // The scales of this thread's stages of a box: two stages of two blocks.  Loaded a box ahead, and not touched before they are used.
+    struct Scales {
+      uint8_t b[4];
+    };
+    auto scales_of = [&](int tile) { return a.scales + (int64_t)min(place(min(tile, a.tiles - 1)).mb * kTileM + at, a.outputs - 1) * a.blocks; };
+    auto fetch_scales = [&](const uint8_t *from, int q, uint32_t it) {
+      Scales r;
+      const int first = 2 * (q * kBoxStages + (int)((it + (uint32_t)set) & 1u));
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int block = 2 * (q * kBoxStages + (int)((it + (uint32_t)set) & 1u) + 2 * j) + i;
-          r |= (block < a.blocks ? (uint32_t)load_plain(from + block) : 127u) << (16 * j + 8 * i);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const int block = first + 4 * (j >> 1) + (j & 1);
+        r.b[j] = 127;
+        if (block < a.blocks) r.b[j] = load_plain(from + block);
+      }
       return r;
     };
     uint32_t it = 0, box = 0;
-    uint32_t next = fetch_scales((int)blockIdx.x, 0, 0u);
+    const uint8_t *from = scales_of((int)blockIdx.x);
+    Scales next = fetch_scales(from, 0, 0u);
     bool ok = true;
     for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x) {
       for (int q = 0; q < tile_boxes; ++q, ++box) {
-        const uint32_t scales = next;
+        const Scales scales = next;
         const int stages_here = min(kBoxStages, a.k_blocks - q * kBoxStages);
-        next = q + 1 < tile_boxes ? fetch_scales(tile, q + 1, it + (uint32_t)stages_here) : fetch_scales(tile + (int)gridDim.x, 0, it + (uint32_t)stages_here);
+        if (q + 1 == tile_boxes) from = scales_of(tile + (int)gridDim.x);
+        next = fetch_scales(from, q + 1 < tile_boxes ? q + 1 : 0, it + (uint32_t)stages_here);
         const uint32_t b = box % kBoxes;
         if (!(ok = arrived(&box_full[b], (box / kBoxes) & 1u))) break;
         const uint32_t row = boxes + b * kBoxBytes + (uint32_t)at * 128u;
@@ -362,18 +389,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
           if (in_box >= stages_here) break;
           const uint4 c0 = lds_b128(row + 16u * ((uint32_t)(2 * in_box) ^ ((uint32_t)at & 7u)));
           const uint4 c1 = lds_b128(row + 16u * ((uint32_t)(2 * in_box + 1) ^ ((uint32_t)at & 7u)));
-          const Scale s0 = scale_of((scales >> (16 * j)) & 255u), s1 = scale_of((scales >> (16 * j + 8)) & 255u);
-          const bool beyond = __any_sync(0xffffffffu, s0.beyond || s1.beyond);
+          const Scale s0 = scale_of(scales.b[2 * j]), s1 = scale_of(scales.b[2 * j + 1]);
           uint32_t v[32];
-          weights_of(c0, s0, beyond, v);
-          weights_of(c1, s1, beyond, v + 16);
+          weights_of(c0.x, s0, number, v), weights_of(c0.y, s0, number, v + 4), weights_of(c0.z, s0, number, v + 8), weights_of(c0.w, s0, number, v + 12);
+          weights_of(c1.x, s1, number, v + 16), weights_of(c1.y, s1, number, v + 20), weights_of(c1.z, s1, number, v + 24), weights_of(c1.w, s1, number, v + 28);
           const uint32_t i = it + (uint32_t)in_box, s = i % kStages;
           if (!(ok = arrived(&empty[s], ((i / kStages) & 1u) ^ 1u))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           tmem_store_32(weights + s * 32u, v);
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(&weighted[s]);
+          if (lane == 0) mbar_arrive(&full[s]);
         }
         if (!ok) break;
         it += (uint32_t)stages_here;
