@@ -12,12 +12,12 @@
 //   warp 1       allocates tensor memory; one lane issues tcgen05.mma.kind::f16 (M 128, N up to 192, K 16, the first operand in tensor memory) and
 //                commits each stage to those who fill it, and each finished accumulator to the epilogue;
 //   warps 2-5    the epilogue, a quarter of the lanes each, under the next tile's products;
-//   warps 6-13   the weights: two sets of four warps, a quarter of the lanes each, take every other stage;
+//   warps 6-13   the weights: two sets of four warps, a quarter of the lanes each, take every other stage of a box;
 //   warp 14      one lane issues the TMA loads of codes into a ring of 4 boxes of 256 values of k, ahead of x.
 // Tensor memory: two accumulators in turn (three numbers: of two parts each), and 4 stages of 32 columns of weights.
 // With three numbers the products of the first one have an accumulator, those of the others, 2^-8 of them, a second; both leave for
 // registers every 256 values of k and are added there in fp32 (the tensor core truncates when it adds; ht_dense_tile.cuh).
-// Every wait is bounded, as in ht_dense_tile.cuh.
+// A tile starts with the first stage of the ring: the last box of a tile may leave stages out.  Every wait is bounded, as in ht_dense_tile.cuh.
 #pragma once
 
 #include "ht_mx4.cuh"
@@ -37,8 +37,6 @@ constexpr uint32_t kWeightColumn = 384;
 // Rows of x in a tile at the most, and the columns of an accumulator.
 template <int P>
 constexpr int kMostRows = P == 1 ? 192 : P == 2 ? 128 : 96;
-template <int P>
-constexpr int kChunk = P == 3 ? 4 : 1 << 24;  // stages between two visits of the registers
 template <int P>
 constexpr size_t kTileBytes = 1024 + (size_t)kStages * P * kMostRows<P> * 128 + (size_t)kBoxes * kBoxBytes + 512;
 
@@ -183,72 +181,77 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
 
   if (warp == 0) {
     const uint32_t one = dense::elect_one();
-    uint32_t it = 0;
+    uint32_t phases = 0xfu, used = 0;  // a bit for each stage
     bool ok = true;
     for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x) {
       const Turn turn = place(tile);
-      for (int kb = 0; kb < a.k_blocks; ++kb, ++it) {
-        const uint32_t s = it % kStages;
-        if (!(ok = arrived(&empty[s], ((it / kStages) & 1u) ^ 1u))) break;
+      for (int kb = 0; kb < a.k_blocks; ++kb) {
+        const uint32_t s = (uint32_t)kb % kStages;  // (a tile starts with the first stage)
+        if (!(ok = arrived(&empty[s], (phases >> s) & 1u))) break;
+        phases ^= 1u << s;
+        used |= 1u << s;
         if (one) mbar_expect_tx(&full[s], stage_bytes);
         dense::load_3d<1>(one, stages + s * stage_bytes, &a.x, kb * kTileK, turn.nb * a.bn, smem_addr(&full[s]));
       }
     }
     if (!ok) give_up();
     // The last use of every stage ends before the CTA leaves, or, where a wait ran out, the copies still in flight.
-    const uint32_t issued = min(it, (uint32_t)kStages);
-    for (uint32_t j = 1; j <= issued; ++j) {
-      const uint32_t i = it - j, s = i % kStages;
-      mbar_wait(ok ? &empty[s] : &full[s], (i / kStages) & 1u, ok ? kMaxSpins : 4096);
-    }
+    for (uint32_t s = 0; s < kStages; ++s)
+      if ((used >> s) & 1u) mbar_wait(ok ? &empty[s] : &full[s], (phases >> s) & 1u, ok ? kMaxSpins : 4096);
   } else if (warp == 1) {
     const uint32_t tmem_d = __reduce_or_sync(0xffffffffu, tmem);  // the same in a uniform register
-    uint32_t chunk = 0, tries = kMaxSpins;
+    uint32_t chunk = 0, tries = kMaxSpins, phases = 0;  // phases: of each stage's barrier, a bit
     const uint32_t plane = (uint32_t)a.bn * 128u >> 4;
-    const int own = (int)blockIdx.x < a.tiles ? (a.tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0, total = own * a.k_blocks;
     const int last_steps = (a.k - (a.k_blocks - 1) * kTileK + 15) / 16;
-    int kb = 0, in_chunk = 0;
-    bool there = passed(&full[0], 0u);
-    for (int base_it = 0; base_it < total; base_it += kStages) {
-      const uint32_t parity = (uint32_t)(base_it / kStages) & 1u;
-#pragma unroll
-      for (int s = 0; s < kStages; ++s) {
-        if (base_it + s >= total) break;
+    bool there[2] = {false, false};
+    for (int tile = (int)blockIdx.x; tile < a.tiles; tile += (int)gridDim.x) {
+      for (int q = 0; q < tile_boxes; ++q) {
         const uint32_t buffer = chunk & 1u, d = tmem_d + buffer * (kWeightColumn / 2);
-        if (in_chunk == 0) wait_for_phase(&drained[buffer], ((chunk >> 1) & 1u) ^ 1u, tries);
-        if (!there) wait_for_phase(&full[s], parity, tries);
-        // the next stage's barrier is looked at under this stage's products
-        there = passed(&full[(s + 1) % kStages], s + 1 == kStages ? parity ^ 1u : parity);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const bool last = kb == a.k_blocks - 1;
-        const int steps = last ? last_steps : 4;
-        const uint64_t db = dense::k_major_descriptor(stages + (uint32_t)s * stage_bytes);
-        const uint32_t wa = tmem_d + kWeightColumn + (uint32_t)s * 32u;
-        if (dense::elect_one()) {
-          auto products = [&](int kk) {
-            const uint32_t more = kk > 0 || in_chunk > 0;
-            if constexpr (P == 3) {
-              const uint32_t small = d + kMostRows<3>;
-              mma_weights(small, wa + 8u * kk, db + 2 * plane + 2u * kk, a.instruction, more);
-              mma_weights(small, wa + 8u * kk, db + plane + 2u * kk, a.instruction, 1u);
-            } else if constexpr (P == 2) {
-              mma_weights(d, wa + 8u * kk, db + plane + 2u * kk, a.instruction, more);
-            }
-            mma_weights(d, wa + 8u * kk, db + 2u * kk, a.instruction, P == 2 ? 1u : more);
-          };
-          if (steps == 4) {
+        const int here = min(kBoxStages, a.k_blocks - q * kBoxStages);
+        const bool last = q == tile_boxes - 1, fresh = P == 3 || q == 0, ends = P == 3 || last;
+        if (fresh) wait_for_phase(&drained[buffer], ((chunk >> 1) & 1u) ^ 1u, tries);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) products(kk);
-          } else {
-            for (int kk = 0; kk < steps; ++kk) products(kk);
+        for (int s = 0; s < kStages; s += 2) {  // two stages at a time; the barriers of the next two are looked at under their products
+          if (s >= here) break;
+          const bool both = s + 1 < here;
+          if (!there[0]) wait_for_phase(&full[s], (phases >> s) & 1u, tries);
+          if (both && !there[1]) wait_for_phase(&full[s + 1], (phases >> (s + 1)) & 1u, tries);
+          phases ^= both ? 3u << s : 1u << s;
+          const int next = s + 2 < here ? s + 2 : 0;
+          there[0] = passed(&full[next], (phases >> next) & 1u);
+          there[1] = passed(&full[next + 1], (phases >> (next + 1)) & 1u);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (dense::elect_one()) {
+            auto products = [&](int stage, int kk) {
+              const uint32_t more = s > 0 || stage > 0 || kk > 0 || !fresh;
+              const uint64_t db = dense::k_major_descriptor(stages + (uint32_t)(s + stage) * stage_bytes) + 2u * (uint32_t)kk;
+              const uint32_t wa = tmem_d + kWeightColumn + (uint32_t)(s + stage) * 32u + 8u * (uint32_t)kk;
+              if constexpr (P == 3) {
+                const uint32_t small = d + kMostRows<3>;
+                mma_weights(small, wa, db + 2 * plane, a.instruction, more);
+                mma_weights(small, wa, db + plane, a.instruction, 1u);
+              } else if constexpr (P == 2) {
+                mma_weights(d, wa, db + plane, a.instruction, more);
+              }
+              mma_weights(d, wa, db, a.instruction, P == 2 ? 1u : more);
+            };
+            const bool ends_here = last && s + 2 >= here;  // the tile's last stage is one of these
+#pragma unroll
+            for (int stage = 0; stage < 2; ++stage) {
+              if (stage == 1 && !both) break;
+              if (ends_here && s + stage == here - 1) {
+                for (int kk = 0; kk < last_steps; ++kk) products(stage, kk);
+              } else {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) products(stage, kk);
+              }
+              commit(&empty[s + stage]);
+            }
+            if (ends && s + 2 >= here) commit(&accumulated[buffer]);
           }
-          commit(&empty[s]);
-          if (last || in_chunk == kChunk<P> - 1) commit(&accumulated[buffer]);
+          __syncwarp();
         }
-        __syncwarp();
-        if (last || in_chunk == kChunk<P> - 1) ++chunk;
-        in_chunk = last || in_chunk == kChunk<P> - 1 ? 0 : in_chunk + 1;
-        kb = last ? 0 : kb + 1;
+        if (ends) ++chunk;
       }
     }
     if (tries == 0) give_up();
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
         for (int u = 0; u < kUnits; ++u)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[u][i] = 0.0f;
-        const int chunks = (a.k_blocks + kChunk<P> - 1) / kChunk<P>;
+        const int chunks = tile_boxes;
         bool there = true;
         for (int c = 0; c < chunks && (there = wait_for(chunk)); ++c, ++chunk) {
           const uint32_t acc = lanes + (chunk & 1u) * (kWeightColumn / 2);
@@ -359,9 +362,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
       uint8_t b[4];
     };
     auto scales_of = [&](int tile) { return a.scales + (int64_t)min(place(min(tile, a.tiles - 1)).mb * kTileM + at, a.outputs - 1) * a.blocks; };
-    auto fetch_scales = [&](const uint8_t *from, int q, uint32_t it) {
+    auto fetch_scales = [&](const uint8_t *from, int q) {
       Scales r;
-      const int first = 2 * (q * kBoxStages + (int)((it + (uint32_t)set) & 1u));
+      const int first = 2 * (q * kBoxStages + set);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int block = first + 4 * (j >> 1) + (j & 1);
@@ -370,22 +373,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
       }
       return r;
     };
-    uint32_t it = 0, box = 0;
+    uint32_t box = 0, phases = 0xfu;
     const uint8_t *from = scales_of((int)blockIdx.x);
-    Scales next = fetch_scales(from, 0, 0u);
+    Scales next = fetch_scales(from, 0);
     bool ok = true;
     for (int tile = (int)blockIdx.x; tile < a.tiles && ok; tile += (int)gridDim.x) {
       for (int q = 0; q < tile_boxes; ++q, ++box) {
         const Scales scales = next;
         const int stages_here = min(kBoxStages, a.k_blocks - q * kBoxStages);
         if (q + 1 == tile_boxes) from = scales_of(tile + (int)gridDim.x);
-        next = fetch_scales(from, q + 1 < tile_boxes ? q + 1 : 0, it + (uint32_t)stages_here);
+        next = fetch_scales(from, q + 1 < tile_boxes ? q + 1 : 0);
         const uint32_t b = box % kBoxes;
         if (!(ok = arrived(&box_full[b], (box / kBoxes) & 1u))) break;
         const uint32_t row = boxes + b * kBoxBytes + (uint32_t)at * 128u;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int in_box = (int)((it + (uint32_t)set) & 1u) + 2 * j;
+          const int in_box = set + 2 * j;
           if (in_box >= stages_here) break;
           const uint4 c0 = lds_b128(row + 16u * ((uint32_t)(2 * in_box) ^ ((uint32_t)at & 7u)));
           const uint4 c1 = lds_b128(row + 16u * ((uint32_t)(2 * in_box + 1) ^ ((uint32_t)at & 7u)));
@@ -393,8 +396,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
           uint32_t v[32];
           weights_of(c0.x, s0, number, v), weights_of(c0.y, s0, number, v + 4), weights_of(c0.z, s0, number, v + 8), weights_of(c0.w, s0, number, v + 12);
           weights_of(c1.x, s1, number, v + 16), weights_of(c1.y, s1, number, v + 20), weights_of(c1.z, s1, number, v + 24), weights_of(c1.w, s1, number, v + 28);
-          const uint32_t i = it + (uint32_t)in_box, s = i % kStages;
-          if (!(ok = arrived(&empty[s], ((i / kStages) & 1u) ^ 1u))) break;
+          const uint32_t s = (uint32_t)in_box;
+          if (!(ok = arrived(&empty[s], (phases >> s) & 1u))) break;
+          phases ^= 1u << s;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           tmem_store_32(weights + s * 32u, v);
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -402,7 +406,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) mx4_tile_kernel(const __grid_
           if (lane == 0) mbar_arrive(&full[s]);
         }
         if (!ok) break;
-        it += (uint32_t)stages_here;
         __syncwarp();
         if (lane == 0) mbar_arrive(&box_empty[b]);
       }
