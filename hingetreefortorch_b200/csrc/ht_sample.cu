@@ -6,18 +6,21 @@
 //     W = sum of w over what counts;  the class is the first i, in the order of classes, whose sum of w up to it is above u W
 //     log_prob = (s_i - m) / T - log W
 //
-// A border that moves by 1e-8 of W picks another class once in some thousand rows of many classes, so weights and sums are 64-bit numbers: the
-// decisions are those of the formulas.  The exponential is table-driven (P. T. P. Tang, Table-driven implementation of the exponential
-// function, ACM TOMS 15, 1989): 2^(k / 64) from a table and a polynomial of degree 4, 4e-14.
+// A border that moves by 1e-8 of W picks another class once in some thousand rows of many classes, so the decisions are those of 64-bit weights
+// and sums.  Where many classes are summed that is done in fp32 first, with a bound on what it is off by; where a border is nearer than that, once
+// more in 64 bits (EXACT).  That exponential is table-driven (P. T. P. Tang, Table-driven implementation of the exponential function, ACM TOMS 15,
+// 1989): 2^(k / 64) from a table and a polynomial of degree 4, 4e-14.
 //
-// A CTA takes a row, which stays in shared memory where it fits.  A prefix of the order is held as its last class, (score, class).  To find it nothing
-// is sorted but a list of up to 1024 classes around the place:
-//   top_k   every thread has the maxima of up to 4 parts of what it has read; the k-th largest of those, found by halving the range,
-//           bounds the k-th largest score from below, and not many more classes than k are above it
+// A row belongs to a CTA, or, where there are few rows, to a cluster of up to 8 that have a part each; it stays in shared memory where it fits.  A
+// prefix of the order is held as its last class, (score, class).  To find it nothing is sorted but a list of up to 1024 classes around the place:
+//   top_k   every thread has the maxima of 4 parts of what it has read; the one of about place k among those, found by halving the
+//           range, bounds the k-th largest score from below, and not many more classes than k are above it
 //   top_p   the same with the first 512 classes, where those hold enough
 //   else    classes are counted, or their weights summed roughly, by 2048 ranges of the score's bits; the range with the place in it is listed, or
 //           divided again, or is one score
-// No sum depends on the order of atomic additions: the same call gives the same bits.
+// What counts of a list is drawn from there; otherwise the row is summed in order, warp by warp, and one warp walks its part.
+// CTAs of a cluster exchange sums, counts, ranges and lists through each other's shared memory and all come to the same decisions.  No sum depends on
+// the order of atomic additions: the same call gives the same bits.
 #include "ht_dense.cuh"
 
 #include <math_constants.h>
@@ -31,7 +34,7 @@ using dense::load_plain;
 using dense::to_float;
 using tile::smem_addr;
 
-constexpr int kMostWarps = 32, kList = 1024, kBins = 2048, kParts = 4;
+constexpr int kMostWarps = 32, kMostCtas = 8, kList = 1024, kBins = 2048, kParts = 4, kCounted = 128;
 constexpr int kFirst = 512;          // classes that are listed first for top_p
 constexpr double kTail = -80.0;      // whatever the classes below exp() of this are, they do not weigh 2^-53 of the row together
 constexpr int kPassed = 0x7fffffff;  // no limit on the class among equal scores
@@ -47,7 +50,7 @@ struct Args {
   const int64_t *row_top_k;
   int64_t *drawn;
   float *log_probs;
-  uint32_t row_bytes;  // of shared memory for a row
+  uint32_t row_bytes;  // of shared memory for a row, or a CTA's part of it
 };
 
 // Larger for larger scores; both zeros are one score.
@@ -59,25 +62,25 @@ __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float
 
 struct Shared {
   double table[64];
-  double sums[kMostWarps];
-  float floats[kMostWarps];
-  uint32_t words[kMostWarps];
-  uint32_t count, low, high, bin;
-  double above;
-  int drawn;
-  float drawn_score;
+  double sums[2][kMostWarps][2];
+  uint32_t words[2][kMostWarps];
+  double cta_sums[2][kMostCtas][2];
+  uint32_t cta_words[2][kMostCtas];
+  uint32_t count, bin[2], bin_before, bin_after, bin_all;
+  uint32_t ranks[kCounted];
   union {
     uint64_t list[kList];
     uint32_t bins[kBins];
   };
 };
-
 constexpr size_t kRowAt = (sizeof(Shared) + 127) / 128 * 128;
+constexpr size_t kMergedBytes = sizeof(uint64_t) * kList;  // of a cluster's list in each of its CTAs, behind that
 
 // w = exp((s - m) / T) as 2^(a / 64) with a = (s - m) 64 / (T ln 2).
 struct Weight {
   double m, c;
   const double *table;
+  float m_, c_;  // of the rough one
   __device__ __forceinline__ double operator()(float s) const {
     const double a = ((double)s - m) * c;
     constexpr double kStep = 0.69314718055994531 / 64.0;
@@ -92,6 +95,15 @@ struct Weight {
     if (power < -1000) return __hiloint2double(__double2hiint(v) + ((power + 100) << 20), __double2loint(v)) * 0x1p-100;  // perhaps subnormal
     return __hiloint2double(__double2hiint(v) + (power << 20), __double2loint(v));
   }
+  // 2^y with y = (s - m) / (T ln 2) in fp32, off by kOff + |y| kOffPower of itself: the hardware's exponential 2^-22, the sum of a vector of them 3 2^-24;
+  // difference, factor and product 2^-24 of y each.
+  static constexpr double kOff = 4.3e-7, kOffPower = 1.25e-7;
+  __device__ __forceinline__ float rough(float s, float &y) const {
+    y = fmaxf((s - m_) * c_, -200.0f);  // (2^-200 is 0)
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return r;
+  }
 };
 
 // The last class of a prefix of the order.
@@ -101,90 +113,221 @@ struct Last {
   __device__ __forceinline__ bool holds(float s, int i) const { return s > score || (s == score && i <= at); }
 };
 
+// A sum and what it may be off by.
+struct Sum {
+  double value, off;
+};
+
 template <typename T>
 struct Row {
   static constexpr int kPer = 16 / (int)sizeof(T);
   const T *base;         // where the row's first 16 bytes start in memory
-  unsigned char *shared; // the same in shared memory, or null
-  int head, classes, vectors;
+  unsigned char *shared; // vector `first` in shared memory, or null
+  int head, classes, vectors, first;
   // Class j kPer - head + i is number i of vector j.
   __device__ __forceinline__ uint4 from_memory(int j) const {
-    const int first = j * kPer - head;
-    if (first >= 0 && first + kPer <= classes) return load_plain(reinterpret_cast<const uint4 *>(base) + j);
+    const int c = j * kPer - head;
+    if (c >= 0 && c + kPer <= classes) return load_plain(reinterpret_cast<const uint4 *>(base) + j);
     T t[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) t[i] = first + i >= 0 && first + i < classes ? base[j * (int64_t)kPer + i] : dense::from_float<T>(-CUDART_INF_F);
+    for (int i = 0; i < kPer; ++i) t[i] = c + i >= 0 && c + i < classes ? base[j * (int64_t)kPer + i] : dense::from_float<T>(-CUDART_INF_F);
     return *reinterpret_cast<const uint4 *>(t);
   }
+  __device__ __forceinline__ uint4 words(int j) const { return shared != nullptr ? reinterpret_cast<const uint4 *>(shared)[j - first] : from_memory(j); }
   __device__ __forceinline__ void values(int j, float (&v)[kPer]) const {
     T t[kPer];
-    *reinterpret_cast<uint4 *>(t) = shared != nullptr ? reinterpret_cast<const uint4 *>(shared)[j] : from_memory(j);
+    *reinterpret_cast<uint4 *>(t) = words(j);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) v[i] = to_float(t[i]);
   }
 };
 
+// The largest scores of 4 parts of what a thread reads, no number where there is one among them, and the least of all, word by word.
 template <typename T>
-struct Team {  // a CTA at work on a row
+struct Extremes {
+  uint32_t top[kParts], low;
+  __device__ __forceinline__ static uint32_t larger(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (sizeof(T) == 4)
+      asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (std::is_same<T, __half>::value)
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ static uint32_t smaller(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (sizeof(T) == 4)
+      asm("min.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (std::is_same<T, __half>::value)
+      asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static constexpr uint32_t kInfinity = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  static constexpr uint32_t kSigns = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+  __device__ __forceinline__ Extremes() : top{kInfinity | kSigns, kInfinity | kSigns, kInfinity | kSigns, kInfinity | kSigns}, low(kInfinity) {}
+  __device__ __forceinline__ void add(const uint4 &q) {
+    top[0] = larger(top[0], q.x), top[1] = larger(top[1], q.y), top[2] = larger(top[2], q.z), top[3] = larger(top[3], q.w);
+    low = smaller(smaller(low, smaller(q.x, q.y)), smaller(q.z, q.w));
+  }
+  __device__ __forceinline__ float least(float (&part_max)[kParts]) const {
+    constexpr int kIn = 4 / (int)sizeof(T);
+    T t[kIn];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      *reinterpret_cast<uint32_t *>(t) = top[i];
+      part_max[i] = to_float(t[0]);
+      if (kIn == 2) asm("max.NaN.f32 %0, %1, %2;" : "=f"(part_max[i]) : "f"(part_max[i]), "f"(to_float(t[kIn - 1])));
+    }
+    *reinterpret_cast<uint32_t *>(t) = low;
+    return fminf(to_float(t[0]), to_float(t[kIn - 1]));
+  }
+};
+
+template <typename T, int C>
+struct Team {  // C CTAs at work on a row
   static constexpr int kPer = Row<T>::kPer;
   Shared &sh;
+  uint64_t *merged;  // the list of all CTAs
   Row<T> row;
-  int lane, warp, warps, first, last;  // of this warp: vectors first .. last - 1
+  int lane, warp, warps, rank, first, last;  // of this warp: vectors first .. last - 1
+  uint32_t turn = 0, far_turn = 0;  // of the buffers that reductions use one after the other, in a CTA and between them
 
-  // f(score, class) for every class of this warp's part of the row.
+  // What follows has seen what all threads of the team did before.
+  __device__ __forceinline__ void meet() const {
+    if constexpr (C > 1) {
+      __syncwarp();
+      dense::cluster_sync();
+    } else
+      __syncthreads();
+  }
+  template <typename V>
+  __device__ __forceinline__ V *of_cta(V *p, int r) const {
+    if constexpr (C == 1) return p;
+    uint64_t to;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(to) : "l"(p), "r"(r));
+    return reinterpret_cast<V *>(to);
+  }
+
+  // f(values, class of the first) for every vector of this warp's part of the row.
   template <typename F>
-  __device__ __forceinline__ void each(F &&f) const {
+  __device__ __forceinline__ void each_vector(F &&f) const {
 #pragma unroll 1
     for (int j = first + lane; j < last; j += 32) {
       float v[kPer];
       row.values(j, v);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) f(v[i], j * kPer - row.head + i);
+      f(v, j * kPer - row.head);
     }
   }
-  __device__ __forceinline__ double warp_sum(double v) const {
+  // f(score, class) for every class.
+  template <typename F>
+  __device__ __forceinline__ void each(F &&f) const {
+    each_vector([&](const float (&v)[kPer], int c) {
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+      for (int i = 0; i < kPer; ++i) f(v[i], c + i);
+    });
+  }
+  // Both numbers of all threads, summed or the larger of them, to all of them.
+  template <bool MAX>
+  __device__ __forceinline__ void reduce(double &a, double &b) {
+    auto with = [](double x, double y) { return MAX ? fmax(x, y) : x + y; };
+    auto in_warp = [&](double &v) {
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) v = with(v, __shfl_xor_sync(0xffffffffu, v, d));
+    };
+    in_warp(a), in_warp(b);
+    if (lane == 0) sh.sums[turn][warp][0] = a, sh.sums[turn][warp][1] = b;
+    __syncthreads();
+    a = lane < warps ? sh.sums[turn][lane][0] : MAX ? -CUDART_INF : 0.0;
+    b = lane < warps ? sh.sums[turn][lane][1] : MAX ? -CUDART_INF : 0.0;
+    in_warp(a), in_warp(b);
+    if constexpr (C > 1) {
+      if (warp == 0 && lane < C) {
+        double *to = of_cta(&sh.cta_sums[far_turn][rank][0], lane);
+        to[0] = a, to[1] = b;
+      }
+      meet();
+      a = sh.cta_sums[far_turn][0][0], b = sh.cta_sums[far_turn][0][1];
+#pragma unroll
+      for (int r = 1; r < C; ++r) a = with(a, sh.cta_sums[far_turn][r][0]), b = with(b, sh.cta_sums[far_turn][r][1]);
+      far_turn ^= 1u;
+    }
+    turn ^= 1u;
+  }
+  __device__ __forceinline__ double sum(double v) {
+    double none = 0.0;
+    reduce<false>(v, none);
     return v;
   }
-  // Of all threads, to all of them; two barriers.
-  __device__ __forceinline__ double sum(double v) const {
-    v = warp_sum(v);
+  // The least, or the sum, of all threads' numbers; of the CTA's alone with `alone`.
+  template <bool LEAST>
+  __device__ __forceinline__ uint32_t words(uint32_t v, bool alone = false) {
+    auto in_warp = [](uint32_t x) { return LEAST ? __reduce_min_sync(0xffffffffu, x) : __reduce_add_sync(0xffffffffu, x); };
+    v = in_warp(v);
+    if (lane == 0) sh.words[turn][warp] = v;
     __syncthreads();
-    if (lane == 0) sh.sums[warp] = v;
-    __syncthreads();
-    return warp_sum(lane < warps ? sh.sums[lane] : 0.0);
-  }
-  __device__ __forceinline__ float largest(float v) const {
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-    __syncthreads();
-    if (lane == 0) sh.floats[warp] = v;
-    __syncthreads();
-    v = lane < warps ? sh.floats[lane] : -CUDART_INF_F;
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    v = in_warp(lane < warps ? sh.words[turn][lane] : LEAST ? 0xffffffffu : 0u);
+    if (C > 1 && !alone) {
+      if (warp == 0 && lane < C) *of_cta(&sh.cta_words[far_turn][rank], lane) = v;
+      meet();
+      v = in_warp(lane < C ? sh.cta_words[far_turn][lane] : LEAST ? 0xffffffffu : 0u);
+      far_turn ^= 1u;
+    }
+    turn ^= 1u;
     return v;
-  }
-  __device__ __forceinline__ uint32_t least(uint32_t v) const {
-    v = __reduce_min_sync(0xffffffffu, v);
-    __syncthreads();
-    if (lane == 0) sh.words[warp] = v;
-    __syncthreads();
-    return __reduce_min_sync(0xffffffffu, lane < warps ? sh.words[lane] : 0xffffffffu);
-  }
-  __device__ __forceinline__ uint32_t total(uint32_t v) const {
-    v = __reduce_add_sync(0xffffffffu, v);
-    __syncthreads();
-    if (lane == 0) sh.words[warp] = v;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, lane < warps ? sh.words[lane] : 0u);
   }
 
-  // Lists the classes that `takes` says, as many as fit, and gives their number; a barrier follows the list.
+  // What a prefix weighs.
+  __device__ __forceinline__ Sum weigh(const Weight &w, const Last &end, bool exact) {
+    double value = 0.0, powers = 0.0;
+    if (exact) {
+      each([&](float s, int i) {
+        if (end.holds(s, i)) value += w(s);
+      });
+      return {sum(value), 0.0};
+    }
+    value = rough_sum(w, end, powers);
+    reduce<false>(value, powers);
+    return {value, 1.01 * (Weight::kOff * value + Weight::kOffPower * powers)};
+  }
+  // This thread's part of that; powers: the sum of w |y|.
+  __device__ __forceinline__ double rough_sum(const Weight &w, const Last &end, double &powers) const {
+    double value = 0.0;
+    float of_powers = 0.0f;
+    auto vector = [&](const float (&v)[kPer]) {
+      float e[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        float y;
+        e[i] = w.rough(v[i], y);
+        of_powers = fmaf(e[i], -y, of_powers);
+      }
+#pragma unroll
+      for (int d = kPer / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int i = 0; i < d; ++i) e[i] += e[i + d];
+      value += (double)e[0];
+    };
+    if (end.score == -CUDART_INF_F) {
+      each_vector([&](const float (&v)[kPer], int) { vector(v); });
+    } else {
+      each_vector([&](const float (&v)[kPer], int c) {
+        float held[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) held[i] = end.holds(v[i], c + i) ? v[i] : -CUDART_INF_F;
+        vector(held);
+      });
+    }
+    powers = (double)of_powers;
+    return value;
+  }
+
+  // Lists the classes that `takes` says, as many as fit, and gives their number; in `merged` for all CTAs.
   template <typename F>
-  __device__ __forceinline__ uint32_t list(F &&takes) const {
-    __syncthreads();
+  __device__ __forceinline__ uint32_t list(F &&takes) {
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     each([&](float s, int i) {
@@ -194,69 +337,121 @@ struct Team {  // a CTA at work on a row
       }
     });
     __syncthreads();
-    return sh.count;
+    uint32_t n = sh.count;
+    if constexpr (C > 1) {
+      if (warp == 0 && lane < C) *of_cta(&sh.cta_words[far_turn][rank], lane) = n;
+      meet();
+      n = 0;
+      for (int r = 0; r < C; ++r) n += sh.cta_words[far_turn][r];
+      if (n <= (uint32_t)kList) {
+        uint32_t at = 0;
+        for (int r = 0; r < C; ++r) {
+          const uint32_t of_r = sh.cta_words[far_turn][r];
+          const uint64_t *from = of_cta(sh.list, r);
+          for (uint32_t i = threadIdx.x; i < of_r; i += blockDim.x) merged[at + i] = from[i];
+          at += of_r;
+        }
+      }
+      far_turn ^= 1u;
+      meet();
+    }
+    return n;
   }
-  // Sorts the list, the largest first: bitonic, as many places as the next power of two.
-  __device__ __forceinline__ void sort(int n) const {
-    int places = 2;
+  // Sorts the list, the largest first: by counting what is larger, or bitonic with as many places as the next power of two.
+  __device__ __forceinline__ void sort(int n) {
+    int places = 32;
     while (places < n) places *= 2;
-    for (int i = n + (int)threadIdx.x; i < places; i += (int)blockDim.x) sh.list[i] = 0;
+    if (places <= kCounted && places <= (int)blockDim.x) {
+      const int e = (int)threadIdx.x & (places - 1), part = (int)threadIdx.x / places, parts = (int)blockDim.x / places;
+      if (threadIdx.x < kCounted) sh.ranks[threadIdx.x] = 0;
+      __syncthreads();
+      const uint64_t own = e < n ? merged[e] : 0;
+      uint32_t larger = 0;
+      if (part < parts)
+        for (int i = part; i < n; i += parts) larger += merged[i] > own ? 1u : 0u;
+      if (e < n && larger > 0u) atomicAdd(&sh.ranks[e], larger);
+      __syncthreads();
+      if (part == 0 && e < n) merged[sh.ranks[e]] = own;
+      __syncthreads();
+      return;
+    }
+    for (int i = n + (int)threadIdx.x; i < places; i += (int)blockDim.x) merged[i] = 0;
     __syncthreads();
     for (int size = 2; size <= places; size *= 2)
       for (int d = size / 2; d >= 1; d /= 2) {
         for (int i = (int)threadIdx.x; i < places / 2; i += (int)blockDim.x) {
           const int a = 2 * i - (i & (d - 1)), b = a + d;
-          const uint64_t x = sh.list[a], y = sh.list[b];
-          if ((x < y) == ((a & size) == 0)) sh.list[a] = y, sh.list[b] = x;
+          const uint64_t x = merged[a], y = merged[b];
+          if ((x < y) == ((a & size) == 0)) merged[a] = y, merged[b] = x;
         }
         __syncthreads();
       }
   }
   __device__ __forceinline__ Last listed(int i) const {
-    const uint64_t e = sh.list[i];
+    const uint64_t e = merged[i];
     return {score_of((uint32_t)(e >> 32)), (int)(0xffffffffu - (uint32_t)e)};
   }
-  // Of the sorted list's first n, with `before` of weight ahead of them: how many start below `target`, and the weight of all n in *weight.
-  __device__ __forceinline__ int places_below(int n, const Weight &w, double before, double target, double *weight) const {
-    // every thread has neighbours: kList / threads of them at the most
-    const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x, from = (int)threadIdx.x * per, to = min(from + per, n);
+  // weight(i) for the list's first n, summed in order: this thread's neighbours from .. to - 1 and what is ahead of them; gives the whole.
+  template <typename F>
+  __device__ __forceinline__ double scan(int n, F &&weight, int &from, int &to, double &ahead) {
+    const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;  // kList / threads at the most
+    from = min((int)threadIdx.x * per, n), to = min(from + per, n);
     double own = 0.0;
-    for (int i = from; i < to; ++i) own += w(listed(i).score);
+    for (int i = from; i < to; ++i) own += weight(i);
     double upto = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double t = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += t;
     }
+    if (lane == 31) sh.sums[turn][warp][0] = upto;
     __syncthreads();
-    if (lane == 31) sh.sums[warp] = upto;
-    __syncthreads();
-    double ahead = 0.0, all = 0.0;
+    double before = 0.0, all = 0.0;
     for (int i = 0; i < warps; ++i) {
-      if (i < warp) ahead += sh.sums[i];
-      all += sh.sums[i];
+      if (i == warp) before = all;
+      all += sh.sums[turn][i][0];
     }
-    *weight = all;
-    double at = before + ahead + (upto - own);
+    turn ^= 1u;
+    ahead = before + (upto - own);
+    return all;
+  }
+  // Of the sorted list's first n, with `before` of weight ahead of them: how many start below `target`, whose own error is `off`: -1 where that
+  // makes a difference.
+  __device__ __forceinline__ int places_below(int n, const Weight &w, double before, double target, double off, double *whole = nullptr) {
+    int from, to;
+    double at;
+    const double all = scan(n, [&](int i) { return w(listed(i).score); }, from, to, at);
+    if (whole != nullptr) *whole = all;
+    at += before;
     uint32_t count = 0;
     for (int i = from; i < to; ++i) {
-      count += at < target ? 1u : 0u;
+      count += (at < target - off ? 1u : 0u) + (at < target + off ? 0x10000u : 0u);
       at += w(listed(i).score);
     }
-    return (int)total(count);
+    count = words<false>(count, true);
+    return (count & 0xffffu) == count >> 16 ? (int)(count >> 16) : -1;
   }
 
   // The class of the n-th (from 1) of those with this score, in the order of classes.
-  __device__ __forceinline__ int nth_of(float score, uint32_t n) const {
+  __device__ __forceinline__ int nth_of(float score, uint32_t n) {
     uint32_t own = 0;
     each([&](float s, int) { own += s == score ? 1u : 0u; });
     own = __reduce_add_sync(0xffffffffu, own);
+    if (lane == 0) sh.words[turn][warp] = own;
     __syncthreads();
-    if (lane == 0) sh.words[warp] = own;
-    if (threadIdx.x == 0) sh.drawn = kPassed;
-    __syncthreads();
-    uint32_t ahead = 0;
-    for (int i = 0; i < warp; ++i) ahead += sh.words[i];
+    uint32_t ahead = 0, of_cta_all = 0;
+    for (int i = 0; i < warps; ++i) {
+      if (i == warp) ahead = of_cta_all;
+      of_cta_all += sh.words[turn][i];
+    }
+    if constexpr (C > 1) {
+      if (warp == 0 && lane < C) *of_cta(&sh.cta_words[far_turn][rank], lane) = of_cta_all;
+      meet();
+      for (int r = 0; r < rank; ++r) ahead += sh.cta_words[far_turn][r];
+      far_turn ^= 1u;
+    }
+    turn ^= 1u;
+    uint32_t found = 0xffffffffu;
     if (ahead < n && n <= ahead + own) {
       for (int j0 = first; j0 < last; j0 += 32) {
         const int j = j0 + lane;
@@ -277,133 +472,162 @@ struct Team {  // a CTA at work on a row
         if (at < n && n <= at + here) {
 #pragma unroll
           for (int i = 0; i < kPer; ++i)
-            if (v[i] == score && ++at == n) sh.drawn = j * kPer - row.head + i;
+            if (v[i] == score && ++at == n) found = (uint32_t)(j * kPer - row.head + i);
         }
         ahead += __shfl_sync(0xffffffffu, upto, 31);
         if (ahead >= n) break;
       }
     }
-    __syncthreads();
-    return sh.drawn;
+    return (int)words<true>(found);
   }
 
   // The last class of the shortest prefix that reaches `target`, counted (WEIGHTS false) or weighed, among the classes that `base` holds and
-  // whose keys are in [low, high]; all others of base are above and are `above` together.  For weights `all` is about what base weighs.
+  // whose keys are in [low, high]; all others of base are above.  For weights `all` is about what base weighs; `off` is target's error, and *sure
+  // is false where that, or what is summed roughly (but with `exact`), makes a difference.
   template <bool WEIGHTS>
-  __device__ __forceinline__ Last narrow(const Weight &w, const Last &base, uint32_t low, uint32_t high, double above, double target, double all) const {
+  __device__ __forceinline__ Last narrow(const Weight &w, const Last &base, uint32_t low, uint32_t high, double target, double off, double all, bool exact, bool *sure) {
+    double above = 0.0;
+    bool by_score = true;
     for (;;) {
-      // by ranges of the key, highest first
+      // By ranges, highest first: of the score at first, over which scores are spread more evenly, and then of its key.  Weights are counted in units
+      // of 2^-31 of what there is.
       const uint32_t width = high - low;
-      int shift = 0;
-      while ((width >> shift) >= (uint32_t)kBins) ++shift;
+      const int shift = max(0, 21 - (int)__clz((int)width));
+      const float slope = by_score ? ((float)kBins - 1.0f) / (w.m_ - score_of(low)) : 0.0f;
+      const uint32_t last_bin = by_score ? (uint32_t)kBins - 1u : width >> shift;
+      auto range_of = [&](float s, uint32_t key) { return by_score ? min((uint32_t)((w.m_ - s) * slope), last_bin) : (high - key) >> shift; };
       const double scale = 2147483648.0 / all;
-      __syncthreads();
+      const float scale_ = (float)scale;
+      meet();
       for (int i = (int)threadIdx.x; i < kBins; i += (int)blockDim.x) sh.bins[i] = 0;
       __syncthreads();
       each([&](float s, int i) {
         const uint32_t key = key_of(s);
-        if (key >= low && key <= high && base.holds(s, i)) atomicAdd(&sh.bins[(high - key) >> shift], WEIGHTS ? (uint32_t)(w(s) * scale + 0.5) : 1u);
+        if (key >= low && key <= high && base.holds(s, i)) {
+          float y;
+          atomicAdd(&sh.bins[range_of(s, key)], WEIGHTS ? (uint32_t)(w.rough(s, y) * scale_ + 0.5f) : 1u);
+        }
       });
-      __syncthreads();
-      // the range in which the sum reaches the target: warps take neighbouring ranges
-      const uint32_t wanted = WEIGHTS ? (uint32_t)fmin(fmax((target - above) * scale, 1.0), 2147483647.0) : (uint32_t)(target - above);
-      if (warp == 0) {
-        uint32_t own = 0;
-        for (int i = 0; i < kBins / 32; ++i) own += sh.bins[lane * (kBins / 32) + i];
-        uint32_t upto = own;
+      meet();
+      const uint32_t *bins = sh.bins;
+      if constexpr (C > 1) {  // of all CTAs together
+        uint32_t *const together = reinterpret_cast<uint32_t *>(merged);
+        for (int i = (int)threadIdx.x; i < kBins; i += (int)blockDim.x) {
+          uint32_t v = 0;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const uint32_t t = __shfl_up_sync(0xffffffffu, upto, d);
-          if (lane >= d) upto += t;
+          for (int r = 0; r < C; ++r) v += of_cta(sh.bins, r)[i];
+          together[i] = v;
         }
-        uint32_t at = upto - own;
-        if (at < wanted && wanted <= upto) {
-          int b = lane * (kBins / 32);
-          while (at + sh.bins[b] < wanted) at += sh.bins[b++];
-          sh.bin = (uint32_t)b;
-        }
-        if (lane == 31 && upto < wanted) sh.bin = width >> shift;  // (rounding: the last)
+        bins = together;
+        meet();  // (the CTAs' own have been read: their place is the list's)
       }
+      // The ranges between which the sum reaches the target: rough weights are off by 2^-16 of themselves (|y| is below 116 here) and half a unit.
+      const uint32_t slack = WEIGHTS ? 32768u + (uint32_t)row.classes / 2u + 2u : 0u;
+      const uint32_t wanted = WEIGHTS ? (uint32_t)fmin(fmax((target - above) * scale, 1.0), 2147483647.0) : (uint32_t)(target - above);
+      const uint32_t wanted_low = wanted > slack ? wanted - slack : 1u, wanted_high = wanted + slack;
+      const int per = kBins / (int)blockDim.x;  // of a thread
+      uint32_t own = 0;
+      for (int i = 0; i < per; ++i) own += bins[(int)threadIdx.x * per + i];
+      uint32_t upto = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += t;
+      }
+      if (lane == 31) sh.words[turn][warp] = upto;
+      if (threadIdx.x == 0) sh.bin[0] = sh.bin[1] = last_bin, sh.bin_before = sh.bin_after = 0;
       __syncthreads();
-      uint32_t bin = sh.bin;
-      const uint32_t last_bin = width >> shift;
-      int moved = 0;  // the way that the range has moved since: it does not come back
-      double over;
-      uint32_t n;
-      Last end;
-      for (;;) {  // (a rough sum may be one range off)
-        const uint32_t top = high - (bin << shift), bottom = top - low < (1u << shift) ? low : top - (1u << shift) + 1u;
-        double mine = 0.0;
-        uint32_t least_key = 0xffffffffu, least_gap = 0xffffffffu;  // of the range: its keys reach from `lowest` to `highest`
-        n = list([&](float s, int i) {
-          const uint32_t key = key_of(s);
-          if (key < bottom || key > high || !base.holds(s, i)) return false;
-          if (key > top) {
-            mine += WEIGHTS ? w(s) : 1.0;
-            return false;
-          }
-          least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
-          return true;
-        });
-        over = above + sum(mine);
-        if (bin > 0u && moved <= 0 && ((WEIGHTS && over >= target) || (n == 0u && moved < 0))) {
-          --bin;
-          moved = -1;
-          continue;
-        }
-        const bool may_rise = bin < last_bin && moved >= 0;
-        if (n == 0u && may_rise) {
-          ++bin;
-          moved = 1;
-          continue;
-        }
-        if (n == 0u) return {score_of(bottom), kPassed};
-        const uint32_t lowest = least(least_key), highest = 0xffffffffu - least(least_gap);
-        if (n <= (uint32_t)kList) {
-          sort((int)n);
-          double weight;
-          int places;
-          if (WEIGHTS) {
-            places = places_below((int)n, w, over, target, &weight);
-            if (over + weight < target && may_rise) {
-              ++bin;
-              moved = 1;
-              continue;
-            }
-          } else {
-            places = (int)(target - over);
-          }
-          end = listed(max(min(places, (int)n), 1) - 1);
-          __syncthreads();
-          return end;
-        }
-        if (lowest == highest) {  // more of one score than the list holds
-          const float s = score_of(lowest);
-          const double one = WEIGHTS ? w(s) : 1.0, missing = target - over;
-          if (WEIGHTS && over + one * n < target && may_rise) {
-            ++bin;
-            moved = 1;
-            continue;
-          }
-          const uint32_t places = one * n <= missing ? n : (uint32_t)fmax(ceil(missing / one), 1.0);
-          // (among those that base holds the first ones are the first ones of all)
-          return {s, nth_of(s, places)};
-        }
-        low = lowest, high = highest;
-        above = over;
-        break;
+      uint32_t at = upto - own;
+      for (int i = 0; i < warp; ++i) at += sh.words[turn][i];
+      turn ^= 1u;
+      for (int i = 0; i < per; ++i) {
+        const uint32_t one = bins[(int)threadIdx.x * per + i];
+        if (at < wanted_low && wanted_low <= at + one) sh.bin[0] = (uint32_t)((int)threadIdx.x * per + i), sh.bin_before = at;
+        if (at < wanted_high && wanted_high <= at + one) sh.bin[1] = (uint32_t)((int)threadIdx.x * per + i), sh.bin_after = at + one;
+        at += one;
       }
+      if ((int)threadIdx.x == (int)blockDim.x - 1) sh.bin_all = at;
+      __syncthreads();
+      const uint32_t end_bin = sh.bin[1], first_bin = min(sh.bin[0], end_bin);
+      const double window = fmax((double)((sh.bin_after > sh.bin_before ? sh.bin_after : sh.bin_all) - sh.bin_before), 1.0) / scale;
+      double over = 0.0, powers = 0.0;
+      uint32_t least_key = 0xffffffffu, least_gap = 0xffffffffu;  // of the ranges: their keys reach from `lowest` to `highest`
+      const uint32_t n = list([&](float s, int i) {
+        const uint32_t key = key_of(s);
+        if (key < low || key > high || !base.holds(s, i)) return false;
+        const uint32_t range = range_of(s, key);
+        if (range < first_bin) {
+          if (WEIGHTS && !exact) {
+            float y;
+            const float one = w.rough(s, y);
+            over += (double)one, powers += (double)(one * -y);
+          } else {
+            over += WEIGHTS ? w(s) : 1.0;
+          }
+        }
+        if (range < first_bin || range > end_bin) return false;
+        least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
+        return true;
+      });
+      reduce<false>(over, powers);
+      if (WEIGHTS && !exact) off += 1.01 * (Weight::kOff * over + Weight::kOffPower * powers);
+      over += above;
+      if (WEIGHTS && over >= target - off) *sure = false;
+      if (n == 0u) return {score_of(low), kPassed};
+      if (n <= (uint32_t)kList) {
+        sort((int)n);
+        int places;
+        if (WEIGHTS) {
+          double weight;
+          places = places_below((int)n, w, over, target, off, &weight);
+          if (places < 0) *sure = false, places = places_below((int)n, w, over, target, 0.0);
+          if (over + weight < target + off && end_bin < last_bin) *sure = false;
+        } else {
+          places = (int)(target - over);
+        }
+        return listed(max(min(places, (int)n), 1) - 1);
+      }
+      const uint32_t lowest = words<true>(least_key), highest = 0xffffffffu - words<true>(least_gap);
+      if (lowest == highest) {  // more of one score than the list holds
+        const float s = score_of(lowest);
+        const double one = WEIGHTS ? w(s) : 1.0, missing = target - over;
+        auto places = [&](double left) { return one * n <= left ? n : (uint32_t)fmax(ceil(left / one), 1.0); };
+        if (WEIGHTS && (places(missing - off) != places(missing + off) || (over + one * n < target + off && end_bin < last_bin))) *sure = false;
+        // (among those that base holds the first ones are the first ones of all)
+        return {s, nth_of(s, places(missing))};
+      }
+      if (WEIGHTS) all = window;
+      if (!by_score && lowest == low && highest == high) {  // the rough weights do not tell: half of the range, by exact ones
+        const uint32_t middle = low + (high - low) / 2u;
+        double upper = 0.0;
+        each([&](float s, int i) {
+          const uint32_t key = key_of(s);
+          if (key > middle && key <= high && base.holds(s, i)) upper += WEIGHTS ? w(s) : 1.0;
+        });
+        upper = sum(upper);
+        if (over + upper < target) {
+          above = over + upper;
+          high = middle;
+        } else {
+          above = over;
+          low = middle + 1u;
+        }
+        continue;
+      }
+      low = lowest, high = highest;
+      above = over;
+      by_score = false;
     }
   }
 };
 
-template <typename T>
+template <typename T, int C>
 __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   extern __shared__ __align__(128) unsigned char sample_smem[];
   Shared &sh = *reinterpret_cast<Shared *>(sample_smem);
   constexpr int kPer = Row<T>::kPer;
   after_previous_kernel();
-  const int64_t r = blockIdx.x;
+  const int64_t r = blockIdx.x / C;
   const T *from = static_cast<const T *>(a.scores) + r * a.stride;
   Row<T> row;
   row.head = (int)((reinterpret_cast<uintptr_t>(from) & 15u) / sizeof(T));
@@ -412,20 +636,24 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   row.vectors = (int)(((int64_t)row.head + a.classes + kPer - 1) / kPer);
   row.shared = nullptr;
   const int warps = (int)blockDim.x / 32, warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
-  const int part = (row.vectors + warps - 1) / warps;
-  Team<T> team = {sh, row, lane, warp, warps, min(warp * part, row.vectors), min((warp + 1) * part, row.vectors)};
+  const int rank = C > 1 ? (int)(blockIdx.x % C) : 0;
+  const int part = (row.vectors + C * warps - 1) / (C * warps), ordinal = rank * warps + warp;
+  row.first = min(rank * warps * part, row.vectors);
+  Team<T, C> team = {sh, C > 1 ? reinterpret_cast<uint64_t *>(sample_smem + kRowAt) : sh.list, row, lane, warp, warps, rank, min(ordinal * part, row.vectors),
+                     min((ordinal + 1) * part, row.vectors)};
 
   // the row into shared memory, and its largest and least score
   if (a.row_bytes > 0) {
-    unsigned char *const to = sample_smem + kRowAt;
+    unsigned char *const to = sample_smem + kRowAt + (C > 1 ? kMergedBytes : 0);
     for (int j = team.first + lane; j < team.last; j += 32) {
       const int first = j * kPer - row.head;
       if (first >= 0 && first + kPer <= a.classes)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to) + 16u * (uint32_t)j), "l"(reinterpret_cast<const uint4 *>(row.base) + j) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(to) + 16u * (uint32_t)(j - row.first)),
+                     "l"(reinterpret_cast<const uint4 *>(row.base) + j)
+                     : "memory");
       else
-        reinterpret_cast<uint4 *>(to)[j] = row.from_memory(j);
+        reinterpret_cast<uint4 *>(to)[j - row.first] = row.from_memory(j);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
     team.row.shared = to;
   }
   if (threadIdx.x < 64) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
@@ -435,29 +663,27 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   const int64_t asked = a.row_top_k != nullptr ? load_plain(a.row_top_k + r) : a.top_k;
   const double u = (double)load_plain(a.uniform + r);
   const int top_k = asked > 0 && asked < a.classes ? (int)asked : a.classes;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (C > 1) team.meet();  // every CTA is there before another one writes to it
 
-  __syncthreads();  // (all of the row: no warp reads another's part, but the table)
-  float part_max[kParts], low = CUDART_INF_F;
-  bool number = true;
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) part_max[i] = -CUDART_INF_F;
+  // (no lane reads another's part of the row; the table comes before the first barrier)
+  float part_max[kParts];
+  Extremes<T> extremes;
 #pragma unroll 1
-  for (int j = team.first + lane; j < team.last; j += 32) {
-    float v[kPer];
-    team.row.values(j, v);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      float &top = part_max[i * kParts / kPer];
-      top = fmaxf(top, v[i]);
-      number &= v[i] == v[i];
-      if (v[i] > -CUDART_INF_F) low = fminf(low, v[i]);
-    }
-  }
-  const float m = team.largest(fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3])));
-  low = -team.largest(-low);
+  for (int j = team.first + lane; j < team.last; j += 32) extremes.add(team.row.words(j));
+  float low_ = extremes.least(part_max);
+  // (no number where one of them is none)
+  const float own_top = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+  const bool number = part_max[0] == part_max[0] && part_max[1] == part_max[1] && part_max[2] == part_max[2] && part_max[3] == part_max[3];
+  double top_ = number ? (double)own_top : CUDART_INF, minus_low = -(double)low_;
+  team.template reduce<true>(top_, minus_low);
+  const float m = (float)top_;
   const bool bounds = temperature >= 0.0 && temperature < CUDART_INF && top_p == top_p && min_p == min_p && u >= 0.0 && u <= 1.0;
-  if (__syncthreads_or(!number) || !bounds || !(m > -CUDART_INF_F && m < CUDART_INF_F)) {
-    if (threadIdx.x == 0) a.drawn[r] = -1, a.log_probs[r] = CUDART_NAN_F;
+  auto answer = [&](int64_t drawn, float log_prob) { a.drawn[r] = drawn, a.log_probs[r] = log_prob; };
+  // (a CTA of a cluster leaves when no other one reads from it any more)
+  if (!bounds || !(m > -CUDART_INF_F && m < CUDART_INF_F)) {
+    if (rank == 0 && threadIdx.x == 0) answer(-1, CUDART_NAN_F);
+    if constexpr (C > 1) team.meet();
     return;
   }
   if (temperature == 0.0 || top_k == 1 || top_p <= 0.0 || min_p > 1.0) {
@@ -465,23 +691,37 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     team.each([&](float s, int i) {
       if (s == m) at = min(at, (uint32_t)i);
     });
-    at = team.least(at);
-    if (threadIdx.x == 0) a.drawn[r] = (int64_t)at, a.log_probs[r] = 0.0f;
+    at = team.template words<true>(at);
+    if (rank == 0 && threadIdx.x == 0) answer((int64_t)at, 0.0f);
+    if constexpr (C > 1) team.meet();
     return;
   }
-  const Weight w = {(double)m, fmin(64.0 * 1.4426950408889634 / temperature, 1e300), sh.table};
+  float low = (float)-minus_low;  // the least finite score
+  if (low == -CUDART_INF_F && (top_k < a.classes || top_p < 1.0)) {
+    float least = CUDART_INF_F;
+    team.each([&](float s, int) { least = fminf(least, s > -CUDART_INF_F ? s : CUDART_INF_F); });
+    double none = -CUDART_INF;
+    minus_low = -(double)least;
+    team.template reduce<true>(minus_low, none);
+    low = (float)-minus_low;
+  }
+  const double factor = fmin(64.0 * 1.4426950408889634 / temperature, 1e300);
+  const Weight w = {(double)m, factor, sh.table, m, (float)fmin(factor / 64.0, 3e38)};
 
-  // what counts: up to `end`
-  const double lowest = fmax((double)low, (double)m + kTail * temperature);
+  const bool rough_fails = w.c_ < 1e-37f;  // a subnormal factor
+
+  // what counts: up to `end`, the first `held` of the sorted list where that is above 0
+  const double tail = fmax((double)low, (double)m + kTail * temperature);
+  const uint32_t high_key = key_of(m), low_key = min(key_of(tail > (double)low ? (float)tail : low), high_key);
   Last end = {-CUDART_INF_F, kPassed};
-  const uint32_t high_key = key_of(m);
-  const uint32_t low_key = min(key_of(lowest > (double)low ? (float)lowest : low), high_key);
+  int held = 0;
   if (top_k < a.classes || top_p < 1.0) {
     const bool by_count = top_k < a.classes;
-    const uint32_t wanted = (uint32_t)(by_count ? top_k : kFirst);
-    // a lower bound for the score of place `wanted`: at least so many of the parts' maxima are not below it
+    // A lower bound for the score of place `wanted`: at least so many of the parts' maxima are not below it.  Of a cluster each CTA has its share
+    // of them and a little more, and what is listed is counted.
+    const uint32_t wanted = (uint32_t)(by_count ? top_k : kFirst), share = C == 1 ? wanted : wanted / C + wanted / (2 * C) + 16u;
     uint32_t bound = 0;
-    if (wanted <= blockDim.x * kParts) {
+    if (share <= blockDim.x * kParts) {
       uint32_t keys[kParts], from_key = key_of(low), to_key = high_key;
 #pragma unroll
       for (int i = 0; i < kParts; ++i) keys[i] = key_of(part_max[i]);
@@ -490,131 +730,211 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
         uint32_t n = 0;
 #pragma unroll
         for (int i = 0; i < kParts; ++i) n += keys[i] >= middle ? 1u : 0u;
-        n = team.total(n);
-        if (n >= wanted) {
+        n = team.template words<false>(n, true);
+        if (n >= share) {
           from_key = middle;
-          if (n <= wanted + wanted / 16u) break;
+          if (n <= share + share / 8u) break;
         } else {
           to_key = middle - 1u;
         }
       }
       bound = from_key;
+      if constexpr (C > 1) bound = 0xffffffffu - team.template words<true>(0xffffffffu - bound);
     }
-    const uint32_t n = bound > 0u ? team.list([&](float s, int) { return key_of(s) >= bound; }) : 0xffffffffu;
-    if (n <= (uint32_t)kList) team.sort((int)n);
-    double all = 0.0;
-    bool done = false;
-    if (by_count) {
-      if (n <= (uint32_t)kList) {
-        end = team.listed(min(top_k, (int)n) - 1);
-        if (top_p < 1.0) {
-          const int held = min(top_k, (int)n);
-          team.places_below(held, w, 0.0, 0.0, &all);
-          double ignored;
-          end = team.listed(max(team.places_below(held, w, 0.0, top_p * all, &ignored), 1) - 1);
-        }
-        done = true;
-        __syncthreads();
+    const float bound_score = score_of(bound);
+    uint32_t n = bound > 0u && wanted <= kList * 3u / 4u ? team.list([&](float s, int) { return s >= bound_score; }) : 0xffffffffu;
+    // (whether all is listed that there is, or the list goes as far as place `wanted`)
+    const bool whole = bound == key_of(low);
+    if (by_count && (n < wanted || (C > 1 && n == 0xffffffffu)) && !whole) n = 0xffffffffu, bound = 0;
+    if (n <= (uint32_t)kList) {
+      team.sort((int)n);
+      held = by_count ? min(top_k, (int)n) : (int)n;
+    }
+    Sum all = {0.0, 0.0};
+    if (by_count && held == 0) {
+      const uint32_t from_key = max(bound, key_of(low));
+      double inside = 0.0;
+      team.each([&](float s, int) { inside += key_of(s) >= from_key ? 1.0 : 0.0; });
+      inside = team.sum(inside);
+      bool sure = true;
+      if (inside >= (double)top_k) end = team.template narrow<false>(w, end, from_key, high_key, (double)top_k, 0.0, 1.0, true, &sure);
+    }
+    if (top_p < 1.0) {
+      if (by_count && held > 0) {
+        team.places_below(held, w, 0.0, 0.0, 0.0, &all.value);
+        held = max(team.places_below(held, w, 0.0, top_p * all.value, 0.0), 1);
       } else {
-        const uint32_t from_key = max(bound, key_of(low));
-        double inside = 0.0;
-        team.each([&](float s, int) { inside += key_of(s) >= from_key ? 1.0 : 0.0; });
-        inside = team.sum(inside);
-        if (inside >= (double)top_k) end = team.template narrow<false>(w, end, from_key, high_key, 0.0, (double)top_k, 1.0);
+        bool exact = rough_fails;
+        int places = -1;
+        for (;;) {
+          all = team.weigh(w, end, exact);
+          double weight = 0.0;
+          if (held > 0) places = team.places_below(held, w, 0.0, top_p * all.value, top_p * all.off, &weight);
+          if (held > 0 && weight < top_p * (all.value + all.off) && !whole) held = 0;  // not enough of them, or perhaps not
+          if (held > 0 && places >= 0) {
+            held = max(places, 1);
+            break;
+          }
+          if (held == 0) {
+            bool sure = true;
+            const Last last = team.template narrow<true>(w, end, max(low_key, key_of(end.score)), high_key, top_p * all.value, top_p * all.off, all.value, exact, &sure);
+            if (sure || exact) {
+              end = last;
+              break;
+            }
+          }
+          exact = true;
+        }
       }
     }
-    if (!done && top_p < 1.0) {
-      double own = 0.0;
-      team.each([&](float s, int i) {
-        if (end.holds(s, i)) own += w(s);
-      });
-      all = team.sum(own);
-      if (!by_count && n <= (uint32_t)kList) {
-        double weight;
-        const int places = team.places_below((int)n, w, 0.0, top_p * all, &weight);
-        if (weight >= top_p * all) {
-          end = team.listed(max(places, 1) - 1);
-          done = true;
-        }
-        __syncthreads();
-      }
-      if (!done) end = team.template narrow<true>(w, end, max(low_key, key_of(end.score)), high_key, 0.0, top_p * all, all);
+  }
+  if (min_p > 0.0) {
+    const float least = __double2float_ru(fmax((double)m + temperature * log(min_p), -3.4028234663852886e38));  // the lowest score that weighs so much
+    if (least > end.score) end = {least, kPassed};
+    if (held > 0) {
+      uint32_t n = 0;
+      for (int i = (int)threadIdx.x; i < held; i += (int)blockDim.x) n += team.listed(i).score >= least ? 1u : 0u;
+      held = (int)max(team.template words<false>(n, true), 1u);
     }
   }
 
-  // the draw: the sums of the warps' parts, then along one part
-  auto weight = [&](float s, int i) {
-    if (!end.holds(s, i)) return 0.0;
-    const double v = w(s);
-    return v >= min_p ? v : 0.0;
-  };
-  double own = 0.0;
-  team.each([&](float s, int i) { own += weight(s, i); });
-  own = team.warp_sum(own);
-  __syncthreads();
-  if (lane == 0) sh.sums[warp] = own;
-  __syncthreads();
-  double all = 0.0, ahead = 0.0;
-  int place = -1;
-  for (int i = 0; i < warps; ++i) all += sh.sums[i];
-  const double target = u * all;
-  for (int i = 0; i < warps; ++i) {  // the first part that ends above the target, or (u = 1, rounding) the last that weighs anything
-    const double s = sh.sums[i];
-    if (s > 0.0) {
-      if (place >= 0) ahead += sh.sums[place];
-      place = i;
-      if (ahead + s > target) break;
+  if (held > 0) {  // drawn from the list: in the order of classes
+    for (int i = (int)threadIdx.x; i < held; i += (int)blockDim.x) team.merged[i] = team.merged[i] << 32 | team.merged[i] >> 32;
+    __syncthreads();
+    team.sort(held);
+    auto score = [&](int i) { return score_of((uint32_t)team.merged[i]); };
+    int first, last;
+    double at;
+    const double all = team.scan(held, [&](int i) { return w(score(i)); }, first, last, at), target = u * all;
+    // the first that passes the target, or the last that weighs anything
+    uint32_t passing = 0xffffffffu, some = 0;
+    for (int i = first; i < last; ++i) {
+      const double one = w(score(i));
+      at += one;
+      if (one > 0.0) {
+        some = (uint32_t)i + 1u;
+        if (at > target) passing = min(passing, (uint32_t)i);
+      }
     }
+    passing = team.template words<true>(passing, true);
+    if (passing == 0xffffffffu) passing = 0xffffffffu - team.template words<true>(0xffffffffu - some, true) - 1u;
+    if (rank == 0 && threadIdx.x == 0)
+      answer((int64_t)(0xffffffffu - (uint32_t)(team.merged[passing] >> 32)), (float)(((double)score((int)passing) - (double)m) / temperature - log(all)));
+    if constexpr (C > 1) team.meet();
+    return;
   }
-  if (warp == place) {
-    int found = -1;
-    float found_score = 0.0f;
-    for (int j0 = team.first; j0 < team.last; j0 += 32) {
-      const int j = j0 + lane;
-      float v[kPer];
-      double here = 0.0;
-      if (j < team.last) {
-        team.row.values(j, v);
+
+  // the sums of the warps' parts, then along one part
+  for (bool exact = rough_fails;; exact = true) {
+    double own = 0.0, powers = 0.0;
+    if (exact)
+      team.each([&](float s, int i) {
+        if (end.holds(s, i)) own += w(s);
+      });
+    else
+      own = team.rough_sum(w, end, powers);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) here += weight(v[i], j * kPer - row.head + i);
+    for (int d = 16; d >= 1; d >>= 1) own += __shfl_xor_sync(0xffffffffu, own, d), powers += __shfl_xor_sync(0xffffffffu, powers, d);
+    const uint32_t turn = team.turn;
+    if (lane == 0) sh.sums[turn][warp][0] = own, sh.sums[turn][warp][1] = powers;
+    __syncthreads();
+    double all = 0.0, all_powers = 0.0, of_cta = 0.0, of_cta_powers = 0.0, ahead_of_cta = 0.0;
+    for (int i = 0; i < warps; ++i) of_cta += sh.sums[turn][i][0], of_cta_powers += sh.sums[turn][i][1];
+    int at_cta = 0;
+    double target;
+    if constexpr (C > 1) {
+      if (warp == 0 && lane < C) {
+        double *to = team.of_cta(&sh.cta_sums[team.far_turn][rank][0], lane);
+        to[0] = of_cta, to[1] = of_cta_powers;
       }
-      double upto = here;
+      team.meet();
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double t = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += t;
+      for (int i = 0; i < C; ++i) all += sh.cta_sums[team.far_turn][i][0], all_powers += sh.cta_sums[team.far_turn][i][1];
+      target = u * all;
+      double ahead = 0.0;
+      at_cta = -1;
+      for (int i = 0; i < C; ++i) {  // as below
+        const double s = sh.cta_sums[team.far_turn][i][0];
+        if (s > 0.0) {
+          if (at_cta >= 0) ahead += sh.cta_sums[team.far_turn][at_cta][0];
+          at_cta = i;
+          if (ahead + s > target) break;
+        }
       }
-      const uint32_t reached = __ballot_sync(0xffffffffu, ahead + upto > target), some = __ballot_sync(0xffffffffu, here > 0.0);
-      // the lane in which the sum passes the target, or (lanes' sums may differ in their last bit) the last one so far that weighs anything
-      const uint32_t passing = reached & some;
-      const int at = passing != 0u ? __ffs((int)passing) - 1 : some != 0u ? 31 - __clz((int)some) : -1;
-      if (lane == at) {
-        double sum = ahead + (upto - here);
-        bool passed = false;
+      ahead_of_cta = ahead;
+      team.far_turn ^= 1u;
+    } else {
+      all = of_cta, all_powers = of_cta_powers;
+      target = u * all;
+    }
+    team.turn ^= 1u;
+    const double off = exact ? 0.0 : 2.02 * (Weight::kOff * all + Weight::kOffPower * all_powers);  // of a sum and of the target together
+    bool sure = true;
+    if (rank == at_cta) {
+      double ahead = ahead_of_cta;
+      int place = -1;
+      for (int i = 0; i < warps; ++i) {  // the first part that ends above the target, or (u = 1, rounding) the last that weighs anything
+        const double s = sh.sums[turn][i][0];
+        if (s > 0.0) {
+          if (place >= 0) ahead += sh.sums[turn][place][0];
+          place = i;
+          if (ahead + s > target) break;
+        }
+      }
+      // that part's vectors, the CTA's threads in order
+      const int part_first = min((rank * warps + place) * part, row.vectors), part_last = min(part_first + part, row.vectors);
+      auto weight = [&](float s, int i) {
+        float y;
+        return !end.holds(s, i) ? 0.0 : exact ? w(s) : (double)w.rough(s, y);
+      };
+      auto of_vector = [&](int i) {
+        float v[kPer];
+        team.row.values(part_first + i, v);
+        double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int c = j * kPer - row.head + i;
-          const double one = weight(v[i], c);
-          sum += one;
-          if (one > 0.0 && !passed) {
-            found = c;
-            found_score = v[i];
-            passed = sum > target;
+        for (int q = 0; q < kPer; ++q) sum += weight(v[q], (part_first + i) * kPer - row.head + q);
+        return sum;
+      };
+      int first, last;
+      double at;
+      team.scan(part_last - part_first, of_vector, first, last, at);
+      at += ahead;
+      // the first class that passes the target, or the last that weighs anything
+      uint32_t passing = 0xffffffffu, some = 0u;
+      float its_score = 0.0f, some_score = 0.0f;
+      bool near = false, some_near = false;
+      for (int i = first; i < last && passing == 0xffffffffu; ++i) {
+        float v[kPer];
+        team.row.values(part_first + i, v);
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          const int c = (part_first + i) * kPer - row.head + q;
+          const double one = weight(v[q], c);
+          if (one > 0.0 && passing == 0xffffffffu) {
+            const double before = at;
+            at += one;
+            some = (uint32_t)c + 1u, some_score = v[q], some_near = true;
+            if (at > target) passing = (uint32_t)c, its_score = v[q], near = target - before <= off || at - target <= off;
           }
         }
       }
-      if (at >= 0) {
-        found = __shfl_sync(0xffffffffu, found, at);
-        found_score = __shfl_sync(0xffffffffu, found_score, at);
+      const uint32_t drawn = team.template words<true>(passing, true);
+      if (drawn == 0xffffffffu) {
+        passing = 0xffffffffu - team.template words<true>(0xffffffffu - some, true) - 1u;
+        if (passing + 1u == some) its_score = some_score, near = some_near;
+        else passing = 0xffffffffu;
+      } else if (passing != drawn) {
+        passing = 0xffffffffu;
       }
-      if (reached != 0u && found >= 0) break;
-      ahead += __shfl_sync(0xffffffffu, upto, 31);
+      if (passing != 0xffffffffu) {
+        sure = exact || !near;
+        if (sure) answer((int64_t)passing, (float)(((double)its_score - (double)m) / temperature - log(all)));
+      }
     }
-    if (lane == 0) {
-      a.drawn[r] = found;
-      a.log_probs[r] = (float)(((double)found_score - (double)m) / temperature - log(all));
-    }
+    if (exact) break;
+    if (team.template words<true>(sure ? 1u : 0u) != 0u) break;
   }
+  if constexpr (C > 1) team.meet();
 }
 
 constexpr size_t kMostBytes = 227 * 1024;
@@ -630,15 +950,33 @@ int screen(const ht_sample_problem *p) {
   return HT_OK;
 }
 
+template <typename T, int C>
+int launch_of(Args a, int64_t vectors, cudaStream_t stream) {
+  const int64_t of_cta = (vectors + C - 1) / C;
+  // 1024 threads an SM, between the CTAs that it holds: as many as shared memory and the rows admit; two vectors a thread at the least
+  const size_t room = kMostBytes / (kRowAt + kMergedBytes + 16 * (size_t)of_cta + 1024);
+  const int64_t resident = std::max<int64_t>(1, std::min<int64_t>((int64_t)room, (a.rows * C + 147) / 148));
+  int threads = 1024;
+  while (threads > 128 && (threads * resident > 1024 || threads * 2 > of_cta)) threads /= 2;
+  const int warps = threads / 32;
+  const size_t row = 16 * (size_t)((vectors + C * warps - 1) / (C * warps) * warps), before = kRowAt + (C > 1 ? kMergedBytes : 0);
+  if (before + row <= kMostBytes) a.row_bytes = (uint32_t)row;
+  return dense::launch_next<sample_kernel<T, C>>(dim3((unsigned)(a.rows * C)), threads, before + a.row_bytes, kMostBytes, stream, C, a);
+}
+
 template <typename T>
 int launch(const ht_sample_problem &p, const void *scores, const float *uniform, int64_t *drawn, float *log_probs, cudaStream_t stream) {
   constexpr int kPer = Row<T>::kPer;
-  Args a = {scores, p.rows, p.stride, (int)p.classes, uniform, p.temperature, p.top_p, p.min_p, p.top_k, p.row_temperature, p.row_top_p, p.row_min_p,
-            p.row_top_k, drawn, log_probs, 0};
+  const Args a = {scores, p.rows, p.stride, (int)p.classes, uniform, p.temperature, p.top_p, p.min_p, p.top_k, p.row_temperature, p.row_top_p, p.row_min_p,
+                  p.row_top_k, drawn, log_probs, 0};
   const int64_t vectors = (p.classes + 2 * kPer - 2) / kPer;
-  if (kRowAt + 16 * (size_t)vectors <= kMostBytes) a.row_bytes = 16u * (uint32_t)vectors;
-  const int threads = vectors >= 4096 ? 1024 : vectors >= 2048 ? 512 : vectors >= 512 ? 256 : 128;
-  return dense::launch_next<sample_kernel<T>>(dim3((unsigned)p.rows), threads, kRowAt + a.row_bytes, kMostBytes, stream, 1, a);
+  // a cluster where the rows leave SMs idle and a CTA's part is still some vectors a thread
+  int ctas = p.rows <= 18 ? 8 : p.rows <= 37 ? 4 : p.rows <= 74 ? 2 : 1;
+  while (ctas > 1 && vectors < 256 * ctas) ctas /= 2;
+  return ctas == 8   ? launch_of<T, 8>(a, vectors, stream)
+         : ctas == 4 ? launch_of<T, 4>(a, vectors, stream)
+         : ctas == 2 ? launch_of<T, 2>(a, vectors, stream)
+                     : launch_of<T, 1>(a, vectors, stream);
 }
 
 }  // namespace

@@ -2,8 +2,9 @@
 
 Packing and unpacking are exact.  A score: a sum of K products loses at most (K + 16) 2^-23 of the sum of their magnitudes (the tensor core truncates when
 it adds), fp32 x is held to 2^-23 (three bf16 numbers), and the result is rounded to its type.  A drawn class is the formula's: weights and sums are held
-to some 1e-13, and no case here comes that near to a border but where both sides are exact; the logarithm of its share is a 64-bit number
-rounded to fp32, 2^-24 of it, and off by 1e-11 before.
+to some 1e-13 where that decides, and no case here comes that near to a border but where both sides are exact.  The logarithm of its share is rounded to
+fp32, 2^-24 of it, and what counts may have been summed in fp32: w = 2^y, y = (s - m) / (T ln 2), with the hardware's exponential (2^-22 of w), sums of
+8 (3 2^-24) and three roundings of y (3 2^-24 |y| ln 2 of w): 2^-22 + 3 2^-24 < 4.2e-7 and 3 2^-24 ln 2 < 1.25e-7 times the mean of |y|.
 """
 import math
 
@@ -212,7 +213,7 @@ def draw(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     import numpy as np
     s, u = scores.double().cpu().numpy(), uniform.double().cpu().numpy()
     rows = [v.double().cpu().numpy() if torch.is_tensor(v) else np.full(len(u), float(v)) for v in (temperature, top_k, top_p, min_p)]
-    classes, logs = np.full(len(u), -1, dtype=np.int64), np.full(len(u), np.nan)
+    classes, logs, powers = np.full(len(u), -1, dtype=np.int64), np.full(len(u), np.nan), np.zeros(len(u))
     for r, (t, k, p, least) in enumerate(zip(*rows)):
         v = s[r]
         if np.isnan(v).any() or not np.isfinite(v.max()) or not (0 <= t < math.inf) or not 0 <= u[r] <= 1 or p != p or least != least:
@@ -235,19 +236,27 @@ def draw(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             at = int(np.flatnonzero(weight > 0)[-1])
         # (not the logarithm of the weight, which may be a subnormal number of few bits)
         classes[r], logs[r] = held[at], (v[held[at]] - v.max()) / (t if t > 0 else 1.0) - np.log(upto[-1])
-    return torch.from_numpy(classes), torch.from_numpy(logs)
+        powers[r] = (weight * np.abs(v[held] - v.max()))[weight > 0].sum() / (t if t > 0 else 1.0) / math.log(2) / upto[-1]
+    return torch.from_numpy(classes), torch.from_numpy(logs), torch.from_numpy(powers)
 
 
 def check_draw(scores, uniform, **bounds):
     got, logs = F.sample_classes(scores, uniform, **bounds)
-    want, exact = draw(scores, uniform, **bounds)
+    want, exact, powers = draw(scores, uniform, **bounds)
     assert got.dtype == torch.int64 and logs.dtype == torch.float32
     wrong = (got.cpu() != want).nonzero()[:, 0]
     assert len(wrong) == 0, [(int(r), int(got[r]), int(want[r])) for r in wrong[:5]]
     logs = logs.cpu().double()
     assert torch.equal(torch.isnan(logs), torch.isnan(exact))
-    off = (logs - exact).abs() / (2.0 ** -24 * exact.abs() + 1e-11)
+    off = (logs - exact).abs() / (2.0 ** -24 * exact.abs() + 4.3e-7 + 1.25e-7 * powers)
     assert not (off > 1).any(), off.max()
+    # the same rows in larger batches, where fewer CTAs share a row
+    for times in (30, 80):
+        if scores.dim() == 2 and 0 < len(scores) < times and not any(torch.is_tensor(v) for v in bounds.values()):
+            k = -(-times // len(scores))
+            more, more_logs = F.sample_classes(scores.repeat(k, 1), uniform.repeat(k), **bounds)
+            assert torch.equal(more, got.repeat(k))
+            assert not ((more_logs.cpu().double() - exact.repeat(k)).abs() > (2.0 ** -24 * exact.abs() + 4.3e-7 + 1.25e-7 * powers).repeat(k)).any()
     return got, logs
 
 
