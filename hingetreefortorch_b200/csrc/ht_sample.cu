@@ -44,13 +44,33 @@ struct Args {
   int64_t rows, stride;
   int classes;
   const float *uniform;
-  double temperature, top_p, min_p;
+  double temperature, factor, top_p, min_p;  // factor: 64 / (T ln 2)
   int64_t top_k;
   const float *row_temperature, *row_top_p, *row_min_p;
   const int64_t *row_top_k;
   int64_t *drawn;
   float *log_probs;
   uint32_t row_bytes;  // of shared memory for a row, or a CTA's part of it
+};
+
+// 2^(k / 64), rounded to nearest.
+__device__ const double kPowers[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
 };
 
 // Larger for larger scores; both zeros are one score.
@@ -60,12 +80,12 @@ __device__ __forceinline__ uint32_t key_of(float s) {
 }
 __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) != 0u ? key & 0x7fffffffu : ~key); }
 
-struct Shared {
+struct alignas(16) Shared {
   double table[64];
   double sums[2][kMostWarps][2];
-  uint32_t words[2][kMostWarps];
+  uint32_t words[2][kMostWarps], lows[2][kMostWarps];
   double cta_sums[2][kMostCtas][2];
-  uint32_t cta_words[2][kMostCtas];
+  uint32_t cta_words[2][kMostCtas], cta_lows[2][kMostCtas];
   uint32_t count, bin[2], bin_before, bin_after, bin_all;
   uint32_t ranks[kCounted];
   union {
@@ -230,19 +250,17 @@ struct Team {  // C CTAs at work on a row
       for (int i = 0; i < kPer; ++i) f(v[i], c + i);
     });
   }
-  // Both numbers of all threads, summed or the larger of them, to all of them.
-  template <bool MAX>
+  // Both numbers of all threads, summed, to all of them.
   __device__ __forceinline__ void reduce(double &a, double &b) {
-    auto with = [](double x, double y) { return MAX ? fmax(x, y) : x + y; };
     auto in_warp = [&](double &v) {
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) v = with(v, __shfl_xor_sync(0xffffffffu, v, d));
+      for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     };
     in_warp(a), in_warp(b);
     if (lane == 0) sh.sums[turn][warp][0] = a, sh.sums[turn][warp][1] = b;
     __syncthreads();
-    a = lane < warps ? sh.sums[turn][lane][0] : MAX ? -CUDART_INF : 0.0;
-    b = lane < warps ? sh.sums[turn][lane][1] : MAX ? -CUDART_INF : 0.0;
+    a = lane < warps ? sh.sums[turn][lane][0] : 0.0;
+    b = lane < warps ? sh.sums[turn][lane][1] : 0.0;
     in_warp(a), in_warp(b);
     if constexpr (C > 1) {
       if (warp == 0 && lane < C) {
@@ -252,14 +270,33 @@ struct Team {  // C CTAs at work on a row
       meet();
       a = sh.cta_sums[far_turn][0][0], b = sh.cta_sums[far_turn][0][1];
 #pragma unroll
-      for (int r = 1; r < C; ++r) a = with(a, sh.cta_sums[far_turn][r][0]), b = with(b, sh.cta_sums[far_turn][r][1]);
+      for (int r = 1; r < C; ++r) a += sh.cta_sums[far_turn][r][0], b += sh.cta_sums[far_turn][r][1];
+      far_turn ^= 1u;
+    }
+    turn ^= 1u;
+  }
+  // The largest and the least of all threads' numbers.
+  __device__ __forceinline__ void range(uint32_t &top, uint32_t &low) {
+    auto in_warp = [&]() { top = __reduce_max_sync(0xffffffffu, top), low = __reduce_min_sync(0xffffffffu, low); };
+    in_warp();
+    if (lane == 0) sh.words[turn][warp] = top, sh.lows[turn][warp] = low;
+    __syncthreads();
+    top = lane < warps ? sh.words[turn][lane] : 0u;
+    low = lane < warps ? sh.lows[turn][lane] : 0xffffffffu;
+    in_warp();
+    if constexpr (C > 1) {
+      if (warp == 0 && lane < C) *of_cta(&sh.cta_words[far_turn][rank], lane) = top, *of_cta(&sh.cta_lows[far_turn][rank], lane) = low;
+      meet();
+      top = lane < C ? sh.cta_words[far_turn][lane] : 0u;
+      low = lane < C ? sh.cta_lows[far_turn][lane] : 0xffffffffu;
+      in_warp();
       far_turn ^= 1u;
     }
     turn ^= 1u;
   }
   __device__ __forceinline__ double sum(double v) {
     double none = 0.0;
-    reduce<false>(v, none);
+    reduce(v, none);
     return v;
   }
   // The least, or the sum, of all threads' numbers; of the CTA's alone with `alone`.
@@ -290,7 +327,7 @@ struct Team {  // C CTAs at work on a row
       return {sum(value), 0.0};
     }
     value = rough_sum(w, end, powers);
-    reduce<false>(value, powers);
+    reduce(value, powers);
     return {value, 1.01 * (Weight::kOff * value + Weight::kOffPower * powers)};
   }
   // This thread's part of that; powers: the sum of w |y|.
@@ -393,7 +430,7 @@ struct Team {  // C CTAs at work on a row
   }
   // weight(i) for the list's first n, summed in order: this thread's neighbours from .. to - 1 and what is ahead of them; gives the whole.
   template <typename F>
-  __device__ __forceinline__ double scan(int n, F &&weight, int &from, int &to, double &ahead) {
+  __device__ __forceinline__ double scan(int n, F &&weight, int &from, int &to, double &ahead, double *mine = nullptr) {
     const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;  // kList / threads at the most
     from = min((int)threadIdx.x * per, n), to = min(from + per, n);
     double own = 0.0;
@@ -413,6 +450,7 @@ struct Team {  // C CTAs at work on a row
     }
     turn ^= 1u;
     ahead = before + (upto - own);
+    if (mine != nullptr) *mine = own;
     return all;
   }
   // Of the sorted list's first n, with `before` of weight ahead of them: how many start below `target`, whose own error is `off`: -1 where that
@@ -569,7 +607,7 @@ struct Team {  // C CTAs at work on a row
         least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
         return true;
       });
-      reduce<false>(over, powers);
+      reduce(over, powers);
       if (WEIGHTS && !exact) off += 1.01 * (Weight::kOff * over + Weight::kOffPower * powers);
       over += above;
       if (WEIGHTS && over >= target - off) *sure = false;
@@ -656,7 +694,8 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     }
     team.row.shared = to;
   }
-  if (threadIdx.x < 64) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  if (threadIdx.x < 32)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_addr(sh.table) + 16u * threadIdx.x), "l"(kPowers + 2 * threadIdx.x) : "memory");
   const double temperature = a.row_temperature != nullptr ? (double)load_plain(a.row_temperature + r) : a.temperature;
   const double top_p = a.row_top_p != nullptr ? (double)load_plain(a.row_top_p + r) : a.top_p;
   const double min_p = a.row_min_p != nullptr ? (double)load_plain(a.row_min_p + r) : a.min_p;
@@ -675,9 +714,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   // (no number where one of them is none)
   const float own_top = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
   const bool number = part_max[0] == part_max[0] && part_max[1] == part_max[1] && part_max[2] == part_max[2] && part_max[3] == part_max[3];
-  double top_ = number ? (double)own_top : CUDART_INF, minus_low = -(double)low_;
-  team.template reduce<true>(top_, minus_low);
-  const float m = (float)top_;
+  uint32_t top_key = number ? key_of(own_top) : 0xffffffffu, low_key_ = key_of(low_);
+  team.range(top_key, low_key_);
+  const float m = top_key == 0xffffffffu ? CUDART_INF_F : score_of(top_key);
   const bool bounds = temperature >= 0.0 && temperature < CUDART_INF && top_p == top_p && min_p == min_p && u >= 0.0 && u <= 1.0;
   auto answer = [&](int64_t drawn, float log_prob) { a.drawn[r] = drawn, a.log_probs[r] = log_prob; };
   // (a CTA of a cluster leaves when no other one reads from it any more)
@@ -696,16 +735,13 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     if constexpr (C > 1) team.meet();
     return;
   }
-  float low = (float)-minus_low;  // the least finite score
+  float low = score_of(low_key_);  // the least finite score
   if (low == -CUDART_INF_F && (top_k < a.classes || top_p < 1.0)) {
     float least = CUDART_INF_F;
     team.each([&](float s, int) { least = fminf(least, s > -CUDART_INF_F ? s : CUDART_INF_F); });
-    double none = -CUDART_INF;
-    minus_low = -(double)least;
-    team.template reduce<true>(minus_low, none);
-    low = (float)-minus_low;
+    low = score_of(team.template words<true>(key_of(least)));
   }
-  const double factor = fmin(64.0 * 1.4426950408889634 / temperature, 1e300);
+  const double factor = a.row_temperature == nullptr ? a.factor : fmin(64.0 * 1.4426950408889634 / temperature, 1e300);
   const Weight w = {(double)m, factor, sh.table, m, (float)fmin(factor / 64.0, 3e38)};
 
   const bool rough_fails = w.c_ < 1e-37f;  // a subnormal factor
@@ -833,102 +869,117 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
       });
     else
       own = team.rough_sum(w, end, powers);
+    // the warps' parts, one after the other
+    const uint32_t turn = team.turn;
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) own += __shfl_xor_sync(0xffffffffu, own, d), powers += __shfl_xor_sync(0xffffffffu, powers, d);
-    const uint32_t turn = team.turn;
     if (lane == 0) sh.sums[turn][warp][0] = own, sh.sums[turn][warp][1] = powers;
     __syncthreads();
-    double all = 0.0, all_powers = 0.0, of_cta = 0.0, of_cta_powers = 0.0, ahead_of_cta = 0.0;
-    for (int i = 0; i < warps; ++i) of_cta += sh.sums[turn][i][0], of_cta_powers += sh.sums[turn][i][1];
+    own = lane < warps ? sh.sums[turn][lane][0] : 0.0;
+    powers = lane < warps ? sh.sums[turn][lane][1] : 0.0;
+    double upto = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += t;
+      powers += __shfl_xor_sync(0xffffffffu, powers, d);
+    }
+    double all = __shfl_sync(0xffffffffu, upto, 31), ahead = 0.0;
     int at_cta = 0;
-    double target;
     if constexpr (C > 1) {
       if (warp == 0 && lane < C) {
         double *to = team.of_cta(&sh.cta_sums[team.far_turn][rank][0], lane);
-        to[0] = of_cta, to[1] = of_cta_powers;
+        to[0] = all, to[1] = powers;
       }
       team.meet();
+      all = powers = 0.0;
 #pragma unroll
-      for (int i = 0; i < C; ++i) all += sh.cta_sums[team.far_turn][i][0], all_powers += sh.cta_sums[team.far_turn][i][1];
-      target = u * all;
-      double ahead = 0.0;
+      for (int i = 0; i < C; ++i) all += sh.cta_sums[team.far_turn][i][0], powers += sh.cta_sums[team.far_turn][i][1];
       at_cta = -1;
-      for (int i = 0; i < C; ++i) {  // as below
+      for (int i = 0; i < C; ++i) {  // the first CTA whose part ends above the target, or (u = 1, rounding) the last that weighs anything
         const double s = sh.cta_sums[team.far_turn][i][0];
         if (s > 0.0) {
           if (at_cta >= 0) ahead += sh.cta_sums[team.far_turn][at_cta][0];
           at_cta = i;
-          if (ahead + s > target) break;
+          if (ahead + s > u * all) break;
         }
       }
-      ahead_of_cta = ahead;
       team.far_turn ^= 1u;
-    } else {
-      all = of_cta, all_powers = of_cta_powers;
-      target = u * all;
     }
+    const double target = u * all;
     team.turn ^= 1u;
-    const double off = exact ? 0.0 : 2.02 * (Weight::kOff * all + Weight::kOffPower * all_powers);  // of a sum and of the target together
+    const double off = exact ? 0.0 : 2.02 * (Weight::kOff * all + Weight::kOffPower * powers);  // of a sum and of the target together
+    // the place of the first of ascending sums that passes the target, among those that weigh anything, or of the last that does
+    auto place_of = [&](bool passes, bool weighs) {
+      const uint32_t some = __ballot_sync(0xffffffffu, weighs), passing = __ballot_sync(0xffffffffu, passes) & some;
+      return passing != 0u ? __ffs((int)passing) - 1 : 31 - __clz((int)some);
+    };
     bool sure = true;
     if (rank == at_cta) {
-      double ahead = ahead_of_cta;
-      int place = -1;
-      for (int i = 0; i < warps; ++i) {  // the first part that ends above the target, or (u = 1, rounding) the last that weighs anything
-        const double s = sh.sums[turn][i][0];
-        if (s > 0.0) {
-          if (place >= 0) ahead += sh.sums[turn][place][0];
-          place = i;
-          if (ahead + s > target) break;
-        }
-      }
+      const int place = place_of(ahead + upto > target, own > 0.0);
+      ahead += __shfl_sync(0xffffffffu, upto - own, place);
       // that part's vectors, the CTA's threads in order
       const int part_first = min((rank * warps + place) * part, row.vectors), part_last = min(part_first + part, row.vectors);
-      auto weight = [&](float s, int i) {
-        float y;
-        return !end.holds(s, i) ? 0.0 : exact ? w(s) : (double)w.rough(s, y);
-      };
-      auto of_vector = [&](int i) {
-        float v[kPer];
-        team.row.values(part_first + i, v);
-        double sum = 0.0;
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) sum += weight(v[q], (part_first + i) * kPer - row.head + q);
-        return sum;
-      };
-      int first, last;
-      double at;
-      team.scan(part_last - part_first, of_vector, first, last, at);
-      at += ahead;
-      // the first class that passes the target, or the last that weighs anything
-      uint32_t passing = 0xffffffffu, some = 0u;
-      float its_score = 0.0f, some_score = 0.0f;
-      bool near = false, some_near = false;
-      for (int i = first; i < last && passing == 0xffffffffu; ++i) {
-        float v[kPer];
+      auto weights_of = [&](int i, float (&v)[kPer], double (&e)[kPer]) {
         team.row.values(part_first + i, v);
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
-          const int c = (part_first + i) * kPer - row.head + q;
-          const double one = weight(v[q], c);
-          if (one > 0.0 && passing == 0xffffffffu) {
+          float y;
+          const bool held = end.holds(v[q], (part_first + i) * kPer - row.head + q);
+          e[q] = !held ? 0.0 : exact ? w(v[q]) : (double)w.rough(v[q], y);
+        }
+      };
+      auto of_vector = [&](int i) {
+        float v[kPer];
+        if (exact) {
+          double e[kPer], sum = 0.0;
+          weights_of(i, v, e);
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) sum += e[q];
+          return sum;
+        }
+        float e[kPer];
+        team.row.values(part_first + i, v);
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          float y;
+          e[q] = w.rough(end.holds(v[q], (part_first + i) * kPer - row.head + q) ? v[q] : -CUDART_INF_F, y);
+        }
+#pragma unroll
+        for (int d = kPer / 2; d >= 1; d /= 2)
+#pragma unroll
+          for (int q = 0; q < d; ++q) e[q] += e[q + d];
+        return (double)e[0];
+      };
+      int first, last;
+      double at, whole;
+      team.scan(part_last - part_first, of_vector, first, last, at, &whole);
+      at += ahead;
+      // the first thread whose sum passes the target, or the last that has any
+      const bool passes = whole > 0.0 && at + whole > target;
+      uint32_t who = team.template words<true>(passes ? threadIdx.x : 0xffffffffu, true);
+      if (who == 0xffffffffu) who = 0xffffffffu - team.template words<true>(0xffffffffu - (whole > 0.0 ? threadIdx.x + 1u : 0u), true) - 1u;
+      if (threadIdx.x == who) {
+        int found = -1;
+        float found_score = 0.0f;
+        bool passed = false, near = true;
+        for (int i = first; i < last && !passed; ++i) {
+          float v[kPer];
+          double e[kPer];
+          weights_of(i, v, e);
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) {
             const double before = at;
-            at += one;
-            some = (uint32_t)c + 1u, some_score = v[q], some_near = true;
-            if (at > target) passing = (uint32_t)c, its_score = v[q], near = target - before <= off || at - target <= off;
+            at += e[q];
+            if (e[q] > 0.0 && !passed) {
+              found = (part_first + i) * kPer - row.head + q, found_score = v[q];
+              passed = at > target;
+              near = target - before <= off || at - target <= off;
+            }
           }
         }
-      }
-      const uint32_t drawn = team.template words<true>(passing, true);
-      if (drawn == 0xffffffffu) {
-        passing = 0xffffffffu - team.template words<true>(0xffffffffu - some, true) - 1u;
-        if (passing + 1u == some) its_score = some_score, near = some_near;
-        else passing = 0xffffffffu;
-      } else if (passing != drawn) {
-        passing = 0xffffffffu;
-      }
-      if (passing != 0xffffffffu) {
         sure = exact || !near;
-        if (sure) answer((int64_t)passing, (float)(((double)its_score - (double)m) / temperature - log(all)));
+        if (sure) answer((int64_t)found, (float)(((double)found_score - (double)m) / temperature - log(all)));
       }
     }
     if (exact) break;
@@ -967,7 +1018,8 @@ int launch_of(Args a, int64_t vectors, cudaStream_t stream) {
 template <typename T>
 int launch(const ht_sample_problem &p, const void *scores, const float *uniform, int64_t *drawn, float *log_probs, cudaStream_t stream) {
   constexpr int kPer = Row<T>::kPer;
-  const Args a = {scores, p.rows, p.stride, (int)p.classes, uniform, p.temperature, p.top_p, p.min_p, p.top_k, p.row_temperature, p.row_top_p, p.row_min_p,
+  const double factor = std::min(64.0 * 1.4426950408889634 / p.temperature, 1e300);
+  const Args a = {scores, p.rows, p.stride, (int)p.classes, uniform, p.temperature, factor, p.top_p, p.min_p, p.top_k, p.row_temperature, p.row_top_p, p.row_min_p,
                   p.row_top_k, drawn, log_probs, 0};
   const int64_t vectors = (p.classes + 2 * kPer - 2) / kPer;
   // a cluster where the rows leave SMs idle and a CTA's part is still some vectors a thread
