@@ -13,9 +13,9 @@
 //
 // A row belongs to a CTA, or, where there are few rows, to a cluster of up to 8 that have a part each; it stays in shared memory where it fits.  A
 // prefix of the order is held as its last class, (score, class).  To find it nothing is sorted but a list of up to 1024 classes around the place:
-//   top_k   every thread has the maxima of 4 parts of what it has read; the one of about place k among those, found by halving the
+//   top_k   up to 200: every thread has the maxima of 4 parts of what it has read; the one of about place k among those, found by halving the
 //           range, bounds the k-th largest score from below, and not many more classes than k are above it
-//   top_p   the same with the first 512 classes, where those hold enough
+//   top_p   the same with the first 192 classes, where those hold enough
 //   else    classes are counted, or their weights summed roughly, by 2048 ranges of the score's bits; the range with the place in it is listed, or
 //           divided again, or is one score
 // What counts of a list is drawn from there; otherwise the row is summed in order, warp by warp, and one warp walks its part.
@@ -34,8 +34,9 @@ using dense::load_plain;
 using dense::to_float;
 using tile::smem_addr;
 
-constexpr int kMostWarps = 32, kMostCtas = 8, kList = 1024, kBins = 2048, kParts = 4, kCounted = 128;
-constexpr int kFirst = 512;          // classes that are listed first for top_p
+constexpr int kMostWarps = 32, kMostCtas = 8, kList = 1024, kBins = 2048, kParts = 4, kCounted = 256;
+constexpr uint32_t kFirst = 192;     // classes that are listed first for top_p
+constexpr uint32_t kListed = 200;   // top_k up to which the classes are listed: what is sorted by counting, a little more at the most
 constexpr double kTail = -80.0;      // whatever the classes below exp() of this are, they do not weigh 2^-53 of the row together
 constexpr int kPassed = 0x7fffffff;  // no limit on the class among equal scores
 
@@ -96,6 +97,8 @@ struct alignas(16) Shared {
 constexpr size_t kRowAt = (sizeof(Shared) + 127) / 128 * 128;
 constexpr size_t kMergedBytes = sizeof(uint64_t) * kList;  // of a cluster's list in each of its CTAs, behind that
 
+constexpr double kStepOf = 0.69314718055994531 / 64.0;  // ln 2 / 64
+
 // w = exp((s - m) / T) as 2^(a / 64) with a = (s - m) 64 / (T ln 2).
 struct Weight {
   double m, c;
@@ -103,7 +106,7 @@ struct Weight {
   float m_, c_;  // of the rough one
   __device__ __forceinline__ double operator()(float s) const {
     const double a = ((double)s - m) * c;
-    constexpr double kStep = 0.69314718055994531 / 64.0;
+    constexpr double kStep = kStepOf;
     if (!(a > -746.0 / kStep)) return 0.0;
     constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52: what is added to it is rounded to a whole number, in the low bits
     const double t = a + kWhole, r = a - (t - kWhole);
@@ -125,6 +128,14 @@ struct Weight {
     return r;
   }
 };
+
+// The logarithm of what counts: fp32's, and a step of Newton's method with the exponential above, log x = y + (x exp(-y) - 1), which leaves the
+// square of its error.  (The 64-bit function took longer than the sums of a row.)
+__device__ __forceinline__ double log_of(double x, const double *table) {
+  const float y = logf((float)x);
+  const Weight w = {0.0, 64.0 * 1.4426950408889634, table, 0.0f, 0.0f};
+  return (double)y + fma(x, w(-y), -1.0);
+}
 
 // The last class of a prefix of the order.
 struct Last {
@@ -189,9 +200,10 @@ struct Extremes {
   static constexpr uint32_t kInfinity = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
   static constexpr uint32_t kSigns = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
   __device__ __forceinline__ Extremes() : top{kInfinity | kSigns, kInfinity | kSigns, kInfinity | kSigns, kInfinity | kSigns}, low(kInfinity) {}
-  __device__ __forceinline__ void add(const uint4 &q) {
+  // (an end of the row holds what is no class of it: of those the least are no matter)
+  __device__ __forceinline__ void add(const uint4 &q, bool end) {
     top[0] = larger(top[0], q.x), top[1] = larger(top[1], q.y), top[2] = larger(top[2], q.z), top[3] = larger(top[3], q.w);
-    low = smaller(smaller(low, smaller(q.x, q.y)), smaller(q.z, q.w));
+    if (!end) low = smaller(smaller(low, smaller(q.x, q.y)), smaller(q.z, q.w));
   }
   __device__ __forceinline__ float least(float (&part_max)[kParts]) const {
     constexpr int kIn = 4 / (int)sizeof(T);
@@ -242,7 +254,35 @@ struct Team {  // C CTAs at work on a row
       f(v, j * kPer - row.head);
     }
   }
-  // f(score, class) for every class.
+  // The same for vectors with a score from `least` on among them.
+  template <typename F>
+  __device__ __forceinline__ void each_vector_from(float least, F &&f) const {
+    if (least == -CUDART_INF_F) {
+      each_vector(f);
+      return;
+    }
+#pragma unroll 2
+    for (int j = first + lane; j < last; j += 32) {
+      const uint4 q = row.words(j);
+      const uint32_t top = Extremes<T>::larger(Extremes<T>::larger(q.x, q.y), Extremes<T>::larger(q.z, q.w));
+      T t[kPer];
+      *reinterpret_cast<uint32_t *>(t) = top;
+      if (!(fmaxf(to_float(t[0]), to_float(t[4 / (int)sizeof(T) - 1])) >= least)) continue;
+      *reinterpret_cast<uint4 *>(t) = q;
+      float v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = to_float(t[i]);
+      f(v, j * kPer - row.head);
+    }
+  }
+  // f(score, class) for every class, or for those of such vectors.
+  template <typename F>
+  __device__ __forceinline__ void each_from(float least, F &&f) const {
+    each_vector_from(least, [&](const float (&v)[kPer], int c) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) f(v[i], c + i);
+    });
+  }
   template <typename F>
   __device__ __forceinline__ void each(F &&f) const {
     each_vector([&](const float (&v)[kPer], int c) {
@@ -317,11 +357,21 @@ struct Team {  // C CTAs at work on a row
     return v;
   }
 
+  // Both numbers of the CTA's threads, summed.
+  __device__ __forceinline__ void counts(uint32_t &a, uint32_t &b) {
+    a = __reduce_add_sync(0xffffffffu, a), b = __reduce_add_sync(0xffffffffu, b);
+    if (lane == 0) sh.words[turn][warp] = a, sh.lows[turn][warp] = b;
+    __syncthreads();
+    a = __reduce_add_sync(0xffffffffu, lane < warps ? sh.words[turn][lane] : 0u);
+    b = __reduce_add_sync(0xffffffffu, lane < warps ? sh.lows[turn][lane] : 0u);
+    turn ^= 1u;
+  }
+
   // What a prefix weighs.
   __device__ __forceinline__ Sum weigh(const Weight &w, const Last &end, bool exact) {
     double value = 0.0, powers = 0.0;
     if (exact) {
-      each([&](float s, int i) {
+      each_from(end.score, [&](float s, int i) {
         if (end.holds(s, i)) value += w(s);
       });
       return {sum(value), 0.0};
@@ -351,7 +401,7 @@ struct Team {  // C CTAs at work on a row
     if (end.score == -CUDART_INF_F) {
       each_vector([&](const float (&v)[kPer], int) { vector(v); });
     } else {
-      each_vector([&](const float (&v)[kPer], int c) {
+      each_vector_from(end.score, [&](const float (&v)[kPer], int c) {
         float held[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) held[i] = end.holds(v[i], c + i) ? v[i] : -CUDART_INF_F;
@@ -362,16 +412,14 @@ struct Team {  // C CTAs at work on a row
     return value;
   }
 
-  // Lists the classes that `takes` says, as many as fit, and gives their number; in `merged` for all CTAs.
+  // Lists the classes that `visit` adds, as many as fit, and gives their number; in `merged` for all CTAs.
   template <typename F>
-  __device__ __forceinline__ uint32_t list(F &&takes) {
+  __device__ __forceinline__ uint32_t list(F &&visit) {
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    each([&](float s, int i) {
-      if (takes(s, i)) {
-        const uint32_t at = atomicAdd(&sh.count, 1u);
-        if (at < (uint32_t)kList) sh.list[at] = (uint64_t)key_of(s) << 32 | (0xffffffffu - (uint32_t)i);
-      }
+    visit([&](float s, int i) {
+      const uint32_t at = atomicAdd(&sh.count, 1u);
+      if (at < (uint32_t)kList) sh.list[at] = (uint64_t)key_of(s) << 32 | (0xffffffffu - (uint32_t)i);
     });
     __syncthreads();
     uint32_t n = sh.count;
@@ -400,7 +448,7 @@ struct Team {  // C CTAs at work on a row
     while (places < n) places *= 2;
     if (places <= kCounted && places <= (int)blockDim.x) {
       const int e = (int)threadIdx.x & (places - 1), part = (int)threadIdx.x / places, parts = (int)blockDim.x / places;
-      if (threadIdx.x < kCounted) sh.ranks[threadIdx.x] = 0;
+      if ((int)threadIdx.x < places) sh.ranks[threadIdx.x] = 0;
       __syncthreads();
       const uint64_t own = e < n ? merged[e] : 0;
       uint32_t larger = 0;
@@ -473,7 +521,7 @@ struct Team {  // C CTAs at work on a row
   // The class of the n-th (from 1) of those with this score, in the order of classes.
   __device__ __forceinline__ int nth_of(float score, uint32_t n) {
     uint32_t own = 0;
-    each([&](float s, int) { own += s == score ? 1u : 0u; });
+    each_from(score, [&](float s, int) { own += s == score ? 1u : 0u; });
     own = __reduce_add_sync(0xffffffffu, own);
     if (lane == 0) sh.words[turn][warp] = own;
     __syncthreads();
@@ -533,17 +581,18 @@ struct Team {  // C CTAs at work on a row
       const int shift = max(0, 21 - (int)__clz((int)width));
       const float slope = by_score ? ((float)kBins - 1.0f) / (w.m_ - score_of(low)) : 0.0f;
       const uint32_t last_bin = by_score ? (uint32_t)kBins - 1u : width >> shift;
-      auto range_of = [&](float s, uint32_t key) { return by_score ? min((uint32_t)((w.m_ - s) * slope), last_bin) : (high - key) >> shift; };
+      const float low_score = score_of(low), high_score = score_of(high);
+      auto inside = [&](float s, int i) { return s >= low_score && s <= high_score && (s != base.score || i <= base.at); };
+      auto range_of = [&](float s) { return by_score ? min((uint32_t)((w.m_ - s) * slope), last_bin) : (high - key_of(s)) >> shift; };
       const double scale = 2147483648.0 / all;
       const float scale_ = (float)scale;
       meet();
       for (int i = (int)threadIdx.x; i < kBins; i += (int)blockDim.x) sh.bins[i] = 0;
       __syncthreads();
-      each([&](float s, int i) {
-        const uint32_t key = key_of(s);
-        if (key >= low && key <= high && base.holds(s, i)) {
+      each_from(low_score, [&](float s, int i) {
+        if (inside(s, i)) {
           float y;
-          atomicAdd(&sh.bins[range_of(s, key)], WEIGHTS ? (uint32_t)(w.rough(s, y) * scale_ + 0.5f) : 1u);
+          atomicAdd(&sh.bins[range_of(s)], WEIGHTS ? (uint32_t)fmaf(w.rough(s, y), scale_, 0.5f) : 1u);
         }
       });
       meet();
@@ -590,23 +639,39 @@ struct Team {  // C CTAs at work on a row
       const double window = fmax((double)((sh.bin_after > sh.bin_before ? sh.bin_after : sh.bin_all) - sh.bin_before), 1.0) / scale;
       double over = 0.0, powers = 0.0;
       uint32_t least_key = 0xffffffffu, least_gap = 0xffffffffu;  // of the ranges: their keys reach from `lowest` to `highest`
-      const uint32_t n = list([&](float s, int i) {
-        const uint32_t key = key_of(s);
-        if (key < low || key > high || !base.holds(s, i)) return false;
-        const uint32_t range = range_of(s, key);
-        if (range < first_bin) {
-          if (WEIGHTS && !exact) {
-            float y;
-            const float one = w.rough(s, y);
-            over += (double)one, powers += (double)(one * -y);
-          } else {
-            over += WEIGHTS ? w(s) : 1.0;
+      float of_powers = 0.0f;
+      const uint32_t n = list([&](auto &&add) {
+        each_vector_from(low_score, [&](const float (&v)[kPer], int c) {
+          float e[kPer];
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            e[i] = 0.0f;
+            if (!inside(v[i], c + i)) continue;
+            const uint32_t range = range_of(v[i]);
+            if (range < first_bin) {
+              if (WEIGHTS && !exact) {
+                float y;
+                e[i] = w.rough(v[i], y);
+                of_powers = fmaf(e[i], -y, of_powers);
+              } else if (WEIGHTS) {
+                over += w(v[i]);
+              } else {
+                e[i] = 1.0f;
+              }
+            } else if (range <= end_bin) {
+              const uint32_t key = key_of(v[i]);
+              least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
+              add(v[i], c + i);
+            }
           }
-        }
-        if (range < first_bin || range > end_bin) return false;
-        least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
-        return true;
+#pragma unroll
+          for (int d = kPer / 2; d >= 1; d /= 2)
+#pragma unroll
+            for (int i = 0; i < d; ++i) e[i] += e[i + d];
+          over += (double)e[0];
+        });
       });
+      powers = (double)of_powers;
       reduce(over, powers);
       if (WEIGHTS && !exact) off += 1.01 * (Weight::kOff * over + Weight::kOffPower * powers);
       over += above;
@@ -638,9 +703,9 @@ struct Team {  // C CTAs at work on a row
       if (!by_score && lowest == low && highest == high) {  // the rough weights do not tell: half of the range, by exact ones
         const uint32_t middle = low + (high - low) / 2u;
         double upper = 0.0;
-        each([&](float s, int i) {
-          const uint32_t key = key_of(s);
-          if (key > middle && key <= high && base.holds(s, i)) upper += WEIGHTS ? w(s) : 1.0;
+        const float middle_score = score_of(middle);
+        each_from(low_score, [&](float s, int i) {
+          if (inside(s, i) && s > middle_score) upper += WEIGHTS ? w(s) : 1.0;
         });
         upper = sum(upper);
         if (over + upper < target) {
@@ -709,8 +774,15 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   float part_max[kParts];
   Extremes<T> extremes;
 #pragma unroll 1
-  for (int j = team.first + lane; j < team.last; j += 32) extremes.add(team.row.words(j));
+  for (int j = team.first + lane; j < team.last; j += 32) extremes.add(team.row.words(j), j == 0 || j == row.vectors - 1);
   float low_ = extremes.least(part_max);
+  for (int j = 0; j < row.vectors; j = j == 0 && row.vectors > 1 ? row.vectors - 1 : row.vectors) {  // the ends
+    if (j < team.first || j >= team.last || (j - team.first) % 32 != lane) continue;
+    float v[kPer];
+    team.row.values(j, v);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) low_ = fminf(low_, v[i] > -CUDART_INF_F ? v[i] : CUDART_INF_F);
+  }
   // (no number where one of them is none)
   const float own_top = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
   const bool number = part_max[0] == part_max[0] && part_max[1] == part_max[1] && part_max[2] == part_max[2] && part_max[3] == part_max[3];
@@ -727,7 +799,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   }
   if (temperature == 0.0 || top_k == 1 || top_p <= 0.0 || min_p > 1.0) {
     uint32_t at = 0xffffffffu;
-    team.each([&](float s, int i) {
+    team.each_from(m, [&](float s, int i) {
       if (s == m) at = min(at, (uint32_t)i);
     });
     at = team.template words<true>(at);
@@ -755,30 +827,50 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     const bool by_count = top_k < a.classes;
     // A lower bound for the score of place `wanted`: at least so many of the parts' maxima are not below it.  Of a cluster each CTA has its share
     // of them and a little more, and what is listed is counted.
-    const uint32_t wanted = (uint32_t)(by_count ? top_k : kFirst), share = C == 1 ? wanted : wanted / C + wanted / (2 * C) + 16u;
+    const uint32_t wanted = by_count ? (uint32_t)top_k : kFirst, share = C == 1 ? wanted : wanted / C + wanted / (4 * C) + 8u;
     uint32_t bound = 0;
     if (share <= blockDim.x * kParts) {
       uint32_t keys[kParts], from_key = key_of(low), to_key = high_key;
 #pragma unroll
       for (int i = 0; i < kParts; ++i) keys[i] = key_of(part_max[i]);
+      // by fifths: the counts of four places at a time, two to a word
       while (from_key < to_key) {
-        const uint32_t middle = from_key + (to_key - from_key) / 2u + 1u;
-        uint32_t n = 0;
+        const uint32_t step = (to_key - from_key) / 5u + 1u;
+        uint32_t place[4], n[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) n += keys[i] >= middle ? 1u : 0u;
-        n = team.template words<false>(n, true);
-        if (n >= share) {
-          from_key = middle;
-          if (n <= share + share / 8u) break;
-        } else {
-          to_key = middle - 1u;
+        for (int q = 0; q < 4; ++q) {
+          place[q] = min(from_key + (uint32_t)(q + 1) * step, to_key);
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) n[q / 2] += keys[i] >= place[q] ? 1u << (16 * (q % 2)) : 0u;
         }
+        team.counts(n[0], n[1]);
+        bool near = false;
+        uint32_t to = to_key;
+#pragma unroll
+        for (int q = 3; q >= 0; --q) {  // the highest place that has enough
+          const uint32_t count = (n[q / 2] >> (16 * (q % 2))) & 0xffffu;
+          if (count < share) {
+            to = place[q] - 1u;
+          } else {
+            from_key = place[q];
+            near = count <= share + share / 8u;
+            break;
+          }
+        }
+        to_key = to;
+        if (near) break;
       }
       bound = from_key;
       if constexpr (C > 1) bound = 0xffffffffu - team.template words<true>(0xffffffffu - bound);
     }
     const float bound_score = score_of(bound);
-    uint32_t n = bound > 0u && wanted <= kList * 3u / 4u ? team.list([&](float s, int) { return s >= bound_score; }) : 0xffffffffu;
+    uint32_t n = 0xffffffffu;
+    if (bound > 0u && wanted <= kListed)
+      n = team.list([&](auto &&add) {
+        team.each_from(bound_score, [&](float s, int i) {
+          if (s >= bound_score) add(s, i);
+        });
+      });
     // (whether all is listed that there is, or the list goes as far as place `wanted`)
     const bool whole = bound == key_of(low);
     if (by_count && (n < wanted || (C > 1 && n == 0xffffffffu)) && !whole) n = 0xffffffffu, bound = 0;
@@ -790,7 +882,8 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     if (by_count && held == 0) {
       const uint32_t from_key = max(bound, key_of(low));
       double inside = 0.0;
-      team.each([&](float s, int) { inside += key_of(s) >= from_key ? 1.0 : 0.0; });
+      const float from_score = score_of(from_key);
+      team.each_from(from_score, [&](float s, int) { inside += s >= from_score ? 1.0 : 0.0; });
       inside = team.sum(inside);
       bool sure = true;
       if (inside >= (double)top_k) end = team.template narrow<false>(w, end, from_key, high_key, (double)top_k, 0.0, 1.0, true, &sure);
@@ -855,7 +948,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     passing = team.template words<true>(passing, true);
     if (passing == 0xffffffffu) passing = 0xffffffffu - team.template words<true>(0xffffffffu - some, true) - 1u;
     if (rank == 0 && threadIdx.x == 0)
-      answer((int64_t)(0xffffffffu - (uint32_t)(team.merged[passing] >> 32)), (float)(((double)score((int)passing) - (double)m) / temperature - log(all)));
+      answer((int64_t)(0xffffffffu - (uint32_t)(team.merged[passing] >> 32)), (float)(((double)score((int)passing) - (double)m) * factor * kStepOf - log_of(all, sh.table)));
     if constexpr (C > 1) team.meet();
     return;
   }
@@ -864,7 +957,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   for (bool exact = rough_fails;; exact = true) {
     double own = 0.0, powers = 0.0;
     if (exact)
-      team.each([&](float s, int i) {
+      team.each_from(end.score, [&](float s, int i) {
         if (end.holds(s, i)) own += w(s);
       });
     else
@@ -979,7 +1072,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
           }
         }
         sure = exact || !near;
-        if (sure) answer((int64_t)found, (float)(((double)found_score - (double)m) / temperature - log(all)));
+        if (sure) answer((int64_t)found, (float)(((double)found_score - (double)m) * factor * kStepOf - log_of(all, sh.table)));
       }
     }
     if (exact) break;
