@@ -69,7 +69,7 @@ __device__ __forceinline__ void load_x(const FewArgs<T> &a, int row, int k, uint
 
 struct Codes {  // a lane's of two outputs
   uint4 a, b;
-  uint32_t scales;  // a's in the low byte, b's in the next
+  uint8_t scale_a, scale_b;  // (as they are loaded: what touches them waits for them)
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -96,18 +96,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
     for (int n = 0; n < NT; ++n) load_x(a, row0 + 8 * n + g, (4 * chunk + j) * kBlock, x[n]);
   };
   auto fetch = [&](int group, int chunk) {
-    Codes c = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u), 0x7f7fu};
+    Codes c = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u), 127, 127};
     const int block = 4 * chunk + j, o = group * 16 + g;
     if (group < groups && block < a.blocks) {
       const int64_t at = (int64_t)min(o, a.outputs - 1) * a.blocks + block, bt = (int64_t)min(o + 8, a.outputs - 1) * a.blocks + block;
       c.a = load_plain(reinterpret_cast<const uint4 *>(a.codes) + at);
       c.b = load_plain(reinterpret_cast<const uint4 *>(a.codes) + bt);
-      c.scales = (uint32_t)load_plain(a.scales + at) | (uint32_t)load_plain(a.scales + bt) << 8;
+      c.scale_a = load_plain(a.scales + at);
+      c.scale_b = load_plain(a.scales + bt);
     }
     return c;
   };
   auto multiply = [&](const Codes &c, float (&sum)[NT][4]) {
-    const Scale sa = scale_of(c.scales & 255u), sb = scale_of(c.scales >> 8);
+    const Scale sa = scale_of(c.scale_a), sb = scale_of(c.scale_b);
     const uint32_t wa[4] = {c.a.x, c.a.y, c.a.z, c.a.w}, wb[4] = {c.b.x, c.b.y, c.b.z, c.b.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {

@@ -23,6 +23,71 @@ struct Shape {
   bool whole;    // rows start on 16 bytes
 };
 
+// 8 values of a row from k on, zeros behind its end.  16-bit rows that start on 2 or 4 bytes are read by words, 5 of them on odd starts, as long as
+// a value follows the last one (`followed`).
+template <typename T>
+__device__ __forceinline__ void load_values(const T *from, int64_t left, bool whole, bool followed, float (&v)[8]) {
+  constexpr int kPer = 16 / (int)sizeof(T);
+  if (whole && left >= 8) {
+#pragma unroll
+    for (int j = 0; j < 8; j += kPer) {
+      T t[kPer];
+      *reinterpret_cast<uint4 *>(t) = load_plain(reinterpret_cast<const uint4 *>(from + j));
+#pragma unroll
+      for (int n = 0; n < kPer; ++n) v[j + n] = to_float(t[n]);
+    }
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (left > 8 || (left == 8 && followed)) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+      const uint32_t *words = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3);
+      const bool odd = (at & 2u) != 0;
+      uint32_t q[5];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) q[j] = j < 4 || odd ? load_plain(words + j) : 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t pair = odd ? __funnelshift_r(q[j], q[j + 1], 16) : q[j];
+        T t[2];
+        *reinterpret_cast<uint32_t *>(t) = pair;
+        v[2 * j] = to_float(t[0]), v[2 * j + 1] = to_float(t[1]);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = j < left ? to_float(from[j]) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ void store_values(T *to, int64_t left, bool whole, const T (&t)[8]) {
+  constexpr int kPer = 16 / (int)sizeof(T);
+  if (whole && left >= 8) {
+#pragma unroll
+    for (int j = 0; j < 8; j += kPer) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(t + j);
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (left >= 8) {  // words from the first even address on
+      const bool odd = (reinterpret_cast<uintptr_t>(to) & 2u) != 0;
+      const uint32_t *pairs = reinterpret_cast<const uint32_t *>(t);
+      if (!odd) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t *>(to)[j] = pairs[j];
+      } else {
+        to[0] = t[0];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) reinterpret_cast<uint32_t *>(to + 1)[j] = __funnelshift_r(pairs[j], pairs[j + 1], 16);
+        to[7] = t[7];
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) to[j] = t[j];
+}
+
 // Codes of 8 values, the first in the lowest bits.
 __device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
   uint32_t r;
@@ -37,41 +102,41 @@ __device__ __forceinline__ uint32_t codes_of(const float (&v)[8]) {
   return r;
 }
 
+// Items of a CTA's rows, kAtOnce of them a thread at a time: their loads are under way together.
+constexpr int kAtOnce = 2;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pack_kernel(const Shape a, const T *w, uint32_t *codes, uint8_t *scales) {
   after_previous_kernel();
-  constexpr int kPer = 16 / (int)sizeof(T);
   for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < a.outputs; row0 += (int64_t)gridDim.x * a.rows) {
     const uint32_t items = (uint32_t)min((int64_t)a.rows, a.outputs - row0) * (uint32_t)a.per_row;  // (a multiple of 4: the lanes of a block go together)
-    for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
-      const uint32_t r = i / (uint32_t)a.per_row, q = i - r * (uint32_t)a.per_row;
-      const int64_t row = row0 + r, k = (int64_t)q * 8;
-      const T *from = w + row * a.stride + k;
-      float v[8];
-      if (a.whole && k + 8 <= a.features) {
+    for (uint32_t i0 = threadIdx.x; i0 < items; i0 += kAtOnce * kThreads) {
+      float v[kAtOnce][8];
+      uint32_t q[kAtOnce];
+      int64_t row[kAtOnce];
 #pragma unroll
-        for (int j = 0; j < 8; j += kPer) {
-          T t[kPer];
-          *reinterpret_cast<uint4 *>(t) = load_plain(reinterpret_cast<const uint4 *>(from + j));
-#pragma unroll
-          for (int n = 0; n < kPer; ++n) v[j + n] = to_float(t[n]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < a.features ? to_float(from[j]) : 0.0f;
+      for (int n = 0; n < kAtOnce; ++n) {
+        const uint32_t i = i0 + n * kThreads, r = i / (uint32_t)a.per_row;
+        q[n] = i - r * (uint32_t)a.per_row;
+        row[n] = row0 + r;
+        const int64_t k = (int64_t)q[n] * 8, left = i < items ? a.features - k : 0;
+        load_values(w + (left > 0 ? row[n] * a.stride + k : 0), left, a.whole, row[n] + 1 < a.outputs, v[n]);
       }
-      uint32_t top = 0;  // the largest magnitude's bits: no number is above infinity
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-      const uint32_t lanes = 0xfu << (threadIdx.x & 28u);
-      top = max(top, __shfl_xor_sync(lanes, top, 1));
-      top = max(top, __shfl_xor_sync(lanes, top, 2));
-      const uint32_t field = top >> 23, b = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
-      const float factor = __uint_as_float((254u - b) << 23);
+      for (int n = 0; n < kAtOnce; ++n) {
+        if (i0 + n * kThreads >= items) break;
+        uint32_t top = 0;  // the largest magnitude's bits: no number is above infinity
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= factor;
-      codes[row * a.per_row + q] = b == 255u ? 0u : codes_of(v);
-      if ((q & 3u) == 0u) scales[row * (a.per_row / 4) + q / 4] = (uint8_t)b;
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[n][j]) & 0x7fffffffu);
+        const uint32_t lanes = 0xfu << (threadIdx.x & 28u);
+        top = max(top, __shfl_xor_sync(lanes, top, 1));
+        top = max(top, __shfl_xor_sync(lanes, top, 2));
+        const uint32_t field = top >> 23, b = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
+        const float factor = __uint_as_float((254u - b) << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[n][j] *= factor;
+        codes[row[n] * a.per_row + q[n]] = b == 255u ? 0u : codes_of(v[n]);
+        if ((q[n] & 3u) == 0u) scales[row[n] * (a.per_row / 4) + q[n] / 4] = (uint8_t)b;
+      }
     }
   }
 }
@@ -79,30 +144,32 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Shape a, const T *
 template <typename T>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(const Shape a, const uint32_t *codes, const uint8_t *scales, T *w) {
   after_previous_kernel();
-  constexpr int kPer = 16 / (int)sizeof(T);
   for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < a.outputs; row0 += (int64_t)gridDim.x * a.rows) {
     const uint32_t items = (uint32_t)min((int64_t)a.rows, a.outputs - row0) * (uint32_t)a.per_row;
-    for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
-      const uint32_t r = i / (uint32_t)a.per_row, q = i - r * (uint32_t)a.per_row;
-      const int64_t row = row0 + r, k = (int64_t)q * 8;
-      if (k >= a.features) continue;
-      const uint32_t c = load_plain(codes + row * a.per_row + q), b = load_plain(scales + row * (a.per_row / 4) + q / 4);
-      const float scale = b == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(b == 0u ? 0x00400000u : b << 23);
-      T t[8];
+    for (uint32_t i0 = threadIdx.x; i0 < items; i0 += kAtOnce * kThreads) {
+      uint32_t c[kAtOnce], b[kAtOnce], q[kAtOnce];
+      int64_t row[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t code = c >> (4 * j);
-        const float number = __uint_as_float((code & 7u) << 22) * 0x1p126f * scale;
-        t[j] = dense::from_float<T>(__uint_as_float(__float_as_uint(number) | (code & 8u) << 28));
+      for (int n = 0; n < kAtOnce; ++n) {
+        const uint32_t i = i0 + n * kThreads, r = i / (uint32_t)a.per_row;
+        q[n] = i - r * (uint32_t)a.per_row;
+        row[n] = row0 + r;
+        c[n] = i < items ? load_plain(codes + row[n] * a.per_row + q[n]) : 0u;
+        b[n] = i < items ? load_plain(scales + row[n] * (a.per_row / 4) + q[n] / 4) : 0u;
       }
-      T *to = w + row * a.stride + k;
-      if (a.whole && k + 8 <= a.features) {
 #pragma unroll
-        for (int j = 0; j < 8; j += kPer) *reinterpret_cast<uint4 *>(to + j) = *reinterpret_cast<const uint4 *>(t + j);
-      } else {
+      for (int n = 0; n < kAtOnce; ++n) {
+        const int64_t k = (int64_t)q[n] * 8;
+        if (i0 + n * kThreads >= items || k >= a.features) continue;
+        const float scale = b[n] == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(b[n] == 0u ? 0x00400000u : b[n] << 23);
+        T t[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (k + j < a.features) to[j] = t[j];
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t code = c[n] >> (4 * j);
+          const float number = __uint_as_float((code & 7u) << 22) * 0x1p126f * scale;
+          t[j] = dense::from_float<T>(__uint_as_float(__float_as_uint(number) | (code & 8u) << 28));
+        }
+        store_values(w + row[n] * a.stride + k, a.features - k, a.whole, t);
       }
     }
   }
