@@ -81,7 +81,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 template <typename T, int NT, int AHEAD>
 __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<T> a) {
   constexpr int P = kNumbers<T>;
-  extern __shared__ __align__(16) float few_sums[];  // [2][warps][NT][32][4]
+  extern __shared__ __align__(16) float few_sums[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
   const int team = warp / a.sharing, part = warp - team * a.sharing, teams = kFewWarps / a.sharing;
   const int row0 = (int)blockIdx.y * (8 * NT);
@@ -95,14 +95,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
 #pragma unroll
     for (int n = 0; n < NT; ++n) load_x(a, row0 + 8 * n + g, (4 * chunk + j) * kBlock, x[n]);
   };
+  // The codes of a chunk of two outputs of a group.
   auto fetch = [&](int group, int chunk) {
     Codes c = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u), 127, 127};
     const int block = 4 * chunk + j, o = group * 16 + g;
-    if (group < groups && block < a.blocks) {
-      const int64_t at = (int64_t)min(o, a.outputs - 1) * a.blocks + block, bt = (int64_t)min(o + 8, a.outputs - 1) * a.blocks + block;
+    const int64_t at = (int64_t)o * a.blocks + block, bt = at + 8 * (int64_t)a.blocks;
+    if (o < a.outputs && block < a.blocks) {
       c.a = load_plain(reinterpret_cast<const uint4 *>(a.codes) + at);
-      c.b = load_plain(reinterpret_cast<const uint4 *>(a.codes) + bt);
       c.scale_a = load_plain(a.scales + at);
+    }
+    if (o + 8 < a.outputs && block < a.blocks) {
+      c.b = load_plain(reinterpret_cast<const uint4 *>(a.codes) + bt);
       c.scale_b = load_plain(a.scales + bt);
     }
     return c;
@@ -132,26 +135,38 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
       }
     }
   };
+  // The warps' sums of AHEAD groups meet: [AHEAD][warps][NT][32] of 4, twice, so that the next ones need not wait for these to have been read.
+  constexpr int kGroupSums = kFewWarps * NT * 32;
+  float4 *const sums = reinterpret_cast<float4 *>(few_sums);
   uint32_t buffer = 0;
-  auto finish = [&](int group, const float (&sum)[NT][4]) {
-    float4 *const own = reinterpret_cast<float4 *>(few_sums) + (size_t)(buffer * kFewWarps) * (NT * 32);
+  auto leave = [&](int d, const float (&sum)[NT][4]) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) own[(warp * NT + n) * 32 + lane] = make_float4(sum[n][0], sum[n][1], sum[n][2], sum[n][3]);
+    for (int n = 0; n < NT; ++n)
+      sums[(buffer * AHEAD + d) * kGroupSums + (warp * NT + n) * 32 + lane] = make_float4(sum[n][0], sum[n][1], sum[n][2], sum[n][3]);
+  };
+  auto finish = [&](int base, int count) {
     if (a.sharing > 1)
       asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(a.sharing * 32) : "memory");
     else
       __syncwarp();
-    // lane's number i is output g + 8 (i / 2) and row 2 j + i % 2
-    const float *sums = reinterpret_cast<const float *>(own) + (size_t)(team * a.sharing) * (NT * 128);
-    for (int f = part * 32 + lane; f < NT * 128; f += a.sharing * 32) {
-      float v = sums[f];
-      for (int p = 1; p < a.sharing; ++p) v += sums[p * (NT * 128) + f];
-      const int n = f >> 7, of = (f >> 2) & 31, i = f & 3;
-      const int o = group * 16 + (of >> 2) + 8 * (i >> 1), r = row0 + 8 * n + 2 * (of & 3) + (i & 1);
-      if (r < a.rows && o < a.outputs) {
-        v *= kHeld;
-        if (a.bias != nullptr) v += to_float(a.bias[o]);
-        a.y[(int64_t)r * a.outputs + o] = dense::from_float<T>(v);
+    for (int f = part * 32 + lane; f < count * NT * 32; f += a.sharing * 32) {
+      const int of = f & 31, n = f / 32 % NT, d = f / (32 * NT);
+      const float4 *from = sums + (buffer * AHEAD + d) * kGroupSums + (team * a.sharing * NT + n) * 32 + of;
+      float4 v = from[0];
+      for (int p = 1; p < a.sharing; ++p) {
+        const float4 q = from[p * NT * 32];
+        v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
+      }
+      // number i of four is output g + 8 (i / 2) and row 2 j + i % 2 of the lane whose they are
+      const int o = (base + d * stride) * 16 + (of >> 2), row = row0 + 8 * n + 2 * (of & 3);
+      const float each[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int to = o + 8 * (i >> 1), at = row + (i & 1);
+        if (at >= a.rows || to >= a.outputs) continue;
+        float y = each[i] * kHeld;
+        if (a.bias != nullptr) y += to_float(a.bias[to]);
+        a.y[(int64_t)at * a.outputs + to] = dense::from_float<T>(y);
       }
     }
     buffer ^= 1u;  // (the next sums go to the other half, and those after them come after the next barrier)
@@ -163,6 +178,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
     for (int d = 0; d < AHEAD; ++d) ahead[d] = fetch(first + d * stride, part);
     fragments(part);
     for (int base = first; base < groups; base += AHEAD * stride) {
+      int count = 0;
 #pragma unroll
       for (int d = 0; d < AHEAD; ++d) {
         const int group = base + d * stride;
@@ -171,8 +187,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
         ahead[d] = fetch(group + AHEAD * stride, part);
         float sum[NT][4] = {};
         multiply(c, sum);
-        finish(group, sum);
+        leave(d, sum);
+        ++count;
       }
+      finish(base, count);
     }
   } else {
     for (int group = first; group < groups; group += stride) {
@@ -184,7 +202,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) few_rows_kernel(const FewArgs<
         fragments(chunk);
         multiply(c, sum);
       }
-      finish(group, sum);
+      leave(0, sum);
+      finish(group, 1);
     }
   }
 }
@@ -199,7 +218,7 @@ int screen(const ht_dense_problem *p) {
 template <typename T, int NT, int AHEAD>
 int launch_few(const FewArgs<T> &a, cudaStream_t stream) {
   const int groups = (a.outputs + 15) / 16;
-  constexpr size_t kBytes = sizeof(float) * 2 * kFewWarps * NT * 128;
+  constexpr size_t kBytes = sizeof(float) * 2 * AHEAD * kFewWarps * NT * 128;
   const dim3 grid((unsigned)std::min(groups, 148), (unsigned)((a.rows + 8 * NT - 1) / (8 * NT)));
   return dense::launch_next<few_rows_kernel<T, NT, AHEAD>>(grid, kFewThreads, kBytes, kBytes, stream, 1, a);
 }

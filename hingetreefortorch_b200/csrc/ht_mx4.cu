@@ -14,12 +14,13 @@ using dense::after_previous_kernel;
 using dense::load_plain;
 using dense::to_float;
 
-constexpr int kThreads = 256, kItems = 2048;  // of a CTA at a time, about
+constexpr int kThreads = 256, kItems = 1024;  // of a CTA at a time, about
 
 struct Shape {
   int64_t outputs, features, stride;
   int per_row;   // items of 8 features, four for each block
   int rows;      // of a CTA at a time
+  uint32_t magic;  // item i of a CTA is in its row i magic / 2^32
   bool whole;    // rows start on 16 bytes
 };
 
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Shape a, const T *
       int64_t row[kAtOnce];
 #pragma unroll
       for (int n = 0; n < kAtOnce; ++n) {
-        const uint32_t i = i0 + n * kThreads, r = i / (uint32_t)a.per_row;
+        const uint32_t i = i0 + n * kThreads, r = __umulhi(i, a.magic);
         q[n] = i - r * (uint32_t)a.per_row;
         row[n] = row0 + r;
         const int64_t k = (int64_t)q[n] * 8, left = i < items ? a.features - k : 0;
@@ -124,9 +125,10 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Shape a, const T *
 #pragma unroll
       for (int n = 0; n < kAtOnce; ++n) {
         if (i0 + n * kThreads >= items) break;
-        uint32_t top = 0;  // the largest magnitude's bits: no number is above infinity
+        float largest = fabsf(v[n][0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[n][j]) & 0x7fffffffu);
+        for (int j = 1; j < 8; ++j) asm("max.NaN.f32 %0, %1, %2;" : "=f"(largest) : "f"(largest), "f"(fabsf(v[n][j])));
+        uint32_t top = __float_as_uint(largest);  // bits: no number is above infinity
         const uint32_t lanes = 0xfu << (threadIdx.x & 28u);
         top = max(top, __shfl_xor_sync(lanes, top, 1));
         top = max(top, __shfl_xor_sync(lanes, top, 2));
@@ -144,6 +146,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const Shape a, const T *
 template <typename T>
 __global__ void __launch_bounds__(kThreads) unpack_kernel(const Shape a, const uint32_t *codes, const uint8_t *scales, T *w) {
   after_previous_kernel();
+  const uint32_t one = opaque_one();
   for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < a.outputs; row0 += (int64_t)gridDim.x * a.rows) {
     const uint32_t items = (uint32_t)min((int64_t)a.rows, a.outputs - row0) * (uint32_t)a.per_row;
     for (uint32_t i0 = threadIdx.x; i0 < items; i0 += kAtOnce * kThreads) {
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const Shape a, const u
       int64_t row[kAtOnce];
 #pragma unroll
       for (int n = 0; n < kAtOnce; ++n) {
-        const uint32_t i = i0 + n * kThreads, r = i / (uint32_t)a.per_row;
+        const uint32_t i = i0 + n * kThreads, r = __umulhi(i, a.magic);
         q[n] = i - r * (uint32_t)a.per_row;
         row[n] = row0 + r;
         c[n] = i < items ? load_plain(codes + row[n] * a.per_row + q[n]) : 0u;
@@ -161,8 +164,24 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const Shape a, const u
       for (int n = 0; n < kAtOnce; ++n) {
         const int64_t k = (int64_t)q[n] * 8;
         if (i0 + n * kThreads >= items || k >= a.features) continue;
-        const float scale = b[n] == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(b[n] == 0u ? 0x00400000u : b[n] << 23);
-        T t[8];
+        alignas(16) T t[8];
+        if (b[n] < 250u) {  // 40 2^(b - 127) is a number of bf16
+          const uint32_t s = b[n] == 0u ? 0x40u : b[n] << 7, offset = 0x8020u | (b[n] + 5u) << 7;
+          uint32_t w4[4];
+          weights_of(c[n], Scale{s | s << 16, offset | offset << 16}, one, w4);
+          if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            *reinterpret_cast<uint4 *>(t) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              t[2 * j] = dense::from_float<T>(__uint_as_float(w4[j] << 16));
+              t[2 * j + 1] = dense::from_float<T>(__uint_as_float(w4[j] & 0xffff0000u));
+            }
+          }
+          store_values(w + row[n] * a.stride + k, a.features - k, a.whole, t);
+          continue;
+        }
+        const float scale = b[n] == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(b[n] << 23);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t code = c[n] >> (4 * j);
@@ -183,6 +202,8 @@ int shape_of(int dtype, int64_t outputs, int64_t features, int64_t stride, const
   s->outputs = outputs, s->features = features, s->stride = stride;
   s->per_row = (int)(4 * blocks_of(features));
   s->rows = std::max(kItems / s->per_row, 1);
+  // (exact where both items and their number in a row are below 2^16; a row alone is row 0)
+  s->magic = s->rows > 1 ? (uint32_t)((0x100000000ull + (uint64_t)s->per_row - 1) / (uint64_t)s->per_row) : 0u;
   s->whole = (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && stride * size % 16 == 0;
   return HT_OK;
 }
@@ -207,7 +228,7 @@ extern "C" int ht_mx4_pack(int dtype, const void *w, int64_t w_stride, int64_t o
   if ((reinterpret_cast<uintptr_t>(codes) & 15u) != 0) return HT_ERR_UNSUPPORTED;
   return by_type(dtype, [&](auto zero) -> int {
     typedef decltype(zero) T;
-    return dense::launch_next<pack_kernel<T>>(dim3(dense::blocks_for(outputs, s.rows, 148 * 8)), kThreads, 0, 0, reinterpret_cast<cudaStream_t>(stream), 1, s,
+    return dense::launch_next<pack_kernel<T>>(dim3(dense::blocks_for(outputs, s.rows, 148 * 64)), kThreads, 0, 0, reinterpret_cast<cudaStream_t>(stream), 1, s,
                                               static_cast<const T *>(w), static_cast<uint32_t *>(codes), static_cast<uint8_t *>(scales));
   });
 }
@@ -221,7 +242,7 @@ extern "C" int ht_mx4_unpack(int dtype, const void *codes, const void *scales, i
   if ((reinterpret_cast<uintptr_t>(codes) & 15u) != 0) return HT_ERR_UNSUPPORTED;
   return by_type(dtype, [&](auto zero) -> int {
     typedef decltype(zero) T;
-    return dense::launch_next<unpack_kernel<T>>(dim3(dense::blocks_for(outputs, s.rows, 148 * 8)), kThreads, 0, 0, reinterpret_cast<cudaStream_t>(stream), 1,
+    return dense::launch_next<unpack_kernel<T>>(dim3(dense::blocks_for(outputs, s.rows, 148 * 64)), kThreads, 0, 0, reinterpret_cast<cudaStream_t>(stream), 1,
                                                 s, static_cast<const uint32_t *>(codes), static_cast<const uint8_t *>(scales), static_cast<T *>(w));
   });
 }
