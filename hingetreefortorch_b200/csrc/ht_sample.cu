@@ -569,9 +569,10 @@ struct Team {  // C CTAs at work on a row
 
   // The last class of the shortest prefix that reaches `target`, counted (WEIGHTS false) or weighed, among the classes that `base` holds and
   // whose keys are in [low, high]; all others of base are above.  For weights `all` is about what base weighs; `off` is target's error, and *sure
-  // is false where that, or what is summed roughly (but with `exact`), makes a difference.
+  // is false where that, or what is summed roughly (but with `exact`), makes a difference; a target is `share` of what base
+  // weighs.
   template <bool WEIGHTS>
-  __device__ __forceinline__ Last narrow(const Weight &w, const Last &base, uint32_t low, uint32_t high, double target, double off, double all, bool exact, bool *sure) {
+  __device__ __forceinline__ Last narrow(const Weight &w, const Last &base, uint32_t low, uint32_t high, double target, double off, double all, double share, bool exact, bool *sure) {
     double above = 0.0;
     bool by_score = true;
     for (;;) {
@@ -637,38 +638,61 @@ struct Team {  // C CTAs at work on a row
       __syncthreads();
       const uint32_t end_bin = sh.bin[1], first_bin = min(sh.bin[0], end_bin);
       const double window = fmax((double)((sh.bin_after > sh.bin_before ? sh.bin_after : sh.bin_all) - sh.bin_before), 1.0) / scale;
+      // The window's ends as scores: the lowest key whose range is below `bin` (a search by 32 places at a time).
+      auto key_below = [&](uint32_t bin) {
+        uint32_t from = low, to = high + 1u;  // (high is below every key that is not a score's)
+        while (from < to) {
+          const uint32_t step = (to - from + 31u) / 32u, place = from + (uint32_t)lane * step;
+          const uint32_t below = __ballot_sync(0xffffffffu, place < to && range_of(score_of(place)) < bin);  // from some lane on
+          const uint32_t first_below = below != 0u ? (uint32_t)__ffs((int)below) - 1u : (to - from + step - 1u) / step;
+          if (first_below == 0u) return from;
+          const uint32_t next = from + first_below * step;
+          from += (first_below - 1u) * step + 1u;
+          if (below != 0u) to = next;
+        }
+        return to;
+      };
+      const uint32_t key_above = key_below(first_bin), key_inside = key_below(end_bin + 1u);
+      const float inside_score = score_of(key_inside);
+      const bool some_above = key_above <= high;
+      const float above_score = some_above ? score_of(key_above) : CUDART_INF_F;  // from here on: above the window
       double over = 0.0, powers = 0.0;
-      uint32_t least_key = 0xffffffffu, least_gap = 0xffffffffu;  // of the ranges: their keys reach from `lowest` to `highest`
+      uint32_t least_key = 0xffffffffu, least_gap = 0xffffffffu;  // of the window: its keys reach from `lowest` to `highest`
       float of_powers = 0.0f;
+      const bool limited = base.score > -CUDART_INF_F;
       const uint32_t n = list([&](auto &&add) {
-        each_vector_from(low_score, [&](const float (&v)[kPer], int c) {
+        each_vector_from(inside_score, [&](const float (&v)[kPer], int c) {
           float e[kPer];
+          bool some = false;
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            e[i] = 0.0f;
-            if (!inside(v[i], c + i)) continue;
-            const uint32_t range = range_of(v[i]);
-            if (range < first_bin) {
-              if (WEIGHTS && !exact) {
-                float y;
-                e[i] = w.rough(v[i], y);
-                of_powers = fmaf(e[i], -y, of_powers);
-              } else if (WEIGHTS) {
-                over += w(v[i]);
-              } else {
-                e[i] = 1.0f;
-              }
-            } else if (range <= end_bin) {
-              const uint32_t key = key_of(v[i]);
-              least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
-              add(v[i], c + i);
+            const bool up = v[i] >= above_score && v[i] <= high_score && (!limited || v[i] != base.score || c + i <= base.at);
+            if (!WEIGHTS) {
+              e[i] = up ? 1.0f : 0.0f;
+            } else if (exact) {
+              e[i] = 0.0f;
+              if (up) over += w(v[i]);
+            } else {
+              float y;
+              e[i] = w.rough(up ? v[i] : -CUDART_INF_F, y);
+              of_powers = fmaf(e[i], -y, of_powers);
             }
+            some |= v[i] >= inside_score && v[i] < above_score;
           }
 #pragma unroll
           for (int d = kPer / 2; d >= 1; d /= 2)
 #pragma unroll
             for (int i = 0; i < d; ++i) e[i] += e[i + d];
           over += (double)e[0];
+          if (some) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+              if (v[i] >= inside_score && v[i] < above_score && inside(v[i], c + i)) {
+                const uint32_t key = key_of(v[i]);
+                least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
+                add(v[i], c + i);
+              }
+          }
         });
       });
       powers = (double)of_powers;
@@ -683,8 +707,20 @@ struct Team {  // C CTAs at work on a row
         if (WEIGHTS) {
           double weight;
           places = places_below((int)n, w, over, target, off, &weight);
-          if (places < 0) *sure = false, places = places_below((int)n, w, over, target, 0.0);
-          if (over + weight < target + off && end_bin < last_bin) *sure = false;
+          if (places < 0 || !*sure || (over + weight < target + off && end_bin < last_bin)) {  // once more, what is above and what there is in 64 bits
+            double whole = 0.0;
+            over = 0.0;
+            each_from(base.score, [&](float s, int i) {
+              if (!base.holds(s, i)) return;
+              const double one = w(s);
+              whole += one;
+              over += s > high_score || (s >= above_score && s <= high_score) ? one : 0.0;
+            });
+            reduce(whole, over);
+            target = share * whole;
+            *sure = over < target && (over + weight >= target || end_bin == last_bin);
+            places = places_below((int)n, w, over, target, 0.0);
+          }
         } else {
           places = (int)(target - over);
         }
@@ -886,7 +922,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
       team.each_from(from_score, [&](float s, int) { inside += s >= from_score ? 1.0 : 0.0; });
       inside = team.sum(inside);
       bool sure = true;
-      if (inside >= (double)top_k) end = team.template narrow<false>(w, end, from_key, high_key, (double)top_k, 0.0, 1.0, true, &sure);
+      if (inside >= (double)top_k) end = team.template narrow<false>(w, end, from_key, high_key, (double)top_k, 0.0, 1.0, 0.0, true, &sure);
     }
     if (top_p < 1.0) {
       if (by_count && held > 0) {
@@ -906,7 +942,10 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
           }
           if (held == 0) {
             bool sure = true;
-            const Last last = team.template narrow<true>(w, end, max(low_key, key_of(end.score)), high_key, top_p * all.value, top_p * all.off, all.value, exact, &sure);
+            // what weighs less than its part of half of 1 - top_p is not held: all of it together is below that half
+            const double slight = (double)m + temperature * log(fmax(0.49 * (1.0 - top_p) * all.value / (double)a.classes, 1e-35));
+            const uint32_t slight_key = slight > (double)low ? min(key_of(__double2float_rd(slight)), high_key) : low_key;
+            const Last last = team.template narrow<true>(w, end, max(max(low_key, slight_key), key_of(end.score)), high_key, top_p * all.value, top_p * all.off, all.value, top_p, exact, &sure);
             if (sure || exact) {
               end = last;
               break;
