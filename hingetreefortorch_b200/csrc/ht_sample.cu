@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
   const double factor = a.row_temperature == nullptr ? a.factor : fmin(64.0 * 1.4426950408889634 / temperature, 1e300);
   const Weight w = {(double)m, factor, sh.table, m, (float)fmin(factor / 64.0, 3e38)};
 
-  const bool rough_fails = w.c_ < 1e-37f;  // a subnormal factor
+  const bool rough_fails = w.c_ < 1e-37f || w.c_ >= 3e38f;  // a factor that fp32 does not hold
 
   // what counts: up to `end`, the first `held` of the sorted list where that is above 0
   const double tail = fmax((double)low, (double)m + kTail * temperature);

@@ -6,6 +6,7 @@ to some 1e-13 where that decides, and no case here comes that near to a border b
 fp32, 2^-24 of it, and what counts may have been summed in fp32: w = 2^y, y = (s - m) / (T ln 2), with the hardware's exponential (2^-22 of w), sums of
 8 (3 2^-24) and three roundings of y (3 2^-24 |y| ln 2 of w): 2^-22 + 3 2^-24 < 4.2e-7 and 3 2^-24 ln 2 < 1.25e-7 times the mean of |y|.
 """
+import gc
 import math
 
 import pytest
@@ -19,6 +20,14 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 NUMBERS = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def nothing_stays():
+    """What these tests leave in the allocator's cache goes before those that count bytes."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 # ---- packed weights ----------------------------------------------------------------------------------------------------
@@ -236,7 +245,8 @@ def draw(scores, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             at = int(np.flatnonzero(weight > 0)[-1])
         # (not the logarithm of the weight, which may be a subnormal number of few bits)
         classes[r], logs[r] = held[at], (v[held[at]] - v.max()) / (t if t > 0 else 1.0) - np.log(upto[-1])
-        powers[r] = (weight * np.abs(v[held] - v.max()))[weight > 0].sum() / (t if t > 0 else 1.0) / math.log(2) / upto[-1]
+        some = weight > 0
+        powers[r] = (weight[some] * np.abs(v[held][some] - v.max())).sum() / (t if t > 0 else 1.0) / math.log(2) / upto[-1]
     return torch.from_numpy(classes), torch.from_numpy(logs), torch.from_numpy(powers)
 
 
@@ -317,6 +327,17 @@ def test_sample_of_hard_rows(kind, name):
     uniform[2] = 1.0 - 2.0 ** -24
     for bounds in BOUNDS:
         check_draw(s.to(kind), uniform, **bounds)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_sample_at_the_ends_of_the_temperature(kind):
+    gen = generator(11)
+    s, u = normal(gen, 10, 3001, scale=2.0, kind=kind), torch.rand(10, generator=gen, device="cuda")
+    s[3] = (s[3] * 2).round()  # equal scores at the top as well
+    for t in (1e-45, 1e-38, 1e-30, 1e-3, 1e3, 1e30, 3e38):
+        for bounds in (dict(), dict(top_p=0.7), dict(top_k=300, top_p=0.9), dict(min_p=0.5)):
+            check_draw(s, u, temperature=torch.full((10,), t, device="cuda"), **bounds)
+            check_draw(s, u, temperature=t, **bounds)
 
 
 def test_sample_rows_without_an_answer():
