@@ -234,13 +234,61 @@ bool few_rows(int64_t rows) {
   return rows <= (kNumbers<T> == 1 ? 16 : 8);
 }
 
+// ---- many rows of bf16 ------------------------------------------------------------------------------------------------
+// Weights decoded once, into memory, as the tile kernel's operands are (2^-5 of their values), and the pair kernel of ht_dense_tile.cuh.  Decoding is
+// bound by memory: 27 MB in and 102 out for 50000 x 1024, 25 us.
+__global__ void __launch_bounds__(256) decode_kernel(const uint32_t *codes, const uint8_t *scales, uint4 *out, int64_t words) {
+  after_previous_kernel();
+  const uint32_t one = opaque_one();
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
+    uint32_t v[4];
+    weights_of(dense::load_plain(codes + i), scale_of(dense::load_plain(scales + i / 4)), one, v);
+    out[i] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
+template <typename T>
+struct ScoresEpilogue {
+  static constexpr bool kPair = false;
+  struct State {};
+  int rows, cols;
+  const T *bias;
+  T *y;  // [rows, cols]
+  int align;
+  __device__ __forceinline__ void begin(State &, const dense::Where &, bool) const {}
+  __device__ __forceinline__ void unit(State &, const dense::Where &w, int col, float (&v)[32]) const {
+    const int n = cols - col, top = w.row - w.lane;
+    if (n <= 0 || top >= rows) return;
+    float b[32];
+    if (bias != nullptr)
+      dense::load_columns(bias + col, b, n);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], kHeld, bias != nullptr ? b[i] : 0.0f);
+    dense::store_box(w, y + (size_t)top * (size_t)cols + col, (size_t)cols, min(32, rows - top), min(32, n), align, v);
+  }
+  __device__ __forceinline__ void end(State &, const dense::Where &) const {}
+};
+
+// Whether that is the way.  us, decoded for every tile and decoded once, in long loops: 8192 x 1024 to 50000 788 and 660, 1024 rows of it 127 and 112, 512
+// rows 66 and 75; 8192 x 784 to 4096 76 and 53; 8192 x 2048 to 1000 38 and 34; 4096 x 200 to 20000 75 and 73; 8192 x 333 to 1001 19 and 26; 1024 x
+// 1024 to 1000 8 and 13.
+template <typename T>
+bool many_rows(const ht_dense_problem &p) {
+  return kNumbers<T> == 1 && p.rows >= 1024 && (double)p.rows * (double)p.features * (double)p.outputs >= 1e10;
+}
+
 template <typename T>
 struct Plan {
   dense::Operand<T, dense::GradKind<T>> x;
+  dense::Matrix w;  // decoded, where the rows are many
   size_t bytes = 0;
   Plan(const ht_dense_problem &p, const void *xp, void *ws) {
     dense::Arena arena(ws);
     if (!few_rows<T>(p.rows)) x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
+    if (many_rows<T>(p)) {
+      w.rows = p.outputs, w.cols = p.features, w.pitch = blocks_of(p.features) * kBlock;
+      w.data = arena.template take<__nv_bfloat16>(w.rows * w.pitch);
+    }
     bytes = arena.used;
   }
 };
@@ -255,6 +303,20 @@ int forward(const ht_dense_problem &p, const void *x, const void *codes, const v
     int sms = 0;
     HT_TRY(dense::sm_count(&sms));
     HT_TRY(dense::lay_out<T>(stream, plan.x));
+    if constexpr (kNumbers<T> == 1)
+      if (plan.w.data != nullptr) {
+        const int64_t words = p.outputs * blocks_of(p.features) * 4;
+        HT_TRY((dense::launch_next<decode_kernel>(dim3(dense::blocks_for(words, 1024, 148 * 16)), 256, 0, 0, stream, 1, static_cast<const uint32_t *>(codes),
+                                                  static_cast<const uint8_t *>(scales), static_cast<uint4 *>(const_cast<void *>(plan.w.data)), words)));
+        dense::TileProblem t;
+        t.a[0] = plan.x.m;
+        t.b[0] = plan.w;
+        t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
+        t.status_word = status_word;
+        const ScoresEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), static_cast<T *>(y),
+                                     dense::row_alignment(y, p.outputs * (int64_t)sizeof(T))};
+        return dense::launch_tiles<1, false, false>(t, e, dense::tile_shape(p.rows, p.outputs, p.features, 1, false), sms, stream);
+      }
     return launch_tiles<T, kNumbers<T>>(plan.x.m, codes, static_cast<const uint8_t *>(scales), static_cast<const T *>(bias), static_cast<T *>(y), p.rows,
                                         p.features, p.outputs, status_word, sms, stream);
   }

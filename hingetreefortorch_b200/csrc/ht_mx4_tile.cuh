@@ -17,7 +17,8 @@
 // Tensor memory: two accumulators in turn (three numbers: of two parts each), and 4 stages of 32 columns of weights.
 // With three numbers the products of the first one have an accumulator, those of the others, 2^-8 of them, a second; both leave for
 // registers every 256 values of k and are added there in fp32 (the tensor core truncates when it adds; ht_dense_tile.cuh).
-// What bounds it: power and the tensor pipe with many rows (8192 x 1024 to 50000 of bf16: 680 to 690 us, 1220 TFLOP/s, where cuBLAS keeps 1376 up);
+// What bounds it: power and the tensor pipe with many rows (8192 x 1024 to 50000 of bf16: 680 to 690 us in a burst, 1220 TFLOP/s, and 790 in a
+// long loop; ht_linear_mx4.cu decodes once there);
 // with few the decoding, 280 cycles for a stage (64 rows 17 us, 17 rows 16.7).  The product with both operands in shared memory needs 48 cycles for 16
 // values of k and 64 columns, this one 32, and 96 with 192, the tensor core's own rate.
 // A tile starts with the first stage of the ring: the last box of a tile may leave stages out.  Every wait is bounded, as in ht_dense_tile.cuh.

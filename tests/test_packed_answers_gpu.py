@@ -182,6 +182,24 @@ def test_linear_by_scale(kind, rows):
     assert torch.isnan(got[:, 7]).all() and not torch.isnan(got[:, :7]).any() and not torch.isnan(got[:, 8:]).any()
 
 
+@pytest.mark.parametrize("rows,features,outputs,apart", [(1024, 1024, 10007, 1024), (1100, 519, 20011, 519), (2050, 200, 26000, 211), (5000, 2049, 1001, 2056)])
+def test_linear_of_many_rows(rows, features, outputs, apart):
+    """bf16 rows and products enough that the weights are decoded once, into memory; blocks of every size, one that holds no number."""
+    gen = generator(rows)
+    wide = normal(gen, rows, apart, kind=torch.bfloat16)
+    codes, scales = F.pack_mx4(normal(gen, outputs, features, scale=1 / math.sqrt(features)))
+    bias = normal(gen, outputs, scale=0.5, kind=torch.bfloat16)
+    first = check_linear(wide[:, :features], codes, scales, bias)
+    assert torch.equal(first, F.linear_mx4(wide[:, :features].contiguous(), codes, scales, bias))
+    for low, high, size in ((0, 40, 2.0 ** 15), (190, 254, 2.0 ** -104)):
+        scales = torch.randint(low, high, scales.shape, generator=gen, device="cuda", dtype=torch.int32).to(torch.uint8)
+        check_linear(wide[:, :features] * size, codes, scales, None)
+    scales[7, -1] = 255
+    got = F.linear_mx4(wide[:, :features] * size, codes, scales)
+    assert torch.isnan(got[:, 7]).all() and not torch.isnan(got[:, :7]).any() and not torch.isnan(got[:, 8:]).any()
+    assert hingetree_cpp.pipeline_status() == 0
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_linear_strides_and_shapes(kind):
     x, codes, scales, bias = linear_inputs(kind, 60, 200, 90)
