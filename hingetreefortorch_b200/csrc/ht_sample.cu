@@ -16,8 +16,8 @@
 //   top_k   up to 200: every thread has the maxima of 4 parts of what it has read; the one of about place k among those, found by halving the
 //           range, bounds the k-th largest score from below, and not many more classes than k are above it
 //   top_p   the same with the first 192 classes, where those hold enough
-//   else    classes are counted, or their weights summed roughly, by 2048 ranges of the score's bits; the range with the place in it is listed, or
-//           divided again, or is one score
+//   else    classes are counted, or their weights summed, by 2048 ranges of the score or of its bits; the ranges that the place may be in are listed, or
+//           divided again, or are one score
 // What counts of a list is drawn from there; otherwise the row is summed in order, warp by warp, and one warp walks its part.
 // CTAs of a cluster exchange sums, counts, ranges and lists through each other's shared memory and all come to the same decisions.  No sum depends on
 // the order of atomic additions: the same call gives the same bits.
@@ -87,7 +87,7 @@ struct alignas(16) Shared {
   uint32_t words[2][kMostWarps], lows[2][kMostWarps];
   double cta_sums[2][kMostCtas][2];
   uint32_t cta_words[2][kMostCtas], cta_lows[2][kMostCtas];
-  uint32_t count, bin[2], bin_before, bin_after, bin_all;
+  uint32_t count, bin[2];
   uint32_t ranks[kCounted];
   union {
     uint64_t list[kList];
@@ -568,24 +568,26 @@ struct Team {  // C CTAs at work on a row
   }
 
   // The last class of the shortest prefix that reaches `target`, counted (WEIGHTS false) or weighed, among the classes that `base` holds and
-  // whose keys are in [low, high]; all others of base are above.  For weights `all` is about what base weighs; `off` is target's error, and *sure
-  // is false where that, or what is summed roughly (but with `exact`), makes a difference; a target is `share` of what base
-  // weighs.
-  template <bool WEIGHTS>
-  __device__ __forceinline__ Last narrow(const Weight &w, const Last &base, uint32_t low, uint32_t high, double target, double off, double all, double share, bool exact, bool *sure) {
+  // whose keys are in [low, high]; all others of base are above, or weigh too little to matter.  For weights `all` is what base weighs; `off` is
+  // target's error, and *sure is false, whatever comes back, where that or what is summed roughly makes a difference (never with EXACT: then all
+  // that is weighed or counted in units is, in 64 bits); a target is `share` of what base weighs.  Two pieces of code, so that rows of rough weights carry
+  // none of the other's (4096 rows of 21841 with wide nuclei 781 us; 917 with the choice at each weight, 793 with the 64-bit one as a call).
+  template <bool WEIGHTS, bool EXACT>
+  __device__ __forceinline__ Last narrow(const Weight &w, const Last &base, uint32_t low, uint32_t high, double target, double off, double all, double share, bool *sure) {
     double above = 0.0;
-    bool by_score = true;
+    uint32_t classes = (uint32_t)row.classes;  // in [low, high], at the most
+    bool by_score = true, split_by_score = true, more_below = false;
     for (;;) {
-      // By ranges, highest first: of the score at first, over which scores are spread more evenly, and then of its key.  Weights are counted in units
-      // of 2^-31 of what there is.
+      // By ranges, highest first: of the score at first, over which scores are spread more evenly, then of its key, and so on in turn.  Weights
+      // are counted in units of 2^-31 of what is in [low, high], so that a count is below 2^32 with half a unit more for each of 2^30 classes.
       const uint32_t width = high - low;
       const int shift = max(0, 21 - (int)__clz((int)width));
-      const float slope = by_score ? ((float)kBins - 1.0f) / (w.m_ - score_of(low)) : 0.0f;
-      const uint32_t last_bin = by_score ? (uint32_t)kBins - 1u : width >> shift;
       const float low_score = score_of(low), high_score = score_of(high);
+      const float slope = by_score ? ((float)kBins - 1.0f) / (high_score - low_score) : 0.0f;
+      const uint32_t last_bin = by_score ? (uint32_t)kBins - 1u : width >> shift;
       auto inside = [&](float s, int i) { return s >= low_score && s <= high_score && (s != base.score || i <= base.at); };
-      auto range_of = [&](float s) { return by_score ? min((uint32_t)((w.m_ - s) * slope), last_bin) : (high - key_of(s)) >> shift; };
-      const double scale = 2147483648.0 / all;
+      auto range_of = [&](float s) { return by_score ? min((uint32_t)((high_score - s) * slope), last_bin) : (high - key_of(s)) >> shift; };
+      const double scale = fmin(2147483648.0 / all, 1e30);  // (as fp32 as well)
       const float scale_ = (float)scale;
       meet();
       for (int i = (int)threadIdx.x; i < kBins; i += (int)blockDim.x) sh.bins[i] = 0;
@@ -593,7 +595,7 @@ struct Team {  // C CTAs at work on a row
       each_from(low_score, [&](float s, int i) {
         if (inside(s, i)) {
           float y;
-          atomicAdd(&sh.bins[range_of(s)], WEIGHTS ? (uint32_t)fmaf(w.rough(s, y), scale_, 0.5f) : 1u);
+          atomicAdd(&sh.bins[range_of(s)], !WEIGHTS ? 1u : EXACT ? (uint32_t)fma(w(s), scale, 0.5) : (uint32_t)fmaf(w.rough(s, y), scale_, 0.5f));
         }
       });
       meet();
@@ -609,10 +611,17 @@ struct Team {  // C CTAs at work on a row
         bins = together;
         meet();  // (the CTAs' own have been read: their place is the list's)
       }
-      // The ranges between which the sum reaches the target: rough weights are off by 2^-16 of themselves (|y| is below 116 here) and half a unit.
-      const uint32_t slack = WEIGHTS ? 32768u + (uint32_t)row.classes / 2u + 2u : 0u;
-      const uint32_t wanted = WEIGHTS ? (uint32_t)fmin(fmax((target - above) * scale, 1.0), 2147483647.0) : (uint32_t)(target - above);
-      const uint32_t wanted_low = wanted > slack ? wanted - slack : 1u, wanted_high = wanted + slack;
+      // The ranges between which the sum reaches the target.  Counts are bounds of weights and not weights: each class is off by half a unit, and rough
+      // weights by 2^-16 of themselves (|y| is below 116 here).  A sum that is in reach of nothing at all starts with the first range, whose
+      // classes may all count 0, and one that is not reached ends with the last.
+      uint32_t wanted_low, wanted_high;
+      if constexpr (WEIGHTS) {
+        const double slack = (EXACT ? 0.0 : 32768.0) + 0.5 * (double)classes + 2.0;
+        wanted_low = (uint32_t)fmin(fmax((target - off - above) * scale - slack, 0.0), 4294967295.0);
+        wanted_high = (uint32_t)fmin(fmax((target + off - above) * scale + slack, 1.0), 4294967295.0);
+      } else {
+        wanted_low = wanted_high = (uint32_t)(target - above);
+      }
       const int per = kBins / (int)blockDim.x;  // of a thread
       uint32_t own = 0;
       for (int i = 0; i < per; ++i) own += bins[(int)threadIdx.x * per + i];
@@ -623,21 +632,19 @@ struct Team {  // C CTAs at work on a row
         if (lane >= d) upto += t;
       }
       if (lane == 31) sh.words[turn][warp] = upto;
-      if (threadIdx.x == 0) sh.bin[0] = sh.bin[1] = last_bin, sh.bin_before = sh.bin_after = 0;
+      if (threadIdx.x == 0) sh.bin[0] = 0, sh.bin[1] = last_bin;
       __syncthreads();
       uint32_t at = upto - own;
       for (int i = 0; i < warp; ++i) at += sh.words[turn][i];
       turn ^= 1u;
       for (int i = 0; i < per; ++i) {
         const uint32_t one = bins[(int)threadIdx.x * per + i];
-        if (at < wanted_low && wanted_low <= at + one) sh.bin[0] = (uint32_t)((int)threadIdx.x * per + i), sh.bin_before = at;
-        if (at < wanted_high && wanted_high <= at + one) sh.bin[1] = (uint32_t)((int)threadIdx.x * per + i), sh.bin_after = at + one;
+        if (at < wanted_low && wanted_low <= at + one) sh.bin[0] = (uint32_t)((int)threadIdx.x * per + i);
+        if (at < wanted_high && wanted_high <= at + one) sh.bin[1] = (uint32_t)((int)threadIdx.x * per + i);
         at += one;
       }
-      if ((int)threadIdx.x == (int)blockDim.x - 1) sh.bin_all = at;
       __syncthreads();
       const uint32_t end_bin = sh.bin[1], first_bin = min(sh.bin[0], end_bin);
-      const double window = fmax((double)((sh.bin_after > sh.bin_before ? sh.bin_after : sh.bin_all) - sh.bin_before), 1.0) / scale;
       // The window's ends as scores: the lowest key whose range is below `bin` (a search by 32 places at a time).
       auto key_below = [&](uint32_t bin) {
         uint32_t from = low, to = high + 1u;  // (high is below every key that is not a score's)
@@ -656,7 +663,7 @@ struct Team {  // C CTAs at work on a row
       const float inside_score = score_of(key_inside);
       const bool some_above = key_above <= high;
       const float above_score = some_above ? score_of(key_above) : CUDART_INF_F;  // from here on: above the window
-      double over = 0.0, powers = 0.0;
+      double over = 0.0, powers = 0.0, within = 0.0;  // what is above the window weighs, and the window
       uint32_t least_key = 0xffffffffu, least_gap = 0xffffffffu;  // of the window: its keys reach from `lowest` to `highest`
       float of_powers = 0.0f;
       const bool limited = base.score > -CUDART_INF_F;
@@ -669,7 +676,7 @@ struct Team {  // C CTAs at work on a row
             const bool up = v[i] >= above_score && v[i] <= high_score && (!limited || v[i] != base.score || c + i <= base.at);
             if (!WEIGHTS) {
               e[i] = up ? 1.0f : 0.0f;
-            } else if (exact) {
+            } else if (EXACT) {
               e[i] = 0.0f;
               if (up) over += w(v[i]);
             } else {
@@ -690,6 +697,10 @@ struct Team {  // C CTAs at work on a row
               if (v[i] >= inside_score && v[i] < above_score && inside(v[i], c + i)) {
                 const uint32_t key = key_of(v[i]);
                 least_key = min(least_key, key), least_gap = min(least_gap, 0xffffffffu - key);
+                if (WEIGHTS) {
+                  float y;
+                  within += EXACT ? w(v[i]) : (double)w.rough(v[i], y);
+                }
                 add(v[i], c + i);
               }
           }
@@ -697,17 +708,18 @@ struct Team {  // C CTAs at work on a row
       });
       powers = (double)of_powers;
       reduce(over, powers);
-      if (WEIGHTS && !exact) off += 1.01 * (Weight::kOff * over + Weight::kOffPower * powers);
+      if (WEIGHTS && !EXACT) off += 1.01 * (Weight::kOff * over + Weight::kOffPower * powers);
       over += above;
       if (WEIGHTS && over >= target - off) *sure = false;
-      if (n == 0u) return {score_of(low), kPassed};
+      more_below |= key_inside > low;
+      if (n == 0u) return {low_score, low_score == base.score ? base.at : kPassed};
       if (n <= (uint32_t)kList) {
         sort((int)n);
         int places;
         if (WEIGHTS) {
           double weight;
           places = places_below((int)n, w, over, target, off, &weight);
-          if (places < 0 || !*sure || (over + weight < target + off && end_bin < last_bin)) {  // once more, what is above and what there is in 64 bits
+          if (!EXACT && (places < 0 || !*sure || (over + weight < target + off && more_below))) {  // once more, what is above and what there is in 64 bits
             double whole = 0.0;
             over = 0.0;
             each_from(base.score, [&](float s, int i) {
@@ -718,7 +730,7 @@ struct Team {  // C CTAs at work on a row
             });
             reduce(whole, over);
             target = share * whole;
-            *sure = over < target && (over + weight >= target || end_bin == last_bin);
+            *sure = over < target && (over + weight >= target || !more_below);
             places = places_below((int)n, w, over, target, 0.0);
           }
         } else {
@@ -731,31 +743,47 @@ struct Team {  // C CTAs at work on a row
         const float s = score_of(lowest);
         const double one = WEIGHTS ? w(s) : 1.0, missing = target - over;
         auto places = [&](double left) { return one * n <= left ? n : (uint32_t)fmax(ceil(left / one), 1.0); };
-        if (WEIGHTS && (places(missing - off) != places(missing + off) || (over + one * n < target + off && end_bin < last_bin))) *sure = false;
+        if (WEIGHTS && (places(missing - off) != places(missing + off) || (over + one * n < target + off && more_below))) *sure = false;
         // (among those that base holds the first ones are the first ones of all)
         return {s, nth_of(s, places(missing))};
       }
-      if (WEIGHTS) all = window;
-      if (!by_score && lowest == low && highest == high) {  // the rough weights do not tell: half of the range, by exact ones
-        const uint32_t middle = low + (high - low) / 2u;
-        double upper = 0.0;
-        const float middle_score = score_of(middle);
-        each_from(low_score, [&](float s, int i) {
-          if (inside(s, i) && s > middle_score) upper += WEIGHTS ? w(s) : 1.0;
-        });
-        upper = sum(upper);
-        if (over + upper < target) {
-          above = over + upper;
-          high = middle;
-        } else {
-          above = over;
-          low = middle + 1u;
-        }
-        continue;
-      }
       low = lowest, high = highest;
       above = over;
-      by_score = false;
+      classes = n;
+      if constexpr (WEIGHTS) {
+        const bool wide = first_bin == 0u && end_bin == last_bin;  // the counts tell nothing
+        if (!EXACT && (wide || !*sure)) {
+          *sure = false;
+          return {low_score, kPassed};
+        }
+        all = sum(within) * (EXACT ? 1.0 : 1.0 + 0x1p-15);
+        if (EXACT && wide) {  // one class may weigh all of the units: half of the scores, or of their keys in turn, by what they weigh
+          uint32_t middle = low + (high - low) / 2u;
+          if (split_by_score) middle = min(max(key_of(0.5f * score_of(low) + 0.5f * score_of(high)), low), high - 1u);
+          split_by_score = !split_by_score;
+          const float middle_score = score_of(middle), lowest_score = score_of(low);
+          double upper = 0.0, lower = 0.0;
+          uint32_t uppers = 0, above_middle = 0xffffffffu, below_middle = 0xffffffffu;
+          each_from(lowest_score, [&](float s, int i) {
+            if (!(s >= lowest_score) || !inside(s, i) || key_of(s) > high) return;
+            const uint32_t key = key_of(s);
+            if (s > middle_score)
+              upper += w(s), ++uppers, above_middle = min(above_middle, key);
+            else
+              lower += w(s), below_middle = min(below_middle, 0xffffffffu - key);
+          });
+          reduce(upper, lower);
+          uppers = words<false>(uppers), above_middle = words<true>(above_middle), below_middle = 0xffffffffu - words<true>(below_middle);
+          if (above + upper < target) {
+            above += upper, high = below_middle, all = lower, classes -= uppers;
+          } else {
+            low = above_middle, all = upper, classes = uppers, more_below = true;
+          }
+          by_score = true;
+          continue;
+        }
+      }
+      by_score = !by_score;
     }
   }
 };
@@ -922,7 +950,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
       team.each_from(from_score, [&](float s, int) { inside += s >= from_score ? 1.0 : 0.0; });
       inside = team.sum(inside);
       bool sure = true;
-      if (inside >= (double)top_k) end = team.template narrow<false>(w, end, from_key, high_key, (double)top_k, 0.0, 1.0, 0.0, true, &sure);
+      if (inside >= (double)top_k) end = team.template narrow<false, true>(w, end, from_key, high_key, (double)top_k, 0.0, 1.0, 0.0, &sure);
     }
     if (top_p < 1.0) {
       if (by_count && held > 0) {
@@ -945,7 +973,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
             // what weighs less than its part of half of 1 - top_p is not held: all of it together is below that half
             const double slight = (double)m + temperature * log(fmax(0.49 * (1.0 - top_p) * all.value / (double)a.classes, 1e-35));
             const uint32_t slight_key = slight > (double)low ? min(key_of(__double2float_rd(slight)), high_key) : low_key;
-            const Last last = team.template narrow<true>(w, end, max(max(low_key, slight_key), key_of(end.score)), high_key, top_p * all.value, top_p * all.off, all.value, top_p, exact, &sure);
+            const uint32_t from_key = max(max(low_key, slight_key), key_of(end.score));
+            const Last last = exact ? team.template narrow<true, true>(w, end, from_key, high_key, top_p * all.value, 0.0, all.value, top_p, &sure)
+                                    : team.template narrow<true, false>(w, end, from_key, high_key, top_p * all.value, top_p * all.off, all.value, top_p, &sure);
             if (sure || exact) {
               end = last;
               break;
