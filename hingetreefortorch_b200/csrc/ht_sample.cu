@@ -25,6 +25,8 @@
 
 #include <math_constants.h>
 
+#include <cstddef>
+
 namespace ht {
 namespace sample {
 namespace {
@@ -54,8 +56,11 @@ struct Args {
   uint32_t row_bytes;  // of shared memory for a row, or a CTA's part of it
 };
 
-// 2^(k / 64), rounded to nearest.
-__device__ const double kPowers[64] = {
+// 2^(k / 64), rounded to nearest; copied 16 bytes at a time.
+struct alignas(16) Powers {
+  double of[64];
+};
+__device__ const Powers kPowers = {{
     0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
     0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
     0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
@@ -72,7 +77,7 @@ __device__ const double kPowers[64] = {
     0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
     0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
     0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
-};
+}};
 
 // Larger for larger scores; both zeros are one score.
 __device__ __forceinline__ uint32_t key_of(float s) {
@@ -823,8 +828,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) sample_kernel(const Args a) {
     }
     team.row.shared = to;
   }
+  static_assert(alignof(Powers) >= 16 && alignof(Shared) >= 16 && offsetof(Shared, table) % 16 == 0, "16 bytes are copied from and to here");
   if (threadIdx.x < 32)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_addr(sh.table) + 16u * threadIdx.x), "l"(kPowers + 2 * threadIdx.x) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_addr(sh.table) + 16u * threadIdx.x), "l"(kPowers.of + 2 * threadIdx.x) : "memory");
   const double temperature = a.row_temperature != nullptr ? (double)load_plain(a.row_temperature + r) : a.temperature;
   const double top_p = a.row_top_p != nullptr ? (double)load_plain(a.row_top_p + r) : a.top_p;
   const double min_p = a.row_min_p != nullptr ? (double)load_plain(a.row_min_p + r) : a.min_p;
