@@ -94,6 +94,7 @@ torch::Tensor linear_mx4(const torch::Tensor &x_, const torch::Tensor &codes_, c
 // A bound of sample_classes: one number for all rows, or a tensor with one a row.
 struct Bound {
   double number = 0.0;
+  int64_t count = 0;  // of one that is a whole number: not every one is a double
   torch::Tensor rows;
 };
 Bound bound_of(const pybind11::object &value, const char *name, torch::ScalarType type, const torch::Tensor &uniform) {
@@ -109,7 +110,10 @@ Bound bound_of(const pybind11::object &value, const char *name, torch::ScalarTyp
     return b;
   }
   try {
-    b.number = type == torch::kInt64 ? (double)pybind11::cast<int64_t>(value) : pybind11::cast<double>(value);
+    if (type == torch::kInt64)
+      b.count = pybind11::cast<int64_t>(value);
+    else
+      b.number = pybind11::cast<double>(value);
   } catch (const pybind11::cast_error &) {
     bad_argument(std::string("Error: ") + name + " must be a number or a tensor with one for each row.");
   }
@@ -126,7 +130,7 @@ std::vector<torch::Tensor> sample_classes(const torch::Tensor &scores_, const to
   const Bound t = bound_of(temperature, "temperature", torch::kFloat32, uniform_), k = bound_of(top_k, "top_k", torch::kInt64, uniform_),
               p = bound_of(top_p, "top_p", torch::kFloat32, uniform_), least = bound_of(min_p, "min_p", torch::kFloat32, uniform_);
   if (!t.rows.defined() && !(t.number >= 0.0 && std::isfinite(t.number))) bad_argument("Error: the temperature must be finite, and 0 at the least.");
-  if (!k.rows.defined() && k.number < 0.0) bad_argument("Error: top_k must be 0 (all classes) or more.");
+  if (!k.rows.defined() && k.count < 0) bad_argument("Error: top_k must be 0 (all classes) or more.");
   if (!p.rows.defined() && !(p.number >= 0.0 && p.number <= 1.0)) bad_argument("Error: top_p must be between 0 and 1.");
   if (!least.rows.defined() && !(least.number >= 0.0 && least.number <= 1.0)) bad_argument("Error: min_p must be between 0 and 1.");
   require_cuda(scores_);
@@ -143,7 +147,7 @@ std::vector<torch::Tensor> sample_classes(const torch::Tensor &scores_, const to
   problem.rows = scores.size(0), problem.classes = scores.size(1);
   problem.stride = scores.size(0) > 1 ? scores.stride(0) : scores.size(1);
   problem.temperature = t.number, problem.top_p = p.number, problem.min_p = least.number;
-  problem.top_k = (int64_t)k.number;
+  problem.top_k = k.count;
   auto rows_of = [](const Bound &b) { return b.rows.defined() ? b.rows.const_data_ptr<float>() : nullptr; };
   problem.row_temperature = rows_of(t), problem.row_top_p = rows_of(p), problem.row_min_p = rows_of(least);
   problem.row_top_k = k.rows.defined() ? k.rows.const_data_ptr<int64_t>() : nullptr;
