@@ -171,6 +171,9 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const Shape a, const u
           const uint32_t s = b[n] == 0u ? 0x40u : b[n] << 7, offset = 0x8020u | (b[n] + 5u) << 7;
           uint32_t w4[4];
           weights_of(c[n], Scale{s | s << 16, offset | offset << 16}, one, w4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // (40 + v) s - 40 s is 0 for both zeros: the sign is the code's
+            w4[j] |= __byte_perm(c[n] << 4, c[n], 0x4000u + 0x1010u * (uint32_t)j) & 0x80008000u;
           if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             *reinterpret_cast<uint4 *>(t) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           } else {

@@ -18,3 +18,21 @@ def test_top_k_up_to_the_largest_whole_number():
         for top_k in (k, torch.full((5,), k, device="cuda")):
             got = F.sample_classes(s, u, top_k=top_k, top_p=0.9)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float16])
+def test_unpacked_zeros_have_the_sign_of_their_code(kind):
+    """Under every scale and at every place of 8 codes, in rows that start on 16 bytes and on fewer; what is packed again is the same."""
+    gen = generator(3)
+    codes = torch.randint(0, 256, (255, 64), generator=gen, device="cuda", dtype=torch.int32).to(torch.uint8)
+    codes[:, :16] = 0x80
+    codes[:, 16:32] = 0x08
+    scales = torch.arange(255, device="cuda", dtype=torch.uint8).view(255, 1).repeat(1, 4)
+    each = torch.stack([codes & 15, codes >> 4], 2).flatten(1)
+    for features in (128, 127, 101):
+        got = F.unpack_mx4(codes, scales, features, dtype=kind)
+        assert torch.equal(torch.signbit(got), each[:, :features] >= 8)
+    w = torch.zeros(3, 64, dtype=kind, device="cuda")
+    w[:, ::3] = -0.0
+    w[1, 5], w[2, 6] = 1.0, -2.0 ** -14
+    assert torch.equal(torch.signbit(F.unpack_mx4(*F.pack_mx4(w), 64, dtype=kind)), torch.signbit(w))
