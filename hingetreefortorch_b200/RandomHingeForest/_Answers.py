@@ -12,8 +12,9 @@ from .. import HingeTree as _F
 class PackedClasses(nn.Module):
     """A class head for answers: nn.Linear whose weight is held as 4-bit numbers with a power of two for each 32 features
     (HingeTree.pack_mx4), 17 bytes for 32 of them.  Buffers ``codes``, ``scales`` (uint8) and, with bias, ``bias``; no parameters, no derivative.
-    x: [..., in_features] in the bias's type (without one: torch.float32, bfloat16 or float16); forward(x) gives the class scores, sample(x, uniform, ...)
-    a class drawn from them and the logarithm of its share (HingeTree.sample_classes).
+    x: [..., in_features] in the bias's type (without one: torch.float32, bfloat16 or float16); forward(x) gives the class scores (x that requires a
+    gradient is refused while gradients are recorded), sample(x, uniform, ...) a class drawn from them and the logarithm of its share
+    (HingeTree.sample_classes), without a gradient whatever x requires.
 
     PackedClasses.of(weight, bias) packs a layer's; LinearClassLoss.packed() and RandomHingeForestFusedLinear.packed_classes() give theirs."""
 
@@ -40,6 +41,7 @@ class PackedClasses(nn.Module):
 
     scores = forward
 
+    @torch.no_grad()
     def sample(self, x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return _F.sample_classes(self(x), uniform, temperature, top_k, top_p, min_p)
 

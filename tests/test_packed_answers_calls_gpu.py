@@ -4,7 +4,7 @@ import sys
 import pytest
 import torch
 
-from hingetreefortorch_b200 import HingeTree as F
+from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R
 from test_dense_gpu import generator, normal
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +36,25 @@ def test_unpacked_zeros_have_the_sign_of_their_code(kind):
     w[:, ::3] = -0.0
     w[1, 5], w[2, 6] = 1.0, -2.0 ** -14
     assert torch.equal(torch.signbit(F.unpack_mx4(*F.pack_mx4(w), 64, dtype=kind)), torch.signbit(w))
+
+
+def test_packed_head_draws_for_features_that_require_a_gradient():
+    """As the heads that it was packed from do: nothing drawn has a derivative."""
+    gen = generator(4)
+    head = R.LinearClassLoss(100, 300).cuda()
+    packed = head.packed()
+    x, u = normal(gen, 20, 100), torch.rand(20, generator=gen, device="cuda")
+    want = packed.sample(x, u, top_k=5)
+    for bounds in (dict(top_k=5), dict(top_k=5, temperature=torch.ones(20, device="cuda", requires_grad=True))):
+        leaf = x.clone().requires_grad_()
+        got = packed.sample(leaf, u, **bounds)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and not got[1].requires_grad
+        head.sample(leaf, u, **bounds)
+    forest = R.RandomHingeForestFusedLinear(12, 70, 30, 4).cuda()
+    rows, v = torch.randn(9, 12, generator=gen, device="cuda"), torch.rand(9, generator=gen, device="cuda")
+    packed = forest.packed_classes()
+    features = forest._function.apply(rows, *forest._tree_params())
+    assert features.requires_grad
+    assert torch.equal(packed.sample(features, v)[0], forest.sample(rows, v, packed=packed)[0])
+    with pytest.raises(RuntimeError, match="no derivative"):
+        packed(features)
