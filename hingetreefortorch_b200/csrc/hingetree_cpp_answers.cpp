@@ -80,8 +80,19 @@ torch::Tensor linear_mx4(const torch::Tensor &x_, const torch::Tensor &codes_, c
   p.rows = x.size(0), p.features = x.size(1), p.outputs = codes.size(0);
   p.x_stride = x.size(0) > 1 ? x.stride(0) : x.size(1);
   torch::Tensor y = fresh({p.rows, p.outputs}, x);
-  const size_t bytes = ht_linear_mx4_workspace_bytes(&p);
-  const torch::Tensor ws = bytes > 0 ? make_workspace(bytes, x) : torch::Tensor();  // (an allocation is a fifth of a small call)
+  size_t bytes = ht_linear_mx4_workspace_bytes(&p);
+  torch::Tensor ws;
+  if (bytes > 0) {  // (an allocation is a fifth of a small call)
+    try {
+      ws = make_workspace(bytes, x);
+    } catch (const c10::OutOfMemoryError &) {  // without decoded weights
+      p.scratch_limit = 1;
+      const size_t least = ht_linear_mx4_workspace_bytes(&p);
+      if (least >= bytes) throw;
+      bytes = least;
+      if (bytes > 0) ws = make_workspace(bytes, x);
+    }
+  }
   raise_status(ht_linear_mx4(&p, x.const_data_ptr(), codes.const_data_ptr(), scales.const_data_ptr(), pointer(bias), y.data_ptr(), bytes > 0 ? ws.data_ptr() : nullptr, bytes,
                              long_lived_word(x), current_stream(x)),
                "linear_mx4");

@@ -253,7 +253,8 @@ struct ScoresEpilogue {
   struct State {};
   int rows, cols;
   const T *bias;
-  T *y;  // [rows, cols]
+  T *y;  // [rows, cols], `pitch` from row to row
+  int64_t pitch;
   int align;
   __device__ __forceinline__ void begin(State &, const dense::Where &, bool) const {}
   __device__ __forceinline__ void unit(State &, const dense::Where &w, int col, float (&v)[32]) const {
@@ -264,7 +265,7 @@ struct ScoresEpilogue {
       dense::load_columns(bias + col, b, n);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], kHeld, bias != nullptr ? b[i] : 0.0f);
-    dense::store_box(w, y + (size_t)top * (size_t)cols + col, (size_t)cols, min(32, rows - top), min(32, n), align, v);
+    dense::store_box(w, y + (size_t)top * (size_t)pitch + col, (size_t)pitch, min(32, rows - top), min(32, n), align, v);
   }
   __device__ __forceinline__ void end(State &, const dense::Where &) const {}
 };
@@ -273,20 +274,31 @@ struct ScoresEpilogue {
 // rows 66 and 75; 8192 x 784 to 4096 76 and 53; 8192 x 2048 to 1000 38 and 34; 4096 x 200 to 20000 75 and 73; 8192 x 333 to 1001 19 and 26; 1024 x
 // 1024 to 1000 8 and 13.
 template <typename T>
-bool many_rows(const ht_dense_problem &p) {
-  return kNumbers<T> == 1 && p.rows >= 1024 && (double)p.rows * (double)p.features * (double)p.outputs >= 1e10;
+bool many_rows(const ht_dense_problem &p, int64_t outputs) {
+  return kNumbers<T> == 1 && p.rows >= 1024 && (double)p.rows * (double)p.features * (double)outputs >= 1e10;
+}
+// Outputs that are decoded at a time: what the caller's limit holds of them, whole tiles; 0 where that is not the way, or where a piece is
+// too little work for it.
+constexpr int64_t kDecodedBytes = (int64_t)512 << 20;
+template <typename T>
+int64_t decoded_outputs(const ht_dense_problem &p) {
+  const int64_t limit = p.scratch_limit > 0 ? std::min(p.scratch_limit, kDecodedBytes) : kDecodedBytes;
+  const int64_t most = limit / (blocks_of(p.features) * kBlock * (int64_t)sizeof(__nv_bfloat16));
+  const int64_t piece = p.outputs <= most ? p.outputs : most / 256 * 256;
+  return many_rows<T>(p, piece) ? piece : 0;
 }
 
 template <typename T>
 struct Plan {
   dense::Operand<T, dense::GradKind<T>> x;
-  dense::Matrix w;  // decoded, where the rows are many
+  dense::Matrix w;  // decoded, where the rows are many: all outputs or a piece of them
   size_t bytes = 0;
   Plan(const ht_dense_problem &p, const void *xp, void *ws) {
     dense::Arena arena(ws);
     if (!few_rows<T>(p.rows)) x.set(arena, static_cast<const T *>(xp), p.rows, p.features, p.x_stride);
-    if (many_rows<T>(p)) {
-      w.rows = p.outputs, w.cols = p.features, w.pitch = blocks_of(p.features) * kBlock;
+    const int64_t piece = decoded_outputs<T>(p);
+    if (piece > 0) {
+      w.rows = piece, w.cols = p.features, w.pitch = blocks_of(p.features) * kBlock;
       w.data = arena.template take<__nv_bfloat16>(w.rows * w.pitch);
     }
     bytes = arena.used;
@@ -305,17 +317,25 @@ int forward(const ht_dense_problem &p, const void *x, const void *codes, const v
     HT_TRY(dense::lay_out<T>(stream, plan.x));
     if constexpr (kNumbers<T> == 1)
       if (plan.w.data != nullptr) {
-        const int64_t words = p.outputs * blocks_of(p.features) * 4;
-        HT_TRY((dense::launch_next<decode_kernel>(dim3(dense::blocks_for(words, 1024, 148 * 16)), 256, 0, 0, stream, 1, static_cast<const uint32_t *>(codes),
-                                                  static_cast<const uint8_t *>(scales), static_cast<uint4 *>(const_cast<void *>(plan.w.data)), words)));
-        dense::TileProblem t;
-        t.a[0] = plan.x.m;
-        t.b[0] = plan.w;
-        t.rows = p.rows, t.cols = p.outputs, t.k = p.features;
-        t.status_word = status_word;
-        const ScoresEpilogue<T> e = {(int)p.rows, (int)p.outputs, static_cast<const T *>(bias), static_cast<T *>(y),
-                                     dense::row_alignment(y, p.outputs * (int64_t)sizeof(T))};
-        return dense::launch_tiles<1, false, false>(t, e, dense::tile_shape(p.rows, p.outputs, p.features, 1, false), sms, stream);
+        const int64_t piece = plan.w.rows, per_output = blocks_of(p.features) * 4;
+        for (int64_t first = 0; first < p.outputs; first += piece) {
+          const int64_t count = std::min(piece, p.outputs - first), words = count * per_output;
+          HT_TRY((dense::launch_next<decode_kernel>(dim3(dense::blocks_for(words, 1024, 148 * 16)), 256, 0, 0, stream, 1,
+                                                    static_cast<const uint32_t *>(codes) + first * per_output,
+                                                    static_cast<const uint8_t *>(scales) + first * per_output / 4,
+                                                    static_cast<uint4 *>(const_cast<void *>(plan.w.data)), words)));
+          dense::TileProblem t;
+          t.a[0] = plan.x.m;
+          t.b[0] = plan.w;
+          t.b[0].rows = count;
+          t.rows = p.rows, t.cols = count, t.k = p.features;
+          t.status_word = status_word;
+          T *const to = static_cast<T *>(y) + first;
+          const ScoresEpilogue<T> e = {(int)p.rows, (int)count, bias != nullptr ? static_cast<const T *>(bias) + first : nullptr, to, p.outputs,
+                                       dense::row_alignment(to, p.outputs * (int64_t)sizeof(T))};
+          HT_TRY((dense::launch_tiles<1, false, false>(t, e, dense::tile_shape(p.rows, count, p.features, 1, false), sms, stream)));
+        }
+        return HT_OK;
       }
     return launch_tiles<T, kNumbers<T>>(plan.x.m, codes, static_cast<const uint8_t *>(scales), static_cast<const T *>(bias), static_cast<T *>(y), p.rows,
                                         p.features, p.outputs, status_word, sms, stream);

@@ -448,7 +448,8 @@ typedef struct ht_dense_problem {
   int64_t rows, features, outputs;
   int64_t x_stride;
   int64_t scratch_limit; /* backward: most bytes of the gradient with respect to the products that are held at a time (0: 512 MiB);
-                          * they are then formed and used a piece of the outputs at a time, 256 of them at the least */
+                          * they are then formed and used a piece of the outputs at a time, 256 of them at the least;
+                          * ht_linear_mx4: of decoded weights */
 } ht_dense_problem;
 
 /* h[n, o] = act(x[n] . gate_weight[o] + gate_bias[o]) * (x[n] . value_weight[o] + value_bias[o]).  The backward forms the projections
@@ -490,8 +491,9 @@ int ht_linear_class_loss_backward(const ht_dense_problem *p, const void *x, cons
 int ht_mx4_pack(int dtype, const void *w, int64_t w_stride, int64_t outputs, int64_t features, void *codes, void *scales, ht_stream_t stream);
 int ht_mx4_unpack(int dtype, const void *codes, const void *scales, int64_t outputs, int64_t features, void *w, int64_t w_stride, ht_stream_t stream);
 
-/* y[n, o] = x[n] . W[o] + bias[o] with W the values of codes and scales; x, bias (may be NULL) and y in the problem's type, sums fp32.  The problem's
- * activation and scratch_limit are not read.  x, bias and y start on 16 bytes (HT_ERR_UNSUPPORTED), the workspace on 256. */
+/* y[n, o] = x[n] . W[o] + bias[o] with W the values of codes and scales; x, bias (may be NULL) and y in the problem's type, sums fp32.  Of many
+ * bf16 rows the weights are decoded into the workspace first, scratch_limit bytes of them at a time at the most (0: 512 MiB), or not at all where that is
+ * too few of them to pay.  The problem's activation is not read.  x, bias and y start on 16 bytes (HT_ERR_UNSUPPORTED), the workspace on 256. */
 size_t ht_linear_mx4_workspace_bytes(const ht_dense_problem *p);
 int ht_linear_mx4(const ht_dense_problem *p, const void *x, const void *codes, const void *scales, const void *bias, void *y, void *workspace,
                   size_t workspace_bytes, uint32_t *status_word, ht_stream_t stream);

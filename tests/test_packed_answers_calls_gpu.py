@@ -1,11 +1,16 @@
 """Calls of the answers' functions that their documentation allows, at the ends of their arguments."""
+import ctypes
+import math
 import sys
 
 import pytest
 import torch
 
-from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R
+from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R, _cabi
+from hingetreefortorch_b200._ext import hingetree_cpp
 from test_dense_gpu import generator, normal
+from test_dense_host import DenseProblem
+from test_packed_answers_gpu import check_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +63,55 @@ def test_packed_head_draws_for_features_that_require_a_gradient():
     assert torch.equal(packed.sample(features, v)[0], forest.sample(rows, v, packed=packed)[0])
     with pytest.raises(RuntimeError, match="no derivative"):
         packed(features)
+
+
+# ---- scores of many rows with little memory ----------------------------------------------------------------------------
+
+def many_rows(rows, features, outputs):
+    gen = generator(outputs)
+    codes, scales = F.pack_mx4(normal(gen, outputs, features, scale=1 / math.sqrt(features)))
+    return normal(gen, rows, features, kind=torch.bfloat16), codes, scales, normal(gen, outputs, scale=0.5, kind=torch.bfloat16)
+
+
+def near(got, want):
+    """Sums of the same products in another order: each is off by half a step of bf16, 2^-9, and by far less in its sums."""
+    assert (got.float() - want.float()).norm() <= 2.0 ** -8 * want.float().norm()
+
+
+def test_decoded_weights_within_a_limit():
+    """Pieces of whole tiles, the last one ragged, and none at all; what lies behind the workspace's end stays as it was."""
+    rows, features, outputs = 1100, 1024, 30011
+    x, codes, scales, bias = many_rows(rows, features, outputs)
+    want = check_linear(x, codes, scales, bias)
+    lib = _cabi.library()
+    lib.ht_linear_mx4_workspace_bytes.restype = ctypes.c_size_t
+    at = lambda t: ctypes.c_void_p(t.data_ptr())
+    for limit, least in ((0, 2 * features * outputs), (1 << 40, 2 * features * outputs), (40 << 20, 36 << 20), (20 << 20, 18 << 20), (10 << 20, 0), (1, 0)):
+        p = DenseProblem(1, 0, rows, features, outputs, features, limit)
+        size = lib.ht_linear_mx4_workspace_bytes(ctypes.byref(p))
+        assert least <= size <= (limit if 1 < limit < 1 << 30 else least + 256), (limit, size)
+        room = torch.full((size + 256,), 77, dtype=torch.uint8, device="cuda")
+        got = torch.empty(rows, outputs, dtype=torch.bfloat16, device="cuda")
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        assert lib.ht_linear_mx4(ctypes.byref(p), at(x), at(codes), at(scales), at(bias), at(got), at(room), ctypes.c_size_t(size), None, stream) == 0
+        assert (room[size:] == 77).all()
+        near(got, want)
+        if size > 0:
+            assert lib.ht_linear_mx4(ctypes.byref(p), at(x), at(codes), at(scales), at(bias), at(got), at(room), ctypes.c_size_t(size - 1), None, stream) == -4
+
+
+def test_scores_without_room_for_decoded_weights():
+    """246 MB of scores are to be had, 123 MB of decoded weights beside them are not: scores all the same."""
+    x, codes, scales, bias = many_rows(4096, 2048, 30000)
+    want = check_linear(x, codes, scales, bias)
+    out = want.numel() * want.element_size()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + out + (60 << 20)) / total)
+    try:
+        got = F.linear_mx4(x, codes, scales, bias)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    near(got, want)
+    assert hingetree_cpp.pipeline_status() == 0
