@@ -8,7 +8,7 @@ import torch
 
 from hingetreefortorch_b200 import HingeTree as F, RandomHingeForest as R, _cabi
 from hingetreefortorch_b200._ext import hingetree_cpp
-from test_dense_gpu import generator, normal
+from test_dense_gpu import generator, lost, normal, within
 from test_dense_host import DenseProblem
 from test_packed_answers_gpu import check_linear
 
@@ -115,3 +115,21 @@ def test_scores_without_room_for_decoded_weights():
         torch.cuda.set_per_process_memory_fraction(1.0)
     near(got, want)
     assert hingetree_cpp.pipeline_status() == 0
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_smallest_numbers_of_fp32(rows):
+    """x as three bf16 numbers is exact from 2^-110 on; of what is smaller the third number leaves 2^-134, half of bf16's smallest.  Weights
+    between 2^98 and 2^108 lift the products into fp32's range, where 2^-140 is no matter."""
+    gen = generator(rows)
+    features = 200
+    codes = torch.randint(0, 256, (90, 16 * 7), generator=gen, device="cuda", dtype=torch.int32).to(torch.uint8)
+    scales = torch.randint(225, 235, (90, 7), generator=gen, device="cuda", dtype=torch.int32).to(torch.uint8)
+    w = F.unpack_mx4(codes, scales, features).double()
+    for size, lost_of_x in ((2.0 ** -106, 0.0), (2.0 ** -118, 2.0 ** -134), (2.0 ** -128, 2.0 ** -134)):
+        x = normal(gen, rows, features, scale=size)
+        if size == 2.0 ** -106:
+            x = torch.where(x.abs() < 2.0 ** -110, torch.zeros_like(x), x)
+        got = F.linear_mx4(x, codes, scales)
+        terms = x.double().abs() @ w.abs().t()
+        within(got, x.double() @ w.t(), (lost(features) + 2.0 ** -23) * terms + lost_of_x * w.abs().sum(1) + 2.0 ** -135, torch.float32)
