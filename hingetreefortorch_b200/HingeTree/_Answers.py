@@ -31,7 +31,8 @@ def linear_mx4(x, codes, scales, bias=None):
 
     x: [..., features], torch.float32, bfloat16 or float16; bias: [outputs] in x's type, or None; the result is in x's type.  Sums are fp32, and
     x enters them exactly: fp32 results are as accurate as fp32 products with the values (of finite numbers: an infinity gives NaN in fp32
-    and fp16).  Large calls of bfloat16 (1024 rows and 10 ** 10 multiplications on) hold decoded weights while they run, 2 bytes each and
+    and fp16; of fp32 numbers below 2 ** -110 what is less than 2 ** -134 is lost).  Those of 16-bit x are the tensor core's, which truncates when it adds:
+    some 3e-8 of a sum for every 16 features, below a step of the type up to 10 ** 5 of them.  Large calls of bfloat16 (1024 rows and 10 ** 10 multiplications on) hold decoded weights while they run, 2 bytes each and
     512 MiB at the most, or none, at a fifth more time, where memory is short.  No
     derivative: tensors that require a gradient are refused while gradients are recorded."""
     return hingetree_cpp.linear_mx4(x, codes, scales, bias)

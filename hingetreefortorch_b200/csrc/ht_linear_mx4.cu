@@ -20,9 +20,12 @@ constexpr int kNumbers = std::is_same<T, __nv_bfloat16>::value ? 1 : std::is_sam
 // are 16 contiguous bytes each, read straight into registers, some groups of outputs ahead.  x, the other operand, is in registers for good where
 // one warp's share of the features never changes: up to 16 warps share a group of outputs, and their sums meet in shared memory, those of four
 // groups at a time.
-// What bounds it: decoding, 11 instructions of half rate for every 8 weights, beside launch and the first loads' latency; the bytes alone would take
-// 4.2 of the 12.6 us.  Measured, 1024 to 50000: 1 to 8 rows of bf16 12.6 us, 16 rows 15.4, 8 rows of fp16 14.4, of fp32 18.5; 784 to 12700, 1 row
-// 5.5, most of it the launch.
+// What bounds it: latency.  The bytes alone take 4.2 us, decoding (11 instructions of half rate for 8 weights) 3.9; issue slots are 48 % and the
+// ALU pipe 47 % in use, and an instruction waits for loads for 2.1 of its 7 cycles, with one CTA of 16 warps an SM, 8 warps to 1024
+// features of 16 outputs, whose sums have to meet, and 11 such groups a team, which are three uneven turns.  Measured, 1024 to 50000: 1 to 8 rows of bf16
+// 12.6 us, 16 rows 15.4, 8 rows of fp16 14.4, of fp32 18.5 (the unpacked layer as torch's bf16 product: 1 row 22.7, 16 rows 23.1); 784 to 12700, 1 row
+// 5.5, most of it the launch.  Beyond 2048 features x does not stay in registers but is loaded for every 16 outputs: 2048 to 50000 24.5 us for 1 to 8 rows
+// and 28 for 16, 4096 to 50000 83 to 89 and 124, of which 17 rows take 55 as a tile.
 constexpr int kFewThreads = 512, kFewWarps = kFewThreads / 32;
 
 template <typename T>
@@ -272,7 +275,8 @@ struct ScoresEpilogue {
 
 // Whether that is the way.  us, decoded for every tile and decoded once, in long loops: 8192 x 1024 to 50000 788 and 660, 1024 rows of it 127 and 112, 512
 // rows 66 and 75; 8192 x 784 to 4096 76 and 53; 8192 x 2048 to 1000 38 and 34; 4096 x 200 to 20000 75 and 73; 8192 x 333 to 1001 19 and 26; 1024 x
-// 1024 to 1000 8 and 13.
+// 1024 to 1000 8 and 13.  fp16 and fp32 rows are not among them: the pair kernel has as many numbers a value on both sides, 3 products for two
+// and 6 for three, where weights of one number take 2 and 3.
 template <typename T>
 bool many_rows(const ht_dense_problem &p, int64_t outputs) {
   return kNumbers<T> == 1 && p.rows >= 1024 && (double)p.rows * (double)p.features * (double)outputs >= 1e10;

@@ -5,7 +5,8 @@
 //
 // Both are bound by memory: a thread takes 8 features, 4 threads a block, and two of those at a time, so that their loads are under way together; a
 // place's row comes by a multiplication (a division by the row's length took a third of the time).  Measured: 50000 x 1024 of fp32 packed in 35 us
-// (6.6 TB/s), unpacked to bf16 in 25 (5.1); 10007 x 771 of fp16, whose rows start on 2 bytes, 7.6 and 10.0 (value by value 24 and 30).
+// (6.6 TB/s), unpacked to bf16 in 26.5 (4.9; issue slots 80 % in use, the sign of zeros is 1.2 of them); 10007 x 771 of fp16, whose rows start on 2 bytes,
+// 7.7 and 10.2 (value by value 24 and 30).
 #include "ht_mx4.cuh"
 
 namespace ht {
